@@ -9,6 +9,20 @@ _c_i64_p = ctypes.c_void_p
 _int = ctypes.c_int
 _stream = ctypes.c_void_p
 
+
+
+class AttentionDesc(ctypes.Structure):
+    """camli_attention of include/camli_hip.h."""
+    _fields_ = [(n, _int) for n in ('type', 'B', 'H', 'Hk', 'Lq', 'Lk', 'D')] + [('scale', ctypes.c_float)] + [
+        (n, ctypes.c_void_p) for n in ('q', 'k', 'v')] + [(n, ctypes.c_int64 * 3) for n in ('q_stride', 'k_stride', 'v_stride')] + [
+        ('kv_lengths', ctypes.c_void_p), ('key_mask', ctypes.c_void_p), ('key_mask_batch_stride', ctypes.c_int64),
+        ('bias_table', ctypes.c_void_p), ('q_pos', ctypes.c_void_p), ('k_pos', ctypes.c_void_p),
+        ('q_pos_batch_stride', ctypes.c_int64), ('k_pos_batch_stride', ctypes.c_int64)] + [
+        (n, _int) for n in ('bias_axes', 'bias_buckets', 'bias_two_sided', 'bias_max_distance')]
+
+
+_desc_p = ctypes.POINTER(AttentionDesc)
+
 # name -> (restype, argtypes); every symbol include/camli_hip.h declares
 PROTOTYPES = {
     "camli_version": (_int, []),
@@ -175,6 +189,24 @@ PROTOTYPES = {
     "camli_weightnet_bwd_workspace_bytes": (ctypes.c_int64, [_int]),
     "camli_weightnet_bwd": (_int, [_c_float_p, _c_float_p, _c_i64_p, _int] + [_c_float_p] * 14
                             + [ctypes.c_int64, _int, _int, _int, _int, _int, _int, _stream]),
+    "camli_group_norm_fwd_workspace_bytes": (ctypes.c_int64, [_int] * 5),
+    "camli_group_norm_fwd": (_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, _int, ctypes.c_void_p,
+                                    _c_float_p, ctypes.c_void_p, ctypes.c_int64, _int, _int, _int, _int, ctypes.c_float, _int, _int, _stream]),
+    "camli_group_norm_bwd_workspace_bytes": (ctypes.c_int64, [_int] * 5),
+    "camli_group_norm_bwd": (_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, _int,
+                                    _c_float_p, ctypes.c_void_p, _c_float_p, _c_float_p, ctypes.c_void_p, ctypes.c_int64, _int, _int, _int,
+                                    _int, _int, _int, _stream]),
+    "camli_rel_bias_borders": (_int, [_int, _int, _int, ctypes.POINTER(_int)]),
+    "camli_rel_bias_fwd": (_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+                           + [_int] * 9 + [_stream]),
+    "camli_rel_bias_bwd_workspace_bytes": (ctypes.c_int64, [_int] * 7),
+    "camli_rel_bias_bwd": (_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                  ctypes.c_void_p, ctypes.c_int64] + [_int] * 9 + [_stream]),
+    "camli_cross_attention_fwd_workspace_bytes": (ctypes.c_int64, [_desc_p]),
+    "camli_cross_attention_fwd": (_int, [_desc_p, ctypes.c_void_p, _c_float_p, ctypes.c_void_p, ctypes.c_int64, _stream]),
+    "camli_cross_attention_bwd_workspace_bytes": (ctypes.c_int64, [_desc_p, _int]),
+    "camli_cross_attention_bwd": (_int, [_desc_p, ctypes.c_void_p, ctypes.c_void_p, _c_float_p] + [ctypes.c_void_p] * 5
+                                  + [ctypes.c_int64, _stream]),
 }
 
 _lib = None

@@ -1,0 +1,312 @@
+"""Cross attention and the bucketed relative position bias (camli_cross_attention_*, camli_rel_bias_*: csrc/hip/xattn.h, relbias.hip).
+
+What an attentive camera-LiDAR fusion needs where the reference gathers one nearest point per pixel (models/clfm.py:7-60): every
+pixel may attend every point and the other way round, with a learned bias by the offset of the two in the image.  Keys and values are
+never expanded over query heads and no score matrix is stored; the backward recomputes the probabilities from each row's log-sum.
+"""
+import ctypes
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .norm import TYPE_CODES, same_device
+from .wrapper import _on_device, _require_cuda, _stream_ptr
+
+MAX_HEAD_DIM = 128
+MAX_BIAS_ROWS = 128
+MAX_BIAS_DISTANCE = 1023
+
+
+# ------------------------------------------------------------------------------------------------
+# the bias: checks, buckets, stand-alone operator
+# ------------------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=64)
+def _bucket_of_offsets(buckets, bidirectional, max_distance):
+    """Bucket of every offset -max_distance .. max_distance, in exact integer arithmetic (the composed formulation's table)."""
+    side = buckets // 2 if bidirectional else buckets
+    exact = side // 2
+    steps = side - exact
+    out = []
+    for offset in range(-max_distance, max_distance + 1):
+        d = abs(offset) if bidirectional else max(-offset, 0)
+        if d < exact:
+            n = d
+        else:
+            n = exact + sum(1 for j in range(1, steps) if d ** steps >= max_distance ** j * exact ** (steps - j))
+        out.append(n + (side if bidirectional and offset > 0 else 0))
+    return out
+
+
+def _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, dtype, heads=None, batch=None, lq=None, lk=None):
+    """-> (table, q_pos, k_pos, batch of the bias or None, axes); positions [B or none, L, axes] int32 contiguous."""
+    if table is None or q_pos is None or k_pos is None:
+        raise ValueError('%s: a position bias needs the table and both positions' % name)
+    if table.dim() != 3 or table.dtype != dtype or dtype not in TYPE_CODES:
+        raise ValueError('%s: the table must be [axes, buckets, heads] of type %s, got %s %s' % (name, dtype, tuple(table.shape), table.dtype))
+    axes, buckets, h = table.shape
+    if axes not in (1, 2) or axes * buckets > MAX_BIAS_ROWS or h < 1 or (heads is not None and h != heads):
+        raise ValueError('%s: the table needs 1 or 2 axes, axes * buckets <= %d%s, got %s' % (
+            name, MAX_BIAS_ROWS, '' if heads is None else ' and %d heads' % heads, tuple(table.shape)))
+    side = buckets // 2 if bidirectional else buckets
+    if side < 2 or (bidirectional and buckets % 2) or not side // 2 < max_distance <= MAX_BIAS_DISTANCE or int(max_distance) != max_distance:
+        raise ValueError('%s: need at least two buckets a side (an even number when bidirectional) and %d < max_distance <= %d, got %d buckets and %r'
+                         % (name, side // 2, MAX_BIAS_DISTANCE, buckets, max_distance))
+    out = []
+    for what, pos, n in (('q_pos', q_pos, lq), ('k_pos', k_pos, lk)):
+        if pos.dtype != torch.int32 or pos.dim() not in (2, 3) or pos.shape[-1] != axes or (n is not None and pos.shape[-2] != n) or (
+                pos.dim() == 3 and batch is not None and pos.shape[0] != batch):
+            raise ValueError('%s: %s must be int32 [L, %d] or [B, L, %d] for the operands\' B and L, got %s %s' % (
+                name, what, axes, axes, tuple(pos.shape), pos.dtype))
+        out.append(pos.contiguous())
+    same_device(name, table, *out)
+    batches = {p.shape[0] for p in out if p.dim() == 3}
+    if len(batches) > 1:
+        raise ValueError('%s: q_pos and k_pos of different batches: %s' % (name, sorted(batches)))
+    return table.contiguous(), out[0], out[1], (batches.pop() if batches else None), axes
+
+
+def _pos_stride(pos):
+    return pos.shape[1] * pos.shape[2] if pos.dim() == 3 else 0
+
+
+def _composed_bias(table, q_pos, k_pos, bidirectional, max_distance):
+    axes, buckets, _ = table.shape
+    lut = torch.tensor(_bucket_of_offsets(buckets, bool(bidirectional), int(max_distance)), device=table.device)
+    total = 0
+    for a in range(axes):
+        offset = k_pos[..., None, :, a].long() - q_pos[..., :, None, a].long()
+        total = total + table[a].float()[lut[offset.clamp(-max_distance, max_distance) + max_distance]]
+    return total.movedim(-1, -3)            # [(B,) H, Lq, Lk]
+
+
+class _RelativeBias(torch.autograd.Function):
+    @staticmethod
+    @torch.amp.custom_fwd(device_type='cuda')
+    def forward(ctx, table, q_pos, k_pos, batch, bidirectional, max_distance):
+        lib = _lib.load()
+        axes, buckets, h = table.shape
+        lq, lk = q_pos.shape[-2], k_pos.shape[-2]
+        lead = (h,) if batch is None else (batch, h)
+        out = torch.empty(lead + (lq, lk), dtype=table.dtype, device=table.device)
+        ctx.save_for_backward(q_pos, k_pos)
+        ctx.args = (axes, buckets, h, batch, lq, lk, bidirectional, max_distance, table.dtype)
+        if out.numel():
+            with _on_device(table):
+                _lib.launch('camli_rel_bias_fwd', lib.camli_rel_bias_fwd, table.data_ptr(), q_pos.data_ptr(), _pos_stride(q_pos), k_pos.data_ptr(),
+                            _pos_stride(k_pos), out.data_ptr(), batch or 1, h, lq, lk, axes, buckets, int(bidirectional), max_distance,
+                            TYPE_CODES[table.dtype], _stream_ptr(table), work=(float(out.numel() * out.element_size()), 'B'))
+        return out
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type='cuda')
+    @once_differentiable
+    def backward(ctx, gout):
+        lib = _lib.load()
+        q_pos, k_pos = ctx.saved_tensors
+        axes, buckets, h, batch, lq, lk, bidirectional, max_distance, dtype = ctx.args
+        if not gout.numel():
+            return torch.zeros((axes, buckets, h), dtype=dtype, device=gout.device), None, None, None, None, None
+        gout = gout.contiguous()
+        gtable = torch.empty((axes, buckets, h), dtype=dtype, device=gout.device)
+        code, b = TYPE_CODES[dtype], batch or 1
+        ws_bytes = int(lib.camli_rel_bias_bwd_workspace_bytes(b, h, lq, lk, axes, buckets, code))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=gout.device)
+        with _on_device(gout):
+            _lib.launch('camli_rel_bias_bwd', lib.camli_rel_bias_bwd, gout.data_ptr(), q_pos.data_ptr(), _pos_stride(q_pos), k_pos.data_ptr(),
+                        _pos_stride(k_pos), gtable.data_ptr(), ws.data_ptr(), ws_bytes, b, h, lq, lk, axes, buckets, int(bidirectional),
+                        max_distance, code, _stream_ptr(gout), work=(float(gout.numel() * gout.element_size()), 'B'))
+        return gtable, None, None, None, None, None
+
+
+def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torch.Tensor, bidirectional=True, max_distance=128,
+                           cpp_impl=True):
+    """The learned bias of every query and key by their bucketed offset, [H, Lq, Lk] ([B, H, Lq, Lk] where a position tensor has a
+    batch): sum over axes a of table[a, bucket(k_pos[j, a] - q_pos[i, a]), h].
+
+    ``table`` [axes, buckets, H] (fp32, bf16 or fp16; the result has its type); ``q_pos`` / ``k_pos`` int32 [L, axes] or [B, L, axes], any
+    whole numbers (the running index of a sequence, pixel coordinates).  ``bidirectional``: half the buckets for each sign, the upper half
+    for keys after the query; otherwise all buckets for keys before the query, and keys after it share bucket 0.  Of the s buckets of a
+    side, e = s // 2 hold one distance each; bucket e + j begins at the first distance >= e (max_distance / e)^(j / (s - e)), and the last
+    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023.  Differentiable in the table (once);
+    the same bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
+    name = 'relative_position_bias'
+    table, q_pos, k_pos, batch, _ = _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, table.dtype if table is not None else None)
+    if (batch or 1) * table.shape[2] > 65535 or q_pos.shape[-2] > 2000000 or k_pos.shape[-2] >= 2 ** 31 - 2 ** 16:
+        raise ValueError('%s: more than 65535 samples x heads, 2000000 queries or 2^31 keys' % name)
+    if not cpp_impl:
+        return _composed_bias(table, q_pos, k_pos, bidirectional, int(max_distance)).to(table.dtype)
+    _require_cuda(name, table)
+    return _RelativeBias.apply(table, q_pos, k_pos, batch, bool(bidirectional), int(max_distance))
+
+
+# ------------------------------------------------------------------------------------------------
+# attention
+# ------------------------------------------------------------------------------------------------
+def _rows16(t):
+    """t itself if its rows are adjacent and start on 16 bytes with non-negative strides, else a dense copy."""
+    size = t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for n, s in zip(t.shape[:3], t.stride()[:3]) if n > 1):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strides(t):
+    return (ctypes.c_int64 * 3)(*[s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])])
+
+
+def _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance):
+    d = _lib.AttentionDesc()
+    d.type = TYPE_CODES[q.dtype]
+    d.B, d.Lq, d.H, d.D = q.shape
+    d.Lk, d.Hk = k.shape[1:3]
+    d.scale = scale
+    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    d.q_stride, d.k_stride, d.v_stride = _strides(q), _strides(k), _strides(v)
+    if kv_lengths is not None:
+        d.kv_lengths = kv_lengths.data_ptr()
+    if key_mask is not None:
+        d.key_mask, d.key_mask_batch_stride = key_mask.data_ptr(), key_mask.shape[1]
+    if table is not None:
+        d.bias_table, d.q_pos, d.k_pos = table.data_ptr(), q_pos.data_ptr(), k_pos.data_ptr()
+        d.q_pos_batch_stride, d.k_pos_batch_stride = _pos_stride(q_pos), _pos_stride(k_pos)
+        d.bias_axes, d.bias_buckets = table.shape[:2]
+        d.bias_two_sided, d.bias_max_distance = int(bidirectional), max_distance
+    return d
+
+
+def _workspace(name, n, like):
+    if n < 0:
+        _lib.check(int(n), name)
+    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=like.device)
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    @torch.amp.custom_fwd(device_type='cuda')
+    def forward(ctx, q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance):
+        lib = _lib.load()
+        b, lq, h, dim = q.shape
+        lk = k.shape[1]
+        ctx.args = (scale, bidirectional, max_distance)
+        if q.numel() == 0 or lk == 0:
+            ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, None, None)
+            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
+        lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad[:4]) else None
+        d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
+        size = q.element_size()
+        with _on_device(q):
+            n = lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d))
+            ws = _workspace('camli_cross_attention_fwd', n, q)
+            _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, ctypes.byref(d), out.data_ptr(),
+                        lse.data_ptr() if lse is not None else None, ws.data_ptr(), n, _stream_ptr(q),
+                        work=(float(size * (2 * q.numel() + 2 * b * lk * k.shape[2] * dim)), 'B'), flop=4.0 * b * h * lq * lk * dim)
+        ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, lse)
+        return out
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type='cuda')
+    @once_differentiable
+    def backward(ctx, gout):
+        lib = _lib.load()
+        q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, lse = ctx.saved_tensors
+        need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
+        nothing = (None,) * 7
+        if out is None:
+            return (torch.zeros_like(q) if need_q else None, torch.zeros_like(k) if need_k else None,
+                    torch.zeros_like(v) if need_v else None, torch.zeros_like(table) if need_t else None) + nothing
+        b, lq, h, dim = q.shape
+        lk, hk = k.shape[1:3]
+        gout = gout.contiguous()
+        if gout.data_ptr() % 16:
+            gout = gout.clone()
+        gq = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device) if need_q else None
+        gk = gv = None
+        if need_k or need_v:
+            gk, gv = (torch.empty((b, lk, hk, dim), dtype=q.dtype, device=q.device) for _ in range(2))
+        gt = torch.empty(table.shape, dtype=table.dtype, device=q.device) if need_t else None
+        d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, *ctx.args)
+        size = q.element_size()
+
+        def ptr(t):
+            return t.data_ptr() if t is not None else None
+        with _on_device(q):
+            n = lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), int(need_t))
+            ws = _workspace('camli_cross_attention_bwd', n, q)
+            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, ctypes.byref(d), out.data_ptr(), gout.data_ptr(),
+                        lse.data_ptr(), ptr(gq), ptr(gk), ptr(gv), ptr(gt), ws.data_ptr(), n, _stream_ptr(q),
+                        work=(float(size * (4 * q.numel() + 4 * b * lk * hk * dim)), 'B'), flop=10.0 * b * h * lq * lk * dim)
+        return (gq, gk if need_k else None, gv if need_v else None, gt) + nothing
+
+
+def _composed_attention(q, k, v, scale, kv_lengths, key_mask, bias):
+    b, lq, h, dim = q.shape
+    lk, hk = k.shape[1:3]
+    qh = q.float().permute(0, 2, 1, 3)
+    kh, vh = (t.float().permute(0, 2, 1, 3).repeat_interleave(h // hk, dim=1) for t in (k, v))
+    keep = torch.ones(b, lk, dtype=torch.bool, device=q.device)
+    if kv_lengths is not None:
+        keep &= torch.arange(lk, device=q.device) < kv_lengths[:, None]
+    if key_mask is not None:
+        keep &= key_mask
+    rows = keep[:, None, :, None]
+    kh, vh = torch.where(rows, kh, torch.zeros_like(kh)), torch.where(rows, vh, torch.zeros_like(vh))
+    scores = torch.matmul(qh, kh.transpose(2, 3).contiguous()) * scale
+    if bias is not None:
+        scores = scores + bias
+    scores = torch.where(keep[:, None, None, :], scores, torch.full_like(scores, -math.inf))
+    if lk == 0:
+        return torch.zeros_like(q)
+    top = scores.amax(dim=-1, keepdim=True).detach()
+    weights = torch.exp(scores - torch.where(top == -math.inf, torch.zeros_like(top), top))
+    total = weights.sum(dim=-1, keepdim=True)
+    return torch.matmul(weights / torch.where(total == 0, torch.ones_like(total), total), vh).permute(0, 2, 1, 3).to(q.dtype)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=None, kv_lengths=None, key_mask=None, bias_table=None,
+                    q_pos=None, k_pos=None, bidirectional=True, max_distance=128, cpp_impl=True):
+    """softmax(scale q k^T + bias) v of queries q [B, Lq, H, D] over keys and values k, v [B, Lk, Hk, D] of another length -> [B, Lq, H, D].
+
+    fp32, bf16 or fp16 (one type for all; sums and softmax in fp32); D a multiple of 8 up to 128; H a multiple of Hk (query heads
+    h share key / value head h // (H / Hk)).  Any strides: rows that are not adjacent or 16-byte aligned are copied first.  ``scale``:
+    positive, default D ** -0.5.  One token (Lq = 1) and other short queries are split over the keys.
+
+    ``kv_lengths`` int32 [B]: keys from there on are padding (values outside 0 .. Lk are clamped); ``key_mask`` bool [B, Lk]: False masks a
+    key; a key is kept if both keep it.  Masked keys and values may hold anything, NaN included, and get zero gradients.  A query that
+    keeps no key gives zeros and takes no part in any gradient.
+
+    ``bias_table`` [axes, buckets, H] of q's type with int32 ``q_pos`` [Lq, axes] or [B, Lq, axes] and ``k_pos`` likewise adds the bias
+    that :func:`relative_position_bias` describes, without storing it.  Differentiable in q, k, v and bias_table (once); the same
+    bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
+    name = 'cross_attention'
+    if any(t.dim() != 4 for t in (q, k, v)) or q.dtype not in TYPE_CODES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('%s: q, k, v must be [B, L, H, D] of one type (fp32, bf16, fp16), got %s' % (
+            name, ', '.join('%s %s' % (tuple(t.shape), t.dtype) for t in (q, k, v))))
+    b, lq, h, dim = q.shape
+    lk, hk = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != dim or hk < 1 or h < 1 or h % hk:
+        raise ValueError('%s: shapes do not belong together: q %s, k %s, v %s' % (name, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM:
+        raise ValueError('%s: the head width must be a multiple of 8 up to %d, got %d' % (name, MAX_HEAD_DIM, dim))
+    scale = float(dim) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError('%s: scale must be positive and finite, got %r' % (name, scale))
+    if kv_lengths is not None and (kv_lengths.shape != (b,) or kv_lengths.dtype != torch.int32):
+        raise ValueError('%s: kv_lengths must be int32 [%d], got %s %s' % (name, b, tuple(kv_lengths.shape), kv_lengths.dtype))
+    if key_mask is not None and (key_mask.shape != (b, lk) or key_mask.dtype != torch.bool):
+        raise ValueError('%s: key_mask must be bool [%d, %d], got %s %s' % (name, b, lk, tuple(key_mask.shape), key_mask.dtype))
+    if bias_table is not None or q_pos is not None or k_pos is not None:
+        bias_table, q_pos, k_pos, _, _ = _check_bias(name, bias_table, q_pos, k_pos, bidirectional, max_distance, q.dtype, h, b, lq, lk)
+    same_device(name, q, k, v, kv_lengths, key_mask, bias_table)
+    if not cpp_impl:
+        bias = _composed_bias(bias_table, q_pos, k_pos, bidirectional, int(max_distance)) if bias_table is not None else None
+        return _composed_attention(q, k, v, scale, kv_lengths, key_mask, bias)
+    _require_cuda(name, q)
+    return _CrossAttention.apply(q, k, v, bias_table, kv_lengths.contiguous() if kv_lengths is not None else None,
+                                 key_mask.contiguous() if key_mask is not None else None, q_pos, k_pos, scale, bool(bidirectional),
+                                 int(max_distance))

@@ -11,7 +11,10 @@ LIB_PATH = os.path.join(HERE, "libcamli_hip.so")
 
 # -ffp-contract=off: KNN / FPS distances are specified UNFUSED (oracle/camli_oracle.c); dot products
 # that may fuse say so explicitly with __builtin_fmaf.
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, which the vectoriser forms from ordinary float code and some of whose forms are not
+# reliable here (the host pass warns that it does not know the feature).
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-source additions.  corr3dmlp: the SLP vectoriser pairs the fmaf chains into v_pk_fma_f32, whose operands must be
 # vector registers -- the 1024 wave-uniform weights then leave the scalar registers (512 VGPRs + scratch instead of 168)
 EXTRA_FLAGS = {"corr3dmlp.hip": ["-fno-slp-vectorize"]}

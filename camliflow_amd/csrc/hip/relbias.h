@@ -1,0 +1,50 @@
+// Learned relative position bias by buckets: what relbias.hip and the attention kernels (xattn.h) share.
+//
+//   bias[h, i, j] = sum_a table[a, bucket(kpos[j, a] - qpos[i, a]), h],    a = 0 .. axes - 1
+//
+// bucket(o), two-sided: side = buckets / 2, d = |o|, + side where o > 0; one-sided: side = buckets, d = max(-o, 0).  Distances
+// below e = side / 2 have a bucket each; beyond, bucket e + j starts at the smallest d with d >= e (limit / e)^(j / (side - e)), and
+// the last one has no end.  The borders are whole numbers found on the host in exact arithmetic (rel_bias_borders); they travel as
+// kernel arguments, so no call uploads anything and a captured graph holds everything it needs.
+//
+// Offsets beyond +-limit share the bucket of the limit: a workgroup expands its heads' table columns to one float per offset in
+// LDS (2 limit + 1 entries), and the bias of a pair is subtract, clamp, one LDS read.
+#pragma once
+#include "typed.h"
+
+#define CAMLI_REL_MAX_LIMIT 1023
+#define CAMLI_REL_MAX_ROWS 128      // axes * buckets
+#define CAMLI_REL_MAX_BORDERS 64
+
+struct RelBias {
+    const void* table;          // [axes][buckets][H]
+    const int *qpos, *kpos;     // [.., L, axes], batch strides in ints (0: shared)
+    int64_t qpos_bs, kpos_bs;
+    int type, axes, buckets, side, exact, two_sided, limit, n_borders;
+    short border[CAMLI_REL_MAX_BORDERS];
+};
+
+// fills r; false (with the error set) for arguments outside the documented range
+bool rel_bias_args(RelBias& r, const char* who, const void* table, int type, const int* qpos, int64_t qpos_bs, const int* kpos,
+                   int64_t kpos_bs, int axes, int buckets, int two_sided, int limit);
+
+// gtable[row][h] = sum over parts of partial[h][part][row], row = a * buckets + n, in a fixed order and in 64 bits
+int rel_bias_join(const float* partial, void* gtable, int type, int H, int nrows, int64_t parts, const char* who, hipStream_t s);
+
+// bucket of the clamped offset index i in 0 .. 2 limit
+__device__ __forceinline__ int rel_bucket(const RelBias& r, int i) {
+    const int o = i - r.limit;
+    const int d = r.two_sided ? abs(o) : max(-o, 0);
+    int n = d;
+    if (d >= r.exact) {
+        n = r.exact;
+        for (int j = 0; j < r.n_borders; ++j) n += r.border[j] <= d ? 1 : 0;
+    }
+    return n + (r.two_sided && o > 0 ? r.side : 0);
+}
+
+// offset index of a pair: saturating, so positions of any size are safe
+__device__ __forceinline__ int rel_index(int kpos, int qpos, int limit) {
+    const int o = __builtin_elementwise_sub_sat(kpos, qpos);
+    return min(max(o, -limit), limit) + limit;
+}

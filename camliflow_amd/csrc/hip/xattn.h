@@ -1,0 +1,823 @@
+// Cross attention over keys and values of another length, with an optional bucketed position bias: forward, both adjoints, gfx950.
+// The three element types instantiate these kernels in files of their own (xattn_f32.hip, xattn_bf16.hip, xattn_f16.hip); checks,
+// split rules and the C entries are in xattn.hip.
+//
+//   s_ij = scale q_i . k_j + bias[h, i, j],   p = softmax_j over the kept keys,   o_i = sum_j p_ij v_j      (no kept key: o_i = 0)
+//   D_i = do_i . o_i,   dp_ij = do_i . v_j,   ds = p (dp - D),   dq = scale ds k,   dk = scale ds^T q,   dv = p^T do,
+//   dtable[a, n, h] = sum of ds over the pairs whose bucket on axis a is n
+//
+// One scheme for all three kernels.  A wave OWNS 32 rows of one side (queries in fwd and dq, keys in dkdv) whose vectors sit in
+// registers as the B operand of 32x32 matrix instructions, one row per lane (lanes l and l + 32 share row l); the other side streams
+// through LDS in row-major tiles that all waves share.  The product tile then has the owned row on the lanes and the streamed rows in
+// the 16 accumulator registers, so
+//   * softmax statistics are per lane: no cross-lane traffic but one half-wave swap per tile,
+//   * the same registers, rounded to the element type, ARE the B operand of the second product (the contraction order over the
+//     streamed rows is free as long as both operands agree on it): P never leaves the registers,
+//   * the A operand of the second product is the streamed tile transposed; 16-bit types read it with the transposing LDS load,
+//     fp32 with plain 4-byte reads, which are conflict-free on row-major tiles.
+// Register i of half h holds streamed row 8 (i / 4) + 4 h + i % 4 of its 32-row block.
+//
+// Two adjoint kernels recompute p instead of one that adds dq with float atomics: 14 D instead of 10 D operations per pair, but
+// every sum has a fixed order (the same bits on every run).  P and dS are rounded to the element type for the second products (their
+// sums stay fp32): half a step of the inputs' own type, as for every operand of a matrix product.
+#pragma once
+#include "camli_hip.h"
+#include "relbias.h"
+
+namespace xattn {
+
+struct Strides {
+    int64_t b, l, h;            // elements
+};
+
+struct Args {
+    const void *q, *k, *v, *o, *go;
+    Strides qs, ks, vs;         // o, go and the gradients are dense [B][L][heads][D]
+    void *out, *dq, *dk, *dv;
+    float *lse;                 // [B][H][Lq], log2 domain; +inf where no key is kept
+    float *delta;               // [B][H][Lq]
+    float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [split][B][H][Lq] (-inf: no key)
+    float *part_dk, *part_dv;   // splits > 1: [split][B][Lk][Hk][D]
+    float *part_table;          // [H][parts][axes * buckets]
+    const int *lengths;         // [B] or null
+    const unsigned char *mask;  // [B][mask_bs] or null
+    int64_t mask_bs;
+    int B, H, Hk, Lq, Lk, D;
+    int pack;                   // query heads of one kv head that share a workgroup's rows (few queries), else 1
+    int row_tiles, splits, tiles_per_split, parts;
+    float scale, scale_log2;
+    RelBias rb;
+};
+
+typedef float acc16 __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef unsigned chunk16 __attribute__((ext_vector_type(4)));       // 16 bytes in flight
+
+// 16-byte fragments: what a lane holds of one operand for one k-step
+template <typename T> struct Mat;
+template <> struct Mat<__bf16> {
+    typedef __bf16 frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ acc16 mma(frag a, frag b, acc16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<_Float16> {
+    typedef _Float16 frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ acc16 mma(frag a, frag b, acc16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<float> {
+    typedef float frag __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ acc16 mma(frag a, frag b, acc16 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <typename T>
+using FragOf = typename Mat<T>::frag;
+
+template <typename T, int DP>
+struct Tile {
+    static constexpr int E = 16 / sizeof(T);            // elements of a 16-byte chunk
+    static constexpr int CHUNKS = DP / E;               // chunks of a row
+    static constexpr int ROWS = sizeof(T) == 2 ? 64 : 32;
+    static constexpr int BLOCKS = ROWS / 32;
+    static constexpr int LD = DP + E;                   // 16 bytes of padding: rows start 4 banks apart (mod 64), no conflicts on either read
+    static constexpr int ELEMS = ROWS * LD;
+    static constexpr int KSTEPS = CHUNKS / 2;           // k-steps of a product over DP
+    static constexpr int PSTEPS = 16 / E;               // k-steps of a product over 32 streamed rows
+    static constexpr int DBLOCKS = DP / 32;
+};
+
+// chunk c of a streamed row: the A operand (row = lane % 32) of products over DP
+template <typename T, int DP>
+__device__ __forceinline__ FragOf<T> read_row(const T* tile, int row, int chunk) {
+    return *reinterpret_cast<const FragOf<T>*>(tile + row * Tile<T, DP>::LD + chunk * Tile<T, DP>::E);
+}
+
+// A operand of products over the streamed rows: lane l = column d0 + l % 32, k-step t of block `row0` in the order the accumulator has
+template <typename T, int DP>
+__device__ __forceinline__ FragOf<T> read_col(const T* tile, int row0, int t, int d0, int lane) {
+    constexpr int LD = Tile<T, DP>::LD;
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        // the transposing load: 16 lanes fetch 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows each
+        typedef __attribute__((address_space(3))) short4v* lds_ptr;
+        const int l = lane & 15;
+        const T* p = tile + (row0 + 16 * t + 4 * h + (l >> 2)) * LD + d0 + (lane & 16) + (l & 3) * 4;
+        union { short4v s[2]; FragOf<T> f; } u;
+        u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(p)));
+        u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(p + 8 * LD)));
+        return u.f;
+    } else {
+        const T* p = tile + (row0 + 8 * t + 4 * h) * LD + d0 + (lane & 31);
+        FragOf<T> f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = p[i * LD];
+        return f;
+    }
+}
+
+// k-step t of the accumulator, rounded to the element type
+template <typename T>
+__device__ __forceinline__ FragOf<T> pack_step(const acc16& x, int t) {
+    constexpr int E = 16 / sizeof(T);
+    FragOf<T> f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = (T)x[t * E + i];
+    return f;
+}
+
+__device__ __forceinline__ int acc_row(int i, int h) { return (i >> 2) * 8 + 4 * h + (i & 3); }
+
+__device__ __forceinline__ float other_half(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
+}
+__device__ __forceinline__ float half_max(float x) { return fmaxf(x, other_half(x)); }
+__device__ __forceinline__ float half_sum(float x) { return x + other_half(x); }
+
+// Workgroups go round-robin over the 8 XCDs: give each XCD a contiguous range of work, so that the workgroups which stream the same
+// keys and values (or queries) share one L2.
+__device__ __forceinline__ int xcd_contiguous(int id, int n) {
+    const int x = id & 7, per = n >> 3, rem = n & 7;
+    return x * per + min(x, rem) + (id >> 3);
+}
+
+// The streamed pair of tiles on its way from memory: registers now, LDS later.  A row at or beyond `limit`, a masked row and columns
+// from D on become zeros (a masked row may hold anything, and 0 * NaN is NaN).
+template <typename T, int DP, int THREADS>
+struct Stream {
+    using TL = Tile<T, DP>;
+    static constexpr int N = TL::ROWS * TL::CHUNKS / THREADS;
+    chunk16 x[N], y[N];
+    unsigned keep;
+
+    __device__ __forceinline__ void load(const T* px, int64_t ldx, const T* py, int64_t ldy, int row0, int limit, int D, const unsigned char* mask) {
+        keep = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int f = threadIdx.x + n * THREADS, row = row0 + f / TL::CHUNKS, c = (f % TL::CHUNKS) * TL::E;
+            x[n] = y[n] = chunk16{0, 0, 0, 0};
+            if (row < limit && c < D) {
+                x[n] = *reinterpret_cast<const chunk16*>(px + row * ldx + c);
+                y[n] = *reinterpret_cast<const chunk16*>(py + row * ldy + c);
+                keep |= (mask == nullptr || mask[row] != 0 ? 1u : 0u) << n;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* tx, T* ty) const {
+        const chunk16 zero = {0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int f = threadIdx.x + n * THREADS, at = (f / TL::CHUNKS) * TL::LD + (f % TL::CHUNKS) * TL::E;
+            const bool k = (keep >> n) & 1;
+            *reinterpret_cast<chunk16*>(tx + at) = k ? x[n] : zero;
+            *reinterpret_cast<chunk16*>(ty + at) = k ? y[n] : zero;
+        }
+    }
+};
+
+// owned row -> B fragments (zeros beyond D and for rows that do not exist)
+template <typename T, int DP>
+__device__ __forceinline__ void load_owned(FragOf<T>* f, const T* row, bool exists, int D, int h) {
+    using TL = Tile<T, DP>;
+#pragma unroll
+    for (int s = 0; s < TL::KSTEPS; ++s) {
+        const int c = (2 * s + h) * TL::E;
+        FragOf<T> z = {};
+        f[s] = z;
+        if (exists && c < D) f[s] = *reinterpret_cast<const FragOf<T>*>(row + c);
+    }
+}
+
+// [DBLOCKS] accumulators (column of the owned row on the lane) -> dense row of elements, or of floats
+template <typename O, int DBLOCKS>
+__device__ __forceinline__ void store_owned(O* row, const acc16 (&o)[DBLOCKS], float mul, int D, int h) {
+#pragma unroll
+    for (int db = 0; db < DBLOCKS; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = db * 32 + acc_row(i, h);
+            if (d < D) {
+                const float v[4] = {o[db][i] * mul, o[db][i + 1] * mul, o[db][i + 2] * mul, o[db][i + 3] * mul};
+                store_f32<O, 4>(row + d, v);
+            }
+        }
+}
+
+__device__ __forceinline__ int kept_length(const Args& a, int b) {
+    return a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
+}
+
+// bit j: key row0 + j is kept.  Called by whole waves.
+__device__ __forceinline__ unsigned long long kept_bits(const unsigned char* mask, int row0, int len, int rows) {
+    const int lane = threadIdx.x & 63, key = row0 + lane;
+    bool k = lane < rows && key < len;
+    if (k && mask) k = mask[key] != 0;
+    return __ballot(k);
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// table columns of `pack` heads, one value per offset: lut[p][axis][2 limit + 1], log2 domain
+template <int AXES, int THREADS>
+__device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0, int pack, int H) {
+    const int span = 2 * r.limit + 1;
+    for (int i = threadIdx.x; i < span; i += THREADS) {
+        const int n = rel_bucket(r, i);
+        for (int p = 0; p < pack; ++p)
+#pragma unroll
+            for (int a = 0; a < AXES; ++a)
+                lut[(p * AXES + a) * span + i] = load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + head0 + p) * LOG2E;
+    }
+}
+
+// positions of the streamed rows: pos[axis][ROWS]
+template <int AXES, int ROWS>
+__device__ __forceinline__ int load_pos(const int* pos, int row0, int limit) {
+    const int t = threadIdx.x;
+    if (t >= AXES * ROWS) return 0;
+    const int row = min(row0 + t % ROWS, limit - 1);
+    return pos[(int64_t)row * AXES + t / ROWS];
+}
+
+// ------------------------------------------------------------------------------------------------------------ forward
+template <typename T, int DP, int AXES>
+__global__ __launch_bounds__(256) void fwd_kernel(Args a) {
+    using TL = Tile<T, DP>;
+    using Frag = FragOf<T>;
+    constexpr int THREADS = 256;
+    extern __shared__ __align__(16) char smem[];
+    T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
+    int* pos = reinterpret_cast<int*>(tiles + 4 * TL::ELEMS);               // [2][AXES][ROWS]
+    float* lut = reinterpret_cast<float*>(pos + 2 * AXES * TL::ROWS);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int groups = a.H / a.pack;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int rt = id % a.row_tiles;
+    id /= a.row_tiles;
+    const int hh = id % groups, b = id / groups, kvh = hh * a.pack / (a.H / a.Hk);
+    const int row = rt * 128 + wave * 32 + (lane & 31), rows = a.pack * a.Lq;
+    const bool exists = row < rows;
+    const int sub = exists ? row / a.Lq : 0, qi = exists ? row - sub * a.Lq : 0, head = hh * a.pack + sub;
+
+    const int len = kept_length(a, b);
+    const int n_tiles = (len + TL::ROWS - 1) / TL::ROWS;
+    const int t0 = split * a.tiles_per_split, t1 = min(n_tiles, t0 + a.tiles_per_split);
+    const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + kvh * a.ks.h;
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
+
+    Frag qf[TL::KSTEPS];
+    load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + qi * a.qs.l + head * a.qs.h, exists, a.D, h);
+    int qp[AXES ? AXES : 1] = {0};
+    const int span = 2 * a.rb.limit + 1;
+    const float* my_lut = lut + sub * AXES * span;
+    const int* kpos = nullptr;
+    if constexpr (AXES > 0) {
+        fill_lut<AXES, THREADS>(a.rb, lut, hh * a.pack, a.pack, a.H);
+        kpos = a.rb.kpos + b * a.rb.kpos_bs;
+#pragma unroll
+        for (int x = 0; x < AXES; ++x) qp[x] = a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x];
+    }
+
+    acc16 o[TL::DBLOCKS];
+#pragma unroll
+    for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = acc16{0};
+    float m = -INFINITY, m_use = 0.0f, l = 0.0f;
+
+    Stream<T, DP, THREADS> st;
+    int pnext = 0, cur = 0;
+    if (t0 < t1) {
+        st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
+        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, t0 * TL::ROWS, len);
+        st.store(tiles, tiles + TL::ELEMS);
+        if constexpr (AXES > 0)
+            if (tid < AXES * TL::ROWS) pos[tid] = pnext;
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
+        if (t + 1 < t1) {
+            st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
+            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, (t + 1) * TL::ROWS, len);
+        }
+        const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
+        const int* pt = pos + cur * AXES * TL::ROWS;
+        if (bits != 0) {
+            acc16 s[TL::BLOCKS];
+            float top = -INFINITY;
+#pragma unroll
+            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+                s[nb] = acc16{0};
+#pragma unroll
+                for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(read_row<T, DP>(kt, nb * 32 + (lane & 31), 2 * ks + h), qf[ks], s[nb]);
+            }
+#pragma unroll
+            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+                if constexpr (AXES > 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = nb * 32 + acc_row(i, h);
+                        float bias = my_lut[rel_index(pt[r], qp[0], a.rb.limit)];
+                        if constexpr (AXES > 1) bias += my_lut[span + rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit)];
+                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, bias);
+                    }
+                }
+                const unsigned half = (unsigned)(bits >> (nb * 32));
+                if (half != 0xffffffffu) {
+                    const unsigned mine = half >> (4 * h);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[nb][i] = (mine >> acc_row(i, 0)) & 1 ? s[nb][i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
+            }
+            top = half_max(top);
+            if constexpr (AXES == 0) top *= a.scale_log2;
+            // the running maximum may lag by 8 (p <= 2^8, sums in fp32): the accumulators are rescaled only when a row passes that
+            if (__any(top > m + 8.0f)) {
+                const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m - use);
+#pragma unroll
+                for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+                l *= alpha;
+                m = mn;
+                m_use = use;
+            }
+#pragma unroll
+            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[nb][i] = __builtin_amdgcn_exp2f(AXES == 0 ? __builtin_fmaf(s[nb][i], a.scale_log2, -m_use) : s[nb][i] - m_use);
+                    l += s[nb][i];
+                }
+#pragma unroll
+                for (int ps = 0; ps < TL::PSTEPS; ++ps) {
+                    const Frag p = pack_step<T>(s[nb], ps);
+#pragma unroll
+                    for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = Mat<T>::mma(read_col<T, DP>(vt, nb * 32, ps, d * 32, lane), p, o[d]);
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
+            st.store(nk, nk + TL::ELEMS);
+            if constexpr (AXES > 0)
+                if (tid < AXES * TL::ROWS) pos[(cur ^ 1) * AXES * TL::ROWS + tid] = pnext;
+        }
+        __syncthreads();
+        cur ^= 1;
+    }
+    l = half_sum(l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (!exists) return;
+    const int64_t at = ((int64_t)b * a.Lq + qi) * a.H + head, stat = ((int64_t)b * a.H + head) * a.Lq + qi;
+    const float lse = m_use + __builtin_amdgcn_logf(l);      // log2
+    if (a.splits > 1) {
+        const int64_t per = (int64_t)a.B * a.Lq * a.H;
+        store_owned<float, TL::DBLOCKS>(a.part_o + (split * per + at) * a.D, o, inv, a.D, h);
+        if (h == 0) a.part_lse[split * per + stat] = l == 0.0f ? -INFINITY : lse;
+    } else {
+        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, h);
+        if (a.lse && h == 0) a.lse[stat] = l == 0.0f ? INFINITY : lse;
+    }
+}
+
+// joins the splits of the forward: one thread per 4 elements of a row
+template <typename T>
+__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
+    const int per_row = a.D / 4;
+    const int64_t rows = (int64_t)a.B * a.Lq * a.H, t = (int64_t)blockIdx.x * 256 + threadIdx.x, at = t / per_row;
+    if (at >= rows) return;
+    const int c = (int)(t - at * per_row) * 4;
+    const int head = (int)(at % a.H);
+    const int64_t bq = at / a.H;
+    const int64_t stat = ((bq / a.Lq) * a.H + head) * a.Lq + bq % a.Lq;
+    float top = -INFINITY;
+    bool bad = false;
+    for (int s = 0; s < a.splits; ++s) {
+        const float v = a.part_lse[s * rows + stat];
+        top = fmaxf(top, v);
+        bad |= v != v;
+    }
+    const float use = top == -INFINITY ? 0.0f : top;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = __builtin_amdgcn_exp2f(a.part_lse[s * rows + stat] - use);
+        if (w == 0.0f) continue;
+        float v[4];
+        load_f32<float, 4>(a.part_o + (s * rows + at) * a.D + c, v);
+        sum += w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = bad ? NAN : acc[i] * inv;
+    store_f32<T, 4>(static_cast<T*>(a.out) + at * a.D + c, acc);
+    if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + __builtin_amdgcn_logf(sum);
+}
+
+// ------------------------------------------------------------------------------------------------------------ dq
+// WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, bucket of every offset,
+// hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
+template <typename T, int DP, int AXES, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
+    using TL = Tile<T, DP>;
+    using Frag = FragOf<T>;
+    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES;
+    extern __shared__ __align__(16) char smem[];
+    T* tiles = reinterpret_cast<T*>(smem);
+    int* pos = reinterpret_cast<int*>(tiles + 4 * TL::ELEMS);
+    float* lut = reinterpret_cast<float*>(pos + 2 * AXES * TL::ROWS);
+    const int span = 2 * a.rb.limit + 1, hist_rows = AXES * a.rb.buckets;
+    float* hist = lut + AXES * span;
+    unsigned short* bucket = reinterpret_cast<unsigned short*>(hist + hist_rows * THREADS);
+    const bool table_grad = AXES > 0 && a.part_table != nullptr;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int rt = id % a.row_tiles;
+    id /= a.row_tiles;
+    const int head = id % a.H, b = id / a.H, kvh = head / (a.H / a.Hk);
+    const int qi = rt * OWN + wave * 32 + (lane & 31);
+    const bool exists = qi < a.Lq;
+    const int q0 = exists ? qi : 0;
+
+    const int len = kept_length(a, b);
+    const int n_tiles = (len + TL::ROWS - 1) / TL::ROWS;
+    const int t0 = split * a.tiles_per_split;
+    const int t1 = a.dq || table_grad ? min(n_tiles, t0 + a.tiles_per_split) : t0;      // else only delta is wanted
+    const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + kvh * a.ks.h;
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
+    const int64_t at = ((int64_t)b * a.Lq + q0) * a.H + head, stat = ((int64_t)b * a.H + head) * a.Lq + q0;
+
+    Frag qf[TL::KSTEPS], gf[TL::KSTEPS];
+    load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + q0 * a.qs.l + head * a.qs.h, exists, a.D, h);
+    load_owned<T, DP>(gf, static_cast<const T*>(a.go) + at * a.D, exists, a.D, h);
+    float delta = 0.0f;
+    {
+        Frag of[TL::KSTEPS];
+        load_owned<T, DP>(of, static_cast<const T*>(a.o) + at * a.D, exists, a.D, h);
+#pragma unroll
+        for (int s = 0; s < TL::KSTEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < TL::E; ++e) delta = __builtin_fmaf((float)of[s][e], (float)gf[s][e], delta);
+        delta = half_sum(delta);
+    }
+    const float lse = exists ? a.lse[stat] : INFINITY;
+    if (exists && split == 0 && h == 0) a.delta[stat] = delta;
+    int qp[AXES ? AXES : 1] = {0};
+    const int* kpos = nullptr;
+    if constexpr (AXES > 0) {
+        fill_lut<AXES, THREADS>(a.rb, lut, head, 1, a.H);
+        kpos = a.rb.kpos + b * a.rb.kpos_bs;
+#pragma unroll
+        for (int x = 0; x < AXES; ++x) qp[x] = a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x];
+        if (table_grad) {
+            for (int i = tid; i < span; i += THREADS) bucket[i] = (unsigned short)rel_bucket(a.rb, i);
+            for (int i = 0; i < hist_rows; ++i) hist[i * THREADS + tid] = 0.0f;
+        }
+    }
+
+    acc16 dq[TL::DBLOCKS];
+#pragma unroll
+    for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = acc16{0};
+
+    Stream<T, DP, THREADS> st;
+    int pnext = 0, cur = 0;
+    if (t0 < t1) {
+        st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
+        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, t0 * TL::ROWS, len);
+        st.store(tiles, tiles + TL::ELEMS);
+        if constexpr (AXES > 0)
+            if (tid < AXES * TL::ROWS) pos[tid] = pnext;
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
+        if (t + 1 < t1) {
+            st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
+            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, (t + 1) * TL::ROWS, len);
+        }
+        const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
+        const int* pt = pos + cur * AXES * TL::ROWS;
+#pragma unroll
+        for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+            const unsigned half = (unsigned)(bits >> (nb * 32));
+            if (half == 0) continue;
+            acc16 s = {0}, dp = {0};
+#pragma unroll
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(read_row<T, DP>(kt, nb * 32 + (lane & 31), 2 * ks + h), qf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(read_row<T, DP>(vt, nb * 32 + (lane & 31), 2 * ks + h), gf[ks], dp);
+            int idx[AXES ? AXES : 1][16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float x;
+                if constexpr (AXES > 0) {
+                    const int r = nb * 32 + acc_row(i, h);
+                    idx[0][i] = rel_index(pt[r], qp[0], a.rb.limit);
+                    float bias = lut[idx[0][i]];
+                    if constexpr (AXES > 1) {
+                        idx[AXES - 1][i] = rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit);
+                        bias += lut[span + idx[AXES - 1][i]];
+                    }
+                    x = __builtin_fmaf(s[i], a.scale_log2, bias) - lse;
+                } else {
+                    x = __builtin_fmaf(s[i], a.scale_log2, -lse);
+                }
+                s[i] = x;
+            }
+            if (half != 0xffffffffu) {
+                const unsigned mine = half >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = (mine >> acc_row(i, 0)) & 1 ? s[i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(s[i]) * (dp[i] - delta);
+            if constexpr (AXES > 0) {
+                if (table_grad) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+#pragma unroll
+                        for (int x = 0; x < AXES; ++x)
+                            __hip_atomic_fetch_add(hist + (x * a.rb.buckets + bucket[idx[x][i]]) * THREADS + tid, dp[i], __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+            }
+#pragma unroll
+            for (int ps = 0; ps < TL::PSTEPS; ++ps) {
+                const Frag p = pack_step<T>(dp, ps);
+#pragma unroll
+                for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = Mat<T>::mma(read_col<T, DP>(kt, nb * 32, ps, d * 32, lane), p, dq[d]);
+            }
+        }
+        if (t + 1 < t1) {
+            T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
+            st.store(nk, nk + TL::ELEMS);
+            if constexpr (AXES > 0)
+                if (tid < AXES * TL::ROWS) pos[(cur ^ 1) * AXES * TL::ROWS + tid] = pnext;
+        }
+        __syncthreads();
+        cur ^= 1;
+    }
+    if (a.dq && exists) {
+        if (a.splits > 1) store_owned<float, TL::DBLOCKS>(a.part_o + ((int64_t)split * a.B * a.Lq * a.H + at) * a.D, dq, a.scale, a.D, h);
+        else store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dq) + at * a.D, dq, a.scale, a.D, h);
+    }
+    if constexpr (AXES > 0) {
+        if (table_grad) {       // rows that do not exist added zeros: lse = +inf makes their p zero
+            const int64_t part = ((int64_t)b * a.row_tiles + rt) * a.splits + split;
+            for (int n = wave; n < hist_rows; n += WAVES) {
+                float v = 0.0f;
+#pragma unroll
+                for (int k = 0; k < WAVES; ++k) v += hist[n * THREADS + k * 64 + lane];
+                v = wave_sum(v);
+                if (lane == 0) a.part_table[((int64_t)head * a.parts + part) * hist_rows + n] = v;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ dk, dv
+template <typename T, int DP, int AXES>
+__global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
+    using TL = Tile<T, DP>;
+    using Frag = FragOf<T>;
+    constexpr int THREADS = 256;
+    extern __shared__ __align__(16) char smem[];
+    T* tiles = reinterpret_cast<T*>(smem);                                              // [2][Q, dO]
+    float* stats = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);                     // [2][lse, delta][ROWS]
+    int* pos = reinterpret_cast<int*>(stats + 4 * TL::ROWS);                            // [2][AXES][ROWS]
+    float* lut = reinterpret_cast<float*>(pos + 2 * AXES * TL::ROWS);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int rt = id % a.row_tiles;
+    id /= a.row_tiles;
+    const int kvh = id % a.Hk, b = id / a.Hk, group = a.H / a.Hk;
+    const int kj = rt * 128 + wave * 32 + (lane & 31);
+    const int len = kept_length(a, b);
+    bool kept = kj < len;
+    if (kept && a.mask) kept = a.mask[b * a.mask_bs + kj] != 0;
+    const float lane_bias = kept ? 0.0f : -INFINITY;
+
+    Frag kf[TL::KSTEPS], vf[TL::KSTEPS];
+    load_owned<T, DP>(kf, static_cast<const T*>(a.k) + b * a.ks.b + (int64_t)kj * a.ks.l + kvh * a.ks.h, kept, a.D, h);
+    load_owned<T, DP>(vf, static_cast<const T*>(a.v) + b * a.vs.b + (int64_t)kj * a.vs.l + kvh * a.vs.h, kept, a.D, h);
+    int kpos[AXES ? AXES : 1] = {0};
+    const int span = 2 * a.rb.limit + 1;
+    const int* qpos = nullptr;
+    if constexpr (AXES > 0) {
+        qpos = a.rb.qpos + b * a.rb.qpos_bs;
+#pragma unroll
+        for (int x = 0; x < AXES; ++x) kpos[x] = kept ? a.rb.kpos[b * a.rb.kpos_bs + (int64_t)kj * AXES + x] : 0;
+    }
+    acc16 dk[TL::DBLOCKS], dv[TL::DBLOCKS];
+#pragma unroll
+    for (int d = 0; d < TL::DBLOCKS; ++d) dk[d] = dv[d] = acc16{0};
+
+    // the streamed sequence: query tiles of every head of the group, one after the other
+    const int q_tiles = (a.Lq + TL::ROWS - 1) / TL::ROWS, n_tiles = q_tiles * group;
+    const int t0 = split * a.tiles_per_split;
+    int t1 = min(n_tiles, t0 + a.tiles_per_split);
+    if (rt * 128 >= len) t1 = t0;        // no key of this workgroup is kept: zeros
+    Stream<T, DP, THREADS> st;
+    float snext = 0.0f;
+    int pnext = 0, cur = 0;
+    auto load = [&](int t) {
+        const int head = kvh * group + t / q_tiles, row0 = (t % q_tiles) * TL::ROWS;
+        st.load(static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h, a.qs.l, static_cast<const T*>(a.go) + ((int64_t)b * a.Lq * a.H + head) * a.D,
+                (int64_t)a.H * a.D, row0, a.Lq, a.D, nullptr);
+        if (tid < 2 * TL::ROWS) {
+            const int r = row0 + tid % TL::ROWS;
+            const float* src = tid < TL::ROWS ? a.lse : a.delta;
+            snext = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
+        }
+        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(qpos, row0, a.Lq);
+    };
+    auto store = [&](int buf) {
+        T* n = tiles + buf * 2 * TL::ELEMS;
+        st.store(n, n + TL::ELEMS);
+        if (tid < 2 * TL::ROWS) stats[buf * 2 * TL::ROWS + tid] = snext;
+        if constexpr (AXES > 0)
+            if (tid < AXES * TL::ROWS) pos[buf * AXES * TL::ROWS + tid] = pnext;
+    };
+    int lut_head = -1;
+    if (t0 < t1) {
+        load(t0);
+        store(0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) load(t + 1);
+        if constexpr (AXES > 0) {
+            const int head = kvh * group + t / q_tiles;
+            if (head != lut_head) {     // the barrier at the end of the last round has ended every read of the old columns
+                fill_lut<AXES, THREADS>(a.rb, lut, head, 1, a.H);
+                lut_head = head;
+                __syncthreads();
+            }
+        }
+        const T *qt = tiles + cur * 2 * TL::ELEMS, *gt = qt + TL::ELEMS;
+        const float *lse = stats + cur * 2 * TL::ROWS, *delta = lse + TL::ROWS;
+        const int* pt = pos + cur * AXES * TL::ROWS;
+#pragma unroll
+        for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+            acc16 s = {0}, dp = {0};
+#pragma unroll
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(read_row<T, DP>(qt, nb * 32 + (lane & 31), 2 * ks + h), kf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(read_row<T, DP>(gt, nb * 32 + (lane & 31), 2 * ks + h), vf[ks], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = nb * 32 + acc_row(i, h);
+                float x = lane_bias - lse[r];
+                if constexpr (AXES > 0) {
+                    x += lut[rel_index(kpos[0], pt[r], a.rb.limit)];
+                    if constexpr (AXES > 1) x += lut[span + rel_index(kpos[AXES - 1], pt[TL::ROWS + r], a.rb.limit)];
+                }
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, x));
+                dp[i] = s[i] * (dp[i] - delta[r]);
+            }
+#pragma unroll
+            for (int ps = 0; ps < TL::PSTEPS; ++ps) {
+                const Frag p = pack_step<T>(s, ps), ds = pack_step<T>(dp, ps);
+#pragma unroll
+                for (int d = 0; d < TL::DBLOCKS; ++d) {
+                    dv[d] = Mat<T>::mma(read_col<T, DP>(gt, nb * 32, ps, d * 32, lane), p, dv[d]);
+                    dk[d] = Mat<T>::mma(read_col<T, DP>(qt, nb * 32, ps, d * 32, lane), ds, dk[d]);
+                }
+            }
+        }
+        if (t + 1 < t1) store(cur ^ 1);
+        __syncthreads();
+        cur ^= 1;
+    }
+    if (kj >= a.Lk) return;
+    const int64_t at = ((int64_t)b * a.Lk + kj) * a.Hk + kvh;
+    if (a.splits > 1) {
+        const int64_t off = (int64_t)split * a.B * a.Lk * a.Hk;
+        store_owned<float, TL::DBLOCKS>(a.part_dk + (off + at) * a.D, dk, a.scale, a.D, h);
+        store_owned<float, TL::DBLOCKS>(a.part_dv + (off + at) * a.D, dv, 1.0f, a.D, h);
+    } else {
+        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dk) + at * a.D, dk, a.scale, a.D, h);
+        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dv) + at * a.D, dv, 1.0f, a.D, h);
+    }
+}
+
+// out[n] = sum of the splits' parts, in order; 4 elements a thread (n is a multiple of 8)
+template <typename T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t n, int splits) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float acc[4], v[4];
+    load_f32<float, 4>(part + i, acc);
+    for (int s = 1; s < splits; ++s) {
+        load_f32<float, 4>(part + s * n + i, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += v[e];
+    }
+    store_f32<T, 4>(out + i, acc);
+}
+
+// ------------------------------------------------------------------------------------------------------------ launches
+constexpr size_t MAX_LDS = 160 * 1024;
+
+template <typename T, int DP>
+constexpr size_t tile_bytes() { return 4 * sizeof(T) * Tile<T, DP>::ELEMS; }
+
+inline size_t lut_bytes(const Args& a, int axes, int heads) { return axes ? sizeof(float) * heads * axes * (2 * a.rb.limit + 1) : 0; }
+
+template <typename K>
+int start(K kernel, const char* what, unsigned long long& done, dim3 grid, int threads, size_t lds, const Args& a, hipStream_t s) {
+    if (lds > MAX_LDS || !camli_reserve_lds((const void*)kernel, MAX_LDS, done)) {
+        camli_set_error("%s: cannot reserve %zu bytes of LDS", what, lds);
+        return CAMLI_ELAUNCH;
+    }
+    kernel<<<grid, threads, lds, s>>>(a);
+    return camli_check_launch(what);
+}
+
+template <typename T, int DP, int AXES>
+int run_fwd(const Args& a, hipStream_t s) {
+    using TL = Tile<T, DP>;
+    static unsigned long long done = 0;
+    const size_t lds = tile_bytes<T, DP>() + sizeof(int) * 2 * AXES * TL::ROWS + lut_bytes(a, AXES, a.pack);
+    const int rc = start(fwd_kernel<T, DP, AXES>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, a, s);
+    if (rc != CAMLI_OK || a.splits == 1) return rc;
+    const int64_t threads = (int64_t)a.B * a.Lq * a.H * (a.D / 4);
+    fwd_join_kernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, s>>>(a);
+    return camli_check_launch("camli_cross_attention_fwd");
+}
+
+template <typename T, int DP, int AXES, int WAVES>
+int run_dq_waves(const Args& a, hipStream_t s) {
+    using TL = Tile<T, DP>;
+    static unsigned long long done = 0;
+    size_t lds = tile_bytes<T, DP>() + sizeof(int) * 2 * AXES * TL::ROWS + lut_bytes(a, AXES, 1);
+    if (AXES && a.part_table) lds += sizeof(float) * AXES * a.rb.buckets * 64 * WAVES + 2 * (2 * a.rb.limit + 2);
+    return start(dq_kernel<T, DP, AXES, WAVES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
+}
+
+template <typename T, int DP, int AXES>
+int run_dq(const Args& a, int waves, hipStream_t s) {
+    int rc;
+    if constexpr (AXES > 0) rc = waves == 2 ? run_dq_waves<T, DP, AXES, 2>(a, s) : run_dq_waves<T, DP, AXES, 4>(a, s);
+    else rc = run_dq_waves<T, DP, AXES, 4>(a, s);
+    if (rc != CAMLI_OK) return rc;
+    if (a.splits > 1 && a.dq) {
+        const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
+        sum_parts_kernel<T><<<dim3((unsigned)((n / 4 + 255) / 256)), 256, 0, s>>>(a.part_o, static_cast<T*>(a.dq), n, a.splits);
+    }
+    return camli_check_launch("camli_cross_attention_bwd");
+}
+
+template <typename T, int DP, int AXES>
+int run_dkdv(const Args& a, hipStream_t s) {
+    using TL = Tile<T, DP>;
+    static unsigned long long done = 0;
+    const size_t lds = tile_bytes<T, DP>() + sizeof(float) * 4 * TL::ROWS + sizeof(int) * 2 * AXES * TL::ROWS + lut_bytes(a, AXES, 1);
+    const int rc = start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);
+    if (rc != CAMLI_OK || a.splits == 1) return rc;
+    const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.D;
+    const dim3 grid((unsigned)((n / 4 + 255) / 256));
+    sum_parts_kernel<T><<<grid, 256, 0, s>>>(a.part_dk, static_cast<T*>(a.dk), n, a.splits);
+    sum_parts_kernel<T><<<grid, 256, 0, s>>>(a.part_dv, static_cast<T*>(a.dv), n, a.splits);
+    return camli_check_launch("camli_cross_attention_bwd");
+}
+
+// the three kernels by head width (padded to 32, 64 or 128) and axes of the bias
+template <typename T>
+struct Launch {
+    static int fwd(const Args& a, int axes, hipStream_t s);
+    static int dq(const Args& a, int axes, int waves, hipStream_t s);
+    static int dkdv(const Args& a, int axes, hipStream_t s);
+};
+
+#define XATTN_SELECT(RUN, ...)                                                                                      \
+    if (a.D <= 32) return axes == 0 ? RUN<T, 32, 0>(__VA_ARGS__) : axes == 1 ? RUN<T, 32, 1>(__VA_ARGS__) : RUN<T, 32, 2>(__VA_ARGS__); \
+    if (a.D <= 64) return axes == 0 ? RUN<T, 64, 0>(__VA_ARGS__) : axes == 1 ? RUN<T, 64, 1>(__VA_ARGS__) : RUN<T, 64, 2>(__VA_ARGS__); \
+    return axes == 0 ? RUN<T, 128, 0>(__VA_ARGS__) : axes == 1 ? RUN<T, 128, 1>(__VA_ARGS__) : RUN<T, 128, 2>(__VA_ARGS__);
+
+#define XATTN_DEFINE_FWD(TYPE) \
+    template <> int Launch<TYPE>::fwd(const Args& a, int axes, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_fwd, a, s) }
+#define XATTN_DEFINE_DQ(TYPE) \
+    template <> int Launch<TYPE>::dq(const Args& a, int axes, int waves, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_dq, a, waves, s) }
+#define XATTN_DEFINE_DKDV(TYPE) \
+    template <> int Launch<TYPE>::dkdv(const Args& a, int axes, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_dkdv, a, s) }
+
+}  // namespace xattn

@@ -1,0 +1,197 @@
+// Cross attention: argument checks, work split and the C entries (kernels: xattn.h).
+#include "xattn.h"
+
+namespace {
+
+using xattn::Args;
+
+int tile_rows(int type) { return type == CAMLI_F32 ? 32 : 64; }
+
+// Few owned rows leave CUs idle: the streamed side is cut until there are two workgroups per CU, but into no less than four tiles a
+// piece (a piece pays for its start and for its part of the join).
+void split_stream(Args& a, int64_t base, int n_tiles) {
+    int splits = 1;
+    if (base < 512) {
+        splits = (int)((512 + base - 1) / base);
+        const int most = n_tiles / 4 < 1 ? 1 : n_tiles / 4;
+        if (splits > most) splits = most;
+    }
+    a.tiles_per_split = n_tiles ? (n_tiles + splits - 1) / splits : 1;
+    a.splits = n_tiles ? (n_tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
+}
+
+void plan_fwd(Args& a, int type, int axes) {
+    const int group = a.H / a.Hk;
+    // the query heads of a kv head share a workgroup where all their rows fit into one and their bias columns into LDS: keys and
+    // values are then read once, not once per head
+    a.pack = group > 1 && (int64_t)a.Lq * group <= 128 && xattn::lut_bytes(a, axes, group) <= 16384 ? group : 1;
+    a.row_tiles = camli_divup(a.pack * a.Lq, 128);
+    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile_rows(type)));
+}
+
+int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.buckets > 64 ? 2 : 4; }
+
+void plan_dq(Args& a, int type, int axes, bool table) {
+    a.pack = 1;
+    a.row_tiles = camli_divup(a.Lq, 32 * dq_waves(a, axes, table));
+    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, tile_rows(type)));
+    a.parts = a.B * a.row_tiles * a.splits;
+}
+
+void plan_dkdv(Args& a, int type) {
+    a.pack = 1;
+    a.row_tiles = camli_divup(a.Lk, 128);
+    split_stream(a, (int64_t)a.row_tiles * a.Hk * a.B, camli_divup(a.Lq, tile_rows(type)) * (a.H / a.Hk));
+}
+
+bool operand_ok(const void* p, const int64_t* stride, int size) {
+    if (!p || ((uintptr_t)p & 15)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (stride[i] < 0 || (stride[i] * size) & 15) return false;
+    return true;
+}
+
+// false (with the error set) for anything the kernels do not take
+bool make_args(Args& a, const camli_attention* d, const char* who) {
+    if (!d) { camli_set_error("%s: null descriptor", who); return false; }
+    if (d->type < 0 || d->type > 2 || d->B < 1 || d->Hk < 1 || d->H < d->Hk || d->H % d->Hk != 0 || d->Lq < 1 || d->Lk < 1 || d->D < 8 || d->D > 128 ||
+        d->D % 8 != 0 || !(d->scale > 0.0f) || !(d->scale < INFINITY)) {
+        camli_set_error("%s: need type 0..2, B, Lq, Lk >= 1, H a multiple of Hk, D a multiple of 8 up to 128, a positive finite scale (type=%d B=%d H=%d Hk=%d Lq=%d Lk=%d D=%d scale=%g)",
+                        who, d->type, d->B, d->H, d->Hk, d->Lq, d->Lk, d->D, (double)d->scale);
+        return false;
+    }
+    const int size = camli_type_size(d->type);
+    // grid sizes and element counts of a workgroup's own arithmetic stay below 2^31
+    if ((int64_t)d->B * d->H * ((int64_t)camli_divup(d->Lq, 32) + 1024) > INT32_MAX || (int64_t)d->B * d->Hk * ((int64_t)camli_divup(d->Lk, 128) + 1024) > INT32_MAX ||
+        (int64_t)camli_divup(d->Lq, 32) * (d->H / d->Hk) > INT32_MAX / 64 || d->Lq > INT32_MAX - 256 || d->Lk > INT32_MAX - 256) {
+        camli_set_error("%s: B * H * Lq or B * Hk * Lk too large", who);
+        return false;
+    }
+    if (!operand_ok(d->q, d->q_stride, size) || !operand_ok(d->k, d->k_stride, size) || !operand_ok(d->v, d->v_stride, size)) {
+        camli_set_error("%s: q, k, v need 16-byte aligned addresses and non-negative strides of whole 16 bytes", who);
+        return false;
+    }
+    a = Args{};
+    a.q = d->q; a.k = d->k; a.v = d->v;
+    a.qs = {d->q_stride[0], d->q_stride[1], d->q_stride[2]};
+    a.ks = {d->k_stride[0], d->k_stride[1], d->k_stride[2]};
+    a.vs = {d->v_stride[0], d->v_stride[1], d->v_stride[2]};
+    a.lengths = d->kv_lengths;
+    a.mask = d->key_mask;
+    a.mask_bs = d->key_mask_batch_stride;
+    a.B = d->B; a.H = d->H; a.Hk = d->Hk; a.Lq = d->Lq; a.Lk = d->Lk; a.D = d->D;
+    a.scale = d->scale;
+    a.scale_log2 = d->scale * xattn::LOG2E;
+    if (d->bias_axes != 0 && !rel_bias_args(a.rb, who, d->bias_table, d->type, d->q_pos, d->q_pos_batch_stride, d->k_pos, d->k_pos_batch_stride,
+                                            d->bias_axes, d->bias_buckets, d->bias_two_sided, d->bias_max_distance))
+        return false;
+    return true;
+}
+
+int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+// workspace of the forward: part_o, part_lse
+int64_t fwd_workspace(Args& a, char* base) {
+    if (a.splits == 1) return 0;
+    const int64_t rows = (int64_t)a.B * a.Lq * a.H, o = align256(4 * rows * a.D * a.splits);
+    a.part_o = reinterpret_cast<float*>(base);
+    a.part_lse = reinterpret_cast<float*>(base + o);
+    return o + align256(4 * rows * a.splits);
+}
+
+struct BwdPlan {
+    Args dq, dkdv;
+    int64_t bytes;
+};
+
+// workspace of the backward: delta; then the parts of dq and of the table, whose place the parts of dk and dv take afterwards
+BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base) {
+    BwdPlan p{a, a, 0};
+    plan_dq(p.dq, d->type, d->bias_axes, table);
+    plan_dkdv(p.dkdv, d->type);
+    const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+    p.dq.delta = p.dkdv.delta = reinterpret_cast<float*>(base);
+    const int64_t start = align256(4 * rows);
+    int64_t end = start;
+    if (p.dq.splits > 1) {
+        p.dq.part_o = reinterpret_cast<float*>(base + end);
+        end += align256(4 * rows * a.D * p.dq.splits);
+    }
+    if (table) {
+        p.dq.part_table = reinterpret_cast<float*>(base + end);
+        end += align256((int64_t)4 * a.H * p.dq.parts * d->bias_axes * d->bias_buckets);
+    }
+    int64_t end2 = start;
+    if (p.dkdv.splits > 1) {
+        const int64_t n = align256((int64_t)4 * a.B * a.Lk * a.Hk * a.D * p.dkdv.splits);
+        p.dkdv.part_dk = reinterpret_cast<float*>(base + start);
+        p.dkdv.part_dv = reinterpret_cast<float*>(base + start + n);
+        end2 += 2 * n;
+    }
+    p.bytes = end > end2 ? end : end2;
+    return p;
+}
+
+}  // namespace
+
+extern "C" int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention* d) {
+    Args a;
+    if (!make_args(a, d, "camli_cross_attention_fwd_workspace_bytes")) return CAMLI_EINVAL;
+    plan_fwd(a, d->type, d->bias_axes);
+    return fwd_workspace(a, nullptr);
+}
+
+extern "C" int camli_cross_attention_fwd(const camli_attention* d, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    Args a;
+    if (!make_args(a, d, "camli_cross_attention_fwd")) return CAMLI_EINVAL;
+    plan_fwd(a, d->type, d->bias_axes);
+    const int64_t need = fwd_workspace(a, static_cast<char*>(workspace));
+    if (!out || ((uintptr_t)out & 15) || (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))) {
+        camli_set_error("camli_cross_attention_fwd: output or workspace missing, unaligned or too small (%lld bytes needed)", (long long)need);
+        return CAMLI_EINVAL;
+    }
+    a.out = out;
+    a.lse = lse;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (d->type == CAMLI_F32) return xattn::Launch<float>::fwd(a, d->bias_axes, s);
+    if (d->type == CAMLI_BF16) return xattn::Launch<__bf16>::fwd(a, d->bias_axes, s);
+    return xattn::Launch<_Float16>::fwd(a, d->bias_axes, s);
+}
+
+extern "C" int64_t camli_cross_attention_bwd_workspace_bytes(const camli_attention* d, int table_gradient) {
+    Args a;
+    if (!make_args(a, d, "camli_cross_attention_bwd_workspace_bytes")) return CAMLI_EINVAL;
+    return plan_bwd(a, d, table_gradient != 0 && d->bias_axes != 0, nullptr).bytes;
+}
+
+extern "C" int camli_cross_attention_bwd(const camli_attention* d, const void* out, const void* gout, const float* lse, void* gq, void* gk,
+                                         void* gv, void* gtable, void* workspace, int64_t workspace_bytes, void* stream) {
+    Args a;
+    if (!make_args(a, d, "camli_cross_attention_bwd")) return CAMLI_EINVAL;
+    if (gtable && d->bias_axes == 0) { camli_set_error("camli_cross_attention_bwd: a table gradient without a table"); return CAMLI_EINVAL; }
+    BwdPlan p = plan_bwd(a, d, gtable != nullptr, static_cast<char*>(workspace));
+    if (!out || !gout || !lse || (gk == nullptr) != (gv == nullptr) || !workspace || workspace_bytes < p.bytes ||
+        (((uintptr_t)out | (uintptr_t)gout | (uintptr_t)gq | (uintptr_t)gk | (uintptr_t)gv | (uintptr_t)workspace) & 15)) {
+        camli_set_error("camli_cross_attention_bwd: an operand is missing or not 16-byte aligned, or the workspace is too small (%lld bytes needed)", (long long)p.bytes);
+        return CAMLI_EINVAL;
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int axes = d->bias_axes, waves = dq_waves(p.dq, axes, gtable != nullptr);
+    p.dq.o = p.dkdv.o = out;
+    p.dq.go = p.dkdv.go = gout;
+    p.dq.lse = p.dkdv.lse = const_cast<float*>(lse);
+    p.dq.dq = gq;
+    p.dkdv.dk = gk;
+    p.dkdv.dv = gv;
+    int rc = d->type == CAMLI_F32 ? xattn::Launch<float>::dq(p.dq, axes, waves, s)
+             : d->type == CAMLI_BF16 ? xattn::Launch<__bf16>::dq(p.dq, axes, waves, s) : xattn::Launch<_Float16>::dq(p.dq, axes, waves, s);
+    if (rc != CAMLI_OK) return rc;
+    if (gtable) {
+        rc = rel_bias_join(p.dq.part_table, gtable, d->type, a.H, axes * d->bias_buckets, p.dq.parts, "camli_cross_attention_bwd", s);
+        if (rc != CAMLI_OK) return rc;
+    }
+    if (!gk) return CAMLI_OK;
+    if (d->type == CAMLI_F32) return xattn::Launch<float>::dkdv(p.dkdv, axes, s);
+    if (d->type == CAMLI_BF16) return xattn::Launch<__bf16>::dkdv(p.dkdv, axes, s);
+    return xattn::Launch<_Float16>::dkdv(p.dkdv, axes, s);
+}

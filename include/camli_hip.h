@@ -715,6 +715,78 @@ int camli_maxpool3x3s2_bwd(const float *gy, const unsigned char *arg, float *gx,
 int camli_transpose_planes(const float *src, int64_t src_batch_stride, int64_t src_row_stride, float *dst,
                            int64_t dst_batch_stride, int64_t dst_row_stride, int B, int rows, int cols, void *stream);
 
+/*
+ * Operators of attentive fusion (camera features attend points and the other way round).  The reference has no counterpart: its
+ * fusion gathers the nearest point per pixel (models/clfm.py:7-60) and normalises with batch / instance / layer norm
+ * (models/mlp.py:43-100).  Element type codes: 0 fp32, 1 bf16, 2 fp16; sums, statistics and softmax are fp32 for all of them.
+ *
+ * Group normalisation with an activation, channels last: y = act((x - mean_g) / sqrt(var_g + eps) * weight[c] + bias[c]).
+ *   x [B,P,C] with any batch stride and pixel pitch (elements; channels adjacent), y, gy, gx dense [B,P,C];
+ *   weight, bias [C] of type wtype, either may be NULL; stat [B,G,2] = (mean, 1/sqrt(var + eps)), NULL if no backward follows;
+ *   act 0 none, 1 relu, 2 leaky_relu (0.1), 3 sigmoid, 6 silu;  C <= 4096, G divides C.
+ *   bwd: gx (may be NULL), gw / gb [C] fp32 (either may be NULL) fully written, no atomics.
+ * workspace_bytes: 0 for sizes outside these limits.
+ */
+int64_t camli_group_norm_fwd_workspace_bytes(int B, int C, int G, int P, int type);
+int camli_group_norm_fwd(const void *x, int64_t x_batch_stride, int64_t x_pixel_stride, const void *weight, const void *bias, int wtype,
+                         void *y, float *stat, void *workspace, int64_t workspace_bytes, int B, int C, int G, int P, float eps, int act,
+                         int type, void *stream);
+int64_t camli_group_norm_bwd_workspace_bytes(int B, int C, int G, int P, int type);
+int camli_group_norm_bwd(const void *gy, const void *x, int64_t x_batch_stride, int64_t x_pixel_stride, const void *weight, const void *bias,
+                         int wtype, const float *stat, void *gx, float *gw, float *gb, void *workspace, int64_t workspace_bytes, int B,
+                         int C, int G, int P, int act, int type, void *stream);
+
+/*
+ * Learned relative position bias by buckets: out[b,h,i,j] = sum_a table[a, bucket(k_pos[b,j,a] - q_pos[b,i,a]), h].
+ *   table [axes,buckets,H] and out [B,H,Lq,Lk] of `type`; positions int32 [B,L,axes], batch strides in ints (0 = shared).
+ *   Two-sided: buckets / 2 per sign (positive offsets in the upper half), distance |o|; else all buckets for max(-o, 0).  With s
+ *   buckets a side, distances below e = s / 2 have a bucket each, bucket e + j starts at the first d >= e (max_distance / e)^(j/(s-e)).
+ *   axes 1 or 2, axes * buckets <= 128, e < max_distance <= 1023.
+ *   bwd: gtable [axes,buckets,H] of `type`, fully written, the same bits on every run.
+ * borders: the first distances of buckets e + 1 ... into border[], returns how many (host only, needs no device).
+ */
+int camli_rel_bias_borders(int buckets, int two_sided, int max_distance, int *border);
+int camli_rel_bias_fwd(const void *table, const int *q_pos, int64_t q_pos_batch_stride, const int *k_pos, int64_t k_pos_batch_stride,
+                       void *out, int B, int H, int Lq, int Lk, int axes, int buckets, int two_sided, int max_distance, int type,
+                       void *stream);
+int64_t camli_rel_bias_bwd_workspace_bytes(int B, int H, int Lq, int Lk, int axes, int buckets, int type);
+int camli_rel_bias_bwd(const void *gout, const int *q_pos, int64_t q_pos_batch_stride, const int *k_pos, int64_t k_pos_batch_stride,
+                       void *gtable, void *workspace, int64_t workspace_bytes, int B, int H, int Lq, int Lk, int axes, int buckets,
+                       int two_sided, int max_distance, int type, void *stream);
+
+/*
+ * Cross attention: out = softmax(scale q k^T + bias) v over the kept keys of each sample; H query heads share Hk key / value heads.
+ *   q [B,Lq,H,D], k, v [B,Lk,Hk,D] of `type`, strides in elements (batch, row, head; D adjacent), 16-byte aligned rows;
+ *   out, gout, gq [B,Lq,H,D] and gk, gv [B,Lk,Hk,D] dense;  D a multiple of 8, at most 128.
+ *   A key is kept if its index is below kv_lengths[b] (NULL: all; clamped to 0..Lk) and key_mask[b,j] != 0 (NULL: all).  Masked keys
+ *   and values may hold anything, NaN included; their gradients are zero.  A row without a kept key (or whose scores are all -inf)
+ *   gives zeros and takes no part in any gradient.
+ *   bias_axes 0: no bias; else as camli_rel_bias_fwd, table [axes,buckets,H] of `type`.
+ *   lse [B,H,Lq]: log2 of each row's softmax sum, +inf for rows without keys; NULL if no backward follows.
+ *   bwd: gq may be NULL, gk and gv both or neither, gtable [axes,buckets,H] may be NULL; everything given is fully written, no atomics
+ *   whose order matters: the same bits on every run.
+ * workspace_bytes: negative (an error code) for a descriptor the kernels do not take.
+ */
+typedef struct camli_attention {
+    int type, B, H, Hk, Lq, Lk, D;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const int *kv_lengths;
+    const unsigned char *key_mask;
+    int64_t key_mask_batch_stride;
+    const void *bias_table;
+    const int *q_pos, *k_pos;
+    int64_t q_pos_batch_stride, k_pos_batch_stride;
+    int bias_axes, bias_buckets, bias_two_sided, bias_max_distance;
+} camli_attention;
+int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention *desc);
+int camli_cross_attention_fwd(const camli_attention *desc, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+                              void *stream);
+int64_t camli_cross_attention_bwd_workspace_bytes(const camli_attention *desc, int table_gradient);
+int camli_cross_attention_bwd(const camli_attention *desc, const void *out, const void *gout, const float *lse, void *gq, void *gk,
+                              void *gv, void *gtable, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,7 +3,7 @@
 // Forward: bound by writing [B, H, Lq, Lk]; a thread keeps the key positions of its 16 bytes of columns in registers over 32 rows.
 // Backward: bound by reading the incoming gradient once.  dtable[a, n, h] adds up to millions of elements into each of a few dozen
 // places; every thread owns a column of an LDS histogram (address = bucket * 256 + thread: no bank conflict, no second writer), so
-// the order of every sum is fixed by the sizes alone.  Columns are added in a fixed order at the end, workgroups in 64 bits.
+// the order of every sum is fixed by the sizes alone and plain reads and writes do.  Columns are added in a fixed order at the end, workgroups in 64 bits.
 #include "relbias.h"
 
 #include <math.h>
@@ -69,15 +69,20 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
         const T* gr = g + (((int64_t)b * H + h) * Lq + i) * Lk;
         for (int j = tx * VEC; j < Lk; j += cols * VEC) {
             float v[VEC];
+            int n[VEC][AXES];
             load_f32<T, VEC>(gr + j, v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
 #pragma unroll
-                for (int a = 0; a < AXES; ++a) {
-                    const int n = lut[rel_index(kpos[(int64_t)(j + e) * AXES + a], qp[a], r.limit)];
-                    // this thread's own column; an LDS add needs no round trip through a register
-                    __hip_atomic_fetch_add(hist + (a * r.buckets + n) * BLOCK + tid, v[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                }
+                for (int a = 0; a < AXES; ++a)
+                    n[e][a] = lut[rel_index(kpos[(int64_t)(j + e) * AXES + a], qp[a], r.limit)] + a * r.buckets;
+            if constexpr (VEC > 1) {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) hist_add2<BLOCK, AXES>(hist + tid, n[e], v[e], n[e + 1], v[e + 1]);
+            } else {
+#pragma unroll
+                for (int a = 0; a < AXES; ++a) hist[n[0][a] * BLOCK + tid] += v[0];
+            }
         }
     }
     __syncthreads();

@@ -521,17 +521,17 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
             for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(read_row<T, DP>(kt, nb * 32 + (lane & 31), 2 * ks + h), qf[ks], s);
 #pragma unroll
             for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(read_row<T, DP>(vt, nb * 32 + (lane & 31), 2 * ks + h), gf[ks], dp);
-            int idx[AXES ? AXES : 1][16];
+            int idx[16][AXES ? AXES : 1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float x;
                 if constexpr (AXES > 0) {
                     const int r = nb * 32 + acc_row(i, h);
-                    idx[0][i] = rel_index(pt[r], qp[0], a.rb.limit);
-                    float bias = lut[idx[0][i]];
+                    idx[i][0] = rel_index(pt[r], qp[0], a.rb.limit);
+                    float bias = lut[idx[i][0]];
                     if constexpr (AXES > 1) {
-                        idx[AXES - 1][i] = rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit);
-                        bias += lut[span + idx[AXES - 1][i]];
+                        idx[i][AXES - 1] = rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit);
+                        bias += lut[span + idx[i][AXES - 1]];
                     }
                     x = __builtin_fmaf(s[i], a.scale_log2, bias) - lse;
                 } else {
@@ -551,9 +551,9 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
 #pragma unroll
-                        for (int x = 0; x < AXES; ++x)
-                            __hip_atomic_fetch_add(hist + (x * a.rb.buckets + bucket[idx[x][i]]) * THREADS + tid, dp[i], __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+                        for (int x = 0; x < AXES; ++x) idx[i][x] = bucket[idx[i][x]] + x * a.rb.buckets;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) hist_add2<THREADS, AXES>(hist + tid, idx[i], dp[i], idx[i + 1], dp[i + 1]);
                 }
             }
 #pragma unroll

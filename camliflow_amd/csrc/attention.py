@@ -193,20 +193,23 @@ class _CrossAttention(torch.autograd.Function):
         lk = k.shape[1]
         ctx.args = (scale, bidirectional, max_distance)
         if q.numel() == 0 or lk == 0:
-            ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, None, None)
+            ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, None, None, None)
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
         out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
-        lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad[:4]) else None
+        lse = rest = None
+        if any(ctx.needs_input_grad[:4]):
+            lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device)
+            rest = torch.empty_like(out) if q.dtype != torch.float32 else None
         d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
         size = q.element_size()
         with _on_device(q):
             n = lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d))
             ws = _workspace('camli_cross_attention_fwd', n, q)
             _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, ctypes.byref(d), out.data_ptr(),
-                        lse.data_ptr() if lse is not None else None, ws.data_ptr(), n, _stream_ptr(q),
+                        rest.data_ptr() if rest is not None else None, lse.data_ptr() if lse is not None else None, ws.data_ptr(), n, _stream_ptr(q),
                         work=(float(size * (2 * q.numel() + 2 * b * lk * k.shape[2] * dim)), 'B'), flop=4.0 * b * h * lq * lk * dim)
-        ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, lse)
+        ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, rest, lse)
         return out
 
     @staticmethod
@@ -214,7 +217,7 @@ class _CrossAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         lib = _lib.load()
-        q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, lse = ctx.saved_tensors
+        q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, rest, lse = ctx.saved_tensors
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
         nothing = (None,) * 7
         if out is None:
@@ -238,7 +241,7 @@ class _CrossAttention(torch.autograd.Function):
         with _on_device(q):
             n = lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), int(need_t))
             ws = _workspace('camli_cross_attention_bwd', n, q)
-            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, ctypes.byref(d), out.data_ptr(), gout.data_ptr(),
+            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, ctypes.byref(d), out.data_ptr(), ptr(rest), gout.data_ptr(),
                         lse.data_ptr(), ptr(gq), ptr(gk), ptr(gv), ptr(gt), ws.data_ptr(), n, _stream_ptr(q),
                         work=(float(size * (4 * q.numel() + 4 * b * lk * hk * dim)), 'B'), flop=10.0 * b * h * lq * lk * dim)
         return (gq, gk if need_k else None, gv if need_v else None, gt) + nothing

@@ -31,9 +31,10 @@ struct Strides {
 };
 
 struct Args {
-    const void *q, *k, *v, *o, *go;
+    const void *q, *k, *v, *o, *o_rest, *go;
     Strides qs, ks, vs;         // o, go and the gradients are dense [B][L][heads][D]
     void *out, *dq, *dk, *dv;
+    void *out_rest;             // 16-bit types in training: out minus its rounding, rounded
     float *lse;                 // [B][H][Lq], log2 domain; +inf where no key is kept
     float *delta;               // [B][H][Lq]
     float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [split][B][H][Lq] (-inf: no key)
@@ -75,47 +76,72 @@ template <> struct Mat<float> {
 template <typename T>
 using FragOf = typename Mat<T>::frag;
 
-template <typename T, int DP>
+// A tile of R streamed rows in LDS.  16-bit rows are unpadded and their 16-byte chunks permuted by an XOR with bits of the row, chosen
+// so that both readers hit every bank equally: 16 lanes reading one chunk of 16 rows, and the transposing load's 8 rows x 64 bytes.
+// fp32 rows are padded by 16 bytes, which does the same for 16-byte row reads and leaves the 4-byte column reads at fixed offsets.
+template <typename T, int DP, int R>
 struct Tile {
     static constexpr int E = 16 / sizeof(T);            // elements of a 16-byte chunk
     static constexpr int CHUNKS = DP / E;               // chunks of a row
-    static constexpr int ROWS = sizeof(T) == 2 ? 64 : 32;
+    static constexpr int ROWS = R;
     static constexpr int BLOCKS = ROWS / 32;
-    static constexpr int LD = DP + E;                   // 16 bytes of padding: rows start 4 banks apart (mod 64), no conflicts on either read
+    static constexpr int LD = sizeof(T) == 2 ? DP : DP + E;
     static constexpr int ELEMS = ROWS * LD;
     static constexpr int KSTEPS = CHUNKS / 2;           // k-steps of a product over DP
     static constexpr int PSTEPS = 16 / E;               // k-steps of a product over 32 streamed rows
     static constexpr int DBLOCKS = DP / 32;
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (sizeof(T) == 4) return 0;
+        else if constexpr (CHUNKS == 4) return (row >> 2) & 3;
+        else if constexpr (CHUNKS == 8) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+        else return (row & 7) << 1 | ((row >> 3) & 1);
+    }
+    static __device__ __forceinline__ int chunk_at(int row, int c) { return row * LD + (c ^ swizzle(row)) * E; }
 };
 
-// chunk c of a streamed row: the A operand (row = lane % 32) of products over DP
+// Where a lane reads in a tile (element offsets from the start of a 32-row block; loop-invariant).
 template <typename T, int DP>
-__device__ __forceinline__ FragOf<T> read_row(const T* tile, int row, int chunk) {
-    return *reinterpret_cast<const FragOf<T>*>(tile + row * Tile<T, DP>::LD + chunk * Tile<T, DP>::E);
-}
+struct LaneMap {
+    using TL = Tile<T, DP, 32>;
+    using Frag = FragOf<T>;
+    int row[TL::KSTEPS];                                        // A operand of products over DP: row lane % 32, chunk 2 s + half
+    int col[sizeof(T) == 2 ? TL::DBLOCKS : 1][2];               // A operand of products over the streamed rows
 
-// A operand of products over the streamed rows: lane l = column d0 + l % 32, k-step t of block `row0` in the order the accumulator has
-template <typename T, int DP>
-__device__ __forceinline__ FragOf<T> read_col(const T* tile, int row0, int t, int d0, int lane) {
-    constexpr int LD = Tile<T, DP>::LD;
-    const int h = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
-        // the transposing load: 16 lanes fetch 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows each
-        typedef __attribute__((address_space(3))) short4v* lds_ptr;
-        const int l = lane & 15;
-        const T* p = tile + (row0 + 16 * t + 4 * h + (l >> 2)) * LD + d0 + (lane & 16) + (l & 3) * 4;
-        union { short4v s[2]; FragOf<T> f; } u;
-        u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(p)));
-        u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(p + 8 * LD)));
-        return u.f;
-    } else {
-        const T* p = tile + (row0 + 8 * t + 4 * h) * LD + d0 + (lane & 31);
-        FragOf<T> f;
+    __device__ __forceinline__ explicit LaneMap(int lane) {
+        const int h = lane >> 5, l = lane & 15;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = p[i * LD];
+        for (int s = 0; s < TL::KSTEPS; ++s) row[s] = TL::chunk_at(lane & 31, 2 * s + h);
+        if constexpr (sizeof(T) == 2) {
+            // the transposing load: 16 lanes fetch 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows each
+#pragma unroll
+            for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int c = d * 32 + (lane & 16) + (l & 3) * 4;
+                    col[d][u] = TL::chunk_at(4 * h + (l >> 2) + 8 * u, c / TL::E) + c % TL::E;
+                }
+        } else {
+            col[0][0] = col[0][1] = 4 * h * TL::LD + (lane & 31);
+        }
+    }
+    __device__ __forceinline__ Frag read_row(const T* block, int s) const { return *reinterpret_cast<const Frag*>(block + row[s]); }
+    // column 32 d + lane % 32 of the rows of k-step t, in the order the accumulator has them
+    __device__ __forceinline__ Frag read_col(const T* block, int t, int d) const {
+        Frag f;
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) short4v* lds_ptr;
+            union { short4v s[2]; Frag f; } u;
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(block + 16 * t * TL::LD + col[d][0])));
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(block + 16 * t * TL::LD + col[d][1])));
+            f = u.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = block[(8 * t + i) * TL::LD + 32 * d + col[0][0]];
+        }
         return f;
     }
-}
+};
 
 // k-step t of the accumulator, rounded to the element type
 template <typename T>
@@ -125,6 +151,13 @@ __device__ __forceinline__ FragOf<T> pack_step(const acc16& x, int t) {
 #pragma unroll
     for (int i = 0; i < E; ++i) f[i] = (T)x[t * E + i];
     return f;
+}
+
+__device__ __forceinline__ acc16 splat(float x) {
+    acc16 v;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = x;
+    return v;
 }
 
 __device__ __forceinline__ int acc_row(int i, int h) { return (i >> 2) * 8 + 4 * h + (i & 3); }
@@ -146,10 +179,11 @@ __device__ __forceinline__ int xcd_contiguous(int id, int n) {
 
 // The streamed pair of tiles on its way from memory: registers now, LDS later.  A row at or beyond `limit`, a masked row and columns
 // from D on become zeros (a masked row may hold anything, and 0 * NaN is NaN).
-template <typename T, int DP, int THREADS>
+template <typename T, int DP, int R, int THREADS>
 struct Stream {
-    using TL = Tile<T, DP>;
-    static constexpr int N = TL::ROWS * TL::CHUNKS / THREADS;
+    using TL = Tile<T, DP, R>;
+    static constexpr int ALL = TL::ROWS * TL::CHUNKS, N = (ALL + THREADS - 1) / THREADS;      // the narrowest tile has chunks for half the threads
+    static_assert(ALL % THREADS == 0 || N == 1, "a whole number of chunks a thread");
     chunk16 x[N], y[N];
     unsigned keep;
 
@@ -159,7 +193,7 @@ struct Stream {
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS, row = row0 + f / TL::CHUNKS, c = (f % TL::CHUNKS) * TL::E;
             x[n] = y[n] = chunk16{0, 0, 0, 0};
-            if (row < limit && c < D) {
+            if (row < limit && c < D && (ALL >= THREADS || f < ALL)) {
                 x[n] = *reinterpret_cast<const chunk16*>(px + row * ldx + c);
                 y[n] = *reinterpret_cast<const chunk16*>(py + row * ldy + c);
                 keep |= (mask == nullptr || mask[row] != 0 ? 1u : 0u) << n;
@@ -170,7 +204,8 @@ struct Stream {
         const chunk16 zero = {0, 0, 0, 0};
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int f = threadIdx.x + n * THREADS, at = (f / TL::CHUNKS) * TL::LD + (f % TL::CHUNKS) * TL::E;
+            const int f = threadIdx.x + n * THREADS, at = TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS);
+            if (ALL < THREADS && f >= ALL) break;
             const bool k = (keep >> n) & 1;
             *reinterpret_cast<chunk16*>(tx + at) = k ? x[n] : zero;
             *reinterpret_cast<chunk16*>(ty + at) = k ? y[n] : zero;
@@ -181,7 +216,7 @@ struct Stream {
 // owned row -> B fragments (zeros beyond D and for rows that do not exist)
 template <typename T, int DP>
 __device__ __forceinline__ void load_owned(FragOf<T>* f, const T* row, bool exists, int D, int h) {
-    using TL = Tile<T, DP>;
+    using TL = Tile<T, DP, 32>;
 #pragma unroll
     for (int s = 0; s < TL::KSTEPS; ++s) {
         const int c = (2 * s + h) * TL::E;
@@ -243,11 +278,23 @@ __device__ __forceinline__ int load_pos(const int* pos, int row0, int limit) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
-template <typename T, int DP, int AXES>
-__global__ __launch_bounds__(256) void fwd_kernel(Args a) {
-    using TL = Tile<T, DP>;
+// Softmax without a running maximum: the scores come out of the matrix unit already relative to m (the accumulators start at -m /
+// scale), and m is taken from the first tile that has a kept key.  p <= 2^30 (2^15 for fp16) is as good as p <= 1 in floating point, so
+// m moves only when a row's sum over a tile passes that: the maximum, its exchange between the half waves and the rescaling of the
+// accumulators leave the loop, but for a test of the sum.
+// TRAIN (16-bit types): out has to be known to more than its own type for the backward's D = do . o, which is subtracted from
+// dp: P enters the product as two terms of the type and the rounding error of out is stored beside it.  Without that the bias table's
+// gradient, a sum over whole rows of ds, is off by twice its own rounding.
+template <typename T>
+constexpr float sum_limit() { return sizeof(T) == 2 && !__is_same(T, __bf16) ? 32768.0f : 1073741824.0f; }
+
+template <typename T, int DP, int AXES, bool TRAIN>
+__global__ __launch_bounds__(256, DP == 128 && (sizeof(T) == 4 || AXES > 0) ? 1 : 2) void fwd_kernel(Args a) {
+    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+    using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
     constexpr int THREADS = 256;
+    constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2;
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
     int* pos = reinterpret_cast<int*>(tiles + 4 * TL::ELEMS);               // [2][AXES][ROWS]
@@ -284,13 +331,17 @@ __global__ __launch_bounds__(256) void fwd_kernel(Args a) {
 #pragma unroll
         for (int x = 0; x < AXES; ++x) qp[x] = a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x];
     }
+    const LaneMap<T, DP> map(lane);
 
     acc16 o[TL::DBLOCKS];
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = acc16{0};
+    // m: the reference of the row's exponents, log2 domain (-inf: no kept key yet, use 0); start: -m / scale in every accumulator
     float m = -INFINITY, m_use = 0.0f, l = 0.0f;
+    acc16 start = splat(0.0f);
+    bool unset = true;
 
-    Stream<T, DP, THREADS> st;
+    Stream<T, DP, R, THREADS> st;
     int pnext = 0, cur = 0;
     if (t0 < t1) {
         st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
@@ -310,61 +361,87 @@ __global__ __launch_bounds__(256) void fwd_kernel(Args a) {
         const int* pt = pos + cur * AXES * TL::ROWS;
         if (bits != 0) {
             acc16 s[TL::BLOCKS];
-            float top = -INFINITY;
+            float sum;
+            bool move = unset;
+            for (int round = 0; round < 2; ++round) {       // a second round only where m had to move
 #pragma unroll
-            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                s[nb] = acc16{0};
+                for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+                    s[nb] = start;
 #pragma unroll
-                for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(read_row<T, DP>(kt, nb * 32 + (lane & 31), 2 * ks + h), qf[ks], s[nb]);
-            }
+                    for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(map.read_row(kt + nb * 32 * TL::LD, ks), qf[ks], s[nb]);
+                }
 #pragma unroll
-            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                if constexpr (AXES > 0) {
+                for (int nb = 0; nb < TL::BLOCKS; ++nb) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int r = nb * 32 + acc_row(i, h);
-                        float bias = my_lut[rel_index(pt[r], qp[0], a.rb.limit)];
-                        if constexpr (AXES > 1) bias += my_lut[span + rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit)];
-                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, bias);
+                        if constexpr (AXES > 0) {
+                            const int r = nb * 32 + acc_row(i, h);
+                            float x = __builtin_fmaf(s[nb][i], a.scale_log2, my_lut[rel_index(pt[r], qp[0], a.rb.limit)]);
+                            if constexpr (AXES > 1) x += my_lut[span + rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit)];
+                            s[nb][i] = x;
+                        } else {
+                            s[nb][i] *= a.scale_log2;
+                        }
+                    }
+                    const unsigned half = (unsigned)(bits >> (nb * 32));
+                    if (half != 0xffffffffu) {
+                        const unsigned mine = half >> (4 * h);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[nb][i] = (mine >> acc_row(i, 0)) & 1 ? s[nb][i] : -INFINITY;
                     }
                 }
-                const unsigned half = (unsigned)(bits >> (nb * 32));
-                if (half != 0xffffffffu) {
-                    const unsigned mine = half >> (4 * h);
+                if (move) {
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[nb][i] = (mine >> acc_row(i, 0)) & 1 ? s[nb][i] : -INFINITY;
+                    for (int nb = 0; nb < TL::BLOCKS; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
+                    top = half_max(top) + m_use;
+                    const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
+                    const float alpha = __builtin_amdgcn_exp2f(m - use), back = m_use - use;
+#pragma unroll
+                    for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+                    l *= alpha;
+                    m = mn;
+                    m_use = use;
+                    start = splat(-use / a.scale_log2);
+                    unset = __any(m == -INFINITY);
+#pragma unroll
+                    for (int nb = 0; nb < TL::BLOCKS; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[nb][i] += back;
                 }
+                sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
+                for (int nb = 0; nb < TL::BLOCKS; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[nb][i] = __builtin_amdgcn_exp2f(s[nb][i]);
+                        sum += s[nb][i];
+                    }
+                if (move || !__any(!(sum <= sum_limit<T>()))) break;
+                move = true;
             }
-            top = half_max(top);
-            if constexpr (AXES == 0) top *= a.scale_log2;
-            // the running maximum may lag by 8 (p <= 2^8, sums in fp32): the accumulators are rescaled only when a row passes that
-            if (__any(top > m + 8.0f)) {
-                const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
-                const float alpha = __builtin_amdgcn_exp2f(m - use);
+            l += sum;
 #pragma unroll
-                for (int d = 0; d < TL::DBLOCKS; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-                l *= alpha;
-                m = mn;
-                m_use = use;
-            }
-#pragma unroll
-            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[nb][i] = __builtin_amdgcn_exp2f(AXES == 0 ? __builtin_fmaf(s[nb][i], a.scale_log2, -m_use) : s[nb][i] - m_use);
-                    l += s[nb][i];
-                }
+            for (int nb = 0; nb < TL::BLOCKS; ++nb)
 #pragma unroll
                 for (int ps = 0; ps < TL::PSTEPS; ++ps) {
                     const Frag p = pack_step<T>(s[nb], ps);
+                    Frag rest;
+                    if constexpr (TWO_TERMS) {
 #pragma unroll
-                    for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = Mat<T>::mma(read_col<T, DP>(vt, nb * 32, ps, d * 32, lane), p, o[d]);
+                        for (int i = 0; i < TL::E; ++i) rest[i] = (T)(s[nb][ps * TL::E + i] - (float)p[i]);
+                    }
+#pragma unroll
+                    for (int d = 0; d < TL::DBLOCKS; ++d) {
+                        const Frag v = map.read_col(vt + nb * 32 * TL::LD, ps, d);
+                        o[d] = Mat<T>::mma(v, p, o[d]);
+                        if constexpr (TWO_TERMS) o[d] = Mat<T>::mma(v, rest, o[d]);
+                    }
                 }
-            }
         }
         if (t + 1 < t1) {
             T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
@@ -386,7 +463,14 @@ __global__ __launch_bounds__(256) void fwd_kernel(Args a) {
         if (h == 0) a.part_lse[split * per + stat] = l == 0.0f ? -INFINITY : lse;
     } else {
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, h);
-        if (a.lse && h == 0) a.lse[stat] = l == 0.0f ? INFINITY : lse;
+        if constexpr (TWO_TERMS) {
+#pragma unroll
+            for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * inv - (float)(T)(o[d][i] * inv);
+            store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out_rest) + at * a.D, o, 1.0f, a.D, h);
+        }
+        if (TRAIN && h == 0) a.lse[stat] = l == 0.0f ? INFINITY : lse;
     }
 }
 
@@ -422,15 +506,22 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = bad ? NAN : acc[i] * inv;
     store_f32<T, 4>(static_cast<T*>(a.out) + at * a.D + c, acc);
+    if (a.out_rest) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] -= (float)(T)acc[i];
+        store_f32<T, 4>(static_cast<T*>(a.out_rest) + at * a.D + c, acc);
+    }
     if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + __builtin_amdgcn_logf(sum);
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
 // WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, bucket of every offset,
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
-template <typename T, int DP, int AXES, int WAVES>
+// HIST: with the table's gradient; its tiles are 32 rows, so that two workgroups still share a CU beside their histograms.
+template <typename T, int DP, int AXES, int WAVES, bool HIST>
 __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
-    using TL = Tile<T, DP>;
+    constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
+    using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
     constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES;
     extern __shared__ __align__(16) char smem[];
@@ -440,7 +531,6 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     const int span = 2 * a.rb.limit + 1, hist_rows = AXES * a.rb.buckets;
     float* hist = lut + AXES * span;
     unsigned short* bucket = reinterpret_cast<unsigned short*>(hist + hist_rows * THREADS);
-    const bool table_grad = AXES > 0 && a.part_table != nullptr;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -456,7 +546,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     const int len = kept_length(a, b);
     const int n_tiles = (len + TL::ROWS - 1) / TL::ROWS;
     const int t0 = split * a.tiles_per_split;
-    const int t1 = a.dq || table_grad ? min(n_tiles, t0 + a.tiles_per_split) : t0;      // else only delta is wanted
+    const int t1 = a.dq || HIST ? min(n_tiles, t0 + a.tiles_per_split) : t0;      // else only delta is wanted
     const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + kvh * a.ks.h;
     const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
     const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
@@ -473,9 +563,19 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         for (int s = 0; s < TL::KSTEPS; ++s)
 #pragma unroll
             for (int e = 0; e < TL::E; ++e) delta = __builtin_fmaf((float)of[s][e], (float)gf[s][e], delta);
+        if constexpr (sizeof(T) == 2) {
+            load_owned<T, DP>(of, static_cast<const T*>(a.o_rest) + at * a.D, exists, a.D, h);
+#pragma unroll
+            for (int s = 0; s < TL::KSTEPS; ++s)
+#pragma unroll
+                for (int e = 0; e < TL::E; ++e) delta = __builtin_fmaf((float)of[s][e], (float)gf[s][e], delta);
+        }
         delta = half_sum(delta);
     }
-    const float lse = exists ? a.lse[stat] : INFINITY;
+    // the accumulators start at -lse / scale and -delta: the products come out as the exponent and as dp - D.  +inf (a row without keys,
+    // or none at all) makes every p zero.
+    const acc16 start_s = splat(-(exists ? a.lse[stat] : INFINITY) / a.scale_log2), start_d = splat(-delta);
+    const LaneMap<T, DP> map(lane);
     if (exists && split == 0 && h == 0) a.delta[stat] = delta;
     int qp[AXES ? AXES : 1] = {0};
     const int* kpos = nullptr;
@@ -484,7 +584,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         kpos = a.rb.kpos + b * a.rb.kpos_bs;
 #pragma unroll
         for (int x = 0; x < AXES; ++x) qp[x] = a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x];
-        if (table_grad) {
+        if constexpr (HIST) {
             for (int i = tid; i < span; i += THREADS) bucket[i] = (unsigned short)rel_bucket(a.rb, i);
             for (int i = 0; i < hist_rows; ++i) hist[i * THREADS + tid] = 0.0f;
         }
@@ -494,7 +594,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = acc16{0};
 
-    Stream<T, DP, THREADS> st;
+    Stream<T, DP, R, THREADS> st;
     int pnext = 0, cur = 0;
     if (t0 < t1) {
         st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
@@ -516,28 +616,27 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
             const unsigned half = (unsigned)(bits >> (nb * 32));
             if (half == 0) continue;
-            acc16 s = {0}, dp = {0};
+            acc16 s = start_s, dp = start_d;
+            const T *kb = kt + nb * 32 * TL::LD, *vb = vt + nb * 32 * TL::LD;
 #pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(read_row<T, DP>(kt, nb * 32 + (lane & 31), 2 * ks + h), qf[ks], s);
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(map.read_row(kb, ks), qf[ks], s);
 #pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(read_row<T, DP>(vt, nb * 32 + (lane & 31), 2 * ks + h), gf[ks], dp);
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(vb, ks), gf[ks], dp);
             int idx[16][AXES ? AXES : 1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float x;
                 if constexpr (AXES > 0) {
                     const int r = nb * 32 + acc_row(i, h);
                     idx[i][0] = rel_index(pt[r], qp[0], a.rb.limit);
-                    float bias = lut[idx[i][0]];
+                    float x = __builtin_fmaf(s[i], a.scale_log2, lut[idx[i][0]]);
                     if constexpr (AXES > 1) {
                         idx[i][AXES - 1] = rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit);
-                        bias += lut[span + idx[i][AXES - 1]];
+                        x += lut[span + idx[i][AXES - 1]];
                     }
-                    x = __builtin_fmaf(s[i], a.scale_log2, bias) - lse;
+                    s[i] = x;
                 } else {
-                    x = __builtin_fmaf(s[i], a.scale_log2, -lse);
+                    s[i] *= a.scale_log2;
                 }
-                s[i] = x;
             }
             if (half != 0xffffffffu) {
                 const unsigned mine = half >> (4 * h);
@@ -545,22 +644,20 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
                 for (int i = 0; i < 16; ++i) s[i] = (mine >> acc_row(i, 0)) & 1 ? s[i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(s[i]) * (dp[i] - delta);
-            if constexpr (AXES > 0) {
-                if (table_grad) {
+            for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(s[i]);
+            if constexpr (HIST) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
+                for (int i = 0; i < 16; ++i)
 #pragma unroll
-                        for (int x = 0; x < AXES; ++x) idx[i][x] = bucket[idx[i][x]] + x * a.rb.buckets;
+                    for (int x = 0; x < AXES; ++x) idx[i][x] = bucket[idx[i][x]] + x * a.rb.buckets;
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) hist_add2<THREADS, AXES>(hist + tid, idx[i], dp[i], idx[i + 1], dp[i + 1]);
-                }
+                for (int i = 0; i < 16; i += 2) hist_add2<THREADS, AXES>(hist + tid, idx[i], dp[i], idx[i + 1], dp[i + 1]);
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
                 const Frag p = pack_step<T>(dp, ps);
 #pragma unroll
-                for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = Mat<T>::mma(read_col<T, DP>(kt, nb * 32, ps, d * 32, lane), p, dq[d]);
+                for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = Mat<T>::mma(map.read_col(kb, ps, d), p, dq[d]);
             }
         }
         if (t + 1 < t1) {
@@ -576,16 +673,14 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         if (a.splits > 1) store_owned<float, TL::DBLOCKS>(a.part_o + ((int64_t)split * a.B * a.Lq * a.H + at) * a.D, dq, a.scale, a.D, h);
         else store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dq) + at * a.D, dq, a.scale, a.D, h);
     }
-    if constexpr (AXES > 0) {
-        if (table_grad) {       // rows that do not exist added zeros: lse = +inf makes their p zero
-            const int64_t part = ((int64_t)b * a.row_tiles + rt) * a.splits + split;
-            for (int n = wave; n < hist_rows; n += WAVES) {
-                float v = 0.0f;
+    if constexpr (HIST) {       // rows that do not exist added zeros
+        const int64_t part = ((int64_t)b * a.row_tiles + rt) * a.splits + split;
+        for (int n = wave; n < hist_rows; n += WAVES) {
+            float v = 0.0f;
 #pragma unroll
-                for (int k = 0; k < WAVES; ++k) v += hist[n * THREADS + k * 64 + lane];
-                v = wave_sum(v);
-                if (lane == 0) a.part_table[((int64_t)head * a.parts + part) * hist_rows + n] = v;
-            }
+            for (int k = 0; k < WAVES; ++k) v += hist[n * THREADS + k * 64 + lane];
+            v = wave_sum(v);
+            if (lane == 0) a.part_table[((int64_t)head * a.parts + part) * hist_rows + n] = v;
         }
     }
 }
@@ -593,7 +688,8 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 // ------------------------------------------------------------------------------------------------------------ dk, dv
 template <typename T, int DP, int AXES>
 __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
-    using TL = Tile<T, DP>;
+    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+    using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
     constexpr int THREADS = 256;
     extern __shared__ __align__(16) char smem[];
@@ -613,7 +709,7 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
     const int len = kept_length(a, b);
     bool kept = kj < len;
     if (kept && a.mask) kept = a.mask[b * a.mask_bs + kj] != 0;
-    const float lane_bias = kept ? 0.0f : -INFINITY;
+    const LaneMap<T, DP> map(lane);
 
     Frag kf[TL::KSTEPS], vf[TL::KSTEPS];
     load_owned<T, DP>(kf, static_cast<const T*>(a.k) + b * a.ks.b + (int64_t)kj * a.ks.l + kvh * a.ks.h, kept, a.D, h);
@@ -635,7 +731,7 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
     const int t0 = split * a.tiles_per_split;
     int t1 = min(n_tiles, t0 + a.tiles_per_split);
     if (rt * 128 >= len) t1 = t0;        // no key of this workgroup is kept: zeros
-    Stream<T, DP, THREADS> st;
+    Stream<T, DP, R, THREADS> st;
     float snext = 0.0f;
     int pnext = 0, cur = 0;
     auto load = [&](int t) {
@@ -645,7 +741,9 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
         if (tid < 2 * TL::ROWS) {
             const int r = row0 + tid % TL::ROWS;
             const float* src = tid < TL::ROWS ? a.lse : a.delta;
-            snext = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
+            // what the accumulators start at: -lse / scale and -delta; a row that does not exist has lse = +inf, so p = 0
+            const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
+            snext = tid < TL::ROWS ? -x / a.scale_log2 : -x;
         }
         if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(qpos, row0, a.Lq);
     };
@@ -673,33 +771,42 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
             }
         }
         const T *qt = tiles + cur * 2 * TL::ELEMS, *gt = qt + TL::ELEMS;
-        const float *lse = stats + cur * 2 * TL::ROWS, *delta = lse + TL::ROWS;
+        const float* start = stats + cur * 2 * TL::ROWS;
         const int* pt = pos + cur * AXES * TL::ROWS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-            acc16 s = {0}, dp = {0};
-#pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(read_row<T, DP>(qt, nb * 32 + (lane & 31), 2 * ks + h), kf[ks], s);
-#pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(read_row<T, DP>(gt, nb * 32 + (lane & 31), 2 * ks + h), vf[ks], dp);
+            const T *qb = qt + nb * 32 * TL::LD, *gb = gt + nb * 32 * TL::LD;
+            acc16 s, dp;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = nb * 32 + acc_row(i, h);
-                float x = lane_bias - lse[r];
+                s[i] = start[r];
+                dp[i] = start[TL::ROWS + r];
+            }
+#pragma unroll
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(map.read_row(qb, ks), kf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(gb, ks), vf[ks], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float x;
                 if constexpr (AXES > 0) {
-                    x += lut[rel_index(kpos[0], pt[r], a.rb.limit)];
+                    const int r = nb * 32 + acc_row(i, h);
+                    x = __builtin_fmaf(s[i], a.scale_log2, lut[rel_index(kpos[0], pt[r], a.rb.limit)]);
                     if constexpr (AXES > 1) x += lut[span + rel_index(kpos[AXES - 1], pt[TL::ROWS + r], a.rb.limit)];
+                } else {
+                    x = s[i] * a.scale_log2;
                 }
-                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, x));
-                dp[i] = s[i] * (dp[i] - delta[r]);
+                s[i] = __builtin_amdgcn_exp2f(x);
+                dp[i] *= s[i];
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
                 const Frag p = pack_step<T>(s, ps), ds = pack_step<T>(dp, ps);
 #pragma unroll
                 for (int d = 0; d < TL::DBLOCKS; ++d) {
-                    dv[d] = Mat<T>::mma(read_col<T, DP>(gt, nb * 32, ps, d * 32, lane), p, dv[d]);
-                    dk[d] = Mat<T>::mma(read_col<T, DP>(qt, nb * 32, ps, d * 32, lane), ds, dk[d]);
+                    dv[d] = Mat<T>::mma(map.read_col(gb, ps, d), p, dv[d]);
+                    dk[d] = Mat<T>::mma(map.read_col(qb, ps, d), ds, dk[d]);
                 }
             }
         }
@@ -708,6 +815,10 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
         cur ^= 1;
     }
     if (kj >= a.Lk) return;
+    if (!kept) {        // a masked key's column of P was computed from zeros and is nobody else's
+#pragma unroll
+        for (int d = 0; d < TL::DBLOCKS; ++d) dk[d] = dv[d] = acc16{0};
+    }
     const int64_t at = ((int64_t)b * a.Lk + kj) * a.Hk + kvh;
     if (a.splits > 1) {
         const int64_t off = (int64_t)split * a.B * a.Lk * a.Hk;
@@ -737,8 +848,8 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict_
 // ------------------------------------------------------------------------------------------------------------ launches
 constexpr size_t MAX_LDS = 160 * 1024;
 
-template <typename T, int DP>
-constexpr size_t tile_bytes() { return 4 * sizeof(T) * Tile<T, DP>::ELEMS; }
+template <typename T, int DP, int R>
+constexpr size_t tile_bytes() { return 4 * sizeof(T) * Tile<T, DP, R>::ELEMS; }
 
 inline size_t lut_bytes(const Args& a, int axes, int heads) { return axes ? sizeof(float) * heads * axes * (2 * a.rb.limit + 1) : 0; }
 
@@ -752,32 +863,41 @@ int start(K kernel, const char* what, unsigned long long& done, dim3 grid, int t
     return camli_check_launch(what);
 }
 
+template <typename T, int DP, int AXES, bool TRAIN>
+int run_fwd_mode(const Args& a, hipStream_t s) {
+    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+    static unsigned long long done = 0;
+    const size_t lds = tile_bytes<T, DP, R>() + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, a.pack);
+    return start(fwd_kernel<T, DP, AXES, TRAIN>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, a, s);
+}
+
 template <typename T, int DP, int AXES>
 int run_fwd(const Args& a, hipStream_t s) {
-    using TL = Tile<T, DP>;
-    static unsigned long long done = 0;
-    const size_t lds = tile_bytes<T, DP>() + sizeof(int) * 2 * AXES * TL::ROWS + lut_bytes(a, AXES, a.pack);
-    const int rc = start(fwd_kernel<T, DP, AXES>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, a, s);
+    const int rc = a.lse ? run_fwd_mode<T, DP, AXES, true>(a, s) : run_fwd_mode<T, DP, AXES, false>(a, s);
     if (rc != CAMLI_OK || a.splits == 1) return rc;
     const int64_t threads = (int64_t)a.B * a.Lq * a.H * (a.D / 4);
     fwd_join_kernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, s>>>(a);
     return camli_check_launch("camli_cross_attention_fwd");
 }
 
-template <typename T, int DP, int AXES, int WAVES>
-int run_dq_waves(const Args& a, hipStream_t s) {
-    using TL = Tile<T, DP>;
+template <typename T, int DP, int AXES, int WAVES, bool HIST>
+int run_dq_mode(const Args& a, hipStream_t s) {
+    constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
     static unsigned long long done = 0;
-    size_t lds = tile_bytes<T, DP>() + sizeof(int) * 2 * AXES * TL::ROWS + lut_bytes(a, AXES, 1);
-    if (AXES && a.part_table) lds += sizeof(float) * AXES * a.rb.buckets * 64 * WAVES + 2 * (2 * a.rb.limit + 2);
-    return start(dq_kernel<T, DP, AXES, WAVES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
+    size_t lds = tile_bytes<T, DP, R>() + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, 1);
+    if (HIST) lds += sizeof(float) * AXES * a.rb.buckets * 64 * WAVES + 2 * (2 * a.rb.limit + 2);
+    return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
 }
 
 template <typename T, int DP, int AXES>
 int run_dq(const Args& a, int waves, hipStream_t s) {
     int rc;
-    if constexpr (AXES > 0) rc = waves == 2 ? run_dq_waves<T, DP, AXES, 2>(a, s) : run_dq_waves<T, DP, AXES, 4>(a, s);
-    else rc = run_dq_waves<T, DP, AXES, 4>(a, s);
+    if constexpr (AXES > 0) {
+        if (!a.part_table) rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
+        else rc = waves == 2 ? run_dq_mode<T, DP, AXES, 2, true>(a, s) : run_dq_mode<T, DP, AXES, 4, true>(a, s);
+    } else {
+        rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
+    }
     if (rc != CAMLI_OK) return rc;
     if (a.splits > 1 && a.dq) {
         const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
@@ -788,9 +908,9 @@ int run_dq(const Args& a, int waves, hipStream_t s) {
 
 template <typename T, int DP, int AXES>
 int run_dkdv(const Args& a, hipStream_t s) {
-    using TL = Tile<T, DP>;
+    constexpr int R = sizeof(T) == 2 ? 64 : 32;
     static unsigned long long done = 0;
-    const size_t lds = tile_bytes<T, DP>() + sizeof(float) * 4 * TL::ROWS + sizeof(int) * 2 * AXES * TL::ROWS + lut_bytes(a, AXES, 1);
+    const size_t lds = tile_bytes<T, DP, R>() + sizeof(float) * 4 * R + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, 1);
     const int rc = start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);
     if (rc != CAMLI_OK || a.splits == 1) return rc;
     const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.D;

@@ -763,6 +763,7 @@ int camli_rel_bias_bwd(const void *gout, const int *q_pos, int64_t q_pos_batch_s
  *   gives zeros and takes no part in any gradient.
  *   bias_axes 0: no bias; else as camli_rel_bias_fwd, table [axes,buckets,H] of `type`.
  *   lse [B,H,Lq]: log2 of each row's softmax sum, +inf for rows without keys; NULL if no backward follows.
+ *   out_rest, like out: what rounding to a 16-bit type took from out, for the backward (unused for fp32 or without lse).
  *   bwd: gq may be NULL, gk and gv both or neither, gtable [axes,buckets,H] may be NULL; everything given is fully written, no atomics
  *   whose order matters: the same bits on every run.
  * workspace_bytes: negative (an error code) for a descriptor the kernels do not take.
@@ -781,11 +782,11 @@ typedef struct camli_attention {
     int bias_axes, bias_buckets, bias_two_sided, bias_max_distance;
 } camli_attention;
 int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention *desc);
-int camli_cross_attention_fwd(const camli_attention *desc, void *out, float *lse, void *workspace, int64_t workspace_bytes,
-                              void *stream);
+int camli_cross_attention_fwd(const camli_attention *desc, void *out, void *out_rest, float *lse, void *workspace,
+                              int64_t workspace_bytes, void *stream);
 int64_t camli_cross_attention_bwd_workspace_bytes(const camli_attention *desc, int table_gradient);
-int camli_cross_attention_bwd(const camli_attention *desc, const void *out, const void *gout, const float *lse, void *gq, void *gk,
-                              void *gv, void *gtable, void *workspace, int64_t workspace_bytes, void *stream);
+int camli_cross_attention_bwd(const camli_attention *desc, const void *out, const void *out_rest, const void *gout, const float *lse,
+                              void *gq, void *gk, void *gv, void *gtable, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

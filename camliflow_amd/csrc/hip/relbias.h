@@ -49,25 +49,25 @@ __device__ __forceinline__ int rel_index(int kpos, int qpos, int limit) {
     return min(max(o, -limit), limit) + limit;
 }
 
-// Two additions to a thread's own histogram column (per axis): cell[n THREADS] += v.  Plain reads and writes, because nobody else
-// touches the column: an LDS float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a
-// dependent read-add-write).  The two cells of an axis may be the same one.
-template <int THREADS, int AXES>
-__device__ __forceinline__ void hist_add2(float* column, const int (&n0)[AXES], float v0, const int (&n1)[AXES], float v1) {
+// Two additions to a thread's own histogram column, per axis, at byte offsets.  Plain reads and writes, because nobody else touches the
+// column: an LDS float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a dependent
+// read-add-write).  The two cells of an axis may be the same one.
+template <int AXES>
+__device__ __forceinline__ void hist_add2(char* column, const unsigned (&at0)[AXES], float v0, const unsigned (&at1)[AXES], float v1) {
     float x0[AXES], x1[AXES];
 #pragma unroll
     for (int a = 0; a < AXES; ++a) {
-        x0[a] = column[n0[a] * THREADS];
-        x1[a] = column[n1[a] * THREADS];
+        x0[a] = *reinterpret_cast<float*>(column + at0[a]);
+        x1[a] = *reinterpret_cast<float*>(column + at1[a]);
     }
 #pragma unroll
     for (int a = 0; a < AXES; ++a) {
         x0[a] += v0;
-        x1[a] = (n0[a] == n1[a] ? x0[a] : x1[a]) + v1;
+        x1[a] = (at0[a] == at1[a] ? x0[a] : x1[a]) + v1;
     }
 #pragma unroll
     for (int a = 0; a < AXES; ++a) {
-        column[n0[a] * THREADS] = x0[a];
-        column[n1[a] * THREADS] = x1[a];
+        *reinterpret_cast<float*>(column + at0[a]) = x0[a];
+        *reinterpret_cast<float*>(column + at1[a]) = x1[a];
     }
 }

@@ -59,6 +59,7 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
     for (int i = tid; i < span; i += BLOCK) lut[i] = (unsigned short)rel_bucket(r, i);
     for (int i = 0; i < nrows; ++i) hist[i * BLOCK + tid] = 0.0f;
     __syncthreads();
+    char* column = reinterpret_cast<char*>(hist + tid);
     const int tx = tid % cols, ty = tid / cols, per = BLOCK / cols;
     for (int64_t row = (int64_t)blockIdx.x * per + ty; row < rows && ty < per; row += (int64_t)gridDim.x * per) {
         const int b = (int)(row / Lq), i = (int)(row - (int64_t)b * Lq);
@@ -69,19 +70,19 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
         const T* gr = g + (((int64_t)b * H + h) * Lq + i) * Lk;
         for (int j = tx * VEC; j < Lk; j += cols * VEC) {
             float v[VEC];
-            int n[VEC][AXES];
+            unsigned n[VEC][AXES];
             load_f32<T, VEC>(gr + j, v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
 #pragma unroll
                 for (int a = 0; a < AXES; ++a)
-                    n[e][a] = lut[rel_index(kpos[(int64_t)(j + e) * AXES + a], qp[a], r.limit)] + a * r.buckets;
+                    n[e][a] = (lut[rel_index(kpos[(int64_t)(j + e) * AXES + a], qp[a], r.limit)] + a * r.buckets) * BLOCK * sizeof(float);
             if constexpr (VEC > 1) {
 #pragma unroll
-                for (int e = 0; e < VEC; e += 2) hist_add2<BLOCK, AXES>(hist + tid, n[e], v[e], n[e + 1], v[e + 1]);
+                for (int e = 0; e < VEC; e += 2) hist_add2<AXES>(column, n[e], v[e], n[e + 1], v[e + 1]);
             } else {
 #pragma unroll
-                for (int a = 0; a < AXES; ++a) hist[n[0][a] * BLOCK + tid] += v[0];
+                for (int a = 0; a < AXES; ++a) *reinterpret_cast<float*>(column + n[0][a]) += v[0];
             }
         }
     }

@@ -52,6 +52,7 @@ struct Args {
 
 typedef float acc16 __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
+typedef unsigned uint2v __attribute__((ext_vector_type(2)));
 typedef unsigned chunk16 __attribute__((ext_vector_type(4)));       // 16 bytes in flight
 
 // 16-byte fragments: what a lane holds of one operand for one k-step
@@ -143,14 +144,42 @@ struct LaneMap {
     }
 };
 
-// k-step t of the accumulator, rounded to the element type
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// k-step t of the accumulator, rounded to the element type (in pairs: one conversion instruction rounds two)
 template <typename T>
 __device__ __forceinline__ FragOf<T> pack_step(const acc16& x, int t) {
     constexpr int E = 16 / sizeof(T);
     FragOf<T> f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) f[i] = (T)x[t * E + i];
+    for (int i = 0; i < E; i += 2) {
+        const float2v v = {x[t * E + i], x[t * E + i + 1]};
+        if constexpr (__is_same(T, __bf16)) {
+            const bf16x2 r = __builtin_convertvector(v, bf16x2);
+            f[i] = r[0];
+            f[i + 1] = r[1];
+        } else if constexpr (__is_same(T, _Float16)) {
+            const f16x2 r = __builtin_convertvector(v, f16x2);
+            f[i] = r[0];
+            f[i + 1] = r[1];
+        } else {
+            f[i] = v[0];
+            f[i + 1] = v[1];
+        }
+    }
     return f;
+}
+
+// what that rounding left
+template <typename T>
+__device__ __forceinline__ FragOf<T> pack_rest(const acc16& x, const FragOf<T>& rounded, int t) {
+    constexpr int E = 16 / sizeof(T);
+    acc16 rest;
+#pragma unroll
+    for (int i = 0; i < E; ++i) rest[i] = x[t * E + i] - (float)rounded[i];
+    return pack_step<T>(rest, 0);
 }
 
 __device__ __forceinline__ acc16 splat(float x) {
@@ -255,7 +284,31 @@ __device__ __forceinline__ unsigned long long kept_bits(const unsigned char* mas
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// table columns of `pack` heads, one value per offset: lut[p][axis][2 limit + 1], log2 domain
+// The bias of a pair from LDS.  Positions are held as multiples of the entry size (scaled once per row, not per pair), and the owned
+// row's carries the address of its table's middle: one subtraction and one clamp of a pair give the LDS address of its entry.
+// Positions beyond +-2^26 count as that, so that no difference overflows.
+// Entries: the bias (log2 domain), and for the table's gradient beside it where the bucket's row of the histogram starts.
+struct Entry8 {
+    float bias;
+    unsigned hist;
+};
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_load(int address) {
+    return *(__attribute__((address_space(3))) const V*)(uintptr_t)(unsigned)address;
+}
+__device__ __forceinline__ int med3(int x, int lo, int hi) {
+    int r;
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(lo), "v"(hi));
+    return r;
+}
+template <int ENTRY>
+__device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 26)), 1 << 26) * ENTRY; }
+
+// tables of `pack` heads: lut[p][axis][2 limit + 1]
 template <int AXES, int THREADS>
 __device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0, int pack, int H) {
     const int span = 2 * r.limit + 1;
@@ -267,33 +320,42 @@ __device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0
                 lut[(p * AXES + a) * span + i] = load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + head0 + p) * LOG2E;
     }
 }
+template <int AXES, int THREADS>
+__device__ __forceinline__ void fill_lut(const RelBias& r, Entry8* lut, int head, int row_bytes, int H) {
+    const int span = 2 * r.limit + 1;
+    for (int i = threadIdx.x; i < span; i += THREADS) {
+        const int n = rel_bucket(r, i);
+#pragma unroll
+        for (int a = 0; a < AXES; ++a)
+            lut[a * span + i] = {load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + head) * LOG2E, (unsigned)((a * r.buckets + n) * row_bytes)};
+    }
+}
 
-// positions of the streamed rows: pos[axis][ROWS]
-template <int AXES, int ROWS>
+// positions of the streamed rows, scaled: pos[axis][ROWS]
+template <int AXES, int ROWS, int ENTRY>
 __device__ __forceinline__ int load_pos(const int* pos, int row0, int limit) {
     const int t = threadIdx.x;
     if (t >= AXES * ROWS) return 0;
     const int row = min(row0 + t % ROWS, limit - 1);
-    return pos[(int64_t)row * AXES + t / ROWS];
+    return scale_pos<ENTRY>(pos[(int64_t)row * AXES + t / ROWS]);
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
 // Softmax without a running maximum: the scores come out of the matrix unit already relative to m (the accumulators start at -m /
-// scale), and m is taken from the first tile that has a kept key.  p <= 2^30 (2^15 for fp16) is as good as p <= 1 in floating point, so
-// m moves only when a row's sum over a tile passes that: the maximum, its exchange between the half waves and the rescaling of the
-// accumulators leave the loop, but for a test of the sum.
+// scale), and m is taken from the first tile that has a kept key.  p <= 2^30 (2^14 for fp16) is as good as p <= 1 in floating point, so
+// m moves only when a score passes that: the exchange between the half waves and the rescaling leave the loop, but for a test.
 // TRAIN (16-bit types): out has to be known to more than its own type for the backward's D = do . o, which is subtracted from
 // dp: P enters the product as two terms of the type and the rounding error of out is stored beside it.  Without that the bias table's
 // gradient, a sum over whole rows of ds, is off by twice its own rounding.
 template <typename T>
-constexpr float sum_limit() { return sizeof(T) == 2 && !__is_same(T, __bf16) ? 32768.0f : 1073741824.0f; }
+constexpr float exponent_limit() { return __is_same(T, _Float16) ? 14.0f : 30.0f; }
 
 template <typename T, int DP, int AXES, bool TRAIN>
-__global__ __launch_bounds__(256, DP == 128 && (sizeof(T) == 4 || AXES > 0) ? 1 : 2) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeof(T) == 2 && AXES == 0) ? 2 : 1) void fwd_kernel(Args a) {
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
-    constexpr int THREADS = 256;
+    constexpr int THREADS = 256, ENTRY = sizeof(float);
     constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2;
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
@@ -321,15 +383,18 @@ __global__ __launch_bounds__(256, DP == 128 && (sizeof(T) == 4 || AXES > 0) ? 1 
 
     Frag qf[TL::KSTEPS];
     load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + qi * a.qs.l + head * a.qs.h, exists, a.D, h);
-    int qp[AXES ? AXES : 1] = {0};
-    const int span = 2 * a.rb.limit + 1;
-    const float* my_lut = lut + sub * AXES * span;
+    int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
     if constexpr (AXES > 0) {
         fill_lut<AXES, THREADS>(a.rb, lut, hh * a.pack, a.pack, a.H);
         kpos = a.rb.kpos + b * a.rb.kpos_bs;
 #pragma unroll
-        for (int x = 0; x < AXES; ++x) qp[x] = a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x];
+        for (int x = 0; x < AXES; ++x) {
+            const int centre = (int)lds_address(lut + (sub * AXES + x) * (2 * a.rb.limit + 1) + a.rb.limit);
+            qa[x] = scale_pos<4>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x]) - centre;
+            lo[x] = centre - 4 * a.rb.limit;
+            hi[x] = centre + 4 * a.rb.limit;
+        }
     }
     const LaneMap<T, DP> map(lane);
 
@@ -345,7 +410,7 @@ __global__ __launch_bounds__(256, DP == 128 && (sizeof(T) == 4 || AXES > 0) ? 1 
     int pnext = 0, cur = 0;
     if (t0 < t1) {
         st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
-        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, t0 * TL::ROWS, len);
+        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
         if constexpr (AXES > 0)
             if (tid < AXES * TL::ROWS) pos[tid] = pnext;
@@ -355,86 +420,70 @@ __global__ __launch_bounds__(256, DP == 128 && (sizeof(T) == 4 || AXES > 0) ? 1 
         const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
         if (t + 1 < t1) {
             st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
-            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, (t + 1) * TL::ROWS, len);
+            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, (t + 1) * TL::ROWS, len);
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
         const int* pt = pos + cur * AXES * TL::ROWS;
         if (bits != 0) {
             acc16 s[TL::BLOCKS];
-            float sum;
-            bool move = unset;
-            for (int round = 0; round < 2; ++round) {       // a second round only where m had to move
+            float top = -INFINITY;
 #pragma unroll
-                for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                    s[nb] = start;
+            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+                s[nb] = start;
 #pragma unroll
-                    for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(map.read_row(kt + nb * 32 * TL::LD, ks), qf[ks], s[nb]);
-                }
+                for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(map.read_row(kt + nb * 32 * TL::LD, ks), qf[ks], s[nb]);
+            }
 #pragma unroll
-                for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if constexpr (AXES > 0) {
-                            const int r = nb * 32 + acc_row(i, h);
-                            float x = __builtin_fmaf(s[nb][i], a.scale_log2, my_lut[rel_index(pt[r], qp[0], a.rb.limit)]);
-                            if constexpr (AXES > 1) x += my_lut[span + rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit)];
-                            s[nb][i] = x;
-                        } else {
-                            s[nb][i] *= a.scale_log2;
-                        }
-                    }
-                    const unsigned half = (unsigned)(bits >> (nb * 32));
-                    if (half != 0xffffffffu) {
-                        const unsigned mine = half >> (4 * h);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[nb][i] = (mine >> acc_row(i, 0)) & 1 ? s[nb][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) {
+                    if constexpr (AXES > 0) {
+                        const int r = nb * 32 + acc_row(i, h);
+                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, lds_load<float>(med3(pt[r] - qa[0], lo[0], hi[0])));
+                        if constexpr (AXES > 1) s[nb][i] += lds_load<float>(med3(pt[TL::ROWS + r] - qa[AXES - 1], lo[AXES - 1], hi[AXES - 1]));
+                    } else {
+                        s[nb][i] *= a.scale_log2;
                     }
                 }
-                if (move) {
-                    float top = -INFINITY;
+                const unsigned half = (unsigned)(bits >> (nb * 32));
+                if (half != 0xffffffffu) {
+                    const unsigned mine = half >> (4 * h);
 #pragma unroll
-                    for (int nb = 0; nb < TL::BLOCKS; ++nb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
-                    top = half_max(top) + m_use;
-                    const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
-                    const float alpha = __builtin_amdgcn_exp2f(m - use), back = m_use - use;
-#pragma unroll
-                    for (int d = 0; d < TL::DBLOCKS; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-                    l *= alpha;
-                    m = mn;
-                    m_use = use;
-                    start = splat(-use / a.scale_log2);
-                    unset = __any(m == -INFINITY);
-#pragma unroll
-                    for (int nb = 0; nb < TL::BLOCKS; ++nb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[nb][i] += back;
+                    for (int i = 0; i < 16; ++i) s[nb][i] = (mine >> acc_row(i, 0)) & 1 ? s[nb][i] : -INFINITY;
                 }
-                sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
+            }
+            if (unset || __any(top > exponent_limit<T>())) {
+                top = half_max(top) + m_use;
+                const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m - use), back = m_use - use;
+#pragma unroll
+                for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+                l *= alpha;
+                m = mn;
+                m_use = use;
+                start = splat(-use / a.scale_log2);
+                unset = __any(m == -INFINITY);
 #pragma unroll
                 for (int nb = 0; nb < TL::BLOCKS; ++nb)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[nb][i] = __builtin_amdgcn_exp2f(s[nb][i]);
-                        sum += s[nb][i];
-                    }
-                if (move || !__any(!(sum <= sum_limit<T>()))) break;
-                move = true;
+                    for (int i = 0; i < 16; ++i) s[nb][i] += back;
             }
-            l += sum;
 #pragma unroll
-            for (int nb = 0; nb < TL::BLOCKS; ++nb)
+            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[nb][i] = __builtin_amdgcn_exp2f(s[nb][i]);
+                    l += s[nb][i];
+                }
 #pragma unroll
                 for (int ps = 0; ps < TL::PSTEPS; ++ps) {
                     const Frag p = pack_step<T>(s[nb], ps);
                     Frag rest;
-                    if constexpr (TWO_TERMS) {
-#pragma unroll
-                        for (int i = 0; i < TL::E; ++i) rest[i] = (T)(s[nb][ps * TL::E + i] - (float)p[i]);
-                    }
+                    if constexpr (TWO_TERMS) rest = pack_rest<T>(s[nb], p, ps);
 #pragma unroll
                     for (int d = 0; d < TL::DBLOCKS; ++d) {
                         const Frag v = map.read_col(vt + nb * 32 * TL::LD, ps, d);
@@ -442,6 +491,7 @@ __global__ __launch_bounds__(256, DP == 128 && (sizeof(T) == 4 || AXES > 0) ? 1 
                         if constexpr (TWO_TERMS) o[d] = Mat<T>::mma(v, rest, o[d]);
                     }
                 }
+            }
         }
         if (t + 1 < t1) {
             T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
@@ -515,7 +565,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
-// WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, bucket of every offset,
+// WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, then
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
 // HIST: with the table's gradient; its tiles are 32 rows, so that two workgroups still share a CU beside their histograms.
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
@@ -523,14 +573,14 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
-    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES;
+    using Entry = __type_pack_element<HIST ? 1 : 0, float, Entry8>;
+    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = sizeof(Entry);
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);
     int* pos = reinterpret_cast<int*>(tiles + 4 * TL::ELEMS);
-    float* lut = reinterpret_cast<float*>(pos + 2 * AXES * TL::ROWS);
+    Entry* lut = reinterpret_cast<Entry*>(pos + 2 * AXES * TL::ROWS);
     const int span = 2 * a.rb.limit + 1, hist_rows = AXES * a.rb.buckets;
-    float* hist = lut + AXES * span;
-    unsigned short* bucket = reinterpret_cast<unsigned short*>(hist + hist_rows * THREADS);
+    float* hist = reinterpret_cast<float*>(lut + AXES * span);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -577,18 +627,22 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     const acc16 start_s = splat(-(exists ? a.lse[stat] : INFINITY) / a.scale_log2), start_d = splat(-delta);
     const LaneMap<T, DP> map(lane);
     if (exists && split == 0 && h == 0) a.delta[stat] = delta;
-    int qp[AXES ? AXES : 1] = {0};
+    int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
     if constexpr (AXES > 0) {
-        fill_lut<AXES, THREADS>(a.rb, lut, head, 1, a.H);
+        fill_lut<AXES, THREADS>(a.rb, lut, head, HIST ? 4 * THREADS : 1, a.H);
         kpos = a.rb.kpos + b * a.rb.kpos_bs;
 #pragma unroll
-        for (int x = 0; x < AXES; ++x) qp[x] = a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x];
-        if constexpr (HIST) {
-            for (int i = tid; i < span; i += THREADS) bucket[i] = (unsigned short)rel_bucket(a.rb, i);
-            for (int i = 0; i < hist_rows; ++i) hist[i * THREADS + tid] = 0.0f;
+        for (int x = 0; x < AXES; ++x) {
+            const int centre = (int)lds_address(lut + x * span + a.rb.limit);
+            qa[x] = scale_pos<ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x]) - centre;
+            lo[x] = centre - ENTRY * a.rb.limit;
+            hi[x] = centre + ENTRY * a.rb.limit;
         }
+        if constexpr (HIST)
+            for (int i = 0; i < hist_rows; ++i) hist[i * THREADS + tid] = 0.0f;
     }
+    char* column = reinterpret_cast<char*>(hist + tid);
 
     acc16 dq[TL::DBLOCKS];
 #pragma unroll
@@ -598,7 +652,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     int pnext = 0, cur = 0;
     if (t0 < t1) {
         st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
-        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, t0 * TL::ROWS, len);
+        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
         if constexpr (AXES > 0)
             if (tid < AXES * TL::ROWS) pos[tid] = pnext;
@@ -608,7 +662,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
         if (t + 1 < t1) {
             st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
-            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(kpos, (t + 1) * TL::ROWS, len);
+            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, (t + 1) * TL::ROWS, len);
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
         const int* pt = pos + cur * AXES * TL::ROWS;
@@ -622,18 +676,24 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
             for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(map.read_row(kb, ks), qf[ks], s);
 #pragma unroll
             for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(vb, ks), gf[ks], dp);
-            int idx[16][AXES ? AXES : 1];
+            unsigned at_hist[16][AXES ? AXES : 1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 if constexpr (AXES > 0) {
-                    const int r = nb * 32 + acc_row(i, h);
-                    idx[i][0] = rel_index(pt[r], qp[0], a.rb.limit);
-                    float x = __builtin_fmaf(s[i], a.scale_log2, lut[idx[i][0]]);
-                    if constexpr (AXES > 1) {
-                        idx[i][AXES - 1] = rel_index(pt[TL::ROWS + r], qp[AXES - 1], a.rb.limit);
-                        x += lut[span + idx[i][AXES - 1]];
+                    float bias[AXES];
+#pragma unroll
+                    for (int x = 0; x < AXES; ++x) {
+                        const int address = med3(pt[x * TL::ROWS + nb * 32 + acc_row(i, h)] - qa[x], lo[x], hi[x]);
+                        if constexpr (HIST) {
+                            const uint2v e = lds_load<uint2v>(address);     // an Entry8
+                            bias[x] = __uint_as_float(e[0]);
+                            at_hist[i][x] = e[1];
+                        } else {
+                            bias[x] = lds_load<float>(address);
+                        }
                     }
-                    s[i] = x;
+                    s[i] = __builtin_fmaf(s[i], a.scale_log2, bias[0]);
+                    if constexpr (AXES > 1) s[i] += bias[AXES - 1];
                 } else {
                     s[i] *= a.scale_log2;
                 }
@@ -647,11 +707,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(s[i]);
             if constexpr (HIST) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int x = 0; x < AXES; ++x) idx[i][x] = bucket[idx[i][x]] + x * a.rb.buckets;
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) hist_add2<THREADS, AXES>(hist + tid, idx[i], dp[i], idx[i + 1], dp[i + 1]);
+                for (int i = 0; i < 16; i += 2) hist_add2<AXES>(column, at_hist[i], dp[i], at_hist[i + 1], dp[i + 1]);
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
@@ -687,11 +743,11 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 
 // ------------------------------------------------------------------------------------------------------------ dk, dv
 template <typename T, int DP, int AXES>
-__global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
+__global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_kernel(Args a) {
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
-    constexpr int THREADS = 256;
+    constexpr int THREADS = 256, ENTRY = sizeof(float);
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                              // [2][Q, dO]
     float* stats = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);                     // [2][lse, delta][ROWS]
@@ -714,13 +770,17 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
     Frag kf[TL::KSTEPS], vf[TL::KSTEPS];
     load_owned<T, DP>(kf, static_cast<const T*>(a.k) + b * a.ks.b + (int64_t)kj * a.ks.l + kvh * a.ks.h, kept, a.D, h);
     load_owned<T, DP>(vf, static_cast<const T*>(a.v) + b * a.vs.b + (int64_t)kj * a.vs.l + kvh * a.vs.h, kept, a.D, h);
-    int kpos[AXES ? AXES : 1] = {0};
-    const int span = 2 * a.rb.limit + 1;
+    int ka[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* qpos = nullptr;
     if constexpr (AXES > 0) {
         qpos = a.rb.qpos + b * a.rb.qpos_bs;
 #pragma unroll
-        for (int x = 0; x < AXES; ++x) kpos[x] = kept ? a.rb.kpos[b * a.rb.kpos_bs + (int64_t)kj * AXES + x] : 0;
+        for (int x = 0; x < AXES; ++x) {
+            const int centre = (int)lds_address(lut + x * (2 * a.rb.limit + 1) + a.rb.limit);
+            ka[x] = (kept ? scale_pos<ENTRY>(a.rb.kpos[b * a.rb.kpos_bs + (int64_t)kj * AXES + x]) : 0) + centre;
+            lo[x] = centre - ENTRY * a.rb.limit;
+            hi[x] = centre + ENTRY * a.rb.limit;
+        }
     }
     acc16 dk[TL::DBLOCKS], dv[TL::DBLOCKS];
 #pragma unroll
@@ -745,7 +805,7 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
             const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
             snext = tid < TL::ROWS ? -x / a.scale_log2 : -x;
         }
-        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS>(qpos, row0, a.Lq);
+        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(qpos, row0, a.Lq);
     };
     auto store = [&](int buf) {
         T* n = tiles + buf * 2 * TL::ELEMS;
@@ -792,8 +852,8 @@ __global__ __launch_bounds__(256) void dkdv_kernel(Args a) {
                 float x;
                 if constexpr (AXES > 0) {
                     const int r = nb * 32 + acc_row(i, h);
-                    x = __builtin_fmaf(s[i], a.scale_log2, lut[rel_index(kpos[0], pt[r], a.rb.limit)]);
-                    if constexpr (AXES > 1) x += lut[span + rel_index(kpos[AXES - 1], pt[TL::ROWS + r], a.rb.limit)];
+                    x = __builtin_fmaf(s[i], a.scale_log2, lds_load<float>(med3(ka[0] - pt[r], lo[0], hi[0])));
+                    if constexpr (AXES > 1) x += lds_load<float>(med3(ka[AXES - 1] - pt[TL::ROWS + r], lo[AXES - 1], hi[AXES - 1]));
                 } else {
                     x = s[i] * a.scale_log2;
                 }
@@ -885,7 +945,7 @@ int run_dq_mode(const Args& a, hipStream_t s) {
     constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
     static unsigned long long done = 0;
     size_t lds = tile_bytes<T, DP, R>() + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, 1);
-    if (HIST) lds += sizeof(float) * AXES * a.rb.buckets * 64 * WAVES + 2 * (2 * a.rb.limit + 2);
+    if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * 64 * WAVES;      // entries of 8 bytes
     return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
 }
 

@@ -9,10 +9,9 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .norm import TYPE_CODES, same_device
+from .norm import TYPE_CODES, address, first_order, same_device
 from .wrapper import _on_device, _require_cuda, _stream_ptr
 
 MAX_HEAD_DIM = 128
@@ -82,42 +81,49 @@ def _composed_bias(table, q_pos, k_pos, bidirectional, max_distance):
     return total.movedim(-1, -3)            # [(B,) H, Lq, Lk]
 
 
+@functools.lru_cache(maxsize=1024)
+def _bias_workspace_bytes(b, h, lq, lk, axes, buckets, code):
+    return int(_lib.load().camli_rel_bias_bwd_workspace_bytes(b, h, lq, lk, axes, buckets, code))
+
+
+def _run_bias(table, q_pos, k_pos, batch, bidirectional, max_distance):
+    axes, buckets, h = table.shape
+    lq, lk = q_pos.shape[-2], k_pos.shape[-2]
+    out = torch.empty((h, lq, lk) if batch is None else (batch, h, lq, lk), dtype=table.dtype, device=table.device)
+    n = out.numel()
+    if n:
+        with _on_device(table):
+            _lib.launch('camli_rel_bias_fwd', _lib.load().camli_rel_bias_fwd, table.data_ptr(), q_pos.data_ptr(), _pos_stride(q_pos),
+                        k_pos.data_ptr(), _pos_stride(k_pos), out.data_ptr(), batch or 1, h, lq, lk, axes, buckets, int(bidirectional),
+                        max_distance, TYPE_CODES[table.dtype], _stream_ptr(table), work=(float(n * out.element_size()), 'B'))
+    return out
+
+
 class _RelativeBias(torch.autograd.Function):
     @staticmethod
-    @torch.amp.custom_fwd(device_type='cuda')
     def forward(ctx, table, q_pos, k_pos, batch, bidirectional, max_distance):
-        lib = _lib.load()
-        axes, buckets, h = table.shape
-        lq, lk = q_pos.shape[-2], k_pos.shape[-2]
-        lead = (h,) if batch is None else (batch, h)
-        out = torch.empty(lead + (lq, lk), dtype=table.dtype, device=table.device)
         ctx.save_for_backward(q_pos, k_pos)
-        ctx.args = (axes, buckets, h, batch, lq, lk, bidirectional, max_distance, table.dtype)
-        if out.numel():
-            with _on_device(table):
-                _lib.launch('camli_rel_bias_fwd', lib.camli_rel_bias_fwd, table.data_ptr(), q_pos.data_ptr(), _pos_stride(q_pos), k_pos.data_ptr(),
-                            _pos_stride(k_pos), out.data_ptr(), batch or 1, h, lq, lk, axes, buckets, int(bidirectional), max_distance,
-                            TYPE_CODES[table.dtype], _stream_ptr(table), work=(float(out.numel() * out.element_size()), 'B'))
-        return out
+        ctx.args = (tuple(table.shape), batch, bidirectional, max_distance, table.dtype)
+        return _run_bias(table, q_pos, k_pos, batch, bidirectional, max_distance)
 
-    @staticmethod
-    @torch.amp.custom_bwd(device_type='cuda')
-    @once_differentiable
+    @first_order
     def backward(ctx, gout):
-        lib = _lib.load()
         q_pos, k_pos = ctx.saved_tensors
-        axes, buckets, h, batch, lq, lk, bidirectional, max_distance, dtype = ctx.args
-        if not gout.numel():
-            return torch.zeros((axes, buckets, h), dtype=dtype, device=gout.device), None, None, None, None, None
+        shape, batch, bidirectional, max_distance, dtype = ctx.args
+        axes, buckets, h = shape
+        lq, lk = q_pos.shape[-2], k_pos.shape[-2]
+        n = gout.numel()
+        if not n:
+            return torch.zeros(shape, dtype=dtype, device=gout.device), None, None, None, None, None
         gout = gout.contiguous()
-        gtable = torch.empty((axes, buckets, h), dtype=dtype, device=gout.device)
+        gtable = torch.empty(shape, dtype=dtype, device=gout.device)
         code, b = TYPE_CODES[dtype], batch or 1
-        ws_bytes = int(lib.camli_rel_bias_bwd_workspace_bytes(b, h, lq, lk, axes, buckets, code))
+        ws_bytes = _bias_workspace_bytes(b, h, lq, lk, axes, buckets, code)
         ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=gout.device)
         with _on_device(gout):
-            _lib.launch('camli_rel_bias_bwd', lib.camli_rel_bias_bwd, gout.data_ptr(), q_pos.data_ptr(), _pos_stride(q_pos), k_pos.data_ptr(),
-                        _pos_stride(k_pos), gtable.data_ptr(), ws.data_ptr(), ws_bytes, b, h, lq, lk, axes, buckets, int(bidirectional),
-                        max_distance, code, _stream_ptr(gout), work=(float(gout.numel() * gout.element_size()), 'B'))
+            _lib.launch('camli_rel_bias_bwd', _lib.load().camli_rel_bias_bwd, gout.data_ptr(), q_pos.data_ptr(), _pos_stride(q_pos),
+                        k_pos.data_ptr(), _pos_stride(k_pos), gtable.data_ptr(), ws.data_ptr(), ws_bytes, b, h, lq, lk, axes, buckets,
+                        int(bidirectional), max_distance, code, _stream_ptr(gout), work=(float(n * gout.element_size()), 'B'))
         return gtable, None, None, None, None, None
 
 
@@ -139,7 +145,8 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
     if not cpp_impl:
         return _composed_bias(table, q_pos, k_pos, bidirectional, int(max_distance)).to(table.dtype)
     _require_cuda(name, table)
-    return _RelativeBias.apply(table, q_pos, k_pos, batch, bool(bidirectional), int(max_distance))
+    run = _RelativeBias.apply if table.requires_grad and torch.is_grad_enabled() else _run_bias
+    return run(table, q_pos, k_pos, batch, bool(bidirectional), int(max_distance))
 
 
 # ------------------------------------------------------------------------------------------------
@@ -184,45 +191,44 @@ def _workspace(name, n, like):
     return torch.empty(max(int(n), 16), dtype=torch.uint8, device=like.device)
 
 
+def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance, train):
+    """-> (out, operands as the kernels read them, out's rounding error, row log-sums)"""
+    b, lq, h, dim = q.shape
+    lk, hk = k.shape[1:3]
+    if q.numel() == 0 or lk == 0:
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device), (q, k, v), None, None
+    lib = _lib.load()
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if train else None
+    rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
+    ref = ctypes.byref(d)
+    with _on_device(q):
+        n = lib.camli_cross_attention_fwd_workspace_bytes(ref)
+        ws = _workspace('camli_cross_attention_fwd', n, q) if n else None
+        _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, ref, out.data_ptr(), address(rest), address(lse), address(ws), n,
+                    _stream_ptr(q), work=(2.0 * q.element_size() * dim * b * (lq * h + lk * hk), 'B'), flop=4.0 * b * h * lq * lk * dim)
+    return out, (q, k, v), rest, lse
+
+
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    @torch.amp.custom_fwd(device_type='cuda')
     def forward(ctx, q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance):
-        lib = _lib.load()
-        b, lq, h, dim = q.shape
-        lk = k.shape[1]
         ctx.args = (scale, bidirectional, max_distance)
-        if q.numel() == 0 or lk == 0:
-            ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, None, None, None)
-            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
-        lse = rest = None
-        if any(ctx.needs_input_grad[:4]):
-            lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device)
-            rest = torch.empty_like(out) if q.dtype != torch.float32 else None
-        d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
-        size = q.element_size()
-        with _on_device(q):
-            n = lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d))
-            ws = _workspace('camli_cross_attention_fwd', n, q)
-            _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, ctypes.byref(d), out.data_ptr(),
-                        rest.data_ptr() if rest is not None else None, lse.data_ptr() if lse is not None else None, ws.data_ptr(), n, _stream_ptr(q),
-                        work=(float(size * (2 * q.numel() + 2 * b * lk * k.shape[2] * dim)), 'B'), flop=4.0 * b * h * lq * lk * dim)
-        ctx.save_for_backward(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, rest, lse)
+        out, operands, rest, lse = _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance, True)
+        ctx.save_for_backward(*operands, table, kv_lengths, key_mask, q_pos, k_pos, out if lse is not None else None, rest, lse)
         return out
 
-    @staticmethod
-    @torch.amp.custom_bwd(device_type='cuda')
-    @once_differentiable
+    @first_order
     def backward(ctx, gout):
-        lib = _lib.load()
         q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, rest, lse = ctx.saved_tensors
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
         nothing = (None,) * 7
         if out is None:
             return (torch.zeros_like(q) if need_q else None, torch.zeros_like(k) if need_k else None,
                     torch.zeros_like(v) if need_v else None, torch.zeros_like(table) if need_t else None) + nothing
+        lib = _lib.load()
         b, lq, h, dim = q.shape
         lk, hk = k.shape[1:3]
         gout = gout.contiguous()
@@ -231,19 +237,17 @@ class _CrossAttention(torch.autograd.Function):
         gq = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device) if need_q else None
         gk = gv = None
         if need_k or need_v:
-            gk, gv = (torch.empty((b, lk, hk, dim), dtype=q.dtype, device=q.device) for _ in range(2))
+            gk = torch.empty((b, lk, hk, dim), dtype=q.dtype, device=q.device)
+            gv = torch.empty_like(gk)
         gt = torch.empty(table.shape, dtype=table.dtype, device=q.device) if need_t else None
         d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, *ctx.args)
-        size = q.element_size()
-
-        def ptr(t):
-            return t.data_ptr() if t is not None else None
+        ref = ctypes.byref(d)
         with _on_device(q):
-            n = lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), int(need_t))
+            n = lib.camli_cross_attention_bwd_workspace_bytes(ref, int(need_t))
             ws = _workspace('camli_cross_attention_bwd', n, q)
-            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, ctypes.byref(d), out.data_ptr(), ptr(rest), gout.data_ptr(),
-                        lse.data_ptr(), ptr(gq), ptr(gk), ptr(gv), ptr(gt), ws.data_ptr(), n, _stream_ptr(q),
-                        work=(float(size * (4 * q.numel() + 4 * b * lk * hk * dim)), 'B'), flop=10.0 * b * h * lq * lk * dim)
+            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, ref, out.data_ptr(), address(rest), gout.data_ptr(),
+                        lse.data_ptr(), address(gq), address(gk), address(gv), address(gt), ws.data_ptr(), n, _stream_ptr(q),
+                        work=(4.0 * q.element_size() * dim * b * (lq * h + lk * hk), 'B'), flop=10.0 * b * h * lq * lk * dim)
         return (gq, gk if need_k else None, gv if need_v else None, gt) + nothing
 
 
@@ -310,6 +314,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
         bias = _composed_bias(bias_table, q_pos, k_pos, bidirectional, int(max_distance)) if bias_table is not None else None
         return _composed_attention(q, k, v, scale, kv_lengths, key_mask, bias)
     _require_cuda(name, q)
-    return _CrossAttention.apply(q, k, v, bias_table, kv_lengths.contiguous() if kv_lengths is not None else None,
-                                 key_mask.contiguous() if key_mask is not None else None, q_pos, k_pos, scale, bool(bidirectional),
-                                 int(max_distance))
+    args = (q, k, v, bias_table, kv_lengths.contiguous() if kv_lengths is not None else None,
+            key_mask.contiguous() if key_mask is not None else None, q_pos, k_pos, scale, bool(bidirectional), int(max_distance))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)):
+        return _CrossAttention.apply(*args)
+    return _run_attention(*args, False)[0]

@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     id /= a.row_tiles;
     const int hh = id % groups, b = id / groups, kvh = hh * a.pack / (a.H / a.Hk);
     const int row = rt * 128 + wave * 32 + (lane & 31), rows = a.pack * a.Lq;
-    const bool exists = row < rows;
+    const bool exists = row < rows, busy = rt * 128 + wave * 32 < rows;         // an idle wave only helps to fetch
     const int sub = exists ? row / a.Lq : 0, qi = exists ? row - sub * a.Lq : 0, head = hh * a.pack + sub;
 
     const int len = kept_length(a, b);
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
         const int* pt = pos + cur * AXES * TL::ROWS;
-        if (bits != 0) {
+        if (bits != 0 && busy) {
             acc16 s[TL::BLOCKS];
             float top = -INFINITY;
 #pragma unroll
@@ -524,35 +524,46 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     }
 }
 
-// joins the splits of the forward: one thread per 4 elements of a row
+// Joins the splits of the forward.  A wave per row: `lanes` (a power of two >= D / 4) lanes hold 4 elements each, the 64 / lanes groups
+// take every (64 / lanes)-th split, and the groups are added at the end -- with one group, 64 splits would be 64 dependent loads.
 template <typename T>
-__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
-    const int per_row = a.D / 4;
-    const int64_t rows = (int64_t)a.B * a.Lq * a.H, t = (int64_t)blockIdx.x * 256 + threadIdx.x, at = t / per_row;
+__global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
+    const int64_t rows = (int64_t)a.B * a.Lq * a.H, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= rows) return;
-    const int c = (int)(t - at * per_row) * 4;
+    const int lane = threadIdx.x & 63, c = (lane & (lanes - 1)) * 4, group = lane / lanes, groups = 64 / lanes;
     const int head = (int)(at % a.H);
     const int64_t bq = at / a.H;
     const int64_t stat = ((bq / a.Lq) * a.H + head) * a.Lq + bq % a.Lq;
     float top = -INFINITY;
     bool bad = false;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = lane; s < a.splits; s += 64) {
         const float v = a.part_lse[s * rows + stat];
         top = fmaxf(top, v);
         bad |= v != v;
     }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    bad = __any(bad);
     const float use = top == -INFINITY ? 0.0f : top;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+    for (int s = group; s < a.splits; s += groups) {
         const float w = __builtin_amdgcn_exp2f(a.part_lse[s * rows + stat] - use);
-        if (w == 0.0f) continue;
-        float v[4];
-        load_f32<float, 4>(a.part_o + (s * rows + at) * a.D + c, v);
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (c < a.D && w != 0.0f) load_f32<float, 4>(a.part_o + (s * rows + at) * a.D + c, v);
         sum += w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
     }
+    for (int off = 32; off >= lanes; off >>= 1) {
+        sum += __shfl_xor(sum, off, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], off, 64);
+    }
+    if (group != 0) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + __builtin_amdgcn_logf(sum);
+    if (c >= a.D) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = bad ? NAN : acc[i] * inv;
     store_f32<T, 4>(static_cast<T*>(a.out) + at * a.D + c, acc);
@@ -561,7 +572,6 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
         for (int i = 0; i < 4; ++i) acc[i] -= (float)(T)acc[i];
         store_f32<T, 4>(static_cast<T*>(a.out_rest) + at * a.D + c, acc);
     }
-    if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + __builtin_amdgcn_logf(sum);
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
@@ -890,19 +900,31 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     }
 }
 
-// out[n] = sum of the splits' parts, in order; 4 elements a thread (n is a multiple of 8)
+// Everything the splits of the backward left to add, in one launch: out[n] = sum of a job's parts, in order, 4 elements a thread (n is a
+// multiple of 8).  Jobs: dq, dk, dv; blockIdx.y selects.
+struct SumJob {
+    const float* part;
+    void* out;
+    int64_t n;
+    int splits;
+};
+struct SumJobs {
+    SumJob job[3];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t n, int splits) {
+__global__ __launch_bounds__(256) void sum_parts_kernel(SumJobs jobs) {
+    const SumJob j = jobs.job[blockIdx.y];
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
+    if (i >= j.n) return;
     float acc[4], v[4];
-    load_f32<float, 4>(part + i, acc);
-    for (int s = 1; s < splits; ++s) {
-        load_f32<float, 4>(part + s * n + i, v);
+    load_f32<float, 4>(j.part + i, acc);
+#pragma unroll 4
+    for (int s = 1; s < j.splits; ++s) {
+        load_f32<float, 4>(j.part + s * j.n + i, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += v[e];
     }
-    store_f32<T, 4>(out + i, acc);
+    store_f32<T, 4>(static_cast<T*>(j.out) + i, acc);
 }
 
 // ------------------------------------------------------------------------------------------------------------ launches
@@ -935,8 +957,9 @@ template <typename T, int DP, int AXES>
 int run_fwd(const Args& a, hipStream_t s) {
     const int rc = a.lse ? run_fwd_mode<T, DP, AXES, true>(a, s) : run_fwd_mode<T, DP, AXES, false>(a, s);
     if (rc != CAMLI_OK || a.splits == 1) return rc;
-    const int64_t threads = (int64_t)a.B * a.Lq * a.H * (a.D / 4);
-    fwd_join_kernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, s>>>(a);
+    int lanes = 2;
+    while (lanes * 4 < a.D) lanes *= 2;
+    fwd_join_kernel<T><<<dim3((unsigned)(((int64_t)a.B * a.Lq * a.H + 3) / 4)), 256, 0, s>>>(a, lanes);
     return camli_check_launch("camli_cross_attention_fwd");
 }
 
@@ -958,12 +981,7 @@ int run_dq(const Args& a, int waves, hipStream_t s) {
     } else {
         rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
     }
-    if (rc != CAMLI_OK) return rc;
-    if (a.splits > 1 && a.dq) {
-        const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
-        sum_parts_kernel<T><<<dim3((unsigned)((n / 4 + 255) / 256)), 256, 0, s>>>(a.part_o, static_cast<T*>(a.dq), n, a.splits);
-    }
-    return camli_check_launch("camli_cross_attention_bwd");
+    return rc;
 }
 
 template <typename T, int DP, int AXES>
@@ -971,13 +989,7 @@ int run_dkdv(const Args& a, hipStream_t s) {
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     static unsigned long long done = 0;
     const size_t lds = tile_bytes<T, DP, R>() + sizeof(float) * 4 * R + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, 1);
-    const int rc = start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);
-    if (rc != CAMLI_OK || a.splits == 1) return rc;
-    const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.D;
-    const dim3 grid((unsigned)((n / 4 + 255) / 256));
-    sum_parts_kernel<T><<<grid, 256, 0, s>>>(a.part_dk, static_cast<T*>(a.dk), n, a.splits);
-    sum_parts_kernel<T><<<grid, 256, 0, s>>>(a.part_dv, static_cast<T*>(a.dv), n, a.splits);
-    return camli_check_launch("camli_cross_attention_bwd");
+    return start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);
 }
 
 // the three kernels by head width (padded to 32, 64 or 128) and axes of the bias
@@ -986,6 +998,7 @@ struct Launch {
     static int fwd(const Args& a, int axes, hipStream_t s);
     static int dq(const Args& a, int axes, int waves, hipStream_t s);
     static int dkdv(const Args& a, int axes, hipStream_t s);
+    static int sum(const SumJobs& jobs, int n, hipStream_t s);
 };
 
 #define XATTN_SELECT(RUN, ...)                                                                                      \
@@ -997,6 +1010,13 @@ struct Launch {
     template <> int Launch<TYPE>::fwd(const Args& a, int axes, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_fwd, a, s) }
 #define XATTN_DEFINE_DQ(TYPE) \
     template <> int Launch<TYPE>::dq(const Args& a, int axes, int waves, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_dq, a, waves, s) }
+#define XATTN_DEFINE_SUM(TYPE)                                                                                     \
+    template <> int Launch<TYPE>::sum(const SumJobs& jobs, int n, hipStream_t s) {                                 \
+        int64_t most = 0;                                                                                          \
+        for (int i = 0; i < n; ++i) most = jobs.job[i].n > most ? jobs.job[i].n : most;                            \
+        sum_parts_kernel<TYPE><<<dim3((unsigned)((most / 4 + 255) / 256), n), 256, 0, s>>>(jobs);                  \
+        return camli_check_launch("camli_cross_attention_bwd");                                                    \
+    }
 #define XATTN_DEFINE_DKDV(TYPE) \
     template <> int Launch<TYPE>::dkdv(const Args& a, int axes, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_dkdv, a, s) }
 

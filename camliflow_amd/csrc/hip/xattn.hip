@@ -7,13 +7,13 @@ using xattn::Args;
 
 int tile_rows(int type, bool histogram = false) { return type == CAMLI_F32 || histogram ? 32 : 64; }
 
-// Few owned rows leave CUs idle: the streamed side is cut until there are two workgroups per CU, but into no less than four tiles a
+// Few owned rows leave CUs idle: the streamed side is cut until there are `want` workgroups, but into no less than `least` tiles a
 // piece (a piece pays for its start and for its part of the join).
-void split_stream(Args& a, int64_t base, int n_tiles) {
+void split_stream(Args& a, int64_t base, int n_tiles, int want, int least) {
     int splits = 1;
-    if (base < 512) {
-        splits = (int)((512 + base - 1) / base);
-        const int most = n_tiles / 4 < 1 ? 1 : n_tiles / 4;
+    if (base < want / 2) {
+        splits = (int)((want + base - 1) / base);
+        const int most = n_tiles / least < 1 ? 1 : n_tiles / least;
         if (splits > most) splits = most;
     }
     a.tiles_per_split = n_tiles ? (n_tiles + splits - 1) / splits : 1;
@@ -26,7 +26,7 @@ void plan_fwd(Args& a, int type, int axes) {
     // values are then read once, not once per head
     a.pack = group > 1 && (int64_t)a.Lq * group <= 128 && xattn::lut_bytes(a, axes, group) <= 16384 ? group : 1;
     a.row_tiles = camli_divup(a.pack * a.Lq, 128);
-    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile_rows(type)));
+    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile_rows(type)), 1024, 4);
 }
 
 int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.buckets > 64 ? 2 : 4; }
@@ -34,14 +34,14 @@ int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.
 void plan_dq(Args& a, int type, int axes, bool table) {
     a.pack = 1;
     a.row_tiles = camli_divup(a.Lq, 32 * dq_waves(a, axes, table));
-    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, tile_rows(type, table)));
+    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, tile_rows(type, table)), 1024, 4);
     a.parts = a.B * a.row_tiles * a.splits;
 }
 
 void plan_dkdv(Args& a, int type) {
     a.pack = 1;
     a.row_tiles = camli_divup(a.Lk, 128);
-    split_stream(a, (int64_t)a.row_tiles * a.Hk * a.B, camli_divup(a.Lq, tile_rows(type)) * (a.H / a.Hk));
+    split_stream(a, (int64_t)a.row_tiles * a.Hk * a.B, camli_divup(a.Lq, tile_rows(type)) * (a.H / a.Hk), 1024, 4);
 }
 
 bool operand_ok(const void* p, const int64_t* stride, int size) {
@@ -104,15 +104,14 @@ struct BwdPlan {
     int64_t bytes;
 };
 
-// workspace of the backward: delta; then the parts of dq and of the table, whose place the parts of dk and dv take afterwards
+// workspace of the backward: delta, then the parts of dq, of the table, of dk and dv
 BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base) {
     BwdPlan p{a, a, 0};
     plan_dq(p.dq, d->type, d->bias_axes, table);
     plan_dkdv(p.dkdv, d->type);
     const int64_t rows = (int64_t)a.B * a.H * a.Lq;
     p.dq.delta = p.dkdv.delta = reinterpret_cast<float*>(base);
-    const int64_t start = align256(4 * rows);
-    int64_t end = start;
+    int64_t end = align256(4 * rows);
     if (p.dq.splits > 1) {
         p.dq.part_o = reinterpret_cast<float*>(base + end);
         end += align256(4 * rows * a.D * p.dq.splits);
@@ -121,14 +120,13 @@ BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base
         p.dq.part_table = reinterpret_cast<float*>(base + end);
         end += align256((int64_t)4 * a.H * p.dq.parts * d->bias_axes * d->bias_buckets);
     }
-    int64_t end2 = start;
     if (p.dkdv.splits > 1) {
         const int64_t n = align256((int64_t)4 * a.B * a.Lk * a.Hk * a.D * p.dkdv.splits);
-        p.dkdv.part_dk = reinterpret_cast<float*>(base + start);
-        p.dkdv.part_dv = reinterpret_cast<float*>(base + start + n);
-        end2 += 2 * n;
+        p.dkdv.part_dk = reinterpret_cast<float*>(base + end);
+        p.dkdv.part_dv = reinterpret_cast<float*>(base + end + n);
+        end += 2 * n;
     }
-    p.bytes = end > end2 ? end : end2;
+    p.bytes = end;
     return p;
 }
 
@@ -193,8 +191,20 @@ extern "C" int camli_cross_attention_bwd(const camli_attention* d, const void* o
         rc = rel_bias_join(p.dq.part_table, gtable, d->type, a.H, axes * d->bias_buckets, p.dq.parts, "camli_cross_attention_bwd", s);
         if (rc != CAMLI_OK) return rc;
     }
-    if (!gk) return CAMLI_OK;
-    if (d->type == CAMLI_F32) return xattn::Launch<float>::dkdv(p.dkdv, axes, s);
-    if (d->type == CAMLI_BF16) return xattn::Launch<__bf16>::dkdv(p.dkdv, axes, s);
-    return xattn::Launch<_Float16>::dkdv(p.dkdv, axes, s);
+    if (gk) {
+        rc = d->type == CAMLI_F32 ? xattn::Launch<float>::dkdv(p.dkdv, axes, s)
+             : d->type == CAMLI_BF16 ? xattn::Launch<__bf16>::dkdv(p.dkdv, axes, s) : xattn::Launch<_Float16>::dkdv(p.dkdv, axes, s);
+        if (rc != CAMLI_OK) return rc;
+    }
+    xattn::SumJobs jobs;
+    int n = 0;
+    if (gq && p.dq.splits > 1) jobs.job[n++] = {p.dq.part_o, gq, (int64_t)a.B * a.Lq * a.H * a.D, p.dq.splits};
+    if (gk && p.dkdv.splits > 1) {
+        jobs.job[n++] = {p.dkdv.part_dk, gk, (int64_t)a.B * a.Lk * a.Hk * a.D, p.dkdv.splits};
+        jobs.job[n++] = {p.dkdv.part_dv, gv, (int64_t)a.B * a.Lk * a.Hk * a.D, p.dkdv.splits};
+    }
+    if (n == 0) return CAMLI_OK;
+    if (d->type == CAMLI_F32) return xattn::Launch<float>::sum(jobs, n, s);
+    if (d->type == CAMLI_BF16) return xattn::Launch<__bf16>::sum(jobs, n, s);
+    return xattn::Launch<_Float16>::sum(jobs, n, s);
 }

@@ -3,4 +3,5 @@
 
 namespace xattn {
 XATTN_DEFINE_DKDV(__bf16)
+XATTN_DEFINE_SUM(__bf16)
 }

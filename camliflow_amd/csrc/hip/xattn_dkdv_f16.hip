@@ -3,4 +3,5 @@
 
 namespace xattn {
 XATTN_DEFINE_DKDV(_Float16)
+XATTN_DEFINE_SUM(_Float16)
 }

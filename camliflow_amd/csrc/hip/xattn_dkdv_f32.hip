@@ -3,4 +3,5 @@
 
 namespace xattn {
 XATTN_DEFINE_DKDV(float)
+XATTN_DEFINE_SUM(float)
 }

@@ -21,7 +21,7 @@ struct RelBias {
     const int *qpos, *kpos;     // [.., L, axes], batch strides in ints (0: shared)
     int64_t qpos_bs, kpos_bs;
     int type, axes, buckets, side, exact, two_sided, limit, n_borders;
-    short border[CAMLI_REL_MAX_BORDERS];
+    int border[CAMLI_REL_MAX_BORDERS];      // INT_MAX from n_borders on
 };
 
 // fills r; false (with the error set) for arguments outside the documented range
@@ -38,7 +38,8 @@ __device__ __forceinline__ int rel_bucket(const RelBias& r, int i) {
     int n = d;
     if (d >= r.exact) {
         n = r.exact;
-        for (int j = 0; j < r.n_borders; ++j) n += r.border[j] <= d ? 1 : 0;
+#pragma unroll          // all of them: the borders come in a few wide scalar loads, a counted loop waits for each
+        for (int j = 0; j < CAMLI_REL_MAX_BORDERS; ++j) n += r.border[j] <= d ? 1 : 0;
     }
     return n + (r.two_sided && o > 0 ? r.side : 0);
 }

@@ -155,8 +155,9 @@ bool rel_bias_args(RelBias& r, const char* who, const void* table, int type, con
         const double near = floor(t + 0.5);
         int d = (int)ceil(t);
         if (fabs(t - near) < 1e-6) d = reaches((int)near, limit, exact, j, steps) ? (int)near : (int)near + 1;
-        r.border[j - 1] = (short)d;
+        r.border[j - 1] = d;
     }
+    for (int j = r.n_borders; j < CAMLI_REL_MAX_BORDERS; ++j) r.border[j] = INT32_MAX;
     return true;
 }
 

@@ -284,8 +284,9 @@ __device__ __forceinline__ unsigned long long kept_bits(const unsigned char* mas
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// The bias of a pair from LDS.  Positions are held as multiples of the entry size (scaled once per row, not per pair), and the owned
-// row's carries the address of its table's middle: one subtraction and one clamp of a pair give the LDS address of its entry.
+// The bias of a pair from LDS.  Positions are held as multiples of the entry size (scaled once per row, not per pair), query positions
+// negated, and the owned row's carries the address of its table's middle: one addition and one clamp of a pair give the LDS
+// address of its entry.
 // Positions beyond +-2^26 count as that, so that no difference overflows.
 // Entries: the bias (log2 domain), and for the table's gradient beside it where the bucket's row of the histogram starts.
 struct Entry8 {
@@ -305,8 +306,8 @@ __device__ __forceinline__ int med3(int x, int lo, int hi) {
     asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(lo), "v"(hi));
     return r;
 }
-template <int ENTRY>
-__device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 26)), 1 << 26) * ENTRY; }
+template <int SCALE>
+__device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 26)), 1 << 26) * SCALE; }
 
 // tables of `pack` heads: lut[p][axis][2 limit + 1]
 template <int AXES, int THREADS>
@@ -331,13 +332,45 @@ __device__ __forceinline__ void fill_lut(const RelBias& r, Entry8* lut, int head
     }
 }
 
-// positions of the streamed rows, scaled: pos[axis][ROWS]
-template <int AXES, int ROWS, int ENTRY>
-__device__ __forceinline__ int load_pos(const int* pos, int row0, int limit) {
-    const int t = threadIdx.x;
-    if (t >= AXES * ROWS) return 0;
-    const int row = min(row0 + t % ROWS, limit - 1);
-    return scale_pos<ENTRY>(pos[(int64_t)row * AXES + t / ROWS]);
+// Positions of the streamed rows stay out of LDS: lane i of each 16-lane row holds the position of the row that accumulator register i
+// stands for (acc_row(i, h): the halves differ), and the subtraction reads it from there by a row broadcast.  As LDS broadcasts the
+// same reads took a quarter of the LDS time.
+template <int AXES, int BLOCKS, int SCALE>
+struct StreamPos {
+    int p[BLOCKS][AXES ? AXES : 1];
+
+    __device__ __forceinline__ void load(const int* pos, int row0, int limit) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int nb = 0; nb < BLOCKS; ++nb) {
+            const int row = min(row0 + nb * 32 + acc_row(lane & 15, lane >> 5), limit - 1);
+#pragma unroll
+            for (int x = 0; x < AXES; ++x) p[nb][x] = scale_pos<SCALE>(pos[(int64_t)row * AXES + x]);
+        }
+    }
+};
+// out[i] = (lane i of the 16-lane row's `lanes`) + own.  One instruction each; the compiler does not fold this broadcast into the addition
+// by itself.  (s_nop: a row broadcast may not read a register within two cycles of its writing.)
+__device__ __forceinline__ void broadcast_plus(int lanes, int own, int (&out)[16]) {
+    asm("s_nop 1\n\t"
+        "v_add_u32_dpp %0, %16, %17 row_newbcast:0 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %1, %16, %17 row_newbcast:1 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %2, %16, %17 row_newbcast:2 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %3, %16, %17 row_newbcast:3 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %4, %16, %17 row_newbcast:4 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %5, %16, %17 row_newbcast:5 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %6, %16, %17 row_newbcast:6 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %7, %16, %17 row_newbcast:7 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %8, %16, %17 row_newbcast:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %9, %16, %17 row_newbcast:9 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %10, %16, %17 row_newbcast:10 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %11, %16, %17 row_newbcast:11 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %12, %16, %17 row_newbcast:12 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %13, %16, %17 row_newbcast:13 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %14, %16, %17 row_newbcast:14 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %15, %16, %17 row_newbcast:15 row_mask:0xf bank_mask:0xf"
+        : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3]), "=&v"(out[4]), "=&v"(out[5]), "=&v"(out[6]), "=&v"(out[7]), "=&v"(out[8]), "=&v"(out[9]), "=&v"(out[10]), "=&v"(out[11]), "=&v"(out[12]), "=&v"(out[13]), "=&v"(out[14]), "=&v"(out[15])
+        : "v"(lanes), "v"(own));
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
@@ -355,12 +388,11 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
-    constexpr int THREADS = 256, ENTRY = sizeof(float);
+    constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
     constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2;
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
-    int* pos = reinterpret_cast<int*>(tiles + 4 * TL::ELEMS);               // [2][AXES][ROWS]
-    float* lut = reinterpret_cast<float*>(pos + 2 * AXES * TL::ROWS);
+    float* lut = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -391,7 +423,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
 #pragma unroll
         for (int x = 0; x < AXES; ++x) {
             const int centre = (int)lds_address(lut + (sub * AXES + x) * (2 * a.rb.limit + 1) + a.rb.limit);
-            qa[x] = scale_pos<4>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x]) - centre;
+            qa[x] = centre + scale_pos<-ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x]);
             lo[x] = centre - 4 * a.rb.limit;
             hi[x] = centre + 4 * a.rb.limit;
         }
@@ -407,23 +439,22 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     bool unset = true;
 
     Stream<T, DP, R, THREADS> st;
-    int pnext = 0, cur = 0;
+    StreamPos<AXES, TL::BLOCKS, ENTRY> pos, pos_next;
+    int cur = 0;
     if (t0 < t1) {
         st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
-        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, t0 * TL::ROWS, len);
+        if constexpr (AXES > 0) pos_next.load(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
-        if constexpr (AXES > 0)
-            if (tid < AXES * TL::ROWS) pos[tid] = pnext;
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
+        if constexpr (AXES > 0) pos = pos_next;
         if (t + 1 < t1) {
             st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
-            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, (t + 1) * TL::ROWS, len);
+            if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
-        const int* pt = pos + cur * AXES * TL::ROWS;
         if (bits != 0 && busy) {
             acc16 s[TL::BLOCKS];
             float top = -INFINITY;
@@ -435,15 +466,18 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
             }
 #pragma unroll
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+                if constexpr (AXES > 0) {
+                    int off[AXES][16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if constexpr (AXES > 0) {
-                        const int r = nb * 32 + acc_row(i, h);
-                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, lds_load<float>(med3(pt[r] - qa[0], lo[0], hi[0])));
-                        if constexpr (AXES > 1) s[nb][i] += lds_load<float>(med3(pt[TL::ROWS + r] - qa[AXES - 1], lo[AXES - 1], hi[AXES - 1]));
-                    } else {
-                        s[nb][i] *= a.scale_log2;
+                    for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], qa[x], off[x]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
+                        if constexpr (AXES > 1) s[nb][i] += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
                     }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[nb][i] *= a.scale_log2;
                 }
                 const unsigned half = (unsigned)(bits >> (nb * 32));
                 if (half != 0xffffffffu) {
@@ -496,8 +530,6 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
         if (t + 1 < t1) {
             T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
             st.store(nk, nk + TL::ELEMS);
-            if constexpr (AXES > 0)
-                if (tid < AXES * TL::ROWS) pos[(cur ^ 1) * AXES * TL::ROWS + tid] = pnext;
         }
         __syncthreads();
         cur ^= 1;
@@ -584,11 +616,10 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
     using Entry = __type_pack_element<HIST ? 1 : 0, float, Entry8>;
-    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = sizeof(Entry);
+    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = (int)sizeof(Entry);
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);
-    int* pos = reinterpret_cast<int*>(tiles + 4 * TL::ELEMS);
-    Entry* lut = reinterpret_cast<Entry*>(pos + 2 * AXES * TL::ROWS);
+    Entry* lut = reinterpret_cast<Entry*>(tiles + 4 * TL::ELEMS);
     const int span = 2 * a.rb.limit + 1, hist_rows = AXES * a.rb.buckets;
     float* hist = reinterpret_cast<float*>(lut + AXES * span);
 
@@ -645,7 +676,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 #pragma unroll
         for (int x = 0; x < AXES; ++x) {
             const int centre = (int)lds_address(lut + x * span + a.rb.limit);
-            qa[x] = scale_pos<ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x]) - centre;
+            qa[x] = centre + scale_pos<-ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x]);
             lo[x] = centre - ENTRY * a.rb.limit;
             hi[x] = centre + ENTRY * a.rb.limit;
         }
@@ -659,23 +690,22 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = acc16{0};
 
     Stream<T, DP, R, THREADS> st;
-    int pnext = 0, cur = 0;
+    StreamPos<AXES, TL::BLOCKS, ENTRY> pos, pos_next;
+    int cur = 0;
     if (t0 < t1) {
         st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
-        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, t0 * TL::ROWS, len);
+        if constexpr (AXES > 0) pos_next.load(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
-        if constexpr (AXES > 0)
-            if (tid < AXES * TL::ROWS) pos[tid] = pnext;
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
+        if constexpr (AXES > 0) pos = pos_next;
         if (t + 1 < t1) {
             st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
-            if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(kpos, (t + 1) * TL::ROWS, len);
+            if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
-        const int* pt = pos + cur * AXES * TL::ROWS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
             const unsigned half = (unsigned)(bits >> (nb * 32));
@@ -687,13 +717,16 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 #pragma unroll
             for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(vb, ks), gf[ks], dp);
             unsigned at_hist[16][AXES ? AXES : 1];
+            if constexpr (AXES > 0) {
+                int off[AXES][16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if constexpr (AXES > 0) {
+                for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], qa[x], off[x]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     float bias[AXES];
 #pragma unroll
                     for (int x = 0; x < AXES; ++x) {
-                        const int address = med3(pt[x * TL::ROWS + nb * 32 + acc_row(i, h)] - qa[x], lo[x], hi[x]);
+                        const int address = med3(off[x][i], lo[x], hi[x]);
                         if constexpr (HIST) {
                             const uint2v e = lds_load<uint2v>(address);     // an Entry8
                             bias[x] = __uint_as_float(e[0]);
@@ -704,9 +737,10 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
                     }
                     s[i] = __builtin_fmaf(s[i], a.scale_log2, bias[0]);
                     if constexpr (AXES > 1) s[i] += bias[AXES - 1];
-                } else {
-                    s[i] *= a.scale_log2;
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] *= a.scale_log2;
             }
             if (half != 0xffffffffu) {
                 const unsigned mine = half >> (4 * h);
@@ -729,8 +763,6 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         if (t + 1 < t1) {
             T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
             st.store(nk, nk + TL::ELEMS);
-            if constexpr (AXES > 0)
-                if (tid < AXES * TL::ROWS) pos[(cur ^ 1) * AXES * TL::ROWS + tid] = pnext;
         }
         __syncthreads();
         cur ^= 1;
@@ -757,12 +789,11 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
-    constexpr int THREADS = 256, ENTRY = sizeof(float);
+    constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                              // [2][Q, dO]
     float* stats = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);                     // [2][lse, delta][ROWS]
-    int* pos = reinterpret_cast<int*>(stats + 4 * TL::ROWS);                            // [2][AXES][ROWS]
-    float* lut = reinterpret_cast<float*>(pos + 2 * AXES * TL::ROWS);
+    float* lut = reinterpret_cast<float*>(stats + 4 * TL::ROWS);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -802,8 +833,9 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     int t1 = min(n_tiles, t0 + a.tiles_per_split);
     if (rt * 128 >= len) t1 = t0;        // no key of this workgroup is kept: zeros
     Stream<T, DP, R, THREADS> st;
+    StreamPos<AXES, TL::BLOCKS, -ENTRY> pos, pos_next;
     float snext = 0.0f;
-    int pnext = 0, cur = 0;
+    int cur = 0;
     auto load = [&](int t) {
         const int head = kvh * group + t / q_tiles, row0 = (t % q_tiles) * TL::ROWS;
         st.load(static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h, a.qs.l, static_cast<const T*>(a.go) + ((int64_t)b * a.Lq * a.H + head) * a.D,
@@ -815,14 +847,12 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
             const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
             snext = tid < TL::ROWS ? -x / a.scale_log2 : -x;
         }
-        if constexpr (AXES > 0) pnext = load_pos<AXES, TL::ROWS, ENTRY>(qpos, row0, a.Lq);
+        if constexpr (AXES > 0) pos_next.load(qpos, row0, a.Lq);
     };
     auto store = [&](int buf) {
         T* n = tiles + buf * 2 * TL::ELEMS;
         st.store(n, n + TL::ELEMS);
         if (tid < 2 * TL::ROWS) stats[buf * 2 * TL::ROWS + tid] = snext;
-        if constexpr (AXES > 0)
-            if (tid < AXES * TL::ROWS) pos[buf * AXES * TL::ROWS + tid] = pnext;
     };
     int lut_head = -1;
     if (t0 < t1) {
@@ -831,6 +861,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
+        if constexpr (AXES > 0) pos = pos_next;
         if (t + 1 < t1) load(t + 1);
         if constexpr (AXES > 0) {
             const int head = kvh * group + t / q_tiles;
@@ -842,7 +873,6 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
         }
         const T *qt = tiles + cur * 2 * TL::ELEMS, *gt = qt + TL::ELEMS;
         const float* start = stats + cur * 2 * TL::ROWS;
-        const int* pt = pos + cur * AXES * TL::ROWS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
             const T *qb = qt + nb * 32 * TL::LD, *gb = gt + nb * 32 * TL::LD;
@@ -857,13 +887,15 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
             for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(map.read_row(qb, ks), kf[ks], s);
 #pragma unroll
             for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(gb, ks), vf[ks], dp);
+            int off[AXES ? AXES : 1][16];
+#pragma unroll
+            for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], ka[x], off[x]);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float x;
                 if constexpr (AXES > 0) {
-                    const int r = nb * 32 + acc_row(i, h);
-                    x = __builtin_fmaf(s[i], a.scale_log2, lds_load<float>(med3(ka[0] - pt[r], lo[0], hi[0])));
-                    if constexpr (AXES > 1) x += lds_load<float>(med3(ka[AXES - 1] - pt[TL::ROWS + r], lo[AXES - 1], hi[AXES - 1]));
+                    x = __builtin_fmaf(s[i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
+                    if constexpr (AXES > 1) x += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
                 } else {
                     x = s[i] * a.scale_log2;
                 }
@@ -949,7 +981,7 @@ template <typename T, int DP, int AXES, bool TRAIN>
 int run_fwd_mode(const Args& a, hipStream_t s) {
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     static unsigned long long done = 0;
-    const size_t lds = tile_bytes<T, DP, R>() + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, a.pack);
+    const size_t lds = tile_bytes<T, DP, R>() + lut_bytes(a, AXES, a.pack);
     return start(fwd_kernel<T, DP, AXES, TRAIN>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, a, s);
 }
 
@@ -967,7 +999,7 @@ template <typename T, int DP, int AXES, int WAVES, bool HIST>
 int run_dq_mode(const Args& a, hipStream_t s) {
     constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
     static unsigned long long done = 0;
-    size_t lds = tile_bytes<T, DP, R>() + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, 1);
+    size_t lds = tile_bytes<T, DP, R>() + lut_bytes(a, AXES, 1);
     if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * 64 * WAVES;      // entries of 8 bytes
     return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
 }
@@ -988,7 +1020,7 @@ template <typename T, int DP, int AXES>
 int run_dkdv(const Args& a, hipStream_t s) {
     constexpr int R = sizeof(T) == 2 ? 64 : 32;
     static unsigned long long done = 0;
-    const size_t lds = tile_bytes<T, DP, R>() + sizeof(float) * 4 * R + sizeof(int) * 2 * AXES * R + lut_bytes(a, AXES, 1);
+    const size_t lds = tile_bytes<T, DP, R>() + sizeof(float) * 4 * R + lut_bytes(a, AXES, 1);
     return start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);
 }
 

@@ -153,9 +153,9 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
 # attention
 # ------------------------------------------------------------------------------------------------
 def _rows16(t):
-    """t itself if its rows are adjacent and start on 16 bytes with non-negative strides, else a dense copy."""
+    """t itself if its elements are adjacent, rows start on 16 bytes and are less than 2^23 elements apart, else a dense copy."""
     size = t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for n, s in zip(t.shape[:3], t.stride()[:3]) if n > 1):
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and t.stride(1) < 2 ** 23 and all(s * size % 16 == 0 for n, s in zip(t.shape[:3], t.stride()[:3]) if n > 1):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -31,15 +31,25 @@ bool rel_bias_args(RelBias& r, const char* who, const void* table, int type, con
 // gtable[row][h] = sum over parts of partial[h][part][row], row = a * buckets + n, in a fixed order and in 64 bits
 int rel_bias_join(const float* partial, void* gtable, int type, int H, int nrows, int64_t parts, const char* who, hipStream_t s);
 
+// The borders in LDS, for rel_bucket (kernel arguments with a lane's own index are memory reads, and all 64 in scalar registers displace
+// what the callers' loops need).  Called by all threads; ends with a barrier.
+__device__ __forceinline__ const int* rel_stage_borders(const RelBias& r) {
+    __shared__ int border[CAMLI_REL_MAX_BORDERS];
+    if (threadIdx.x < CAMLI_REL_MAX_BORDERS) border[threadIdx.x] = r.border[threadIdx.x];
+    __syncthreads();
+    return border;
+}
+
 // bucket of the clamped offset index i in 0 .. 2 limit
-__device__ __forceinline__ int rel_bucket(const RelBias& r, int i) {
+__device__ __forceinline__ int rel_bucket(const RelBias& r, const int* border, int i) {
     const int o = i - r.limit;
     const int d = r.two_sided ? abs(o) : max(-o, 0);
     int n = d;
     if (d >= r.exact) {
-        n = r.exact;
-#pragma unroll          // all of them: the borders come in a few wide scalar loads, a counted loop waits for each
-        for (int j = 0; j < CAMLI_REL_MAX_BORDERS; ++j) n += r.border[j] <= d ? 1 : 0;
+        int below = 0;          // borders at or below d, by bisection: at most 63 are in use, the others are INT_MAX
+#pragma unroll
+        for (int step = CAMLI_REL_MAX_BORDERS / 2; step >= 1; step >>= 1) below += border[below + step - 1] <= d ? step : 0;
+        n = r.exact + below;
     }
     return n + (r.two_sided && o > 0 ? r.side : 0);
 }

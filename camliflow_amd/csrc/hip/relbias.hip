@@ -18,8 +18,9 @@ template <typename T, int VEC, int AXES>
 __global__ __launch_bounds__(BLOCK) void rel_bias_fwd_kernel(RelBias r, T* __restrict__ out, int H, int Lq, int Lk, int cols) {
     extern __shared__ float tab[];
     const int h = blockIdx.z % H, b = blockIdx.z / H, tid = threadIdx.x, span = 2 * r.limit + 1;
+    const int* border = rel_stage_borders(r);
     for (int i = tid; i < span; i += BLOCK) {
-        const int n = rel_bucket(r, i);
+        const int n = rel_bucket(r, border, i);
 #pragma unroll
         for (int a = 0; a < AXES; ++a) tab[a * span + i] = load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + h);
     }
@@ -56,7 +57,8 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
     extern __shared__ float hist[];
     const int h = blockIdx.y, tid = threadIdx.x, span = 2 * r.limit + 1, nrows = AXES * r.buckets;
     unsigned short* lut = reinterpret_cast<unsigned short*>(hist + nrows * BLOCK);
-    for (int i = tid; i < span; i += BLOCK) lut[i] = (unsigned short)rel_bucket(r, i);
+    const int* border = rel_stage_borders(r);
+    for (int i = tid; i < span; i += BLOCK) lut[i] = (unsigned short)rel_bucket(r, border, i);
     for (int i = 0; i < nrows; ++i) hist[i * BLOCK + tid] = 0.0f;
     __syncthreads();
     char* column = reinterpret_cast<char*>(hist + tid);

@@ -207,30 +207,62 @@ __device__ __forceinline__ int xcd_contiguous(int id, int n) {
 }
 
 // The streamed pair of tiles on its way from memory: registers now, LDS later.  A row at or beyond `limit`, a masked row and columns
-// from D on become zeros (a masked row may hold anything, and 0 * NaN is NaN).
+// from D on become zeros (a masked row may hold anything, and 0 * NaN is NaN); a whole, unmasked tile skips those tests.
+// A thread's place in a tile is a 32-bit byte offset computed once (row strides are below 2^23 elements); the tile's base is uniform.
 template <typename T, int DP, int R, int THREADS>
 struct Stream {
     using TL = Tile<T, DP, R>;
     static constexpr int ALL = TL::ROWS * TL::CHUNKS, N = (ALL + THREADS - 1) / THREADS;      // the narrowest tile has chunks for half the threads
     static_assert(ALL % THREADS == 0 || N == 1, "a whole number of chunks a thread");
     chunk16 x[N], y[N];
+    unsigned at_x[N], at_y[N];
     unsigned keep;
+    bool whole;
 
-    __device__ __forceinline__ void load(const T* px, int64_t ldx, const T* py, int64_t ldy, int row0, int limit, int D, const unsigned char* mask) {
+    __device__ __forceinline__ void init(int64_t ldx, int64_t ldy) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int f = threadIdx.x + n * THREADS;
+            const unsigned c = (f % TL::CHUNKS) * 16;
+            at_x[n] = (unsigned)(f / TL::CHUNKS) * (unsigned)(ldx * (int)sizeof(T)) + c;
+            at_y[n] = (unsigned)(f / TL::CHUNKS) * (unsigned)(ldy * (int)sizeof(T)) + c;
+        }
+    }
+    // px, py: the tile's first row
+    __device__ __forceinline__ void load(const T* px, const T* py, int row0, int limit, int D, const unsigned char* mask) {
+        const char *bx = reinterpret_cast<const char*>(px), *by = reinterpret_cast<const char*>(py);
+        whole = ALL >= THREADS && row0 + TL::ROWS <= limit && D == DP && mask == nullptr;
+        if (whole) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                x[n] = *reinterpret_cast<const chunk16*>(bx + at_x[n]);
+                y[n] = *reinterpret_cast<const chunk16*>(by + at_y[n]);
+            }
+            return;
+        }
         keep = 0;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS, row = row0 + f / TL::CHUNKS, c = (f % TL::CHUNKS) * TL::E;
             x[n] = y[n] = chunk16{0, 0, 0, 0};
             if (row < limit && c < D && (ALL >= THREADS || f < ALL)) {
-                x[n] = *reinterpret_cast<const chunk16*>(px + row * ldx + c);
-                y[n] = *reinterpret_cast<const chunk16*>(py + row * ldy + c);
+                x[n] = *reinterpret_cast<const chunk16*>(bx + at_x[n]);
+                y[n] = *reinterpret_cast<const chunk16*>(by + at_y[n]);
                 keep |= (mask == nullptr || mask[row] != 0 ? 1u : 0u) << n;
             }
         }
     }
     __device__ __forceinline__ void store(T* tx, T* ty) const {
         const chunk16 zero = {0, 0, 0, 0};
+        if (whole) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int f = threadIdx.x + n * THREADS, at = TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS);
+                *reinterpret_cast<chunk16*>(tx + at) = x[n];
+                *reinterpret_cast<chunk16*>(ty + at) = y[n];
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS, at = TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS);
@@ -276,9 +308,11 @@ __device__ __forceinline__ int kept_length(const Args& a, int b) {
 
 // bit j: key row0 + j is kept.  Called by whole waves.
 __device__ __forceinline__ unsigned long long kept_bits(const unsigned char* mask, int row0, int len, int rows) {
+    const unsigned long long all = rows == 64 ? ~0ull : (1ull << rows) - 1;
+    if (mask == nullptr) return row0 + rows <= len ? all : (1ull << (len - row0)) - 1;      // row0 < len
     const int lane = threadIdx.x & 63, key = row0 + lane;
     bool k = lane < rows && key < len;
-    if (k && mask) k = mask[key] != 0;
+    if (k) k = mask[key] != 0;
     return __ballot(k);
 }
 
@@ -313,8 +347,9 @@ __device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 2
 template <int AXES, int THREADS>
 __device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0, int pack, int H) {
     const int span = 2 * r.limit + 1;
+    const int* border = rel_stage_borders(r);
     for (int i = threadIdx.x; i < span; i += THREADS) {
-        const int n = rel_bucket(r, i);
+        const int n = rel_bucket(r, border, i);
         for (int p = 0; p < pack; ++p)
 #pragma unroll
             for (int a = 0; a < AXES; ++a)
@@ -324,8 +359,9 @@ __device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0
 template <int AXES, int THREADS>
 __device__ __forceinline__ void fill_lut(const RelBias& r, Entry8* lut, int head, int row_bytes, int H) {
     const int span = 2 * r.limit + 1;
+    const int* border = rel_stage_borders(r);
     for (int i = threadIdx.x; i < span; i += THREADS) {
-        const int n = rel_bucket(r, i);
+        const int n = rel_bucket(r, border, i);
 #pragma unroll
         for (int a = 0; a < AXES; ++a)
             lut[a * span + i] = {load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + head) * LOG2E, (unsigned)((a * r.buckets + n) * row_bytes)};
@@ -440,9 +476,10 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
 
     Stream<T, DP, R, THREADS> st;
     StreamPos<AXES, TL::BLOCKS, ENTRY> pos, pos_next;
+    st.init(a.ks.l, a.vs.l);
     int cur = 0;
     if (t0 < t1) {
-        st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
+        st.load(kp + t0 * (int64_t)TL::ROWS * a.ks.l, vp + t0 * (int64_t)TL::ROWS * a.vs.l, t0 * TL::ROWS, len, a.D, mask);
         if constexpr (AXES > 0) pos_next.load(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
     }
@@ -451,7 +488,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
         const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
         if constexpr (AXES > 0) pos = pos_next;
         if (t + 1 < t1) {
-            st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
+            st.load(kp + (t + 1) * (int64_t)TL::ROWS * a.ks.l, vp + (t + 1) * (int64_t)TL::ROWS * a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
             if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
@@ -691,9 +728,10 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
 
     Stream<T, DP, R, THREADS> st;
     StreamPos<AXES, TL::BLOCKS, ENTRY> pos, pos_next;
+    st.init(a.ks.l, a.vs.l);
     int cur = 0;
     if (t0 < t1) {
-        st.load(kp, a.ks.l, vp, a.vs.l, t0 * TL::ROWS, len, a.D, mask);
+        st.load(kp + t0 * (int64_t)TL::ROWS * a.ks.l, vp + t0 * (int64_t)TL::ROWS * a.vs.l, t0 * TL::ROWS, len, a.D, mask);
         if constexpr (AXES > 0) pos_next.load(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
     }
@@ -702,7 +740,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
         const unsigned long long bits = kept_bits(mask, t * TL::ROWS, len, TL::ROWS);
         if constexpr (AXES > 0) pos = pos_next;
         if (t + 1 < t1) {
-            st.load(kp, a.ks.l, vp, a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
+            st.load(kp + (t + 1) * (int64_t)TL::ROWS * a.ks.l, vp + (t + 1) * (int64_t)TL::ROWS * a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
             if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
         const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
@@ -834,12 +872,13 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     if (rt * 128 >= len) t1 = t0;        // no key of this workgroup is kept: zeros
     Stream<T, DP, R, THREADS> st;
     StreamPos<AXES, TL::BLOCKS, -ENTRY> pos, pos_next;
+    st.init(a.qs.l, (int64_t)a.H * a.D);
     float snext = 0.0f;
     int cur = 0;
     auto load = [&](int t) {
         const int head = kvh * group + t / q_tiles, row0 = (t % q_tiles) * TL::ROWS;
-        st.load(static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h, a.qs.l, static_cast<const T*>(a.go) + ((int64_t)b * a.Lq * a.H + head) * a.D,
-                (int64_t)a.H * a.D, row0, a.Lq, a.D, nullptr);
+        st.load(static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h + row0 * a.qs.l,
+                static_cast<const T*>(a.go) + (((int64_t)b * a.Lq + row0) * a.H + head) * a.D, row0, a.Lq, a.D, nullptr);
         if (tid < 2 * TL::ROWS) {
             const int r = row0 + tid % TL::ROWS;
             const float* src = tid < TL::ROWS ? a.lse : a.delta;
@@ -960,7 +999,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(SumJobs jobs) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ launches
-constexpr size_t MAX_LDS = 160 * 1024;
+constexpr size_t MAX_LDS = 159 * 1024;      // of a CU's 160 KB; the bias borders are static
 
 template <typename T, int DP, int R>
 constexpr size_t tile_bytes() { return 4 * sizeof(T) * Tile<T, DP, R>::ELEMS; }

@@ -48,7 +48,7 @@ bool operand_ok(const void* p, const int64_t* stride, int size) {
     if (!p || ((uintptr_t)p & 15)) return false;
     for (int i = 0; i < 3; ++i)
         if (stride[i] < 0 || (stride[i] * size) & 15) return false;
-    return true;
+    return stride[1] < (1 << 23);       // a thread's place in a tile of 64 rows is a 32-bit byte offset
 }
 
 // false (with the error set) for anything the kernels do not take
@@ -63,12 +63,12 @@ bool make_args(Args& a, const camli_attention* d, const char* who) {
     const int size = camli_type_size(d->type);
     // grid sizes and element counts of a workgroup's own arithmetic stay below 2^31
     if ((int64_t)d->B * d->H * ((int64_t)camli_divup(d->Lq, 32) + 1024) > INT32_MAX || (int64_t)d->B * d->Hk * ((int64_t)camli_divup(d->Lk, 128) + 1024) > INT32_MAX ||
-        (int64_t)camli_divup(d->Lq, 32) * (d->H / d->Hk) > INT32_MAX / 64 || d->Lq > INT32_MAX - 256 || d->Lk > INT32_MAX - 256) {
+        (int64_t)camli_divup(d->Lq, 32) * (d->H / d->Hk) > INT32_MAX / 64 || (int64_t)d->H * d->D >= (1 << 23) || d->Lq > INT32_MAX - 256 || d->Lk > INT32_MAX - 256) {
         camli_set_error("%s: B * H * Lq or B * Hk * Lk too large", who);
         return false;
     }
     if (!operand_ok(d->q, d->q_stride, size) || !operand_ok(d->k, d->k_stride, size) || !operand_ok(d->v, d->v_stride, size)) {
-        camli_set_error("%s: q, k, v need 16-byte aligned addresses and non-negative strides of whole 16 bytes", who);
+        camli_set_error("%s: q, k, v need 16-byte aligned addresses and non-negative strides of whole 16 bytes, row strides below 2^23 elements", who);
         return false;
     }
     a = Args{};

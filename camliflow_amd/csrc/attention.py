@@ -140,8 +140,8 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
     the same bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
     name = 'relative_position_bias'
     table, q_pos, k_pos, batch, _ = _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, table.dtype if table is not None else None)
-    if (batch or 1) * table.shape[2] > 65535 or q_pos.shape[-2] > 2000000 or k_pos.shape[-2] >= 2 ** 31 - 2 ** 16:
-        raise ValueError('%s: more than 65535 samples x heads, 2000000 queries or 2^31 keys' % name)
+    if (batch or 1) * table.shape[2] > 65535 or q_pos.shape[-2] > 2000000 or k_pos.shape[-2] > 16000000:
+        raise ValueError('%s: more than 65535 samples x heads, 2000000 queries or 16000000 keys' % name)
     if not cpp_impl:
         return _composed_bias(table, q_pos, k_pos, bidirectional, int(max_distance)).to(table.dtype)
     _require_cuda(name, table)

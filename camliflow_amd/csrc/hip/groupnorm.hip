@@ -12,6 +12,8 @@
 //   stats   one workgroup per (sample, chunk of pixels), all channels: thread = 16 bytes of channels x every rows-th pixel.  Each
 //           thread sums (x - pivot) and its square about ITS first value, so a mean far from zero costs no digits; threads, channels
 //           and chunks are joined as (count, mean, M2) triples in a fixed order -- no atomics, the same bits on every run.
+//   small   a group of at most 16384 values whose channels fit whole vectors: one workgroup of 1024 threads per (sample, group) holds it in
+//           registers, so one launch and one reading do (1 x 128 x 17 x 30 fp32: 12 -> 6 us on the GPU).
 //   apply   the workgroup joins its sample's chunk triples (a few KB from L2) and writes its chunk.  It takes the chunks in the
 //           reverse of the order in which stats read them, so that what stats read last is still in the last-level cache.
 //   sums    (backward) per channel sum dz and sum dz xhat of a chunk;  finish: joins the chunks per channel and group;
@@ -29,6 +31,7 @@ struct GnArgs {
     const void *weight, *bias;
     int wtype;
     int C, G, P, chunks, chunk_px, act;
+    bool stream;              // the map is larger than the caches: its second reading and the result are not kept in them
     float eps;
 };
 
@@ -175,11 +178,75 @@ __global__ __launch_bounds__(BLOCK) void gn_apply_kernel(GnArgs a, const float2*
 #pragma unroll 4
         for (int p = r; p < len; p += rows) {
             float v[VEC];
-            load_f32<T, VEC>(xb + (int64_t)p * a.x_ld + c, v);
+            load_f32<T, VEC>(xb + (int64_t)p * a.x_ld + c, v, a.stream);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = act_value(__builtin_fmaf(v[e] - mean[e], scale[e], shift[e]), a.act);
-            store_f32<T, VEC>(yb + (int64_t)p * a.C + c, v);
+            store_f32<T, VEC>(yb + (int64_t)p * a.C + c, v, a.stream);
         }
+    }
+}
+
+constexpr int SMALL_THREADS = 1024, SMALL_VALUES = 16;       // per thread
+
+__device__ __forceinline__ float block_sum_1024(float v, float* red) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float t = red[threadIdx.x & 15];
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) t += __shfl_xor(t, off, CAMLI_WAVE);
+    __syncthreads();
+    return t;
+}
+
+// grid (G, B)
+template <typename T, int VEC>
+__global__ __launch_bounds__(SMALL_THREADS) void gn_small_kernel(GnArgs a, T* __restrict__ y, float2* __restrict__ stat_out) {
+    __shared__ float red[SMALL_THREADS / 64];
+    constexpr int N = SMALL_VALUES / VEC;
+    const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, cpg = a.C / a.G;
+    const int w = cpg / VEC, rows = SMALL_THREADS / w, r = tid / w, c = g * cpg + (tid - r * w) * VEC;
+    const T* xb = static_cast<const T*>(a.x) + b * a.x_bs + c;
+    float v[N][VEC], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int p = r + i * rows;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
+        if (r < rows && p < a.P) load_f32<T, VEC>(xb + (int64_t)p * a.x_ld, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += v[i][e];
+    const float n = (float)a.P * (float)cpg, mean = block_sum_1024(sum, red) / n;
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (r < rows && r + i * rows < a.P) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[i][e] -= mean;
+                sum = __builtin_fmaf(v[i][e], v[i][e], sum);
+            }
+        }
+    const float rstd = 1.0f / sqrtf(block_sum_1024(sum, red) / n + a.eps);
+    if (stat_out && tid == 0) stat_out[(int64_t)b * a.G + g] = make_float2(mean, rstd);
+    if (r >= rows) return;
+    float scale[VEC], shift[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        scale[e] = a.weight ? rstd * load_param(a.weight, a.wtype, c + e) : rstd;
+        shift[e] = a.bias ? load_param(a.bias, a.wtype, c + e) : 0.0f;
+    }
+    T* yb = y + (int64_t)b * a.P * a.C + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int p = r + i * rows;
+        if (p >= a.P) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = act_value(__builtin_fmaf(v[i][e], scale[e], shift[e]), a.act);
+        store_f32<T, VEC>(yb + (int64_t)p * a.C, v[i]);
     }
 }
 
@@ -315,25 +382,28 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_dx_kernel(GnArgs a, const T* __r
 #pragma unroll 2
         for (int p = r; p < len; p += rows) {
             float v[VEC], g[VEC];
-            load_f32<T, VEC>(xb + (int64_t)p * a.x_ld + c, v);
-            load_f32<T, VEC>(gy + dense + (int64_t)p * a.C + c, g);
+            load_f32<T, VEC>(xb + (int64_t)p * a.x_ld + c, v, a.stream);
+            load_f32<T, VEC>(gy + dense + (int64_t)p * a.C + c, g, a.stream);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float d = v[e] - mean[e], xhat = d * rstd[e];
                 const float dz = g[e] * act_slope(__builtin_fmaf(d, rstd[e] * wt[e], shift[e]), a.act);
                 v[e] = rstd[e] * (__builtin_fmaf(wt[e], dz, -m0[e]) - xhat * m1[e]);
             }
-            store_f32<T, VEC>(gx + dense + (int64_t)p * a.C + c, v);
+            store_f32<T, VEC>(gx + dense + (int64_t)p * a.C + c, v, a.stream);
         }
     }
 }
 
-// Chunks per sample: enough workgroups for four per CU, but at least 8 KB of the map in each (below that the fixed cost of a
-// workgroup shows), and at most 256 (every apply workgroup reads its sample's chunk moments).
+// Chunks per sample.  A workgroup has a fixed cost (its tree of sums, in apply the joining of its sample's chunk moments), a small map needs
+// workgroups more than long ones: 32 KB of the map each, but 256 workgroups at least and 2048 at most, none below 8 KB, and at most 256
+// a sample.  (8 x 128 x 68 x 120 fp32, 36 MB: apply 24 us with 2048 workgroups, 17 with 1024; 267 MB: stats 58 us with 2048, 75 with 1024.)
 int gn_chunk_px(int B, int C, int P, int type) {
-    const int64_t px_bytes = (int64_t)C * camli_type_size(type);
+    const int64_t px_bytes = (int64_t)C * camli_type_size(type), total = px_bytes * P * B;
+    int64_t want = total >> 15;
+    want = want < 256 ? 256 : want > 2048 ? 2048 : want;
+    want = (want + B - 1) / B < 256 ? (want + B - 1) / B : 256;
     int64_t px = (8192 + px_bytes - 1) / px_bytes;
-    const int64_t want = (1024 + B - 1) / B < 256 ? (1024 + B - 1) / B : 256;
     const int64_t even = (P + want - 1) / want;
     if (px < even) px = even;
     return (int)(px < P ? px : P);
@@ -358,11 +428,19 @@ GnArgs make_args(const void* x, int64_t x_bs, int64_t x_ld, const void* weight, 
     a.C = C; a.G = G; a.P = P; a.act = act; a.eps = eps;
     a.chunk_px = gn_chunk_px(B, C, P, type);
     a.chunks = camli_divup(P, a.chunk_px);
+    // half of the 256 MB last-level cache.  At 16 x 64 x 272 x 480 bf16 (267 MB) keeping nothing of the result leaves what the first
+    // reading brought for the second: 196 -> 161 us forward, 305 -> 285 us backward; a smaller map is left for its next reader.
+    a.stream = (int64_t)B * P * C * camli_type_size(type) >= ((int64_t)128 << 20);
     return a;
 }
 
 template <typename T, int VEC>
 int run_fwd(const GnArgs& a, void* y, float2* stat, float2* partial, int B, hipStream_t s) {
+    const int cpg = a.C / a.G, w = cpg / VEC;
+    if (cpg % VEC == 0 && w <= SMALL_THREADS && (int64_t)a.P <= (int64_t)(SMALL_THREADS / w) * (SMALL_VALUES / VEC)) {
+        gn_small_kernel<T, VEC><<<dim3(a.G, B), SMALL_THREADS, 0, s>>>(a, static_cast<T*>(y), stat);
+        return camli_check_launch("camli_group_norm_fwd");
+    }
     const size_t lds = sizeof(float2) * ((size_t)a.C + BLOCK * VEC);
     gn_stats_kernel<T, VEC><<<dim3(a.chunks, B), BLOCK, lds, s>>>(a, partial);
     gn_apply_kernel<T, VEC><<<dim3(a.chunks, B), BLOCK, sizeof(float2) * a.G, s>>>(a, partial, static_cast<T*>(y), stat);

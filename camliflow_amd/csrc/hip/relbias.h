@@ -8,7 +8,7 @@
 // kernel arguments, so no call uploads anything and a captured graph holds everything it needs.
 //
 // Offsets beyond +-limit share the bucket of the limit: a workgroup expands its heads' table columns to one float per offset in
-// LDS (2 limit + 1 entries), and the bias of a pair is subtract, clamp, one LDS read.
+// LDS (2 limit + 1 entries).
 #pragma once
 #include "typed.h"
 
@@ -54,11 +54,23 @@ __device__ __forceinline__ int rel_bucket(const RelBias& r, const int* border, i
     return n + (r.two_sided && o > 0 ? r.side : 0);
 }
 
-// offset index of a pair: saturating, so positions of any size are safe
-__device__ __forceinline__ int rel_index(int kpos, int qpos, int limit) {
-    const int o = __builtin_elementwise_sub_sat(kpos, qpos);
-    return min(max(o, -limit), limit) + limit;
+// A pair's table entry in LDS by one addition and one clamp.  Positions are held as multiples of the entry size (scaled once per row, not
+// per pair), one side negated and carrying the address of the table's middle.  Positions beyond +-2^26 count as that, so that no
+// difference overflows.
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
+template <typename V>
+__device__ __forceinline__ V lds_load(int address) {
+    return *(__attribute__((address_space(3))) const V*)(uintptr_t)(unsigned)address;
+}
+__device__ __forceinline__ int med3(int x, int lo, int hi) {
+    int r;
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(lo), "v"(hi));
+    return r;
+}
+template <int SCALE>
+__device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 26)), 1 << 26) * SCALE; }
 
 // Two additions to a thread's own histogram column, per axis, at byte offsets.  Plain reads and writes, because nobody else touches the
 // column: an LDS float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a dependent

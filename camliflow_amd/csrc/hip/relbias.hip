@@ -28,74 +28,102 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_fwd_kernel(RelBias r, T* __res
     const int tx = tid % cols, ty = tid / cols, per = BLOCK / cols;
     const int j = (blockIdx.x * cols + tx) * VEC;
     if (j >= Lk) return;
-    int kp[AXES][VEC];
+    int kp[AXES][VEC], lo[AXES], hi[AXES];
     const int* kpos = r.kpos + b * r.kpos_bs;
     const int* qpos = r.qpos + b * r.qpos_bs;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
+    for (int a = 0; a < AXES; ++a) {
+        const int centre = (int)lds_address(tab + a * span + r.limit);
+        lo[a] = centre - 4 * r.limit;
+        hi[a] = centre + 4 * r.limit;
 #pragma unroll
-        for (int a = 0; a < AXES; ++a) kp[a][e] = kpos[(int64_t)(j + e) * AXES + a];
+        for (int e = 0; e < VEC; ++e) kp[a][e] = centre + scale_pos<4>(kpos[(int64_t)(j + e) * AXES + a]);
+    }
     const int i1 = min(Lq, ((int)blockIdx.y + 1) * ROWS * per);
     for (int i = blockIdx.y * ROWS * per + ty; i < i1; i += per) {
         float v[VEC];
         int qp[AXES];
 #pragma unroll
-        for (int a = 0; a < AXES; ++a) qp[a] = qpos[(int64_t)i * AXES + a];
+        for (int a = 0; a < AXES; ++a) qp[a] = scale_pos<4>(qpos[(int64_t)i * AXES + a]);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            v[e] = tab[rel_index(kp[0][e], qp[0], r.limit)];
-            if (AXES > 1) v[e] += tab[span + rel_index(kp[AXES - 1][e], qp[AXES - 1], r.limit)];
+            v[e] = lds_load<float>(med3(kp[0][e] - qp[0], lo[0], hi[0]));
+            if (AXES > 1) v[e] += lds_load<float>(med3(kp[AXES - 1][e] - qp[AXES - 1], lo[AXES - 1], hi[AXES - 1]));
         }
         store_f32<T, VEC>(out + ((int64_t)blockIdx.z * Lq + i) * Lk + j, v);
     }
 }
 
-// dynamic LDS: float hist[axes * buckets][BLOCK], then unsigned short bucket[2 limit + 1].  grid (workgroups, H)
+// dynamic LDS: float hist[axes * buckets][BLOCK], then unsigned short bucket[2 limit + 1] (two bytes an entry: the usual tables fit one
+// dword per bank, so lanes with different offsets do not collide).
+// grid (row parts, column tiles, H): as in the forward a thread keeps its columns' positions in registers and walks over rows; the next
+// row's gradient is on its way while one is added.
 template <typename T, int VEC, int AXES>
 __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T* __restrict__ g, float* __restrict__ partial, int H, int Lq,
                                                              int Lk, int64_t rows, int cols) {
     extern __shared__ float hist[];
-    const int h = blockIdx.y, tid = threadIdx.x, span = 2 * r.limit + 1, nrows = AXES * r.buckets;
-    unsigned short* lut = reinterpret_cast<unsigned short*>(hist + nrows * BLOCK);
+    const int h = blockIdx.z, tid = threadIdx.x, span = 2 * r.limit + 1, nrows = AXES * r.buckets;
+    unsigned short* bucket = reinterpret_cast<unsigned short*>(hist + nrows * BLOCK);
     const int* border = rel_stage_borders(r);
-    for (int i = tid; i < span; i += BLOCK) lut[i] = (unsigned short)rel_bucket(r, border, i);
+    for (int i = tid; i < span; i += BLOCK) bucket[i] = (unsigned short)rel_bucket(r, border, i);
     for (int i = 0; i < nrows; ++i) hist[i * BLOCK + tid] = 0.0f;
     __syncthreads();
     char* column = reinterpret_cast<char*>(hist + tid);
-    const int tx = tid % cols, ty = tid / cols, per = BLOCK / cols;
-    for (int64_t row = (int64_t)blockIdx.x * per + ty; row < rows && ty < per; row += (int64_t)gridDim.x * per) {
-        const int b = (int)(row / Lq), i = (int)(row - (int64_t)b * Lq);
-        const int* kpos = r.kpos + b * r.kpos_bs;
-        int qp[AXES];
+    const int tx = tid % cols, ty = tid / cols, per = BLOCK / cols, j = (blockIdx.y * cols + tx) * VEC;
+    const int64_t first = (int64_t)blockIdx.x * per + ty;
+    const int step = gridDim.x * per;
+    if (j < Lk && first < rows) {
+        const int centre = (int)lds_address(bucket + r.limit), lo = centre - 2 * r.limit, hi = centre + 2 * r.limit, B = (int)(rows / Lq);
+        int b = (int)(first / Lq), i = (int)(first - (int64_t)b * Lq), of = -1;      // of: the sample whose positions kp holds
+        int kp[AXES][VEC], q[AXES];
+        float v[VEC];
+        load_f32<T, VEC>(g + (((int64_t)b * H + h) * Lq + i) * Lk + j, v);
 #pragma unroll
-        for (int a = 0; a < AXES; ++a) qp[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + a];
-        const T* gr = g + (((int64_t)b * H + h) * Lq + i) * Lk;
-        for (int j = tx * VEC; j < Lk; j += cols * VEC) {
-            float v[VEC];
-            unsigned n[VEC][AXES];
-            load_f32<T, VEC>(gr + j, v);
+        for (int a = 0; a < AXES; ++a) q[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + a];
+        while (b < B) {
+            float now[VEC];
+            int qs[AXES];
+            const int sample = b;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
+            for (int e = 0; e < VEC; ++e) now[e] = v[e];
+#pragma unroll
+            for (int a = 0; a < AXES; ++a) qs[a] = scale_pos<2>(q[a]);
+            for (i += step; i >= Lq; i -= Lq) ++b;
+            if (b < B) {
+                load_f32<T, VEC>(g + (((int64_t)b * H + h) * Lq + i) * Lk + j, v);
+#pragma unroll
+                for (int a = 0; a < AXES; ++a) q[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + a];
+            }
+            if (sample != of) {
+                of = sample;
 #pragma unroll
                 for (int a = 0; a < AXES; ++a)
-                    n[e][a] = (lut[rel_index(kpos[(int64_t)(j + e) * AXES + a], qp[a], r.limit)] + a * r.buckets) * BLOCK * sizeof(float);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) kp[a][e] = centre + scale_pos<2>(r.kpos[sample * r.kpos_bs + (int64_t)(j + e) * AXES + a]);
+            }
+            unsigned n[VEC][AXES];
+#pragma unroll
+            for (int a = 0; a < AXES; ++a)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) n[e][a] = (a * r.buckets + lds_load<unsigned short>(med3(kp[a][e] - qs[a], lo, hi))) * (BLOCK * (unsigned)sizeof(float));
             if constexpr (VEC > 1) {
 #pragma unroll
-                for (int e = 0; e < VEC; e += 2) hist_add2<AXES>(column, n[e], v[e], n[e + 1], v[e + 1]);
+                for (int e = 0; e < VEC; e += 2) hist_add2<AXES>(column, n[e], now[e], n[e + 1], now[e + 1]);
             } else {
 #pragma unroll
-                for (int a = 0; a < AXES; ++a) *reinterpret_cast<float*>(column + n[0][a]) += v[0];
+                for (int a = 0; a < AXES; ++a) *reinterpret_cast<float*>(column + n[0][a]) += now[0];
             }
         }
     }
     __syncthreads();
     const int wave = tid >> 6, lane = tid & 63;
+    const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, parts = (int64_t)gridDim.x * gridDim.y;
     for (int n = wave; n < nrows; n += BLOCK / 64) {
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < BLOCK / 64; ++k) s += hist[n * BLOCK + k * 64 + lane];
         s = wave_sum(s);
-        if (lane == 0) partial[((int64_t)h * gridDim.x + blockIdx.x) * nrows + n] = s;
+        if (lane == 0) partial[(h * parts + part) * nrows + n] = s;
     }
 }
 
@@ -176,12 +204,12 @@ int pow2_cols(int n) {      // threads along a row: the power of two that covers
     return c;
 }
 
+// row parts per column tile: 512 workgroups (two per CU fit beside each other), but 16 row groups in each: a workgroup pays for its table
+// and for clearing and adding up its histogram
 int bwd_parts(int64_t rows, int Lk, int H, int vec) {
-    const int per = BLOCK / pow2_cols(camli_divup(Lk, vec));
-    const int64_t blocks = (rows + per - 1) / per;
-    const int64_t most = H < 512 ? (1024 + H - 1) / H : 2;
-    const int64_t few = (blocks + 3) / 4;      // four row groups a workgroup at least: each pays for clearing its histogram
-    return (int)(few < 1 ? 1 : few < most ? few : most);
+    const int cols = pow2_cols(camli_divup(Lk, vec)), per = BLOCK / cols, tiles = camli_divup(Lk, cols * vec);
+    const int64_t most = (512 + (int64_t)H * tiles - 1) / ((int64_t)H * tiles), few = ((rows + per - 1) / per + 15) / 16;
+    return (int)(few < most ? few : most);
 }
 
 template <typename T, int VEC, int AXES>
@@ -201,14 +229,15 @@ int bwd(const RelBias& r, const void* g, void* gtable, float* ws, int B, int H, 
     }
     const int64_t rows = (int64_t)B * Lq;
     const int nrows = AXES * r.buckets, cols = pow2_cols(camli_divup(Lk, VEC)), parts = bwd_parts(rows, Lk, H, VEC);
+    const int tiles = camli_divup(Lk, cols * VEC);
     const size_t lds = sizeof(float) * nrows * BLOCK + 2 * (2 * r.limit + 2);
-    rel_bias_bwd_kernel<T, VEC, AXES><<<dim3(parts, H), BLOCK, lds, s>>>(r, static_cast<const T*>(g), ws, H, Lq, Lk, rows, cols);
-    return rel_bias_join(ws, gtable, r.type, H, nrows, parts, "camli_rel_bias_bwd", s);
+    rel_bias_bwd_kernel<T, VEC, AXES><<<dim3(parts, tiles, H), BLOCK, lds, s>>>(r, static_cast<const T*>(g), ws, H, Lq, Lk, rows, cols);
+    return rel_bias_join(ws, gtable, r.type, H, nrows, (int64_t)parts * tiles, "camli_rel_bias_bwd", s);
 }
 
 bool sizes_ok(int B, int H, int Lq, int Lk, const char* who) {
-    if (B < 1 || H < 1 || Lq < 1 || Lk < 1 || (int64_t)B * H > 65535 || Lq > 2000000) {
-        camli_set_error("%s: need B, H, Lq, Lk >= 1, B * H <= 65535, Lq <= 2000000 (B=%d H=%d Lq=%d Lk=%d)", who, B, H, Lq, Lk);
+    if (B < 1 || H < 1 || Lq < 1 || Lk < 1 || (int64_t)B * H > 65535 || Lq > 2000000 || Lk > 16000000) {
+        camli_set_error("%s: need B, H, Lq, Lk >= 1, B * H <= 65535, Lq <= 2000000, Lk <= 16000000 (B=%d H=%d Lq=%d Lk=%d)", who, B, H, Lq, Lk);
         return false;
     }
     return true;
@@ -258,7 +287,9 @@ extern "C" int64_t camli_rel_bias_bwd_workspace_bytes(int B, int H, int Lq, int 
     if (!sizes_ok(B, H, Lq, Lk, "camli_rel_bias_bwd_workspace_bytes") || axes < 1 || axes > 2 || buckets < 1 || type < 0 || type > 2) return 0;
     const int vec = 16 / camli_type_size(type);
     const int64_t rows = (int64_t)B * Lq;
-    const int a = bwd_parts(rows, Lk, H, vec), c = bwd_parts(rows, Lk, H, 1);      // whichever form the alignment allows
+    // whichever form the alignment allows
+    const int64_t a = (int64_t)bwd_parts(rows, Lk, H, vec) * camli_divup(Lk, pow2_cols(camli_divup(Lk, vec)) * vec);
+    const int64_t c = (int64_t)bwd_parts(rows, Lk, H, 1) * camli_divup(Lk, pow2_cols(Lk));
     return (int64_t)sizeof(float) * H * (a > c ? a : c) * axes * buckets;
 }
 

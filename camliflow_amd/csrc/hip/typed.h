@@ -30,6 +30,37 @@ __device__ __forceinline__ void store_f32(T* p, const float (&in)[N]) {
     *reinterpret_cast<TypedVec<T, N>*>(p) = t;
 }
 
+typedef unsigned vec16_t __attribute__((ext_vector_type(4)));
+
+// as load_f32 / store_f32, with a choice of not keeping the line in the caches
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T* p, float (&out)[N], bool stream) {
+    if constexpr (sizeof(T) * N == 16) {
+        if (stream) {
+            union { TypedVec<T, N> t; vec16_t u; } v;
+            v.u = __builtin_nontemporal_load(reinterpret_cast<const vec16_t*>(p));
+#pragma unroll
+            for (int i = 0; i < N; ++i) out[i] = (float)v.t.v[i];
+            return;
+        }
+    }
+    load_f32<T, N>(p, out);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T* p, const float (&in)[N], bool stream) {
+    if constexpr (sizeof(T) * N == 16) {
+        if (stream) {
+            union { TypedVec<T, N> t; vec16_t u; } v;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v.t.v[i] = (T)in[i];
+            __builtin_nontemporal_store(v.u, reinterpret_cast<vec16_t*>(p));
+            return;
+        }
+    }
+    store_f32<T, N>(p, in);
+}
+
 // element i of a small parameter vector whose type is a run-time code
 __device__ __forceinline__ float load_param(const void* p, int type, int64_t i) {
     if (type == CAMLI_F32) return static_cast<const float*>(p)[i];

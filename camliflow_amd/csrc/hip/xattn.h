@@ -199,11 +199,22 @@ __device__ __forceinline__ float other_half(float x) {
 __device__ __forceinline__ float half_max(float x) { return fmaxf(x, other_half(x)); }
 __device__ __forceinline__ float half_sum(float x) { return x + other_half(x); }
 
-// Workgroups go round-robin over the 8 XCDs: give each XCD a contiguous range of work, so that the workgroups which stream the same
-// keys and values (or queries) share one L2.
-__device__ __forceinline__ int xcd_contiguous(int id, int n) {
-    const int x = id & 7, per = n >> 3, rem = n & 7;
-    return x * per + min(x, rem) + (id >> 3);
+// Workgroups go round-robin over the 8 XCDs.  The `chunk` workgroups of a unit (a sample's head: they stream the same keys and values, or
+// queries) are kept on one XCD, so that they share its L2, and units alternate between the XCDs, so that samples of different lengths
+// spread over them (contiguous ranges of samples per XCD took twice as long with lengths from 0 to 16384).
+__device__ __forceinline__ int unit_per_xcd(int id, int n, int chunk) {
+    const int units = n / chunk, full = (units >> 3) * 8 * chunk;
+    int unit, k;
+    if (id < full) {
+        const int group = id / (8 * chunk), rem = id - group * 8 * chunk;
+        unit = group * 8 + (rem & 7);
+        k = rem >> 3;
+    } else {
+        const int left = units & 7, rem = id - full;
+        unit = units - left + rem % left;
+        k = rem / left;
+    }
+    return unit * chunk + k;
 }
 
 // The streamed pair of tiles on its way from memory: registers now, LDS later.  A row at or beyond `limit`, a masked row and columns
@@ -318,30 +329,12 @@ __device__ __forceinline__ unsigned long long kept_bits(const unsigned char* mas
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// The bias of a pair from LDS.  Positions are held as multiples of the entry size (scaled once per row, not per pair), query positions
-// negated, and the owned row's carries the address of its table's middle: one addition and one clamp of a pair give the LDS
-// address of its entry.
-// Positions beyond +-2^26 count as that, so that no difference overflows.
+// The bias of a pair comes from a table in LDS (rel_bias: relbias.h); query positions are the negated side.
 // Entries: the bias (log2 domain), and for the table's gradient beside it where the bucket's row of the histogram starts.
 struct Entry8 {
     float bias;
     unsigned hist;
 };
-
-__device__ __forceinline__ unsigned lds_address(const void* p) {
-    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
-}
-template <typename V>
-__device__ __forceinline__ V lds_load(int address) {
-    return *(__attribute__((address_space(3))) const V*)(uintptr_t)(unsigned)address;
-}
-__device__ __forceinline__ int med3(int x, int lo, int hi) {
-    int r;
-    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(lo), "v"(hi));
-    return r;
-}
-template <int SCALE>
-__device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 26)), 1 << 26) * SCALE; }
 
 // tables of `pack` heads: lut[p][axis][2 limit + 1]
 template <int AXES, int THREADS>
@@ -431,7 +424,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     float* lut = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    int id = unit_per_xcd(blockIdx.x, gridDim.x, a.row_tiles * a.splits);
     const int groups = a.H / a.pack;
     const int split = id % a.splits;
     id /= a.splits;
@@ -646,7 +639,8 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
 // ------------------------------------------------------------------------------------------------------------ dq
 // WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, then
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
-// HIST: with the table's gradient; its tiles are 32 rows, so that two workgroups still share a CU beside their histograms.
+// HIST: with the table's gradient; its tiles are 32 rows in one buffer, so that two workgroups still share a CU beside their histograms
+// (one waits at a barrier while the other computes).
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
 __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
@@ -656,12 +650,12 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
     constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = (int)sizeof(Entry);
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);
-    Entry* lut = reinterpret_cast<Entry*>(tiles + 4 * TL::ELEMS);
+    Entry* lut = reinterpret_cast<Entry*>(tiles + (HIST ? 2 : 4) * TL::ELEMS);
     const int span = 2 * a.rb.limit + 1, hist_rows = AXES * a.rb.buckets;
     float* hist = reinterpret_cast<float*>(lut + AXES * span);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    int id = unit_per_xcd(blockIdx.x, gridDim.x, a.row_tiles * a.splits);
     const int split = id % a.splits;
     id /= a.splits;
     const int rt = id % a.row_tiles;
@@ -743,7 +737,7 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
             st.load(kp + (t + 1) * (int64_t)TL::ROWS * a.ks.l, vp + (t + 1) * (int64_t)TL::ROWS * a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
             if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
-        const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
+        const T *kt = HIST ? tiles : tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
             const unsigned half = (unsigned)(bits >> (nb * 32));
@@ -798,8 +792,9 @@ __global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
                 for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = Mat<T>::mma(map.read_col(kb, ps, d), p, dq[d]);
             }
         }
+        if constexpr (HIST) __syncthreads();
         if (t + 1 < t1) {
-            T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
+            T* nk = HIST ? tiles : tiles + (cur ^ 1) * 2 * TL::ELEMS;
             st.store(nk, nk + TL::ELEMS);
         }
         __syncthreads();
@@ -834,7 +829,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     float* lut = reinterpret_cast<float*>(stats + 4 * TL::ROWS);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    int id = unit_per_xcd(blockIdx.x, gridDim.x, a.row_tiles * a.splits);
     const int split = id % a.splits;
     id /= a.splits;
     const int rt = id % a.row_tiles;
@@ -1038,7 +1033,7 @@ template <typename T, int DP, int AXES, int WAVES, bool HIST>
 int run_dq_mode(const Args& a, hipStream_t s) {
     constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
     static unsigned long long done = 0;
-    size_t lds = tile_bytes<T, DP, R>() + lut_bytes(a, AXES, 1);
+    size_t lds = tile_bytes<T, DP, R>() / (HIST ? 2 : 1) + lut_bytes(a, AXES, 1);
     if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * 64 * WAVES;      // entries of 8 bytes
     return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
 }

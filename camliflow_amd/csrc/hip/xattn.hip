@@ -26,7 +26,9 @@ void plan_fwd(Args& a, int type, int axes) {
     // values are then read once, not once per head
     a.pack = group > 1 && (int64_t)a.Lq * group <= 128 && xattn::lut_bytes(a, axes, group) <= 16384 ? group : 1;
     a.row_tiles = camli_divup(a.pack * a.Lq, 128);
-    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile_rows(type)), 1024, 4);
+    // one wave of rows: the pieces are short, bound by latency, and cost little to join
+    const int least = a.pack * (int64_t)a.Lq <= 32 ? 2 : 4;
+    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile_rows(type)), 1024, least);
 }
 
 int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.buckets > 64 ? 2 : 4; }

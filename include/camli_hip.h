@@ -741,7 +741,8 @@ int camli_group_norm_bwd(const void *gy, const void *x, int64_t x_batch_stride, 
  *   table [axes,buckets,H] and out [B,H,Lq,Lk] of `type`; positions int32 [B,L,axes], batch strides in ints (0 = shared).
  *   Two-sided: buckets / 2 per sign (positive offsets in the upper half), distance |o|; else all buckets for max(-o, 0).  With s
  *   buckets a side, distances below e = s / 2 have a bucket each, bucket e + j starts at the first d >= e (max_distance / e)^(j/(s-e)).
- *   axes 1 or 2, axes * buckets <= 128, e < max_distance <= 1023.
+ *   axes 1 or 2, axes * buckets <= 128, e < max_distance <= 1023; positions beyond +-2^26 count as that.
+ *   B * H <= 65535, Lq <= 2000000, Lk <= 16000000.
  *   bwd: gtable [axes,buckets,H] of `type`, fully written, the same bits on every run.
  * borders: the first distances of buckets e + 1 ... into border[], returns how many (host only, needs no device).
  */

@@ -3,6 +3,7 @@
 Parameter names (``conv_fn``, ``norm_fn``, ``convs.N``) are those of the reference so that its
 checkpoints load; the classes are generated from one dimension-generic implementation.
 """
+import math
 import os
 
 import torch
@@ -38,6 +39,20 @@ class LayerNormCF2d(_LayerNormCF):
     extra_dims = 2
 
 
+class GroupNormAct(nn.GroupNorm):
+    """Group normalisation and activation of a map [B, C, ...] in one operator (``csrc.group_norm_act``: fp32 statistics, channels-last
+    result; under the 'composed' backend the same formula from torch primitives).  No counterpart in the reference, whose norms are
+    batch / instance / layer norm (mlp.py:43-100).  Eight groups, or as many as divide the channels."""
+
+    def __init__(self, channels, act=None, eps=1e-5):
+        super().__init__(math.gcd(channels, 8), channels, eps=eps)
+        self.act = act
+
+    def forward(self, x):
+        from ..csrc import norm
+        return norm.group_norm_act(x, self.num_groups, self.weight, self.bias, eps=self.eps, act=self.act, cpp_impl=runtime.fused())
+
+
 def make_activation(act):
     if act == 'relu':
         return nn.ReLU(inplace=True)
@@ -61,6 +76,8 @@ def _make_norm(norm, channels, dims):
         return inorm(channels, affine=True)
     if norm == 'layer_norm':
         return ln(channels)
+    if norm == 'group_norm':
+        return GroupNormAct(channels)
     if norm is None:
         return nn.Identity()
     raise NotImplementedError('Unknown normalization function: %s' % norm)
@@ -77,11 +94,15 @@ class _ConvNormAct(nn.Module):
                             dilation=dilation, groups=groups, bias=norm is None)
         self.norm_fn = _make_norm(norm, out_channels, self.dims)
         self.act_fn = make_activation(act)
+        if norm == 'group_norm':        # the normalisation applies the activation
+            self.norm_fn.act, self.act_fn = act, nn.Identity()
         self._epilogue = act if (norm is None and act in (None, 'relu', 'leaky_relu', 'sigmoid')) else False
 
     def forward(self, x):
         if self._epilogue is not False and epilogue_ok(x):
             return conv_bias_act(self.conv_fn, x, self._epilogue)
+        if self.dims == 2 and runtime.fused() and isinstance(self.norm_fn, GroupNormAct):
+            x = x.contiguous(memory_format=torch.channels_last)     # the library's NHWC convolution hands the norm the layout it reads
         return self.act_fn(self.norm_fn(self.conv_fn(x)))
 
 

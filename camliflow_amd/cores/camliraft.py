@@ -33,16 +33,17 @@ class CamLiRAFT_Core(nn.Module):
         self.corr_radius = 4
         self.branch_2d = RAFTCore(cfgs)
         self.branch_3d = CamLiRAFT_L_Core(cfgs)
+        fusion_fn = getattr(cfgs, 'fusion_fn', 'sk')        # 'attn': cross attention between pixels and points (fusion.CrossAttend)
         if cfgs.fuse_fnet:
-            self.clfm_fnet = CLFM(128, 128, norm='batch_norm')
+            self.clfm_fnet = CLFM(128, 128, fusion_fn, norm='batch_norm')
         if cfgs.fuse_cnet:
-            self.clfm_cnet = CLFM(128, 128, norm='batch_norm')
+            self.clfm_cnet = CLFM(128, 128, fusion_fn, norm='batch_norm')
         if cfgs.fuse_corr:
-            self.clfm_corr = CLFM(81 * 4, 128)
+            self.clfm_corr = CLFM(81 * 4, 128, fusion_fn)
         if cfgs.fuse_motion:
-            self.clfm_motion = CLFM(128, 128)
+            self.clfm_motion = CLFM(128, 128, fusion_fn)
         if cfgs.fuse_hidden:
-            self.clfm_hidden = CLFM(128, 128)
+            self.clfm_hidden = CLFM(128, 128, fusion_fn)
 
     def _project_to_feature_grid(self, xyz, camera_info, feat_hw):
         return project_pc2image(xyz, camera_info, grid_hw=feat_hw)

@@ -4,16 +4,18 @@
 score MLP on the pixel offset gates the point feature, then a 1x1 conv.
 3D<-2D: bilinear sample of the image feature at the projected points.
 Both directions are merged by selective-kernel fusion (``SKFusion``, the default) or the add /
-concat / gated variants.  Inputs to the cross paths are detached exactly where the reference
+concat / gated variants.  ``fusion_fn='attn'`` (not in the reference) replaces nearest point, sample and merge by cross attention: every
+pixel attends every point and the other way round (``CrossAttend``).  Inputs to the cross paths are detached exactly where the reference
 detaches them (clfm.py:34,37-38).
 """
 import torch
 import torch.nn as nn
 from torch.nn.functional import softmax
 
+from ..csrc import attention as _attention
 from ..csrc import wrapper as _ops
 from . import runtime
-from .blocks import Conv1dNormRelu, Conv2dNormRelu
+from .blocks import Conv1dNormRelu, Conv2dNormRelu, GroupNormAct
 from .geometry import batch_indexing, grid_sample_wrapper, mesh_grid
 
 
@@ -154,6 +156,36 @@ class SKFusion(nn.Module):
         return feat_2d * weight[..., 0].reshape(bshape) + feat_3d * weight[..., 1].reshape(bshape)
 
 
+class CrossAttend(nn.Module):
+    """x + out(attention(q(norm(x)), kv(norm(context)))) with a learned bias by the bucketed image offset of query and key, per axis.
+
+    x [B, Cx, ...] and context [B, Cc, ...] are maps of any spatial shape (pixels or points); positions are int32 [L, 2] or [B, L, 2] pixel
+    coordinates.  Heads are 32 wide.  The output projection starts at zero: a fresh module passes x through."""
+    HEAD = 32
+
+    def __init__(self, channels, context_channels, buckets=32, max_distance=64):
+        super().__init__()
+        self.heads = max(1, channels // self.HEAD)
+        self.max_distance = max_distance
+        inner = self.heads * self.HEAD
+        self.norm_x, self.norm_context = GroupNormAct(channels), GroupNormAct(context_channels)
+        self.to_q = nn.Linear(channels, inner, bias=False)
+        self.to_kv = nn.Linear(context_channels, 2 * inner, bias=False)
+        self.out = nn.Linear(inner, channels)
+        nn.init.zeros_(self.out.weight)
+        nn.init.zeros_(self.out.bias)
+        self.bias_table = nn.Parameter(torch.zeros(2, buckets, self.heads))
+
+    def forward(self, x, context, x_pos, context_pos):
+        rows = self.norm_x(x).movedim(1, -1).flatten(1, -2)                         # [B, L, C], a view: the norm's memory is that
+        context_rows = self.norm_context(context).movedim(1, -1).flatten(1, -2)
+        q = self.to_q(rows).unflatten(-1, (self.heads, self.HEAD))
+        k, v = self.to_kv(context_rows).unflatten(-1, (2, self.heads, self.HEAD)).unbind(2)
+        att = _attention.cross_attention(q, k, v, bias_table=self.bias_table.to(q.dtype), q_pos=x_pos, k_pos=context_pos,
+                                         max_distance=self.max_distance, cpp_impl=runtime.fused())
+        return x + self.out(att.flatten(2)).transpose(1, 2).reshape(x.shape)
+
+
 _FUSIONS = {'add': (AddFusion, {}), 'concat': (ConcatFusion, {}), 'gated': (GatedFusion, {}),
             'sk': (SKFusion, {'reduction': 2})}
 
@@ -161,6 +193,11 @@ _FUSIONS = {'add': (AddFusion, {}), 'concat': (ConcatFusion, {}), 'gated': (Gate
 class CLFM(nn.Module):
     def __init__(self, in_channels_2d, in_channels_3d, fusion_fn='sk', norm=None):
         super().__init__()
+        self.attends = fusion_fn == 'attn'
+        if self.attends:
+            self.attend2d = CrossAttend(in_channels_2d, in_channels_3d)
+            self.attend3d = CrossAttend(in_channels_3d, in_channels_2d)
+            return
         self.interp = FusionAwareInterp(in_channels_3d, k=1, norm=norm)
         self.mlps3d = Conv1dNormRelu(in_channels_2d, in_channels_2d, norm=norm)
         if fusion_fn not in _FUSIONS:
@@ -169,8 +206,22 @@ class CLFM(nn.Module):
         self.fuse2d = cls(in_channels_2d, in_channels_3d, in_channels_2d, 'nchw', norm, **extra)
         self.fuse3d = cls(in_channels_2d, in_channels_3d, in_channels_3d, 'ncm', norm, **extra)
 
+    def _attend(self, uv, feat_2d, feat_3d):
+        bs, _, image_h, image_w = feat_2d.shape
+        pixels = mesh_grid(1, image_h, image_w, uv.device).reshape(2, -1).t().to(torch.int32).contiguous()            # [HW, 2]
+        # projections far outside the image share the last bucket anyway
+        points = uv.detach().nan_to_num().clamp(-2.0 ** 20, 2.0 ** 20).round().to(torch.int32).transpose(1, 2).contiguous()
+        branch = runtime.Branch(feat_2d, feat_3d, points, pixels, slot=2)
+        with branch:
+            out3d = self.attend3d(feat_3d, feat_2d.detach(), points, pixels)
+        out2d = self.attend2d(feat_2d, feat_3d.detach(), pixels, points)
+        branch.join(out3d)
+        return out2d, out3d
+
     def forward(self, uv, feat_2d, feat_3d):
         feat_2d, feat_3d = feat_2d.float(), feat_3d.float()
+        if self.attends:
+            return self._attend(uv, feat_2d, feat_3d)
         # the two directions are independent chains: 3D<-2D (a dozen kernels on [B,C,2048] tensors, latency-sized) goes to
         # an auxiliary stream next to 2D<-3D (runtime.Branch; one stream when the lanes are off)
         branch = runtime.Branch(feat_2d, feat_3d, uv, slot=2)

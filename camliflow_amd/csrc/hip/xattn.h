@@ -419,6 +419,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     using Frag = FragOf<T>;
     constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
     constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2;
+    constexpr unsigned long long ALL_KEPT = R == 64 ? ~0ull : (1ull << R) - 1;
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
     float* lut = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);
@@ -462,7 +463,8 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     acc16 o[TL::DBLOCKS];
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = acc16{0};
-    // m: the reference of the row's exponents, log2 domain (-inf: no kept key yet, use 0); start: -m / scale in every accumulator
+    // m: the reference of the row's exponents, log2 domain (-inf: no kept key yet, use 0); start: -m / scale in every accumulator (with
+    // a bias; without one the exponent's multiply-add subtracts m at no cost)
     float m = -INFINITY, m_use = 0.0f, l = 0.0f;
     acc16 start = splat(0.0f);
     bool unset = true;
@@ -490,13 +492,13 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
             float top = -INFINITY;
 #pragma unroll
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                s[nb] = start;
+                s[nb] = AXES > 0 ? start : acc16{0};
 #pragma unroll
                 for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(map.read_row(kt + nb * 32 * TL::LD, ks), qf[ks], s[nb]);
             }
+            if constexpr (AXES > 0) {
 #pragma unroll
-            for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                if constexpr (AXES > 0) {
+                for (int nb = 0; nb < TL::BLOCKS; ++nb) {
                     int off[AXES][16];
 #pragma unroll
                     for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], qa[x], off[x]);
@@ -505,42 +507,47 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
                         s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
                         if constexpr (AXES > 1) s[nb][i] += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[nb][i] *= a.scale_log2;
                 }
-                const unsigned half = (unsigned)(bits >> (nb * 32));
-                if (half != 0xffffffffu) {
-                    const unsigned mine = half >> (4 * h);
+            }
+            if (bits != ALL_KEPT) {
+#pragma unroll
+                for (int nb = 0; nb < TL::BLOCKS; ++nb) {
+                    const unsigned mine = (unsigned)(bits >> (nb * 32)) >> (4 * h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[nb][i] = (mine >> acc_row(i, 0)) & 1 ? s[nb][i] : -INFINITY;
                 }
+            }
+#pragma unroll
+            for (int nb = 0; nb < TL::BLOCKS; ++nb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
-            }
+            if constexpr (AXES == 0) top = __builtin_fmaf(top, a.scale_log2, -m_use);
             if (unset || __any(top > exponent_limit<T>())) {
                 top = half_max(top) + m_use;
                 const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
-                const float alpha = __builtin_amdgcn_exp2f(m - use), back = m_use - use;
+                const float alpha = __builtin_amdgcn_exp2f(m - use);
 #pragma unroll
                 for (int d = 0; d < TL::DBLOCKS; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
                 l *= alpha;
+                if constexpr (AXES > 0) {
+                    const float back = m_use - use;
+                    start = splat(-use / a.scale_log2);
+#pragma unroll
+                    for (int nb = 0; nb < TL::BLOCKS; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[nb][i] += back;
+                }
                 m = mn;
                 m_use = use;
-                start = splat(-use / a.scale_log2);
                 unset = __any(m == -INFINITY);
-#pragma unroll
-                for (int nb = 0; nb < TL::BLOCKS; ++nb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[nb][i] += back;
             }
 #pragma unroll
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[nb][i] = __builtin_amdgcn_exp2f(s[nb][i]);
+                    s[nb][i] = __builtin_amdgcn_exp2f(AXES > 0 ? s[nb][i] : __builtin_fmaf(s[nb][i], a.scale_log2, -m_use));
                     l += s[nb][i];
                 }
 #pragma unroll
@@ -642,7 +649,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
 // HIST: with the table's gradient; its tiles are 32 rows in one buffer, so that two workgroups still share a CU beside their histograms
 // (one waits at a barrier while the other computes).
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
-__global__ __launch_bounds__(64 * WAVES) void dq_kernel(Args a) {
+__global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
     constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;

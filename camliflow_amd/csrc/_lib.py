@@ -1,6 +1,7 @@
 """ctypes binding of libcamli_hip.so (prototypes: include/camli_hip.h)."""
 import ctypes
 import os
+import struct
 
 from .build import LIB_PATH
 
@@ -21,7 +22,10 @@ class AttentionDesc(ctypes.Structure):
         (n, _int) for n in ('bias_axes', 'bias_buckets', 'bias_two_sided', 'bias_max_distance')]
 
 
-_desc_p = ctypes.POINTER(AttentionDesc)
+# a call hands over an AttentionDesc by reference, or its bytes packed with this format (a tenth of the time of 30 attribute writes)
+ATTENTION_PACK = struct.Struct('@7if3P9q2Pq3P2q4i').pack
+assert struct.calcsize('@7if3P9q2Pq3P2q4i') == ctypes.sizeof(AttentionDesc)
+_desc_p = ctypes.c_void_p
 
 # name -> (restype, argtypes); every symbol include/camli_hip.h declares
 PROTOTYPES = {

@@ -53,18 +53,18 @@ def _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, dtype, h
     if side < 2 or (bidirectional and buckets % 2) or not side // 2 < max_distance <= MAX_BIAS_DISTANCE or int(max_distance) != max_distance:
         raise ValueError('%s: need at least two buckets a side (an even number when bidirectional) and %d < max_distance <= %d, got %d buckets and %r'
                          % (name, side // 2, MAX_BIAS_DISTANCE, buckets, max_distance))
-    out = []
+    leads = []
     for what, pos, n in (('q_pos', q_pos, lq), ('k_pos', k_pos, lk)):
-        if pos.dtype != torch.int32 or pos.dim() not in (2, 3) or pos.shape[-1] != axes or (n is not None and pos.shape[-2] != n) or (
-                pos.dim() == 3 and batch is not None and pos.shape[0] != batch):
-            raise ValueError('%s: %s must be int32 [L, %d] or [B, L, %d] for the operands\' B and L, got %s %s' % (
-                name, what, axes, axes, tuple(pos.shape), pos.dtype))
-        out.append(pos.contiguous())
-    same_device(name, table, *out)
-    batches = {p.shape[0] for p in out if p.dim() == 3}
-    if len(batches) > 1:
-        raise ValueError('%s: q_pos and k_pos of different batches: %s' % (name, sorted(batches)))
-    return table.contiguous(), out[0], out[1], (batches.pop() if batches else None), axes
+        shape = pos.shape
+        if pos.dtype != torch.int32 or len(shape) not in (2, 3) or shape[-1] != axes or (n is not None and shape[-2] != n) or (
+                len(shape) == 3 and batch is not None and shape[0] != batch) or pos.device != table.device:
+            raise ValueError('%s: %s must be int32 [L, %d] or [B, L, %d] for the operands\' B and L, beside the table on %s; got %s %s on %s' % (
+                name, what, axes, axes, table.device, tuple(shape), pos.dtype, pos.device))
+        if len(shape) == 3:
+            leads.append(shape[0])
+    if len(leads) == 2 and leads[0] != leads[1]:
+        raise ValueError('%s: q_pos and k_pos of different batches: %s' % (name, leads))
+    return table.contiguous(), q_pos.contiguous(), k_pos.contiguous(), (leads[0] if leads else None), axes
 
 
 def _pos_stride(pos):
@@ -162,33 +162,45 @@ def _rows16(t):
 
 
 def _strides(t):
-    return (ctypes.c_int64 * 3)(*[s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])])
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
 
 
 def _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance):
-    d = _lib.AttentionDesc()
-    d.type = TYPE_CODES[q.dtype]
-    d.B, d.Lq, d.H, d.D = q.shape
-    d.Lk, d.Hk = k.shape[1:3]
-    d.scale = scale
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    d.q_stride, d.k_stride, d.v_stride = _strides(q), _strides(k), _strides(v)
-    if kv_lengths is not None:
-        d.kv_lengths = kv_lengths.data_ptr()
-    if key_mask is not None:
-        d.key_mask, d.key_mask_batch_stride = key_mask.data_ptr(), key_mask.shape[1]
+    """the bytes of a camli_attention (include/camli_hip.h)"""
+    b, lq, h, dim = q.shape
+    lk, hk = k.shape[1:3]
+    bias = (0, 0, 0, 0, 0, 0, 0, 0, 0)
     if table is not None:
-        d.bias_table, d.q_pos, d.k_pos = table.data_ptr(), q_pos.data_ptr(), k_pos.data_ptr()
-        d.q_pos_batch_stride, d.k_pos_batch_stride = _pos_stride(q_pos), _pos_stride(k_pos)
-        d.bias_axes, d.bias_buckets = table.shape[:2]
-        d.bias_two_sided, d.bias_max_distance = int(bidirectional), max_distance
-    return d
+        axes, buckets, _ = table.shape
+        bias = (table.data_ptr(), q_pos.data_ptr(), k_pos.data_ptr(), _pos_stride(q_pos), _pos_stride(k_pos), axes, buckets, bidirectional,
+                max_distance)
+    return _lib.ATTENTION_PACK(TYPE_CODES[q.dtype], b, h, hk, lq, lk, dim, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                               *_strides(q), *_strides(k), *_strides(v), 0 if kv_lengths is None else kv_lengths.data_ptr(),
+                               0 if key_mask is None else key_mask.data_ptr(), lk, *bias)
 
 
-def _workspace(name, n, like):
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace_bytes(backward, table_gradient, head, bias):
+    """by sizes alone: head = (type, B, H, Hk, Lq, Lk, D), bias = (axes, buckets, bidirectional, max_distance)"""
+    lib = _lib.load()
+    d = _lib.AttentionDesc(*head)
+    d.scale = 1.0
+    d.q = d.k = d.v = 16
+    if bias[0]:
+        d.bias_table = d.q_pos = d.k_pos = 16
+        d.bias_axes, d.bias_buckets, d.bias_two_sided, d.bias_max_distance = bias
+    n = (lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), int(table_gradient)) if backward
+         else lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d)))
     if n < 0:
-        _lib.check(int(n), name)
-    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=like.device)
+        _lib.check(int(n), 'camli_cross_attention_%s_workspace_bytes' % ('bwd' if backward else 'fwd'))
+    return int(n)
+
+
+def _sizes(q, k, table, bidirectional, max_distance):
+    b, lq, h, dim = q.shape
+    lk, hk = k.shape[1:3]
+    return ((TYPE_CODES[q.dtype], b, h, hk, lq, lk, dim),
+            (0, 0, 0, 0) if table is None else (table.shape[0], table.shape[1], int(bidirectional), max_distance))
 
 
 def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance, train):
@@ -202,12 +214,11 @@ def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bi
     out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if train else None
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
-    d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
-    ref = ctypes.byref(d)
+    desc = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
+    n = _attention_workspace_bytes(False, False, *_sizes(q, k, table, bidirectional, max_distance))
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     with _on_device(q):
-        n = lib.camli_cross_attention_fwd_workspace_bytes(ref)
-        ws = _workspace('camli_cross_attention_fwd', n, q) if n else None
-        _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, ref, out.data_ptr(), address(rest), address(lse), address(ws), n,
+        _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, desc, out.data_ptr(), address(rest), address(lse), address(ws), n,
                     _stream_ptr(q), work=(2.0 * q.element_size() * dim * b * (lq * h + lk * hk), 'B'), flop=4.0 * b * h * lq * lk * dim)
     return out, (q, k, v), rest, lse
 
@@ -240,12 +251,11 @@ class _CrossAttention(torch.autograd.Function):
             gk = torch.empty((b, lk, hk, dim), dtype=q.dtype, device=q.device)
             gv = torch.empty_like(gk)
         gt = torch.empty(table.shape, dtype=table.dtype, device=q.device) if need_t else None
-        d = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, *ctx.args)
-        ref = ctypes.byref(d)
+        desc = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, *ctx.args)
+        n = _attention_workspace_bytes(True, need_t, *_sizes(q, k, table, *ctx.args[1:]))
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         with _on_device(q):
-            n = lib.camli_cross_attention_bwd_workspace_bytes(ref, int(need_t))
-            ws = _workspace('camli_cross_attention_bwd', n, q)
-            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, ref, out.data_ptr(), address(rest), gout.data_ptr(),
+            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, desc, out.data_ptr(), address(rest), gout.data_ptr(),
                         lse.data_ptr(), address(gq), address(gk), address(gv), address(gt), ws.data_ptr(), n, _stream_ptr(q),
                         work=(4.0 * q.element_size() * dim * b * (lq * h + lk * hk), 'B'), flop=10.0 * b * h * lq * lk * dim)
         return (gq, gk if need_k else None, gv if need_v else None, gt) + nothing

@@ -291,7 +291,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
 
     fp32, bf16 or fp16 (one type for all; sums and softmax in fp32); D a multiple of 8 up to 128; H a multiple of Hk (query heads
     h share key / value head h // (H / Hk)).  Any strides: rows that are not adjacent or 16-byte aligned are copied first.  ``scale``:
-    positive, default D ** -0.5.  One token (Lq = 1) and other short queries are split over the keys.
+    from 1e-15 to 1e15, default D ** -0.5.  One token (Lq = 1) and other short queries are split over the keys.
 
     ``kv_lengths`` int32 [B]: keys from there on are padding (values outside 0 .. Lk are clamped); ``key_mask`` bool [B, Lk]: False masks a
     key; a key is kept if both keep it.  Masked keys and values may hold anything, NaN included, and get zero gradients.  A query that
@@ -311,8 +311,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
     if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM:
         raise ValueError('%s: the head width must be a multiple of 8 up to %d, got %d' % (name, MAX_HEAD_DIM, dim))
     scale = float(dim) ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError('%s: scale must be positive and finite, got %r' % (name, scale))
+    if not 1e-15 <= scale <= 1e15:
+        raise ValueError('%s: scale must be positive, from 1e-15 to 1e15, got %r' % (name, scale))
+    if b * h * ((lq + 31) // 32) >= 2 ** 24 or b * hk * ((lk + 127) // 128) >= 2 ** 24 or h * dim >= 2 ** 23:
+        raise ValueError('%s: too many samples x heads x rows for one launch: q %s, k %s' % (name, tuple(q.shape), tuple(k.shape)))
     if kv_lengths is not None and (kv_lengths.shape != (b,) or kv_lengths.dtype != torch.int32):
         raise ValueError('%s: kv_lengths must be int32 [%d], got %s %s' % (name, b, tuple(kv_lengths.shape), kv_lengths.dtype))
     if key_mask is not None and (key_mask.shape != (b, lk) or key_mask.dtype != torch.bool):

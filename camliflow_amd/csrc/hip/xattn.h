@@ -17,6 +17,10 @@
 //     fp32 with plain 4-byte reads, which are conflict-free on row-major tiles.
 // Register i of half h holds streamed row 8 (i / 4) + 4 h + i % 4 of its 32-row block.
 //
+// fp16 dS: p (dp - D) of a long row is of the size of |go| / Lk, below fp16's normal numbers for quite ordinary gradients.  go is therefore taken
+// times a power of two that brings its largest element to 1 .. 2 (a row's own in dq, where the contraction is over keys; the kv head's
+// in dkdv, where it is over queries), and P times 2^10 in dkdv; both are undone exactly when the gradients are written.
+//
 // Two adjoint kernels recompute p instead of one that adds dq with float atomics: 14 D instead of 10 D operations per pair, but
 // every sum has a fixed order (the same bits on every run).  P and dS are rounded to the element type for the second products (their
 // sums stay fp32): half a step of the inputs' own type, as for every operand of a matrix product.
@@ -37,6 +41,7 @@ struct Args {
     void *out_rest;             // 16-bit types in training: out minus its rounding, rounded
     float *lse;                 // [B][H][Lq], log2 domain; +inf where no key is kept
     float *delta;               // [B][H][Lq]
+    float *go_max;              // [B][H][Lq] fp16 only: largest |go| of a row
     float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [split][B][H][Lq] (-inf: no key)
     float *part_dk, *part_dv;   // splits > 1: [split][B][Lk][Hk][D]
     float *part_table;          // [H][parts][axes * buckets]
@@ -643,6 +648,12 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
     }
 }
 
+// power of two that brings x to 1 .. 2 (1 for zero, infinity and NaN)
+__device__ __forceinline__ float unit_scale(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
+    return x > 0.0f && e < 128 ? __uint_as_float((unsigned)(127 - e) << 23) : 1.0f;
+}
+
 // ------------------------------------------------------------------------------------------------------------ dq
 // WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, then
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
@@ -701,11 +712,28 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
         }
         delta = half_sum(delta);
     }
+    if (exists && split == 0 && h == 0) a.delta[stat] = delta;
+    float unscale = 1.0f;
+    if constexpr (__is_same(T, _Float16)) {
+        float most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < TL::KSTEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < TL::E; ++e) most = fmaxf(most, fabsf((float)gf[s][e]));
+        most = half_max(most);
+        if (exists && split == 0 && h == 0) a.go_max[stat] = most;
+        const float f = unit_scale(most);
+        unscale = unit_scale(f);
+        delta *= f;
+#pragma unroll
+        for (int s = 0; s < TL::KSTEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < TL::E; ++e) gf[s][e] = (T)((float)gf[s][e] * f);
+    }
     // the accumulators start at -lse / scale and -delta: the products come out as the exponent and as dp - D.  +inf (a row without keys,
     // or none at all) makes every p zero.
     const acc16 start_s = splat(-(exists ? a.lse[stat] : INFINITY) / a.scale_log2), start_d = splat(-delta);
     const LaneMap<T, DP> map(lane);
-    if (exists && split == 0 && h == 0) a.delta[stat] = delta;
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
     if constexpr (AXES > 0) {
@@ -790,7 +818,10 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(s[i]);
             if constexpr (HIST) {
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) hist_add2<AXES>(column, at_hist[i], dp[i], at_hist[i + 1], dp[i + 1]);
+                for (int i = 0; i < 16; i += 2) {
+                    if constexpr (__is_same(T, _Float16)) hist_add2<AXES>(column, at_hist[i], dp[i] * unscale, at_hist[i + 1], dp[i + 1] * unscale);
+                    else hist_add2<AXES>(column, at_hist[i], dp[i], at_hist[i + 1], dp[i + 1]);
+                }
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
@@ -808,8 +839,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
         cur ^= 1;
     }
     if (a.dq && exists) {
-        if (a.splits > 1) store_owned<float, TL::DBLOCKS>(a.part_o + ((int64_t)split * a.B * a.Lq * a.H + at) * a.D, dq, a.scale, a.D, h);
-        else store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dq) + at * a.D, dq, a.scale, a.D, h);
+        if (a.splits > 1) store_owned<float, TL::DBLOCKS>(a.part_o + ((int64_t)split * a.B * a.Lq * a.H + at) * a.D, dq, a.scale * unscale, a.D, h);
+        else store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dq) + at * a.D, dq, a.scale * unscale, a.D, h);
     }
     if constexpr (HIST) {       // rows that do not exist added zeros
         const int64_t part = ((int64_t)b * a.row_tiles + rt) * a.splits + split;
@@ -863,6 +894,23 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
             hi[x] = centre + ENTRY * a.rb.limit;
         }
     }
+    constexpr bool HALF = __is_same(T, _Float16);
+    constexpr float P_LOG2 = HALF ? 10.0f : 0.0f, P_UNSCALE = HALF ? 1.0f / 1024.0f : 1.0f;
+    float ds_scale = 1.0f, ds_unscale = 1.0f;       // of dS beside that of P
+    if constexpr (HALF) {
+        __shared__ float most[THREADS / 64];
+        float x = 0.0f;
+        const float* rows = a.go_max + ((int64_t)b * a.H + kvh * group) * a.Lq;
+        const int64_t n = (int64_t)group * a.Lq;
+        for (int64_t i = tid; i < n; i += THREADS) x = fmaxf(x, rows[i]);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+        if (lane == 0) most[wave] = x;
+        __syncthreads();
+        const float f = unit_scale(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+        ds_scale = f * P_UNSCALE;
+        ds_unscale = unit_scale(f);
+    }
     acc16 dk[TL::DBLOCKS], dv[TL::DBLOCKS];
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) dk[d] = dv[d] = acc16{0};
@@ -886,7 +934,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
             const float* src = tid < TL::ROWS ? a.lse : a.delta;
             // what the accumulators start at: -lse / scale and -delta; a row that does not exist has lse = +inf, so p = 0
             const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
-            snext = tid < TL::ROWS ? -x / a.scale_log2 : -x;
+            snext = tid < TL::ROWS ? (P_LOG2 - x) / a.scale_log2 : -x;
         }
         if constexpr (AXES > 0) pos_next.load(qpos, row0, a.Lq);
     };
@@ -941,7 +989,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
                     x = s[i] * a.scale_log2;
                 }
                 s[i] = __builtin_amdgcn_exp2f(x);
-                dp[i] *= s[i];
+                dp[i] *= HALF ? s[i] * ds_scale : s[i];
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
@@ -965,11 +1013,11 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     const int64_t at = ((int64_t)b * a.Lk + kj) * a.Hk + kvh;
     if (a.splits > 1) {
         const int64_t off = (int64_t)split * a.B * a.Lk * a.Hk;
-        store_owned<float, TL::DBLOCKS>(a.part_dk + (off + at) * a.D, dk, a.scale, a.D, h);
-        store_owned<float, TL::DBLOCKS>(a.part_dv + (off + at) * a.D, dv, 1.0f, a.D, h);
+        store_owned<float, TL::DBLOCKS>(a.part_dk + (off + at) * a.D, dk, a.scale * ds_unscale, a.D, h);
+        store_owned<float, TL::DBLOCKS>(a.part_dv + (off + at) * a.D, dv, P_UNSCALE, a.D, h);
     } else {
-        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dk) + at * a.D, dk, a.scale, a.D, h);
-        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dv) + at * a.D, dv, 1.0f, a.D, h);
+        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dk) + at * a.D, dk, a.scale * ds_unscale, a.D, h);
+        store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dv) + at * a.D, dv, P_UNSCALE, a.D, h);
     }
 }
 

@@ -57,16 +57,16 @@ bool operand_ok(const void* p, const int64_t* stride, int size) {
 bool make_args(Args& a, const camli_attention* d, const char* who) {
     if (!d) { camli_set_error("%s: null descriptor", who); return false; }
     if (d->type < 0 || d->type > 2 || d->B < 1 || d->Hk < 1 || d->H < d->Hk || d->H % d->Hk != 0 || d->Lq < 1 || d->Lk < 1 || d->D < 8 || d->D > 128 ||
-        d->D % 8 != 0 || !(d->scale > 0.0f) || !(d->scale < INFINITY)) {
-        camli_set_error("%s: need type 0..2, B, Lq, Lk >= 1, H a multiple of Hk, D a multiple of 8 up to 128, a positive finite scale (type=%d B=%d H=%d Hk=%d Lq=%d Lk=%d D=%d scale=%g)",
+        d->D % 8 != 0 || !(d->scale >= 1e-15f) || !(d->scale <= 1e15f)) {
+        camli_set_error("%s: need type 0..2, B, Lq, Lk >= 1, H a multiple of Hk, D a multiple of 8 up to 128, a scale from 1e-15 to 1e15 (type=%d B=%d H=%d Hk=%d Lq=%d Lk=%d D=%d scale=%g)",
                         who, d->type, d->B, d->H, d->Hk, d->Lq, d->Lk, d->D, (double)d->scale);
         return false;
     }
     const int size = camli_type_size(d->type);
-    // grid sizes and element counts of a workgroup's own arithmetic stay below 2^31
-    if ((int64_t)d->B * d->H * ((int64_t)camli_divup(d->Lq, 32) + 1024) > INT32_MAX || (int64_t)d->B * d->Hk * ((int64_t)camli_divup(d->Lk, 128) + 1024) > INT32_MAX ||
-        (int64_t)camli_divup(d->Lq, 32) * (d->H / d->Hk) > INT32_MAX / 64 || (int64_t)d->H * d->D >= (1 << 23) || d->Lq > INT32_MAX - 256 || d->Lk > INT32_MAX - 256) {
-        camli_set_error("%s: B * H * Lq or B * Hk * Lk too large", who);
+    // a launch has fewer than 2^32 threads: 2^24 workgroups of 256
+    if ((int64_t)d->B * d->H * camli_divup(d->Lq > INT32_MAX - 256 ? 0 : d->Lq, 32) >= (1 << 24) || (int64_t)d->B * d->Hk * camli_divup(d->Lk > INT32_MAX - 256 ? 0 : d->Lk, 128) >= (1 << 24) ||
+        (int64_t)camli_divup(d->Lq > INT32_MAX - 256 ? 0 : d->Lq, 32) * (d->H / d->Hk) >= (1 << 24) || (int64_t)d->H * d->D >= (1 << 23) || d->Lq > INT32_MAX - 256 || d->Lk > INT32_MAX - 256) {
+        camli_set_error("%s: B * H * Lq / 32, B * Hk * Lk / 128 (at most 2^24) or H * D (2^23) too large", who);
         return false;
     }
     if (!operand_ok(d->q, d->q_stride, size) || !operand_ok(d->k, d->k_stride, size) || !operand_ok(d->v, d->v_stride, size)) {
@@ -114,6 +114,10 @@ BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base
     const int64_t rows = (int64_t)a.B * a.H * a.Lq;
     p.dq.delta = p.dkdv.delta = reinterpret_cast<float*>(base);
     int64_t end = align256(4 * rows);
+    if (d->type == CAMLI_F16) {
+        p.dq.go_max = p.dkdv.go_max = reinterpret_cast<float*>(base + end);
+        end += align256(4 * rows);
+    }
     if (p.dq.splits > 1) {
         p.dq.part_o = reinterpret_cast<float*>(base + end);
         end += align256(4 * rows * a.D * p.dq.splits);

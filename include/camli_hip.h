@@ -759,7 +759,7 @@ int camli_rel_bias_bwd(const void *gout, const int *q_pos, int64_t q_pos_batch_s
  * Cross attention: out = softmax(scale q k^T + bias) v over the kept keys of each sample; H query heads share Hk key / value heads.
  *   q [B,Lq,H,D], k, v [B,Lk,Hk,D] of `type`, strides in elements (batch, row, head; D adjacent), 16-byte aligned rows,
  *   row strides below 2^23;
- *   out, gout, gq [B,Lq,H,D] and gk, gv [B,Lk,Hk,D] dense;  D a multiple of 8, at most 128.
+ *   out, gout, gq [B,Lq,H,D] and gk, gv [B,Lk,Hk,D] dense;  D a multiple of 8, at most 128;  scale from 1e-15 to 1e15.
  *   A key is kept if its index is below kv_lengths[b] (NULL: all; clamped to 0..Lk) and key_mask[b,j] != 0 (NULL: all).  Masked keys
  *   and values may hold anything, NaN included; their gradients are zero.  A row without a kept key (or whose scores are all -inf)
  *   gives zeros and takes no part in any gradient.

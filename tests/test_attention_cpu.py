@@ -22,7 +22,7 @@ def _pos(n, axes=1):
 @pytest.mark.parametrize('change', [
     dict(q=torch.zeros(2, 5, 4)), dict(q=torch.zeros(2, 5, 4, 16, dtype=torch.float64)), dict(k=torch.zeros(2, 7, 2, 16, dtype=torch.bfloat16)),
     dict(v=torch.zeros(2, 8, 2, 16)), dict(k=torch.zeros(3, 7, 2, 16), v=torch.zeros(3, 7, 2, 16)), dict(k=torch.zeros(2, 7, 3, 16), v=torch.zeros(2, 7, 3, 16)),
-    dict(k=torch.zeros(2, 7, 0, 16), v=torch.zeros(2, 7, 0, 16)), dict(scale=0.0), dict(scale=-1.0), dict(scale=float('inf')), dict(scale=float('nan')),
+    dict(k=torch.zeros(2, 7, 0, 16), v=torch.zeros(2, 7, 0, 16)), dict(scale=0.0), dict(scale=-1.0), dict(scale=float('inf')), dict(scale=float('nan')), dict(scale=1e-16), dict(scale=1e16),
     dict(kv_lengths=torch.zeros(2, dtype=torch.int64)), dict(kv_lengths=torch.zeros(3, dtype=torch.int32)), dict(key_mask=torch.ones(2, 7)),
     dict(key_mask=torch.ones(7, dtype=torch.bool)), dict(bias_table=torch.zeros(1, 8, 4)), dict(q_pos=_pos(5)),
     dict(bias_table=torch.zeros(1, 8, 3), q_pos=_pos(5), k_pos=_pos(7)), dict(bias_table=torch.zeros(8, 4), q_pos=_pos(5), k_pos=_pos(7)),
@@ -76,6 +76,13 @@ def test_operators_refuse_cpu_tensors():
         csrc.relative_position_bias(torch.zeros(1, 8, 2), _pos(3), _pos(3))
 
 
+def test_attention_refuses_what_one_launch_cannot_hold():
+    one = torch.zeros(1)
+    for q, k in (((2 ** 24, 1, 1, 8), (2 ** 24, 1, 1, 8)), ((1, 1, 2 ** 20, 8), (1, 1, 1, 8)), ((1, 2 ** 29, 1, 8), (1, 1, 1, 8))):
+        with pytest.raises(ValueError, match='too many'):
+            cross_attention(one.expand(q), one.expand(k), one.expand(k))
+
+
 def test_c_entries_refuse_and_report():
     """the C boundary checks for itself: nothing is launched and no exception crosses it"""
     lib = _lib.load()
@@ -97,7 +104,7 @@ def test_c_entries_refuse_and_report():
         s[0], s[1], s[2] = 0, 64, 32
     assert lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d)) >= 0
     assert lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), 0) > 0
-    for name, bad in (('D', 36), ('D', 0), ('H', 3), ('Lk', 0), ('B', 0), ('type', 3), ('scale', 0.0), ('k', 8200), ('bias_axes', 1), ('Lq', 2 ** 31 - 1)):
+    for name, bad in (('D', 36), ('D', 0), ('H', 3), ('Lk', 0), ('B', 0), ('type', 3), ('scale', 0.0), ('scale', 1e-16), ('k', 8200), ('bias_axes', 1), ('Lq', 2 ** 31 - 1)):
         keep = getattr(d, name)
         d.Hk = 2 if name == 'H' else 1
         setattr(d, name, bad)

@@ -121,6 +121,11 @@ def test_attention_masked_places_may_hold_anything(dtype, poison):
     assert not clean['dk'][hidden.expand_as(c['k']).cuda()].any() and not clean['dv'][hidden.expand_as(c['v']).cuda()].any()
 
 
+@pytest.mark.parametrize('scale', [1e-15, 1e-4, 3.0])
+def test_attention_scales(scale):
+    _check(_case(1, 20, 90, 2, 2, 32, torch.float32, axes=1, seed=16), scale=scale)
+
+
 def test_attention_lengths_are_clamped():
     c = _case(3, 9, 50, 2, 2, 32, torch.float32, lengths=[50, 0, 50], seed=8)
     got = _run(c)
@@ -207,6 +212,24 @@ def test_attention_gradients_against_differences():
         mine = float((got['d' + name].cpu().double() * direction).sum())
         # differences: step^2 times a third derivative of order 10^2; gradients: fp32
         assert abs(slope - mine) < 1e-5 * max(1.0, float((got['d' + name].cpu().double().abs() * direction.abs()).sum()))
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('factor', [2.0 ** -12, 2.0 ** 8])
+def test_attention_gradients_scale_with_the_incoming_gradient(dtype, factor):
+    """a long row's dS is 1 / Lk of the gradient: it must not sink into fp16's subnormal numbers, nor a large gradient overflow them"""
+    c = _case(1, 64, 5000, 2, 1, 32, dtype, axes=1, seed=15)
+    c['go'] = (c['go'] / 64).to(dtype)
+    base = _run(c)
+    c['go'] = c['go'] * factor          # exact: a power of two, and no element of this go is below 2^-13 / 64 but by chance
+    scaled = _run(c)
+    for name in ('dq', 'dk', 'dv', 'dtable'):
+        a, b = scaled[name].double() / factor, base[name].double()
+        # both are roundings of the same numbers: a step of the larger one's type, or of the subnormal numbers it was written as
+        step = torch.finfo(dtype).eps * b.abs() + 2 * attnref.SUBNORMAL[dtype] * max(1.0, 1.0 / factor)
+        # elements of go that became subnormal: each off by half a step of 2^-24, through sums of at most 5000 weights that add up to 1
+        lost = 2 ** -24 * 64 / factor if dtype == torch.float16 and factor < 1 else 0.0
+        assert ((a - b).abs() <= 2 * step + lost + 1e-6 * b.abs().max()).all(), name
 
 
 def test_attention_same_bits_every_run_and_refuses_double_backward():

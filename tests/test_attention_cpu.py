@@ -80,7 +80,7 @@ def test_attention_refuses_what_one_launch_cannot_hold():
     one = torch.zeros(1)
     for q, k in (((2 ** 24, 1, 1, 8), (2 ** 24, 1, 1, 8)), ((1, 1, 2 ** 20, 8), (1, 1, 1, 8)), ((1, 2 ** 29, 1, 8), (1, 1, 1, 8))):
         with pytest.raises(ValueError, match='too many'):
-            cross_attention(one.expand(q), one.expand(k), one.expand(k))
+            csrc.cross_attention(one.expand(q), one.expand(k), one.expand(k))
 
 
 def test_c_entries_refuse_and_report():

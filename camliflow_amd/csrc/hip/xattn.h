@@ -414,6 +414,10 @@ __device__ __forceinline__ void broadcast_plus(int lanes, int own, int (&out)[16
 // TRAIN (16-bit types): out has to be known to more than its own type for the backward's D = do . o, which is subtracted from
 // dp: P enters the product as two terms of the type and the rounding error of out is stored beside it.  Without that the bias table's
 // gradient, a sum over whole rows of ds, is off by twice its own rounding.
+// fp32 with a bias starts at zero and subtracts m at the end: at -m / scale every step of the product rounds to a few bits less (a relative
+// error of p of 1e-6), which is nothing to a 16-bit product and shows in an fp32 gradient.  The adjoints do the same with the log-sum.
+template <typename T>
+constexpr bool fold_start() { return sizeof(T) == 2; }
 template <typename T>
 constexpr float exponent_limit() { return __is_same(T, _Float16) ? 14.0f : 30.0f; }
 
@@ -423,7 +427,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
     constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
-    constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2;
+    constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2, FOLD = AXES > 0 && fold_start<T>();
     constexpr unsigned long long ALL_KEPT = R == 64 ? ~0ull : (1ull << R) - 1;
     extern __shared__ __align__(16) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
@@ -468,8 +472,8 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     acc16 o[TL::DBLOCKS];
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = acc16{0};
-    // m: the reference of the row's exponents, log2 domain (-inf: no kept key yet, use 0); start: -m / scale in every accumulator (with
-    // a bias; without one the exponent's multiply-add subtracts m at no cost)
+    // m: the reference of the row's exponents, log2 domain (-inf: no kept key yet, use 0); start: -m / scale in every accumulator (FOLD:
+    // with a bias; without one the exponent's multiply-add subtracts m at no cost)
     float m = -INFINITY, m_use = 0.0f, l = 0.0f;
     acc16 start = splat(0.0f);
     bool unset = true;
@@ -497,7 +501,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
             float top = -INFINITY;
 #pragma unroll
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                s[nb] = AXES > 0 ? start : acc16{0};
+                s[nb] = FOLD ? start : acc16{0};
 #pragma unroll
                 for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(map.read_row(kt + nb * 32 * TL::LD, ks), qf[ks], s[nb]);
             }
@@ -527,6 +531,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
             if constexpr (AXES == 0) top = __builtin_fmaf(top, a.scale_log2, -m_use);
+            else if constexpr (!FOLD) top -= m_use;
             if (unset || __any(top > exponent_limit<T>())) {
                 top = half_max(top) + m_use;
                 const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
@@ -536,7 +541,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
                 l *= alpha;
-                if constexpr (AXES > 0) {
+                if constexpr (FOLD) {
                     const float back = m_use - use;
                     start = splat(-use / a.scale_log2);
 #pragma unroll
@@ -552,7 +557,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[nb][i] = __builtin_amdgcn_exp2f(AXES > 0 ? s[nb][i] : __builtin_fmaf(s[nb][i], a.scale_log2, -m_use));
+                    s[nb][i] = __builtin_amdgcn_exp2f(FOLD ? s[nb][i] : AXES > 0 ? s[nb][i] - m_use : __builtin_fmaf(s[nb][i], a.scale_log2, -m_use));
                     l += s[nb][i];
                 }
 #pragma unroll
@@ -732,7 +737,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
     }
     // the accumulators start at -lse / scale and -delta: the products come out as the exponent and as dp - D.  +inf (a row without keys,
     // or none at all) makes every p zero.
-    const acc16 start_s = splat(-(exists ? a.lse[stat] : INFINITY) / a.scale_log2), start_d = splat(-delta);
+    constexpr bool FOLD = fold_start<T>();
+    const float lse = exists ? a.lse[stat] : INFINITY;
+    const acc16 start_s = FOLD ? splat(-lse / a.scale_log2) : acc16{0}, start_d = splat(-delta);
     const LaneMap<T, DP> map(lane);
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
@@ -804,10 +811,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
                     }
                     s[i] = __builtin_fmaf(s[i], a.scale_log2, bias[0]);
                     if constexpr (AXES > 1) s[i] += bias[AXES - 1];
+                    if constexpr (!FOLD) s[i] -= lse;
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] *= a.scale_log2;
+                for (int i = 0; i < 16; ++i) s[i] = FOLD ? s[i] * a.scale_log2 : __builtin_fmaf(s[i], a.scale_log2, -lse);
             }
             if (half != 0xffffffffu) {
                 const unsigned mine = half >> (4 * h);
@@ -894,7 +902,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
             hi[x] = centre + ENTRY * a.rb.limit;
         }
     }
-    constexpr bool HALF = __is_same(T, _Float16);
+    constexpr bool HALF = __is_same(T, _Float16), FOLD = fold_start<T>();
     constexpr float P_LOG2 = HALF ? 10.0f : 0.0f, P_UNSCALE = HALF ? 1.0f / 1024.0f : 1.0f;
     float ds_scale = 1.0f, ds_unscale = 1.0f;       // of dS beside that of P
     if constexpr (HALF) {
@@ -932,9 +940,9 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
         if (tid < 2 * TL::ROWS) {
             const int r = row0 + tid % TL::ROWS;
             const float* src = tid < TL::ROWS ? a.lse : a.delta;
-            // what the accumulators start at: -lse / scale and -delta; a row that does not exist has lse = +inf, so p = 0
+            // what the accumulators start at: -lse / scale (fp32: -lse, added at the end) and -delta; a row that does not exist has lse = +inf, so p = 0
             const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
-            snext = tid < TL::ROWS ? (P_LOG2 - x) / a.scale_log2 : -x;
+            snext = tid < TL::ROWS && FOLD ? (P_LOG2 - x) / a.scale_log2 : -x;
         }
         if constexpr (AXES > 0) pos_next.load(qpos, row0, a.Lq);
     };
@@ -969,7 +977,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = nb * 32 + acc_row(i, h);
-                s[i] = start[r];
+                s[i] = FOLD ? start[r] : 0.0f;
                 dp[i] = start[TL::ROWS + r];
             }
 #pragma unroll
@@ -988,6 +996,7 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
                 } else {
                     x = s[i] * a.scale_log2;
                 }
+                if constexpr (!FOLD) x += start[nb * 32 + acc_row(i, h)];
                 s[i] = __builtin_amdgcn_exp2f(x);
                 dp[i] *= HALF ? s[i] * ds_scale : s[i];
             }

@@ -74,23 +74,28 @@ __device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 2
 
 // Two additions to a thread's own histogram column, per axis, at byte offsets.  Plain reads and writes, because nobody else touches the
 // column: an LDS float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a dependent
-// read-add-write).  The two cells of an axis may be the same one.
+// read-add-write).  The two cells of an axis may be the same one.  What stands between fetch and add covers the read's way.
 template <int AXES>
-__device__ __forceinline__ void hist_add2(char* column, const unsigned (&at0)[AXES], float v0, const unsigned (&at1)[AXES], float v1) {
+struct HistPair {
     float x0[AXES], x1[AXES];
+
+    __device__ __forceinline__ void fetch(const char* column, const unsigned (&at0)[AXES], const unsigned (&at1)[AXES]) {
 #pragma unroll
-    for (int a = 0; a < AXES; ++a) {
-        x0[a] = *reinterpret_cast<float*>(column + at0[a]);
-        x1[a] = *reinterpret_cast<float*>(column + at1[a]);
+        for (int a = 0; a < AXES; ++a) {
+            x0[a] = *reinterpret_cast<const float*>(column + at0[a]);
+            x1[a] = *reinterpret_cast<const float*>(column + at1[a]);
+        }
     }
+    __device__ __forceinline__ void add(char* column, const unsigned (&at0)[AXES], float v0, const unsigned (&at1)[AXES], float v1) {
 #pragma unroll
-    for (int a = 0; a < AXES; ++a) {
-        x0[a] += v0;
-        x1[a] = (at0[a] == at1[a] ? x0[a] : x1[a]) + v1;
-    }
+        for (int a = 0; a < AXES; ++a) {
+            x0[a] += v0;
+            x1[a] = (at0[a] == at1[a] ? x0[a] : x1[a]) + v1;
+        }
 #pragma unroll
-    for (int a = 0; a < AXES; ++a) {
-        *reinterpret_cast<float*>(column + at0[a]) = x0[a];
-        *reinterpret_cast<float*>(column + at1[a]) = x1[a];
+        for (int a = 0; a < AXES; ++a) {
+            *reinterpret_cast<float*>(column + at0[a]) = x0[a];
+            *reinterpret_cast<float*>(column + at1[a]) = x1[a];
+        }
     }
-}
+};

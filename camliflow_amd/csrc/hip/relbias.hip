@@ -71,7 +71,7 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
     char* column = reinterpret_cast<char*>(hist + tid);
     const int tx = tid % cols, ty = tid / cols, per = BLOCK / cols, j = (blockIdx.y * cols + tx) * VEC;
     const int64_t first = (int64_t)blockIdx.x * per + ty;
-    const int step = gridDim.x * per;
+    const int step = gridDim.x * per, step_b = step / Lq, step_i = step - step_b * Lq;
     if (j < Lk && first < rows) {
         const int centre = (int)lds_address(bucket + r.limit), lo = centre - 2 * r.limit, hi = centre + 2 * r.limit, B = (int)(rows / Lq);
         int b = (int)(first / Lq), i = (int)(first - (int64_t)b * Lq), of = -1;      // of: the sample whose positions kp holds
@@ -88,7 +88,12 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
             for (int e = 0; e < VEC; ++e) now[e] = v[e];
 #pragma unroll
             for (int a = 0; a < AXES; ++a) qs[a] = scale_pos<2>(q[a]);
-            for (i += step; i >= Lq; i -= Lq) ++b;
+            b += step_b;
+            i += step_i;
+            if (i >= Lq) {
+                i -= Lq;
+                ++b;
+            }
             if (b < B) {
                 load_f32<T, VEC>(g + (((int64_t)b * H + h) * Lq + i) * Lk + j, v);
 #pragma unroll
@@ -108,7 +113,11 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
                 for (int e = 0; e < VEC; ++e) n[e][a] = (a * r.buckets + lds_load<unsigned short>(med3(kp[a][e] - qs[a], lo, hi))) * (BLOCK * (unsigned)sizeof(float));
             if constexpr (VEC > 1) {
 #pragma unroll
-                for (int e = 0; e < VEC; e += 2) hist_add2<AXES>(column, n[e], now[e], n[e + 1], now[e + 1]);
+                for (int e = 0; e < VEC; e += 2) {
+                    HistPair<AXES> cell;
+                    cell.fetch(column, n[e], n[e + 1]);
+                    cell.add(column, n[e], now[e], n[e + 1], now[e + 1]);
+                }
             } else {
 #pragma unroll
                 for (int a = 0; a < AXES; ++a) *reinterpret_cast<float*>(column + n[0][a]) += now[0];

@@ -332,6 +332,13 @@ __device__ __forceinline__ unsigned long long kept_bits(const unsigned char* mas
     return __ballot(k);
 }
 
+// is streamed row acc_row(i, this lane's half) kept: the lanes' answers as a scalar mask, no vector instruction
+__device__ __forceinline__ bool kept_row(unsigned kept, int i) {
+    const int r = acc_row(i, 0);
+    const unsigned lo = (unsigned)((int)(kept << (31 - r)) >> 31), hi = (unsigned)((int)(kept << (27 - r)) >> 31);
+    return __builtin_amdgcn_inverse_ballot_w64((unsigned long long)hi << 32 | lo);
+}
+
 constexpr float LOG2E = 1.4426950408889634f;
 
 // The bias of a pair comes from a table in LDS (rel_bias: relbias.h); query positions are the negated side.
@@ -664,9 +671,11 @@ __device__ __forceinline__ float unit_scale(float x) {
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
 // HIST: with the table's gradient; its tiles are 32 rows in one buffer, so that two workgroups still share a CU beside their histograms
 // (one waits at a barrier while the other computes).
+constexpr int dq_tile_rows(int size, int dp, bool hist) { return size == 2 && (!hist || dp == 32) ? 64 : 32; }
+
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
 __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
-    constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
+    constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
     using TL = Tile<T, DP, R>;
     using Frag = FragOf<T>;
     using Entry = __type_pack_element<HIST ? 1 : 0, float, Entry8>;
@@ -761,7 +770,6 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
     acc16 dq[TL::DBLOCKS];
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = acc16{0};
-
     Stream<T, DP, R, THREADS> st;
     StreamPos<AXES, TL::BLOCKS, ENTRY> pos, pos_next;
     st.init(a.ks.l, a.vs.l);
@@ -818,17 +826,18 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
                 for (int i = 0; i < 16; ++i) s[i] = FOLD ? s[i] * a.scale_log2 : __builtin_fmaf(s[i], a.scale_log2, -lse);
             }
             if (half != 0xffffffffu) {
-                const unsigned mine = half >> (4 * h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = (mine >> acc_row(i, 0)) & 1 ? s[i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) s[i] = kept_row(half, i) ? s[i] : -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(s[i]);
             if constexpr (HIST) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    if constexpr (__is_same(T, _Float16)) hist_add2<AXES>(column, at_hist[i], dp[i] * unscale, at_hist[i + 1], dp[i + 1] * unscale);
-                    else hist_add2<AXES>(column, at_hist[i], dp[i], at_hist[i + 1], dp[i + 1]);
+                    const float d0 = __is_same(T, _Float16) ? dp[i] * unscale : dp[i], d1 = __is_same(T, _Float16) ? dp[i + 1] * unscale : dp[i + 1];
+                    HistPair<AXES> cell;
+                    cell.fetch(column, at_hist[i], at_hist[i + 1]);
+                    cell.add(column, at_hist[i], d0, at_hist[i + 1], d1);
                 }
             }
 #pragma unroll
@@ -1095,7 +1104,7 @@ int run_fwd(const Args& a, hipStream_t s) {
 
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
 int run_dq_mode(const Args& a, hipStream_t s) {
-    constexpr int R = sizeof(T) == 2 && !HIST ? 64 : 32;
+    constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
     static unsigned long long done = 0;
     size_t lds = tile_bytes<T, DP, R>() / (HIST ? 2 : 1) + lut_bytes(a, AXES, 1);
     if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * 64 * WAVES;      // entries of 8 bytes

@@ -5,7 +5,7 @@ namespace {
 
 using xattn::Args;
 
-int tile_rows(int type, bool histogram = false) { return type == CAMLI_F32 || histogram ? 32 : 64; }
+int tile_rows(int type) { return type == CAMLI_F32 ? 32 : 64; }
 
 // Few owned rows leave CUs idle: the streamed side is cut until there are `want` workgroups, but into no less than `least` tiles a
 // piece (a piece pays for its start and for its part of the join).
@@ -36,7 +36,7 @@ int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.
 void plan_dq(Args& a, int type, int axes, bool table) {
     a.pack = 1;
     a.row_tiles = camli_divup(a.Lq, 32 * dq_waves(a, axes, table));
-    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, tile_rows(type, table)), 1024, 4);
+    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, xattn::dq_tile_rows(camli_type_size(type), a.D <= 32 ? 32 : 64, table)), 1024, 4);
     a.parts = a.B * a.row_tiles * a.splits;
 }
 

@@ -13,8 +13,7 @@
 //   * softmax statistics are per lane: no cross-lane traffic but one half-wave swap per tile,
 //   * the same registers, rounded to the element type, ARE the B operand of the second product (the contraction order over the
 //     streamed rows is free as long as both operands agree on it): P never leaves the registers,
-//   * the A operand of the second product is the streamed tile transposed; 16-bit types read it with the transposing LDS load,
-//     fp32 with plain 4-byte reads, which are conflict-free on row-major tiles.
+//   * the A operand of the second product is the streamed tile transposed, read with the transposing LDS load.
 // Register i of half h holds streamed row 8 (i / 4) + 4 h + i % 4 of its 32-row block.
 //
 // fp16 dS: p (dp - D) of a long row is of the size of |go| / Lk, below fp16's normal numbers for quite ordinary gradients.  go is therefore taken
@@ -61,7 +60,7 @@ typedef unsigned uint2v __attribute__((ext_vector_type(2)));
 typedef unsigned chunk16 __attribute__((ext_vector_type(4)));       // 16 bytes in flight
 
 // 16-byte fragments: what a lane holds of one operand for one k-step
-template <typename T> struct Mat;
+template <typename L> struct Mat;
 template <> struct Mat<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ acc16 mma(frag a, frag b, acc16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -70,121 +69,158 @@ template <> struct Mat<_Float16> {
     typedef _Float16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ acc16 mma(frag a, frag b, acc16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
-template <> struct Mat<float> {
-    typedef float frag __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ acc16 mma(frag a, frag b, acc16 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-        return c;
-    }
+
+// fp32 operands are held as three bf16 parts, x = x0 + x1 + x2 exactly (each the rounding of what is left: 8 + 8 + 8 bits), and a product
+// is the six terms a0 b0, a0 b1, a1 b0, a1 b1, a0 b2, a2 b0 in fp32 accumulators, smallest first.  What is left out, a1 b2 + a2 b1 + a2 b2,
+// is at most 2^-25 of |a| |b|: less than fp32's own rounding of the product.  A 32 x 32 x 32 product takes 384 cycles of the matrix
+// unit so, 1024 as fp32 instructions (2 x 2048 queries x 8160 keys x 4 heads of 32 with a two-axis bias, forward and backward: 854 -> 588 us;
+// heads of 128 without one: 2650 -> 1730 us).  (An infinity has no parts: it comes out as NaN.)
+template <typename T> struct Parts {
+    typedef T Lds;
+    static constexpr int N = 1;
+};
+template <> struct Parts<float> {
+    typedef __bf16 Lds;
+    static constexpr int N = 3;
 };
 
 template <typename T>
-using FragOf = typename Mat<T>::frag;
-
-// A tile of R streamed rows in LDS.  16-bit rows are unpadded and their 16-byte chunks permuted by an XOR with bits of the row, chosen
-// so that both readers hit every bank equally: 16 lanes reading one chunk of 16 rows, and the transposing load's 8 rows x 64 bytes.
-// fp32 rows are padded by 16 bytes, which does the same for 16-byte row reads and leaves the 4-byte column reads at fixed offsets.
-template <typename T, int DP, int R>
-struct Tile {
-    static constexpr int E = 16 / sizeof(T);            // elements of a 16-byte chunk
-    static constexpr int CHUNKS = DP / E;               // chunks of a row
-    static constexpr int ROWS = R;
-    static constexpr int BLOCKS = ROWS / 32;
-    static constexpr int LD = sizeof(T) == 2 ? DP : DP + E;
-    static constexpr int ELEMS = ROWS * LD;
-    static constexpr int KSTEPS = CHUNKS / 2;           // k-steps of a product over DP
-    static constexpr int PSTEPS = 16 / E;               // k-steps of a product over 32 streamed rows
-    static constexpr int DBLOCKS = DP / 32;
-
-    static __device__ __forceinline__ int swizzle(int row) {
-        if constexpr (sizeof(T) == 4) return 0;
-        else if constexpr (CHUNKS == 4) return (row >> 2) & 3;
-        else if constexpr (CHUNKS == 8) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
-        else return (row & 7) << 1 | ((row >> 3) & 1);
-    }
-    static __device__ __forceinline__ int chunk_at(int row, int c) { return row * LD + (c ^ swizzle(row)) * E; }
+struct Frag {
+    typename Mat<typename Parts<T>::Lds>::frag part[Parts<T>::N];
 };
 
-// Where a lane reads in a tile (element offsets from the start of a 32-row block; loop-invariant).
-template <typename T, int DP>
-struct LaneMap {
-    using TL = Tile<T, DP, 32>;
-    using Frag = FragOf<T>;
-    int row[TL::KSTEPS];                                        // A operand of products over DP: row lane % 32, chunk 2 s + half
-    int col[sizeof(T) == 2 ? TL::DBLOCKS : 1][2];               // A operand of products over the streamed rows
-
-    __device__ __forceinline__ explicit LaneMap(int lane) {
-        const int h = lane >> 5, l = lane & 15;
-#pragma unroll
-        for (int s = 0; s < TL::KSTEPS; ++s) row[s] = TL::chunk_at(lane & 31, 2 * s + h);
-        if constexpr (sizeof(T) == 2) {
-            // the transposing load: 16 lanes fetch 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows each
-#pragma unroll
-            for (int d = 0; d < TL::DBLOCKS; ++d)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int c = d * 32 + (lane & 16) + (l & 3) * 4;
-                    col[d][u] = TL::chunk_at(4 * h + (l >> 2) + 8 * u, c / TL::E) + c % TL::E;
-                }
-        } else {
-            col[0][0] = col[0][1] = 4 * h * TL::LD + (lane & 31);
-        }
+template <typename T>
+__device__ __forceinline__ acc16 mma(const Frag<T>& a, const Frag<T>& b, acc16 c) {
+    using M = Mat<typename Parts<T>::Lds>;
+    if constexpr (Parts<T>::N == 3) {
+        c = M::mma(a.part[2], b.part[0], c);
+        c = M::mma(a.part[0], b.part[2], c);
+        c = M::mma(a.part[1], b.part[1], c);
+        c = M::mma(a.part[1], b.part[0], c);
+        c = M::mma(a.part[0], b.part[1], c);
     }
-    __device__ __forceinline__ Frag read_row(const T* block, int s) const { return *reinterpret_cast<const Frag*>(block + row[s]); }
-    // column 32 d + lane % 32 of the rows of k-step t, in the order the accumulator has them
-    __device__ __forceinline__ Frag read_col(const T* block, int t, int d) const {
-        Frag f;
-        if constexpr (sizeof(T) == 2) {
-            typedef __attribute__((address_space(3))) short4v* lds_ptr;
-            union { short4v s[2]; Frag f; } u;
-            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(block + 16 * t * TL::LD + col[d][0])));
-            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<T*>(block + 16 * t * TL::LD + col[d][1])));
-            f = u.f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = block[(8 * t + i) * TL::LD + 32 * d + col[0][0]];
-        }
-        return f;
-    }
-};
+    return M::mma(a.part[0], b.part[0], c);
+}
 
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// k-step t of the accumulator, rounded to the element type (in pairs: one conversion instruction rounds two)
+// 8 floats -> the parts of type T (in pairs: one conversion instruction rounds two)
 template <typename T>
-__device__ __forceinline__ FragOf<T> pack_step(const acc16& x, int t) {
-    constexpr int E = 16 / sizeof(T);
-    FragOf<T> f;
+__device__ __forceinline__ Frag<T> to_frag(const float (&x)[8]) {
+    typedef typename Parts<T>::Lds L;
+    typedef L pair __attribute__((ext_vector_type(2)));
+    Frag<T> f;
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-        const float2v v = {x[t * E + i], x[t * E + i + 1]};
-        if constexpr (__is_same(T, __bf16)) {
-            const bf16x2 r = __builtin_convertvector(v, bf16x2);
-            f[i] = r[0];
-            f[i + 1] = r[1];
-        } else if constexpr (__is_same(T, _Float16)) {
-            const f16x2 r = __builtin_convertvector(v, f16x2);
-            f[i] = r[0];
-            f[i + 1] = r[1];
-        } else {
-            f[i] = v[0];
-            f[i + 1] = v[1];
+    for (int i = 0; i < 8; i += 2) {
+        float2v v = {x[i], x[i + 1]};
+#pragma unroll
+        for (int n = 0; n < Parts<T>::N; ++n) {
+            const pair r = __builtin_convertvector(v, pair);
+            f.part[n][i] = r[0];
+            f.part[n][i + 1] = r[1];
+            v[0] -= (float)r[0];
+            v[1] -= (float)r[1];
         }
     }
     return f;
 }
 
-// what that rounding left
-template <typename T>
-__device__ __forceinline__ FragOf<T> pack_rest(const acc16& x, const FragOf<T>& rounded, int t) {
-    constexpr int E = 16 / sizeof(T);
-    acc16 rest;
+// A tile of R streamed rows in LDS, one plane per part.  Rows are unpadded and their 16-byte chunks permuted by an XOR with bits of the row,
+// chosen so that both readers hit every bank equally: 16 lanes reading one chunk of 16 rows, and the transposing load's 8 rows x 64 bytes.
+template <typename T, int DP, int R>
+struct Tile {
+    using Lds = typename Parts<T>::Lds;
+    static constexpr int E = 8;                         // elements of a 16-byte chunk
+    static constexpr int CHUNKS = DP / E;               // chunks of a row
+    static constexpr int ROWS = R;
+    static constexpr int BLOCKS = ROWS / 32;
+    static constexpr int PLANE = ROWS * DP;
+    static constexpr int ELEMS = Parts<T>::N * PLANE;
+    static constexpr int KSTEPS = CHUNKS / 2;           // k-steps of a product over DP
+    static constexpr int PSTEPS = 2;                    // k-steps of a product over 32 streamed rows
+    static constexpr int DBLOCKS = DP / 32;
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (CHUNKS == 4) return (row >> 2) & 3;
+        else if constexpr (CHUNKS == 8) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+        else return (row & 7) << 1 | ((row >> 3) & 1);
+    }
+    static __device__ __forceinline__ int chunk_at(int row, int c) { return row * DP + (c ^ swizzle(row)) * E; }
+};
+
+// rows of a streamed tile: what a thread of 256 can fetch at once in narrow heads, what two buffers leave room for in wide fp32 ones
+constexpr int tile_rows(int size, int dp) { return size == 2 || dp == 32 ? 64 : 32; }
+// dq with a histogram beside one buffer: two workgroups a CU need tiles of at most 12 KB
+constexpr int dq_tile_rows(int size, int dp, bool hist) { return !hist ? tile_rows(size, dp) : size == 2 && dp == 32 ? 64 : 32; }
+
+// Where a lane reads in a tile (element offsets from the start of a 32-row block; loop-invariant).
+template <typename TL, typename T>
+struct LaneMap {
+    using L = typename TL::Lds;
+    int row[TL::KSTEPS];                                        // A operand of products over DP: row lane % 32, chunk 2 s + half
+    int col[TL::DBLOCKS][2];                                    // A operand of products over the streamed rows
+
+    __device__ __forceinline__ explicit LaneMap(int lane) {
+        const int h = lane >> 5, l = lane & 15;
 #pragma unroll
-    for (int i = 0; i < E; ++i) rest[i] = x[t * E + i] - (float)rounded[i];
-    return pack_step<T>(rest, 0);
+        for (int s = 0; s < TL::KSTEPS; ++s) row[s] = TL::chunk_at(lane & 31, 2 * s + h);
+        // the transposing load: 16 lanes fetch 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows each
+#pragma unroll
+        for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int c = d * 32 + (lane & 16) + (l & 3) * 4;
+                col[d][u] = TL::chunk_at(4 * h + (l >> 2) + 8 * u, c / TL::E) + c % TL::E;
+            }
+    }
+    __device__ __forceinline__ Frag<T> read_row(const L* block, int s) const {
+        Frag<T> f;
+#pragma unroll
+        for (int n = 0; n < Parts<T>::N; ++n) f.part[n] = *reinterpret_cast<const typename Mat<L>::frag*>(block + n * TL::PLANE + row[s]);
+        return f;
+    }
+    // column 32 d + lane % 32 of the rows of k-step t, in the order the accumulator has them
+    __device__ __forceinline__ Frag<T> read_col(const L* block, int t, int d) const {
+        typedef __attribute__((address_space(3))) short4v* lds_ptr;
+        Frag<T> f;
+#pragma unroll
+        for (int n = 0; n < Parts<T>::N; ++n) {
+            union { short4v s[2]; typename Mat<L>::frag f; } u;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                u.s[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<L*>(block + n * TL::PLANE + 16 * t * 32 * TL::DBLOCKS + col[d][i])));
+            f.part[n] = u.f;
+        }
+        return f;
+    }
+};
+
+// c + block . own over DP
+template <typename T, typename TL>
+__device__ __forceinline__ acc16 product(const LaneMap<TL, T>& map, const typename TL::Lds* block, const Frag<T>* own, acc16 c) {
+#pragma unroll
+    for (int ks = 0; ks < TL::KSTEPS; ++ks) c = mma<T>(map.read_row(block, ks), own[ks], c);
+    return c;
+}
+
+// k-step t of the accumulator as an operand of type T
+template <typename T>
+__device__ __forceinline__ Frag<T> pack_step(const acc16& x, int t) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[t * 8 + i];
+    return to_frag<T>(v);
+}
+
+// what that rounding left (16-bit types)
+template <typename T>
+__device__ __forceinline__ Frag<T> pack_rest(const acc16& x, const Frag<T>& rounded, int t) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[t * 8 + i] - (float)rounded.part[0][i];
+    return to_frag<T>(v);
 }
 
 __device__ __forceinline__ acc16 splat(float x) {
@@ -228,9 +264,11 @@ __device__ __forceinline__ int unit_per_xcd(int id, int n, int chunk) {
 template <typename T, int DP, int R, int THREADS>
 struct Stream {
     using TL = Tile<T, DP, R>;
-    static constexpr int ALL = TL::ROWS * TL::CHUNKS, N = (ALL + THREADS - 1) / THREADS;      // the narrowest tile has chunks for half the threads
+    using L = typename TL::Lds;
+    static constexpr int ALL = TL::ROWS * TL::CHUNKS, N = (ALL + THREADS - 1) / THREADS;      // the smallest tile has chunks for half the threads
+    static constexpr int C = TL::E * sizeof(T) / 16;                                           // loads a chunk
     static_assert(ALL % THREADS == 0 || N == 1, "a whole number of chunks a thread");
-    chunk16 x[N], y[N];
+    chunk16 x[N][C], y[N][C];
     unsigned at_x[N], at_y[N];
     unsigned keep;
     bool whole;
@@ -239,7 +277,7 @@ struct Stream {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS;
-            const unsigned c = (f % TL::CHUNKS) * 16;
+            const unsigned c = (f % TL::CHUNKS) * 16 * C;
             at_x[n] = (unsigned)(f / TL::CHUNKS) * (unsigned)(ldx * (int)sizeof(T)) + c;
             at_y[n] = (unsigned)(f / TL::CHUNKS) * (unsigned)(ldy * (int)sizeof(T)) + c;
         }
@@ -250,56 +288,95 @@ struct Stream {
         whole = ALL >= THREADS && row0 + TL::ROWS <= limit && D == DP && mask == nullptr;
         if (whole) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                x[n] = *reinterpret_cast<const chunk16*>(bx + at_x[n]);
-                y[n] = *reinterpret_cast<const chunk16*>(by + at_y[n]);
-            }
+            for (int n = 0; n < N; ++n) fetch(n, bx, by);
             return;
         }
         keep = 0;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS, row = row0 + f / TL::CHUNKS, c = (f % TL::CHUNKS) * TL::E;
-            x[n] = y[n] = chunk16{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < C; ++i) x[n][i] = y[n][i] = chunk16{0, 0, 0, 0};
             if (row < limit && c < D && (ALL >= THREADS || f < ALL)) {
-                x[n] = *reinterpret_cast<const chunk16*>(bx + at_x[n]);
-                y[n] = *reinterpret_cast<const chunk16*>(by + at_y[n]);
+                fetch(n, bx, by);
                 keep |= (mask == nullptr || mask[row] != 0 ? 1u : 0u) << n;
             }
         }
     }
-    __device__ __forceinline__ void store(T* tx, T* ty) const {
-        const chunk16 zero = {0, 0, 0, 0};
-        if (whole) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int f = threadIdx.x + n * THREADS, at = TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS);
-                *reinterpret_cast<chunk16*>(tx + at) = x[n];
-                *reinterpret_cast<chunk16*>(ty + at) = y[n];
-            }
-            return;
-        }
+    __device__ __forceinline__ void store(L* tx, L* ty) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS, at = TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS);
             if (ALL < THREADS && f >= ALL) break;
-            const bool k = (keep >> n) & 1;
-            *reinterpret_cast<chunk16*>(tx + at) = k ? x[n] : zero;
-            *reinterpret_cast<chunk16*>(ty + at) = k ? y[n] : zero;
+            put(tx + at, x[n], whole || ((keep >> n) & 1));
+            put(ty + at, y[n], whole || ((keep >> n) & 1));
+        }
+    }
+
+private:
+    __device__ __forceinline__ void fetch(int n, const char* bx, const char* by) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            x[n][i] = *reinterpret_cast<const chunk16*>(bx + at_x[n] + 16 * i);
+            y[n][i] = *reinterpret_cast<const chunk16*>(by + at_y[n] + 16 * i);
+        }
+    }
+    static __device__ __forceinline__ void put(L* to, const chunk16 (&v)[C], bool kept) {
+        const chunk16 zero = {0, 0, 0, 0};
+        if constexpr (C == 1) {
+            *reinterpret_cast<chunk16*>(to) = kept ? v[0] : zero;
+        } else {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = kept ? __uint_as_float(v[i / 4][i % 4]) : 0.0f;
+            const Frag<T> parts = to_frag<T>(f);
+#pragma unroll
+            for (int n = 0; n < Parts<T>::N; ++n) *reinterpret_cast<typename Mat<L>::frag*>(to + n * TL::PLANE) = parts.part[n];
         }
     }
 };
 
-// owned row -> B fragments (zeros beyond D and for rows that do not exist)
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        load_f32<T, 8>(p, v);
+    } else {
+        float a[4], b[4];
+        load_f32<T, 4>(p, a);
+        load_f32<T, 4>(p + 4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    }
+}
+
+// The matrix unit aligns the terms of a sum to the largest and cuts what is below, downwards: every fp32 dp comes out 4e-8 (at |dp| of 6) too low,
+// nothing to a gradient's element, but the bias table's gradient adds whole rows of ds that cancel and was off by 2e-5 of its size.  So every
+// other owned row enters dp with its sign turned, and the shifts cancel.
+template <typename T>
+__device__ __forceinline__ float dp_sign(int lane) { return sizeof(T) == 4 && (lane & 1) ? -1.0f : 1.0f; }
+
+// owned row, times sign (fp32) -> B fragments (zeros beyond D and for rows that do not exist)
 template <typename T, int DP>
-__device__ __forceinline__ void load_owned(FragOf<T>* f, const T* row, bool exists, int D, int h) {
+__device__ __forceinline__ void load_owned(Frag<T>* f, const T* row, bool exists, int D, int h, float sign = 1.0f) {
     using TL = Tile<T, DP, 32>;
 #pragma unroll
     for (int s = 0; s < TL::KSTEPS; ++s) {
         const int c = (2 * s + h) * TL::E;
-        FragOf<T> z = {};
-        f[s] = z;
-        if (exists && c < D) f[s] = *reinterpret_cast<const FragOf<T>*>(row + c);
+        f[s] = Frag<T>{};
+        if (exists && c < D) {
+            if constexpr (sizeof(T) == 2) {
+                f[s].part[0] = *reinterpret_cast<const typename Mat<T>::frag*>(row + c);
+            } else {
+                float v[8];
+                load8(row + c, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= sign;
+                f[s] = to_frag<T>(v);
+            }
+        }
     }
 }
 
@@ -429,15 +506,15 @@ template <typename T>
 constexpr float exponent_limit() { return __is_same(T, _Float16) ? 14.0f : 30.0f; }
 
 template <typename T, int DP, int AXES, bool TRAIN>
-__global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeof(T) == 2 && AXES == 0) ? 2 : 1) void fwd_kernel(Args a) {
-    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+__global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : DP == 64 || (sizeof(T) == 2 && AXES == 0) ? 2 : 1) void fwd_kernel(Args a) {
+    constexpr int R = tile_rows(sizeof(T), DP);
     using TL = Tile<T, DP, R>;
-    using Frag = FragOf<T>;
+    using L = typename TL::Lds;
     constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
     constexpr bool TWO_TERMS = TRAIN && sizeof(T) == 2, FOLD = AXES > 0 && fold_start<T>();
     constexpr unsigned long long ALL_KEPT = R == 64 ? ~0ull : (1ull << R) - 1;
     extern __shared__ __align__(16) char smem[];
-    T* tiles = reinterpret_cast<T*>(smem);                                  // [2][K, V]
+    L* tiles = reinterpret_cast<L*>(smem);                                  // [2][K, V]
     float* lut = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
@@ -459,7 +536,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
     const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
     const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
 
-    Frag qf[TL::KSTEPS];
+    Frag<T> qf[TL::KSTEPS];
     load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + qi * a.qs.l + head * a.qs.h, exists, a.D, h);
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
@@ -474,7 +551,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
             hi[x] = centre + 4 * a.rb.limit;
         }
     }
-    const LaneMap<T, DP> map(lane);
+    const LaneMap<TL, T> map(lane);
 
     acc16 o[TL::DBLOCKS];
 #pragma unroll
@@ -502,15 +579,13 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
             st.load(kp + (t + 1) * (int64_t)TL::ROWS * a.ks.l, vp + (t + 1) * (int64_t)TL::ROWS * a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
             if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
-        const T *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
+        const L *kt = tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
         if (bits != 0 && busy) {
             acc16 s[TL::BLOCKS];
             float top = -INFINITY;
 #pragma unroll
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-                s[nb] = FOLD ? start : acc16{0};
-#pragma unroll
-                for (int ks = 0; ks < TL::KSTEPS; ++ks) s[nb] = Mat<T>::mma(map.read_row(kt + nb * 32 * TL::LD, ks), qf[ks], s[nb]);
+                s[nb] = product<T, TL>(map, kt + nb * 32 * DP, qf, FOLD ? start : acc16{0});
             }
             if constexpr (AXES > 0) {
 #pragma unroll
@@ -569,20 +644,20 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES ? 3 : 4) : DP == 64 || (sizeo
                 }
 #pragma unroll
                 for (int ps = 0; ps < TL::PSTEPS; ++ps) {
-                    const Frag p = pack_step<T>(s[nb], ps);
-                    Frag rest;
+                    const Frag<T> p = pack_step<T>(s[nb], ps);
+                    Frag<T> rest;
                     if constexpr (TWO_TERMS) rest = pack_rest<T>(s[nb], p, ps);
 #pragma unroll
                     for (int d = 0; d < TL::DBLOCKS; ++d) {
-                        const Frag v = map.read_col(vt + nb * 32 * TL::LD, ps, d);
-                        o[d] = Mat<T>::mma(v, p, o[d]);
-                        if constexpr (TWO_TERMS) o[d] = Mat<T>::mma(v, rest, o[d]);
+                        const Frag<T> v = map.read_col(vt + nb * 32 * DP, ps, d);
+                        o[d] = mma<T>(v, p, o[d]);
+                        if constexpr (TWO_TERMS) o[d] = mma<T>(v, rest, o[d]);
                     }
                 }
             }
         }
         if (t + 1 < t1) {
-            T* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
+            L* nk = tiles + (cur ^ 1) * 2 * TL::ELEMS;
             st.store(nk, nk + TL::ELEMS);
         }
         __syncthreads();
@@ -671,17 +746,15 @@ __device__ __forceinline__ float unit_scale(float x) {
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
 // HIST: with the table's gradient; its tiles are 32 rows in one buffer, so that two workgroups still share a CU beside their histograms
 // (one waits at a barrier while the other computes).
-constexpr int dq_tile_rows(int size, int dp, bool hist) { return size == 2 && (!hist || dp == 32) ? 64 : 32; }
-
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
-__global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
+__global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof(T) == 4 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
     constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
     using TL = Tile<T, DP, R>;
-    using Frag = FragOf<T>;
+    using L = typename TL::Lds;
     using Entry = __type_pack_element<HIST ? 1 : 0, float, Entry8>;
     constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = (int)sizeof(Entry);
     extern __shared__ __align__(16) char smem[];
-    T* tiles = reinterpret_cast<T*>(smem);
+    L* tiles = reinterpret_cast<L*>(smem);
     Entry* lut = reinterpret_cast<Entry*>(tiles + (HIST ? 2 : 4) * TL::ELEMS);
     const int span = 2 * a.rb.limit + 1, hist_rows = AXES * a.rb.buckets;
     float* hist = reinterpret_cast<float*>(lut + AXES * span);
@@ -706,34 +779,33 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
     const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
     const int64_t at = ((int64_t)b * a.Lq + q0) * a.H + head, stat = ((int64_t)b * a.H + head) * a.Lq + q0;
 
-    Frag qf[TL::KSTEPS], gf[TL::KSTEPS];
+    Frag<T> qf[TL::KSTEPS], gf[TL::KSTEPS];
     load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + q0 * a.qs.l + head * a.qs.h, exists, a.D, h);
-    load_owned<T, DP>(gf, static_cast<const T*>(a.go) + at * a.D, exists, a.D, h);
-    float delta = 0.0f;
-    {
-        Frag of[TL::KSTEPS];
-        load_owned<T, DP>(of, static_cast<const T*>(a.o) + at * a.D, exists, a.D, h);
+    const float sign = dp_sign<T>(lane);
+    load_owned<T, DP>(gf, static_cast<const T*>(a.go) + at * a.D, exists, a.D, h, sign);
+    float delta = 0.0f, most = 0.0f;
 #pragma unroll
-        for (int s = 0; s < TL::KSTEPS; ++s)
+    for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+        const int c = (2 * ks + h) * TL::E;
+        if (exists && c < a.D) {
+            float g[8], o[8];
+            load8(static_cast<const T*>(a.go) + at * a.D + c, g);
+            load8(static_cast<const T*>(a.o) + at * a.D + c, o);
 #pragma unroll
-            for (int e = 0; e < TL::E; ++e) delta = __builtin_fmaf((float)of[s][e], (float)gf[s][e], delta);
-        if constexpr (sizeof(T) == 2) {
-            load_owned<T, DP>(of, static_cast<const T*>(a.o_rest) + at * a.D, exists, a.D, h);
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(o[e], g[e], delta);
+            if constexpr (sizeof(T) == 2) {
+                load8(static_cast<const T*>(a.o_rest) + at * a.D + c, o);
 #pragma unroll
-            for (int s = 0; s < TL::KSTEPS; ++s)
+                for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(o[e], g[e], delta);
+            }
 #pragma unroll
-                for (int e = 0; e < TL::E; ++e) delta = __builtin_fmaf((float)of[s][e], (float)gf[s][e], delta);
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(g[e]));
         }
-        delta = half_sum(delta);
     }
+    delta = half_sum(delta);
     if (exists && split == 0 && h == 0) a.delta[stat] = delta;
     float unscale = 1.0f;
     if constexpr (__is_same(T, _Float16)) {
-        float most = 0.0f;
-#pragma unroll
-        for (int s = 0; s < TL::KSTEPS; ++s)
-#pragma unroll
-            for (int e = 0; e < TL::E; ++e) most = fmaxf(most, fabsf((float)gf[s][e]));
         most = half_max(most);
         if (exists && split == 0 && h == 0) a.go_max[stat] = most;
         const float f = unit_scale(most);
@@ -742,14 +814,14 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
 #pragma unroll
         for (int s = 0; s < TL::KSTEPS; ++s)
 #pragma unroll
-            for (int e = 0; e < TL::E; ++e) gf[s][e] = (T)((float)gf[s][e] * f);
+            for (int e = 0; e < TL::E; ++e) gf[s].part[0][e] = (T)((float)gf[s].part[0][e] * f);
     }
     // the accumulators start at -lse / scale and -delta: the products come out as the exponent and as dp - D.  +inf (a row without keys,
     // or none at all) makes every p zero.
     constexpr bool FOLD = fold_start<T>();
     const float lse = exists ? a.lse[stat] : INFINITY;
-    const acc16 start_s = FOLD ? splat(-lse / a.scale_log2) : acc16{0}, start_d = splat(-delta);
-    const LaneMap<T, DP> map(lane);
+    const acc16 start_s = FOLD ? splat(-lse / a.scale_log2) : acc16{0}, start_d = FOLD ? splat(-delta) : acc16{0};
+    const LaneMap<TL, T> map(lane);
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
     if constexpr (AXES > 0) {
@@ -787,17 +859,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
             st.load(kp + (t + 1) * (int64_t)TL::ROWS * a.ks.l, vp + (t + 1) * (int64_t)TL::ROWS * a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
             if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
         }
-        const T *kt = HIST ? tiles : tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
+        const L *kt = HIST ? tiles : tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
             const unsigned half = (unsigned)(bits >> (nb * 32));
             if (half == 0) continue;
-            acc16 s = start_s, dp = start_d;
-            const T *kb = kt + nb * 32 * TL::LD, *vb = vt + nb * 32 * TL::LD;
-#pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(map.read_row(kb, ks), qf[ks], s);
-#pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(vb, ks), gf[ks], dp);
+            const L *kb = kt + nb * 32 * DP, *vb = vt + nb * 32 * DP;
+            acc16 s = product<T, TL>(map, kb, qf, start_s), dp = product<T, TL>(map, vb, gf, start_d);
             unsigned at_hist[16][AXES ? AXES : 1];
             if constexpr (AXES > 0) {
                 int off[AXES][16];
@@ -830,7 +898,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
                 for (int i = 0; i < 16; ++i) s[i] = kept_row(half, i) ? s[i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(s[i]);
+            for (int i = 0; i < 16; ++i) dp[i] = (FOLD ? dp[i] : __builtin_fmaf(dp[i], sign, -delta)) * __builtin_amdgcn_exp2f(s[i]);
             if constexpr (HIST) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
@@ -842,14 +910,14 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
-                const Frag p = pack_step<T>(dp, ps);
+                const Frag<T> p = pack_step<T>(dp, ps);
 #pragma unroll
-                for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = Mat<T>::mma(map.read_col(kb, ps, d), p, dq[d]);
+                for (int d = 0; d < TL::DBLOCKS; ++d) dq[d] = mma<T>(map.read_col(kb, ps, d), p, dq[d]);
             }
         }
         if constexpr (HIST) __syncthreads();
         if (t + 1 < t1) {
-            T* nk = HIST ? tiles : tiles + (cur ^ 1) * 2 * TL::ELEMS;
+            L* nk = HIST ? tiles : tiles + (cur ^ 1) * 2 * TL::ELEMS;
             st.store(nk, nk + TL::ELEMS);
         }
         __syncthreads();
@@ -873,13 +941,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 ? 2 : 3) 
 
 // ------------------------------------------------------------------------------------------------------------ dk, dv
 template <typename T, int DP, int AXES>
-__global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_kernel(Args a) {
-    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+__global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64 ? 2 : 1) void dkdv_kernel(Args a) {
+    constexpr int R = tile_rows(sizeof(T), DP);
     using TL = Tile<T, DP, R>;
-    using Frag = FragOf<T>;
+    using L = typename TL::Lds;
     constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
     extern __shared__ __align__(16) char smem[];
-    T* tiles = reinterpret_cast<T*>(smem);                                              // [2][Q, dO]
+    L* tiles = reinterpret_cast<L*>(smem);                                              // [2][Q, dO]
     float* stats = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);                     // [2][lse, delta][ROWS]
     float* lut = reinterpret_cast<float*>(stats + 4 * TL::ROWS);
 
@@ -894,11 +962,12 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
     const int len = kept_length(a, b);
     bool kept = kj < len;
     if (kept && a.mask) kept = a.mask[b * a.mask_bs + kj] != 0;
-    const LaneMap<T, DP> map(lane);
+    const LaneMap<TL, T> map(lane);
 
-    Frag kf[TL::KSTEPS], vf[TL::KSTEPS];
+    Frag<T> kf[TL::KSTEPS], vf[TL::KSTEPS];
+    const float sign = dp_sign<T>(lane);
     load_owned<T, DP>(kf, static_cast<const T*>(a.k) + b * a.ks.b + (int64_t)kj * a.ks.l + kvh * a.ks.h, kept, a.D, h);
-    load_owned<T, DP>(vf, static_cast<const T*>(a.v) + b * a.vs.b + (int64_t)kj * a.vs.l + kvh * a.vs.h, kept, a.D, h);
+    load_owned<T, DP>(vf, static_cast<const T*>(a.v) + b * a.vs.b + (int64_t)kj * a.vs.l + kvh * a.vs.h, kept, a.D, h, sign);
     int ka[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* qpos = nullptr;
     if constexpr (AXES > 0) {
@@ -949,14 +1018,14 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
         if (tid < 2 * TL::ROWS) {
             const int r = row0 + tid % TL::ROWS;
             const float* src = tid < TL::ROWS ? a.lse : a.delta;
-            // what the accumulators start at: -lse / scale (fp32: -lse, added at the end) and -delta; a row that does not exist has lse = +inf, so p = 0
+            // what the accumulators start at: -lse / scale (fp32: -lse, and both are added at the end) and -delta; a row that does not exist has lse = +inf, so p = 0
             const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
             snext = tid < TL::ROWS && FOLD ? (P_LOG2 - x) / a.scale_log2 : -x;
         }
         if constexpr (AXES > 0) pos_next.load(qpos, row0, a.Lq);
     };
     auto store = [&](int buf) {
-        T* n = tiles + buf * 2 * TL::ELEMS;
+        L* n = tiles + buf * 2 * TL::ELEMS;
         st.store(n, n + TL::ELEMS);
         if (tid < 2 * TL::ROWS) stats[buf * 2 * TL::ROWS + tid] = snext;
     };
@@ -977,22 +1046,20 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
                 __syncthreads();
             }
         }
-        const T *qt = tiles + cur * 2 * TL::ELEMS, *gt = qt + TL::ELEMS;
+        const L *qt = tiles + cur * 2 * TL::ELEMS, *gt = qt + TL::ELEMS;
         const float* start = stats + cur * 2 * TL::ROWS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-            const T *qb = qt + nb * 32 * TL::LD, *gb = gt + nb * 32 * TL::LD;
+            const L *qb = qt + nb * 32 * DP, *gb = gt + nb * 32 * DP;
             acc16 s, dp;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = nb * 32 + acc_row(i, h);
                 s[i] = FOLD ? start[r] : 0.0f;
-                dp[i] = start[TL::ROWS + r];
+                dp[i] = FOLD ? start[TL::ROWS + r] : 0.0f;
             }
-#pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) s = Mat<T>::mma(map.read_row(qb, ks), kf[ks], s);
-#pragma unroll
-            for (int ks = 0; ks < TL::KSTEPS; ++ks) dp = Mat<T>::mma(map.read_row(gb, ks), vf[ks], dp);
+            s = product<T, TL>(map, qb, kf, s);
+            dp = product<T, TL>(map, gb, vf, dp);
             int off[AXES ? AXES : 1][16];
 #pragma unroll
             for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], ka[x], off[x]);
@@ -1005,17 +1072,20 @@ __global__ __launch_bounds__(256, DP == 32 ? 3 : DP == 64 ? 2 : 1) void dkdv_ker
                 } else {
                     x = s[i] * a.scale_log2;
                 }
-                if constexpr (!FOLD) x += start[nb * 32 + acc_row(i, h)];
+                if constexpr (!FOLD) {
+                    x += start[nb * 32 + acc_row(i, h)];
+                    dp[i] = __builtin_fmaf(dp[i], sign, start[TL::ROWS + nb * 32 + acc_row(i, h)]);
+                }
                 s[i] = __builtin_amdgcn_exp2f(x);
                 dp[i] *= HALF ? s[i] * ds_scale : s[i];
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
-                const Frag p = pack_step<T>(s, ps), ds = pack_step<T>(dp, ps);
+                const Frag<T> p = pack_step<T>(s, ps), ds = pack_step<T>(dp, ps);
 #pragma unroll
                 for (int d = 0; d < TL::DBLOCKS; ++d) {
-                    dv[d] = Mat<T>::mma(map.read_col(gb, ps, d), p, dv[d]);
-                    dk[d] = Mat<T>::mma(map.read_col(qb, ps, d), ds, dk[d]);
+                    dv[d] = mma<T>(map.read_col(gb, ps, d), p, dv[d]);
+                    dk[d] = mma<T>(map.read_col(qb, ps, d), ds, dk[d]);
                 }
             }
         }
@@ -1070,7 +1140,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(SumJobs jobs) {
 constexpr size_t MAX_LDS = 159 * 1024;      // of a CU's 160 KB; the bias borders are static
 
 template <typename T, int DP, int R>
-constexpr size_t tile_bytes() { return 4 * sizeof(T) * Tile<T, DP, R>::ELEMS; }
+constexpr size_t tile_bytes() { return 4 * sizeof(typename Parts<T>::Lds) * Tile<T, DP, R>::ELEMS; }
 
 inline size_t lut_bytes(const Args& a, int axes, int heads) { return axes ? sizeof(float) * heads * axes * (2 * a.rb.limit + 1) : 0; }
 
@@ -1086,7 +1156,7 @@ int start(K kernel, const char* what, unsigned long long& done, dim3 grid, int t
 
 template <typename T, int DP, int AXES, bool TRAIN>
 int run_fwd_mode(const Args& a, hipStream_t s) {
-    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+    constexpr int R = tile_rows(sizeof(T), DP);
     static unsigned long long done = 0;
     const size_t lds = tile_bytes<T, DP, R>() + lut_bytes(a, AXES, a.pack);
     return start(fwd_kernel<T, DP, AXES, TRAIN>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, a, s);
@@ -1125,7 +1195,7 @@ int run_dq(const Args& a, int waves, hipStream_t s) {
 
 template <typename T, int DP, int AXES>
 int run_dkdv(const Args& a, hipStream_t s) {
-    constexpr int R = sizeof(T) == 2 ? 64 : 32;
+    constexpr int R = tile_rows(sizeof(T), DP);
     static unsigned long long done = 0;
     const size_t lds = tile_bytes<T, DP, R>() + sizeof(float) * 4 * R + lut_bytes(a, AXES, 1);
     return start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);

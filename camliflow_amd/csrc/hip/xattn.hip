@@ -5,11 +5,13 @@ namespace {
 
 using xattn::Args;
 
-int tile_rows(int type) { return type == CAMLI_F32 ? 32 : 64; }
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int tile_rows(const Args& a, int type) { return xattn::tile_rows(camli_type_size(type), padded(a.D)); }
 
-// Few owned rows leave CUs idle: the streamed side is cut until there are `want` workgroups, but into no less than `least` tiles a
-// piece (a piece pays for its start and for its part of the join).
-void split_stream(Args& a, int64_t base, int n_tiles, int want, int least) {
+// Few owned rows leave CUs idle: the streamed side is cut until there are `want` workgroups, but into no less than `least_rows` rows a
+// piece (a piece pays for its start and for its part of the join; fp32 rows take twice the time of 16-bit ones).
+void split_stream(Args& a, int64_t base, int n_tiles, int tile, int want, int least_rows) {
+    const int least = camli_divup(least_rows, tile);
     int splits = 1;
     if (base < want / 2) {
         splits = (int)((want + base - 1) / base);
@@ -27,8 +29,8 @@ void plan_fwd(Args& a, int type, int axes) {
     a.pack = group > 1 && (int64_t)a.Lq * group <= 128 && xattn::lut_bytes(a, axes, group) <= 16384 ? group : 1;
     a.row_tiles = camli_divup(a.pack * a.Lq, 128);
     // one wave of rows: the pieces are short, bound by latency, and cost little to join
-    const int least = a.pack * (int64_t)a.Lq <= 32 ? 2 : 4;
-    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile_rows(type)), 1024, least);
+    const int least = (a.pack * (int64_t)a.Lq <= 32 ? 128 : 256) / (type == CAMLI_F32 ? 2 : 1), tile = tile_rows(a, type);
+    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile), tile, 1024, least);
 }
 
 int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.buckets > 64 ? 2 : 4; }
@@ -36,14 +38,16 @@ int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.
 void plan_dq(Args& a, int type, int axes, bool table) {
     a.pack = 1;
     a.row_tiles = camli_divup(a.Lq, 32 * dq_waves(a, axes, table));
-    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, xattn::dq_tile_rows(camli_type_size(type), a.D <= 32 ? 32 : 64, table)), 1024, 4);
+    const int tile = xattn::dq_tile_rows(camli_type_size(type), padded(a.D), table);
+    split_stream(a, (int64_t)a.row_tiles * a.H * a.B, camli_divup(a.Lk, tile), tile, 1024, type == CAMLI_F32 || table ? 128 : 256);
     a.parts = a.B * a.row_tiles * a.splits;
 }
 
 void plan_dkdv(Args& a, int type) {
     a.pack = 1;
     a.row_tiles = camli_divup(a.Lk, 128);
-    split_stream(a, (int64_t)a.row_tiles * a.Hk * a.B, camli_divup(a.Lq, tile_rows(type)) * (a.H / a.Hk), 1024, 4);
+    const int tile = tile_rows(a, type);
+    split_stream(a, (int64_t)a.row_tiles * a.Hk * a.B, camli_divup(a.Lq, tile) * (a.H / a.Hk), tile, 1024, type == CAMLI_F32 ? 128 : 256);
 }
 
 bool operand_ok(const void* p, const int64_t* stride, int size) {

@@ -17,6 +17,8 @@ from .wrapper import _on_device, _require_cuda, _stream_ptr
 MAX_HEAD_DIM = 128
 MAX_BIAS_ROWS = 128
 MAX_BIAS_DISTANCE = 1023
+MAX_BIAS_HEADS = 65535
+MAX_POSITION = 2 ** 26
 
 
 # ------------------------------------------------------------------------------------------------
@@ -46,9 +48,9 @@ def _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, dtype, h
     if table.dim() != 3 or table.dtype != dtype or dtype not in TYPE_CODES:
         raise ValueError('%s: the table must be [axes, buckets, heads] of type %s, got %s %s' % (name, dtype, tuple(table.shape), table.dtype))
     axes, buckets, h = table.shape
-    if axes not in (1, 2) or axes * buckets > MAX_BIAS_ROWS or h < 1 or (heads is not None and h != heads):
-        raise ValueError('%s: the table needs 1 or 2 axes, axes * buckets <= %d%s, got %s' % (
-            name, MAX_BIAS_ROWS, '' if heads is None else ' and %d heads' % heads, tuple(table.shape)))
+    if axes not in (1, 2) or axes * buckets > MAX_BIAS_ROWS or not 1 <= h <= MAX_BIAS_HEADS or (heads is not None and h != heads):
+        raise ValueError('%s: the table needs 1 or 2 axes, axes * buckets <= %d and %s heads, got %s' % (
+            name, MAX_BIAS_ROWS, heads if heads is not None and heads <= MAX_BIAS_HEADS else '1 .. %d' % MAX_BIAS_HEADS, tuple(table.shape)))
     side = buckets // 2 if bidirectional else buckets
     if side < 2 or (bidirectional and buckets % 2) or not side // 2 < max_distance <= MAX_BIAS_DISTANCE or int(max_distance) != max_distance:
         raise ValueError('%s: need at least two buckets a side (an even number when bidirectional) and %d < max_distance <= %d, got %d buckets and %r'
@@ -76,7 +78,8 @@ def _composed_bias(table, q_pos, k_pos, bidirectional, max_distance):
     lut = torch.tensor(_bucket_of_offsets(buckets, bool(bidirectional), int(max_distance)), device=table.device)
     total = 0
     for a in range(axes):
-        offset = k_pos[..., None, :, a].long() - q_pos[..., :, None, a].long()
+        offset = (k_pos[..., None, :, a].clamp(-MAX_POSITION, MAX_POSITION).long()
+                  - q_pos[..., :, None, a].clamp(-MAX_POSITION, MAX_POSITION).long())
         total = total + table[a].float()[lut[offset.clamp(-max_distance, max_distance) + max_distance]]
     return total.movedim(-1, -3)            # [(B,) H, Lq, Lk]
 
@@ -132,11 +135,11 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
     """The learned bias of every query and key by their bucketed offset, [H, Lq, Lk] ([B, H, Lq, Lk] where a position tensor has a
     batch): sum over axes a of table[a, bucket(k_pos[j, a] - q_pos[i, a]), h].
 
-    ``table`` [axes, buckets, H] (fp32, bf16 or fp16; the result has its type); ``q_pos`` / ``k_pos`` int32 [L, axes] or [B, L, axes], any
-    whole numbers (the running index of a sequence, pixel coordinates).  ``bidirectional``: half the buckets for each sign, the upper half
+    ``table`` [axes, buckets, H] (fp32, bf16 or fp16; the result has its type); ``q_pos`` / ``k_pos`` int32 [L, axes] or [B, L, axes], whole
+    numbers (the running index of a sequence, pixel coordinates); beyond -2^26 .. 2^26 they count as that bound.  ``bidirectional``: half the buckets for each sign, the upper half
     for keys after the query; otherwise all buckets for keys before the query, and keys after it share bucket 0.  Of the s buckets of a
     side, e = s // 2 hold one distance each; bucket e + j begins at the first distance >= e (max_distance / e)^(j / (s - e)), and the last
-    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023.  Differentiable in the table (once);
+    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023; at most 65535 samples x heads, 2000000 queries, 16000000 keys.  Differentiable in the table (once);
     the same bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
     name = 'relative_position_bias'
     table, q_pos, k_pos, batch, _ = _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, table.dtype if table is not None else None)
@@ -289,7 +292,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
                     q_pos=None, k_pos=None, bidirectional=True, max_distance=128, cpp_impl=True):
     """softmax(scale q k^T + bias) v of queries q [B, Lq, H, D] over keys and values k, v [B, Lk, Hk, D] of another length -> [B, Lq, H, D].
 
-    fp32, bf16 or fp16 (one type for all; sums and softmax in fp32); D a multiple of 8 up to 128; H a multiple of Hk (query heads
+    fp32, bf16 or fp16 (one type for all; sums and softmax in fp32; fp32 factors go through the matrix unit as three bf16 parts each, exact to
+    2^-25, so an infinity or a value beyond 3.38e38 among kept fp32 operands gives NaN); D a multiple of 8 up to 128; H a multiple of Hk (query heads
     h share key / value head h // (H / Hk)).  Any strides: rows that are not adjacent or 16-byte aligned are copied first.  ``scale``:
     from 1e-15 to 1e15, default D ** -0.5.  One token (Lq = 1) and other short queries are split over the keys.
 

@@ -88,6 +88,10 @@ bool make_args(Args& a, const camli_attention* d, const char* who) {
     a.B = d->B; a.H = d->H; a.Hk = d->Hk; a.Lq = d->Lq; a.Lk = d->Lk; a.D = d->D;
     a.scale = d->scale;
     a.scale_log2 = d->scale * xattn::LOG2E;
+    if (d->bias_axes != 0 && d->H > 65535) {
+        camli_set_error("%s: a position bias takes at most 65535 heads (H=%d)", who, d->H);
+        return false;
+    }
     if (d->bias_axes != 0 && !rel_bias_args(a.rb, who, d->bias_table, d->type, d->q_pos, d->q_pos_batch_stride, d->k_pos, d->k_pos_batch_stride,
                                             d->bias_axes, d->bias_buckets, d->bias_two_sided, d->bias_max_distance))
         return false;

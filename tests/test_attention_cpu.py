@@ -66,6 +66,21 @@ def test_bias_refuses():
             csrc.relative_position_bias(table, q, k, cpp_impl=False, **kw)
 
 
+def test_bias_refuses_more_heads_than_a_launch_holds():
+    wide = torch.zeros(1).expand(1, 8, 65536)
+    with pytest.raises(ValueError, match='65535'):
+        csrc.relative_position_bias(wide, _pos(3), _pos(3), cpp_impl=False)
+    with pytest.raises(ValueError, match='65535'):
+        csrc.cross_attention(torch.zeros(1).expand(1, 3, 65536, 8), *[torch.zeros(1, 3, 1, 8)] * 2, bias_table=wide, q_pos=_pos(3), k_pos=_pos(3), cpp_impl=False)
+
+
+def test_bias_positions_count_as_their_bound():
+    table = torch.arange(8, dtype=torch.float32).view(1, 8, 1)
+    far = torch.tensor([[2 ** 31 - 1], [2 ** 26], [2 ** 26 - 1], [-2 ** 31]], dtype=torch.int32)
+    got = csrc.relative_position_bias(table, far, far, max_distance=8, cpp_impl=False)[0]
+    assert got.tolist() == [[0, 0, 1, 3], [0, 0, 1, 3], [5, 5, 0, 3], [7, 7, 7, 0]]
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason='CPU-only behaviour')
 def test_operators_refuse_cpu_tensors():
     with pytest.raises(_lib.CamliHipError):

@@ -232,6 +232,84 @@ def test_attention_gradients_scale_with_the_incoming_gradient(dtype, factor):
         assert ((a - b).abs() <= 2 * step + lost + 1e-6 * b.abs().max()).all(), name
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('exponent', [-90, 60])
+def test_attention_gradients_keep_their_bits_under_powers_of_two(dtype, exponent):
+    """every step is linear in the incoming gradient and these types have range to spare: the same bits, shifted"""
+    c = _case(1, 70, 150, 2, 1, 40, dtype, axes=2, seed=17)
+    base = _run(c)
+    c['go'] = c['go'] * 2.0 ** exponent
+    for name, t in _run(c).items():
+        assert torch.equal(t.double(), base[name].double() * (1.0 if name == 'out' else 2.0 ** exponent)), name
+
+
+@pytest.mark.parametrize('magnitude', [1e-30, 1e30])
+def test_attention_fp32_products_over_the_range(magnitude):
+    """values and keys far from 1: an fp32 factor's three parts still hold all of its bits"""
+    c = _case(1, 33, 130, 2, 1, 32, torch.float32, seed=18)
+    c['v'], c['k'], c['q'] = c['v'] * magnitude, c['k'] * magnitude, c['q'] / magnitude
+    c['go'] = c['go'] / magnitude
+    _check(c)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('dim,axes,buckets,bidirectional', [(128, 2, 64, True), (64, 1, 128, False), (32, 2, 64, False)])
+def test_attention_largest_tables(dtype, dim, axes, buckets, bidirectional):
+    """what takes the most shared memory: two columns of 2047 offsets and 128 histogram rows beside the widest tiles"""
+    c = _case(1, 140, 200, 2, 1, dim, dtype, axes=axes, buckets=buckets, max_distance=1023, seed=19)
+    c['qp'], c['kp'] = c['qp'] * 12, c['kp'] * 12
+    _check(c, bidirectional=bidirectional)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+def test_attention_rows_without_keys_take_no_part(dtype):
+    """a sample without keys, by length or by mask: its gradient may be anything and reaches nothing"""
+    c = _case(3, 37, 65, 2, 2, 32, dtype, axes=2, lengths=[65, 0, 65], masked=0.2, seed=20)
+    c['mask'][2] = False
+    c['keep'][2] = False
+    c['go'][1:] = 0
+    want = _run(c)
+    c['go'][1] = float('nan')
+    c['go'][2] = float('inf')
+    for name, t in _run(c).items():
+        assert torch.equal(t, want[name]), name
+    assert not want['dq'][1:].any() and not want['dk'][1:].any() and not want['dv'][1:].any()
+
+
+def test_attention_broadcast_gradient_and_strided_masks():
+    from camliflow_amd import csrc
+    c = _case(2, 50, 90, 4, 2, 64, torch.bfloat16, axes=1, lengths=[90, 41], masked=0.3, seed=21)
+    c['go'] = torch.ones_like(c['go'])
+    want = _run(c)
+    kvl = torch.stack([c['kvl'], c['kvl']], dim=1).cuda()[:, 0]
+    mask = c['mask'].t().contiguous().cuda().t()
+    pos = torch.cat([c['qp'], c['qp']], dim=1).cuda()[:, :1]
+    assert not kvl.is_contiguous() and not mask.is_contiguous() and not pos.is_contiguous()
+    leaves = {n: c[n].cuda().requires_grad_(True) for n in ('q', 'k', 'v', 'table')}
+    out = csrc.cross_attention(leaves['q'], leaves['k'], leaves['v'], kv_lengths=kvl, key_mask=mask, bias_table=leaves['table'], q_pos=pos,
+                               k_pos=c['kp'].cuda(), max_distance=c['max_distance'])
+    out.sum().backward()            # an expanded gradient
+    for name, leaf in leaves.items():
+        assert torch.equal(leaf.grad, want['d' + name])
+
+
+def test_attention_two_streams_at_once():
+    """calls of different sizes in flight on two streams do not touch each other's workspaces"""
+    cases = [_case(2, 300, 700, 4, 2, 32, torch.bfloat16, axes=2, seed=22), _case(1, 1, 3000, 4, 1, 64, torch.float32, seed=23)]
+    want = [_run(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for _ in range(5):
+        for c, stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                got.append(_run(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for name, t in g.items():
+            assert torch.equal(t, want[i % 2][name]), name
+
+
 def test_attention_same_bits_every_run_and_refuses_double_backward():
     c = _case(2, 150, 333, 4, 2, 64, torch.bfloat16, axes=2, lengths=[333, 100], seed=12)
     first = _run(c)
@@ -300,6 +378,20 @@ def test_bias_extreme_positions():
     kp = torch.tensor([[hi], [1], [lo]], dtype=torch.int32).cuda()
     got = csrc.relative_position_bias(table, qp, kp)[0].cpu() / 2
     assert got.tolist() == [[31, 31, 0], [31, 17, 15], [0, 15, 15]]
+
+
+def test_bias_many_short_samples():
+    """one query a sample: the backward's rows walk over many samples at a step"""
+    from camliflow_amd import csrc
+    g = torch.Generator().manual_seed(0)
+    table = torch.zeros(1, 8, 2).cuda().requires_grad_(True)
+    qp = torch.randint(-9, 9, (9000, 1, 1), generator=g, dtype=torch.int32).cuda()
+    kp = torch.randint(-9, 9, (9000, 3, 1), generator=g, dtype=torch.int32).cuda()
+    out = csrc.relative_position_bias(table, qp, kp, max_distance=8)
+    go = torch.randint(-4, 5, out.shape, generator=g).float().cuda()        # whole numbers: every sum is exact
+    grad, = torch.autograd.grad(out, table, go)
+    plain, = torch.autograd.grad(csrc.relative_position_bias(table, qp, kp, max_distance=8, cpp_impl=False), table, go)
+    assert torch.equal(grad, plain)
 
 
 # ------------------------------------------------------------------------------------------------ group norm

@@ -207,7 +207,7 @@ def _sizes(q, k, table, bidirectional, max_distance):
 
 
 def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance, train):
-    """-> (out, operands as the kernels read them, out's rounding error, row log-sums)"""
+    """-> (out, operands as the kernels read them, 16-bit types' out before its rounding, row log-sums)"""
     b, lq, h, dim = q.shape
     lk, hk = k.shape[1:3]
     if q.numel() == 0 or lk == 0:
@@ -216,30 +216,30 @@ def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bi
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if train else None
-    rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    out_f32 = torch.empty(out.shape, dtype=torch.float32, device=q.device) if train and q.dtype != torch.float32 else None
     desc = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
     n = _attention_workspace_bytes(False, False, *_sizes(q, k, table, bidirectional, max_distance))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     with _on_device(q):
-        _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, desc, out.data_ptr(), address(rest), address(lse), address(ws), n,
+        _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, desc, out.data_ptr(), address(out_f32), address(lse), address(ws), n,
                     _stream_ptr(q), work=(2.0 * q.element_size() * dim * b * (lq * h + lk * hk), 'B'), flop=4.0 * b * h * lq * lk * dim)
-    return out, (q, k, v), rest, lse
+    return out, (q, k, v), out_f32, lse
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance):
         ctx.args = (scale, bidirectional, max_distance)
-        out, operands, rest, lse = _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance, True)
-        ctx.save_for_backward(*operands, table, kv_lengths, key_mask, q_pos, k_pos, out if lse is not None else None, rest, lse)
+        out, operands, out_f32, lse = _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bidirectional, max_distance, True)
+        ctx.save_for_backward(*operands, table, kv_lengths, key_mask, q_pos, k_pos, out if out_f32 is None and lse is not None else out_f32, lse)
         return out
 
     @first_order
     def backward(ctx, gout):
-        q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out, rest, lse = ctx.saved_tensors
+        q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, out_f32, lse = ctx.saved_tensors
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
         nothing = (None,) * 7
-        if out is None:
+        if lse is None:
             return (torch.zeros_like(q) if need_q else None, torch.zeros_like(k) if need_k else None,
                     torch.zeros_like(v) if need_v else None, torch.zeros_like(table) if need_t else None) + nothing
         lib = _lib.load()
@@ -258,7 +258,7 @@ class _CrossAttention(torch.autograd.Function):
         n = _attention_workspace_bytes(True, need_t, *_sizes(q, k, table, *ctx.args[1:]))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         with _on_device(q):
-            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, desc, out.data_ptr(), address(rest), gout.data_ptr(),
+            _lib.launch('camli_cross_attention_bwd', lib.camli_cross_attention_bwd, desc, out_f32.data_ptr(), gout.data_ptr(),
                         lse.data_ptr(), address(gq), address(gk), address(gv), address(gt), ws.data_ptr(), n, _stream_ptr(q),
                         work=(4.0 * q.element_size() * dim * b * (lq * h + lk * hk), 'B'), flop=10.0 * b * h * lq * lk * dim)
         return (gq, gk if need_k else None, gv if need_v else None, gt) + nothing

@@ -35,22 +35,42 @@ struct GnArgs {
     float eps;
 };
 
+// e = exp(-|z|): with it sigmoid(|z|) = 1 / (1 + e) and its complement e / (1 + e) lose no digits where the sigmoid saturates.  fp32 maps
+// carry the rounding of the product along (plain exp2(-|z| log2 e) is off by |z| 2^-24).
+template <typename T>
+__device__ __forceinline__ float exp_minus(float z) {
+    constexpr float L = 1.44269502162933349609375f, L_REST = 1.92596299e-8f;      // log2 e
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_amdgcn_exp2f(-fabsf(z) * L);
+    } else {
+        const float a = fabsf(z), x = a > 87.0f ? -87.0f : -a;
+        const float t = x * L, rest = __builtin_fmaf(x, L_REST, __builtin_fmaf(x, L, -t));
+        const float e = __builtin_amdgcn_exp2f(t);
+        return __builtin_fmaf(e, rest * 0.693147181f, e);
+    }
+}
+
+template <typename T>
 __device__ __forceinline__ float act_value(float z, int act) {
     switch (act) {
         case 1: return z > 0.0f || z != z ? z : 0.0f;
         case 2: return z > 0.0f ? z : 0.1f * z;
-        case 3: return 1.0f / (1.0f + __expf(-z));
-        case 6: return z / (1.0f + __expf(-z));
+        case 3: { const float e = exp_minus<T>(z); return (z < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e); }
+        case 6: { const float e = exp_minus<T>(z); return z * ((z < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e)); }
         default: return z;
     }
 }
 
+template <typename T>
 __device__ __forceinline__ float act_slope(float z, int act) {
     switch (act) {
         case 1: return z > 0.0f ? 1.0f : 0.0f;
         case 2: return z > 0.0f ? 1.0f : 0.1f;
-        case 3: { const float s = 1.0f / (1.0f + __expf(-z)); return s * (1.0f - s); }
-        case 6: { const float s = 1.0f / (1.0f + __expf(-z)); return s * __builtin_fmaf(z, 1.0f - s, 1.0f); }
+        case 3: { const float e = exp_minus<T>(z), r = __builtin_amdgcn_rcpf(1.0f + e); return e * r * r; }
+        case 6: {
+            const float e = exp_minus<T>(z), r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+            return (z < 0.0f ? er : r) * __builtin_fmaf(z, z < 0.0f ? r : er, 1.0f);
+        }
         default: return 1.0f;
     }
 }
@@ -180,7 +200,7 @@ __global__ __launch_bounds__(BLOCK) void gn_apply_kernel(GnArgs a, const float2*
             float v[VEC];
             load_f32<T, VEC>(xb + (int64_t)p * a.x_ld + c, v, a.stream);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = act_value(__builtin_fmaf(v[e] - mean[e], scale[e], shift[e]), a.act);
+            for (int e = 0; e < VEC; ++e) v[e] = act_value<T>(__builtin_fmaf(v[e] - mean[e], scale[e], shift[e]), a.act);
             store_f32<T, VEC>(yb + (int64_t)p * a.C + c, v, a.stream);
         }
     }
@@ -245,7 +265,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void gn_small_kernel(GnArgs a, T* __
         const int p = r + i * rows;
         if (p >= a.P) break;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = act_value(__builtin_fmaf(v[i][e], scale[e], shift[e]), a.act);
+        for (int e = 0; e < VEC; ++e) v[i][e] = act_value<T>(__builtin_fmaf(v[i][e], scale[e], shift[e]), a.act);
         store_f32<T, VEC>(yb + (int64_t)p * a.C, v[i]);
     }
 }
@@ -285,7 +305,7 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_sums_kernel(GnArgs a, const T* _
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const float xhat = (v[e] - mean[e]) * rstd[e];
-                    const float dz = g[e] * act_slope(__builtin_fmaf(v[e] - mean[e], rstd[e] * wt[e], shift[e]), a.act);
+                    const float dz = g[e] * act_slope<T>(__builtin_fmaf(v[e] - mean[e], rstd[e] * wt[e], shift[e]), a.act);
                     s0[e] += dz;
                     s1[e] = __builtin_fmaf(dz, xhat, s1[e]);
                 }
@@ -387,7 +407,7 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_dx_kernel(GnArgs a, const T* __r
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float d = v[e] - mean[e], xhat = d * rstd[e];
-                const float dz = g[e] * act_slope(__builtin_fmaf(d, rstd[e] * wt[e], shift[e]), a.act);
+                const float dz = g[e] * act_slope<T>(__builtin_fmaf(d, rstd[e] * wt[e], shift[e]), a.act);
                 v[e] = rstd[e] * (__builtin_fmaf(wt[e], dz, -m0[e]) - xhat * m1[e]);
             }
             store_f32<T, VEC>(gx + dense + (int64_t)p * a.C + c, v, a.stream);

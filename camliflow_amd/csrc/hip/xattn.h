@@ -34,10 +34,11 @@ struct Strides {
 };
 
 struct Args {
-    const void *q, *k, *v, *o, *o_rest, *go;
+    const void *q, *k, *v, *go;
+    const float *o;
     Strides qs, ks, vs;         // o, go and the gradients are dense [B][L][heads][D]
     void *out, *dq, *dk, *dv;
-    void *out_rest;             // 16-bit types in training: out minus its rounding, rounded
+    float *out_f32;             // 16-bit types in training: out before its rounding
     float *lse;                 // [B][H][Lq], log2 domain; +inf where no key is kept
     float *delta;               // [B][H][Lq]
     float *go_max;              // [B][H][Lq] fp16 only: largest |go| of a row
@@ -496,7 +497,7 @@ __device__ __forceinline__ void broadcast_plus(int lanes, int own, int (&out)[16
 // scale), and m is taken from the first tile that has a kept key.  p <= 2^30 (2^14 for fp16) is as good as p <= 1 in floating point, so
 // m moves only when a score passes that: the exchange between the half waves and the rescaling leave the loop, but for a test.
 // TRAIN (16-bit types): out has to be known to more than its own type for the backward's D = do . o, which is subtracted from
-// dp: P enters the product as two terms of the type and the rounding error of out is stored beside it.  Without that the bias table's
+// dp: P enters the product as two terms of the type and out is stored before its rounding as well.  Without that the bias table's
 // gradient, a sum over whole rows of ds, is off by twice its own rounding.
 // fp32 with a bias starts at zero and subtracts m at the end: at -m / scale every step of the product rounds to a few bits less (a relative
 // error of p of 1e-6), which is nothing to a 16-bit product and shows in an fp32 gradient.  The adjoints do the same with the log-sum.
@@ -674,13 +675,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
         if (h == 0) a.part_lse[split * per + stat] = l == 0.0f ? -INFINITY : lse;
     } else {
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, h);
-        if constexpr (TWO_TERMS) {
-#pragma unroll
-            for (int d = 0; d < TL::DBLOCKS; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * inv - (float)(T)(o[d][i] * inv);
-            store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out_rest) + at * a.D, o, 1.0f, a.D, h);
-        }
+        if constexpr (TWO_TERMS) store_owned<float, TL::DBLOCKS>(a.out_f32 + at * a.D, o, inv, a.D, h);
         if (TRAIN && h == 0) a.lse[stat] = l == 0.0f ? INFINITY : lse;
     }
 }
@@ -728,11 +723,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = bad ? NAN : acc[i] * inv;
     store_f32<T, 4>(static_cast<T*>(a.out) + at * a.D + c, acc);
-    if (a.out_rest) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] -= (float)(T)acc[i];
-        store_f32<T, 4>(static_cast<T*>(a.out_rest) + at * a.D + c, acc);
-    }
+    if (a.out_f32) store_f32<float, 4>(a.out_f32 + at * a.D + c, acc);
 }
 
 // power of two that brings x to 1 .. 2 (1 for zero, infinity and NaN)
@@ -790,14 +781,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
         if (exists && c < a.D) {
             float g[8], o[8];
             load8(static_cast<const T*>(a.go) + at * a.D + c, g);
-            load8(static_cast<const T*>(a.o) + at * a.D + c, o);
+            load8(a.o + at * a.D + c, o);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(o[e], g[e], delta);
-            if constexpr (sizeof(T) == 2) {
-                load8(static_cast<const T*>(a.o_rest) + at * a.D + c, o);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(o[e], g[e], delta);
-            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(g[e]));
         }

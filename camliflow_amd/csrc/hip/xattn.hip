@@ -153,18 +153,18 @@ extern "C" int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attenti
     return fwd_workspace(a, nullptr);
 }
 
-extern "C" int camli_cross_attention_fwd(const camli_attention* d, void* out, void* out_rest, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int camli_cross_attention_fwd(const camli_attention* d, void* out, float* out_f32, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
     Args a;
     if (!make_args(a, d, "camli_cross_attention_fwd")) return CAMLI_EINVAL;
     plan_fwd(a, d->type, d->bias_axes);
     const int64_t need = fwd_workspace(a, static_cast<char*>(workspace));
-    const bool rest = lse && d->type != CAMLI_F32;
-    if (!out || (((uintptr_t)out | (uintptr_t)out_rest) & 15) || (rest && !out_rest) || (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))) {
+    const bool two = lse && d->type != CAMLI_F32;
+    if (!out || (((uintptr_t)out | (uintptr_t)out_f32) & 15) || (two && !out_f32) || (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))) {
         camli_set_error("camli_cross_attention_fwd: output or workspace missing, unaligned or too small (%lld bytes needed)", (long long)need);
         return CAMLI_EINVAL;
     }
     a.out = out;
-    a.out_rest = rest ? out_rest : nullptr;
+    a.out_f32 = two ? out_f32 : nullptr;
     a.lse = lse;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (d->type == CAMLI_F32) return xattn::Launch<float>::fwd(a, d->bias_axes, s);
@@ -178,21 +178,20 @@ extern "C" int64_t camli_cross_attention_bwd_workspace_bytes(const camli_attenti
     return plan_bwd(a, d, table_gradient != 0 && d->bias_axes != 0, nullptr).bytes;
 }
 
-extern "C" int camli_cross_attention_bwd(const camli_attention* d, const void* out, const void* out_rest, const void* gout, const float* lse, void* gq, void* gk,
+extern "C" int camli_cross_attention_bwd(const camli_attention* d, const float* out_f32, const void* gout, const float* lse, void* gq, void* gk,
                                          void* gv, void* gtable, void* workspace, int64_t workspace_bytes, void* stream) {
     Args a;
     if (!make_args(a, d, "camli_cross_attention_bwd")) return CAMLI_EINVAL;
     if (gtable && d->bias_axes == 0) { camli_set_error("camli_cross_attention_bwd: a table gradient without a table"); return CAMLI_EINVAL; }
     BwdPlan p = plan_bwd(a, d, gtable != nullptr, static_cast<char*>(workspace));
-    if (!out || !gout || !lse || (d->type != CAMLI_F32 && !out_rest) || (gk == nullptr) != (gv == nullptr) || !workspace || workspace_bytes < p.bytes ||
-        (((uintptr_t)out | (uintptr_t)out_rest | (uintptr_t)gout | (uintptr_t)gq | (uintptr_t)gk | (uintptr_t)gv | (uintptr_t)workspace) & 15)) {
+    if (!out_f32 || !gout || !lse || (gk == nullptr) != (gv == nullptr) || !workspace || workspace_bytes < p.bytes ||
+        (((uintptr_t)out_f32 | (uintptr_t)gout | (uintptr_t)gq | (uintptr_t)gk | (uintptr_t)gv | (uintptr_t)workspace) & 15)) {
         camli_set_error("camli_cross_attention_bwd: an operand is missing or not 16-byte aligned, or the workspace is too small (%lld bytes needed)", (long long)p.bytes);
         return CAMLI_EINVAL;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int axes = d->bias_axes, waves = dq_waves(p.dq, axes, gtable != nullptr);
-    p.dq.o = p.dkdv.o = out;
-    p.dq.o_rest = out_rest;
+    p.dq.o = out_f32;
     p.dq.go = p.dkdv.go = gout;
     p.dq.lse = p.dkdv.lse = const_cast<float*>(lse);
     p.dq.dq = gq;

@@ -766,7 +766,7 @@ int camli_rel_bias_bwd(const void *gout, const int *q_pos, int64_t q_pos_batch_s
  *   bias_axes 0: no bias; else as camli_rel_bias_fwd, table [axes,buckets,H] of `type`, H <= 65535.
  *   fp32 factors are multiplied as three bf16 parts each (exact to 2^-25): a kept infinity, or a value beyond 3.38e38, gives NaN.
  *   lse [B,H,Lq]: log2 of each row's softmax sum, +inf for rows without keys; NULL if no backward follows.
- *   out_rest, like out: what rounding to a 16-bit type took from out, for the backward (unused for fp32 or without lse).
+ *   out_f32 [B,Lq,H,D]: out before its rounding to a 16-bit type, for the backward (fwd: unused for fp32 or without lse; bwd: fp32 out itself).
  *   bwd: gq may be NULL, gk and gv both or neither, gtable [axes,buckets,H] may be NULL; everything given is fully written, no atomics
  *   whose order matters: the same bits on every run.
  * workspace_bytes: negative (an error code) for a descriptor the kernels do not take.
@@ -785,10 +785,10 @@ typedef struct camli_attention {
     int bias_axes, bias_buckets, bias_two_sided, bias_max_distance;
 } camli_attention;
 int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention *desc);
-int camli_cross_attention_fwd(const camli_attention *desc, void *out, void *out_rest, float *lse, void *workspace,
+int camli_cross_attention_fwd(const camli_attention *desc, void *out, float *out_f32, float *lse, void *workspace,
                               int64_t workspace_bytes, void *stream);
 int64_t camli_cross_attention_bwd_workspace_bytes(const camli_attention *desc, int table_gradient);
-int camli_cross_attention_bwd(const camli_attention *desc, const void *out, const void *out_rest, const void *gout, const float *lse,
+int camli_cross_attention_bwd(const camli_attention *desc, const float *out_f32, const void *gout, const float *lse,
                               void *gq, void *gk, void *gv, void *gtable, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

@@ -124,15 +124,15 @@ def test_c_entries_refuse_and_report():
         d.Hk = 2 if name == 'H' else 1
         setattr(d, name, bad)
         assert lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d)) == -22, name
-        assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, 16, 16, 16, 16, 16, 16, null, 16, 1 << 30, null) == -22, name
+        assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, 16, 16, 16, 16, 16, null, 16, 1 << 30, null) == -22, name
         setattr(d, name, keep)
     for row in (-64, 2 ** 23, 66):
         d.k_stride[1] = row
         assert lib.camli_cross_attention_fwd(ctypes.byref(d), 16, null, null, 16, 1 << 30, null) == -22
     d.k_stride[1] = 64
     assert lib.camli_cross_attention_fwd(ctypes.byref(d), 24, null, null, 16, 1 << 30, null) == -22       # unaligned output
-    assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, null, 16, 16, 16, 16, null, null, 16, 1 << 30, null) == -22     # one of gk, gv
-    assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, null, 16, 16, 16, 16, 16, null, 16, 0, null) == -22            # no workspace
+    assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, 16, 16, 16, 16, null, null, 16, 1 << 30, null) == -22     # one of gk, gv
+    assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, 16, 16, 16, 16, 16, null, 16, 0, null) == -22            # no workspace
 
 
 @pytest.mark.parametrize('buckets,two_sided,limit', [(32, 1, 128), (32, 0, 128), (8, 1, 48), (64, 0, 100), (64, 1, 1023), (128, 0, 1023), (4, 1, 2), (2, 0, 2),

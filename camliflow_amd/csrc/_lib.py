@@ -206,7 +206,7 @@ PROTOTYPES = {
     "camli_rel_bias_bwd_workspace_bytes": (ctypes.c_int64, [_int] * 7),
     "camli_rel_bias_bwd": (_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                   ctypes.c_void_p, ctypes.c_int64] + [_int] * 9 + [_stream]),
-    "camli_cross_attention_fwd_workspace_bytes": (ctypes.c_int64, [_desc_p]),
+    "camli_cross_attention_fwd_workspace_bytes": (ctypes.c_int64, [_desc_p, _int]),
     "camli_cross_attention_fwd": (_int, [_desc_p, ctypes.c_void_p, _c_float_p, _c_float_p, ctypes.c_void_p, ctypes.c_int64, _stream]),
     "camli_cross_attention_bwd_workspace_bytes": (ctypes.c_int64, [_desc_p, _int]),
     "camli_cross_attention_bwd": (_int, [_desc_p, _c_float_p, ctypes.c_void_p, _c_float_p] + [ctypes.c_void_p] * 5

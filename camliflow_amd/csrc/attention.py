@@ -183,8 +183,8 @@ def _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidir
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace_bytes(backward, table_gradient, head, bias):
-    """by sizes alone: head = (type, B, H, Hk, Lq, Lk, D), bias = (axes, buckets, bidirectional, max_distance)"""
+def _attention_workspace_bytes(backward, flag, head, bias):
+    """by sizes alone; flag: training (forward), a table gradient (backward); head = (type, B, H, Hk, Lq, Lk, D), bias = (axes, buckets, bidirectional, max_distance)"""
     lib = _lib.load()
     d = _lib.AttentionDesc(*head)
     d.scale = 1.0
@@ -192,8 +192,7 @@ def _attention_workspace_bytes(backward, table_gradient, head, bias):
     if bias[0]:
         d.bias_table = d.q_pos = d.k_pos = 16
         d.bias_axes, d.bias_buckets, d.bias_two_sided, d.bias_max_distance = bias
-    n = (lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), int(table_gradient)) if backward
-         else lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d)))
+    n = (lib.camli_cross_attention_bwd_workspace_bytes if backward else lib.camli_cross_attention_fwd_workspace_bytes)(ctypes.byref(d), int(flag))
     if n < 0:
         _lib.check(int(n), 'camli_cross_attention_%s_workspace_bytes' % ('bwd' if backward else 'fwd'))
     return int(n)
@@ -218,7 +217,7 @@ def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bi
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if train else None
     out_f32 = torch.empty(out.shape, dtype=torch.float32, device=q.device) if train and q.dtype != torch.float32 else None
     desc = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
-    n = _attention_workspace_bytes(False, False, *_sizes(q, k, table, bidirectional, max_distance))
+    n = _attention_workspace_bytes(False, train, *_sizes(q, k, table, bidirectional, max_distance))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     with _on_device(q):
         _lib.launch('camli_cross_attention_fwd', lib.camli_cross_attention_fwd, desc, out.data_ptr(), address(out_f32), address(lse), address(ws), n,

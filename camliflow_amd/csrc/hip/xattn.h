@@ -49,6 +49,7 @@ struct Args {
     const unsigned char *mask;  // [B][mask_bs] or null
     int64_t mask_bs;
     int B, H, Hk, Lq, Lk, D;
+    bool few;                   // fwd_few_kernel
     int pack;                   // query heads of one kv head that share a workgroup's rows (few queries), else 1
     int row_tiles, splits, tiles_per_split, parts;
     float scale, scale_log2;
@@ -259,6 +260,38 @@ __device__ __forceinline__ int unit_per_xcd(int id, int n, int chunk) {
     return unit * chunk + k;
 }
 
+// 8 elements as they came from memory (one or two 16-byte loads) -> the parts of type T
+template <typename T, int C>
+__device__ __forceinline__ Frag<T> chunk_frag(const chunk16 (&v)[C]) {
+    if constexpr (C == 1) {
+        Frag<T> f;
+        f.part[0] = __builtin_bit_cast(typename Mat<T>::frag, v[0]);
+        return f;
+    } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[i / 4][i % 4]);
+        return to_frag<T>(x);
+    }
+}
+// ... into a chunk of a tile, zeros if not kept
+template <typename T, typename TL, int C>
+__device__ __forceinline__ void put_chunk(typename TL::Lds* to, const chunk16 (&v)[C], bool kept) {
+    using L = typename TL::Lds;
+    chunk16 k[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) k[i] = kept ? v[i] : chunk16{0, 0, 0, 0};
+    const Frag<T> parts = chunk_frag<T>(k);
+#pragma unroll
+    for (int n = 0; n < Parts<T>::N; ++n) *reinterpret_cast<typename Mat<L>::frag*>(to + n * TL::PLANE) = parts.part[n];
+}
+// orders a wave's LDS accesses (they execute in order; this keeps the compiler from moving them)
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The streamed pair of tiles on its way from memory: registers now, LDS later.  A row at or beyond `limit`, a masked row and columns
 // from D on become zeros (a masked row may hold anything, and 0 * NaN is NaN); a whole, unmasked tile skips those tests.
 // A thread's place in a tile is a 32-bit byte offset computed once (row strides are below 2^23 elements); the tile's base is uniform.
@@ -309,8 +342,8 @@ struct Stream {
         for (int n = 0; n < N; ++n) {
             const int f = threadIdx.x + n * THREADS, at = TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS);
             if (ALL < THREADS && f >= ALL) break;
-            put(tx + at, x[n], whole || ((keep >> n) & 1));
-            put(ty + at, y[n], whole || ((keep >> n) & 1));
+            put_chunk<T, TL>(tx + at, x[n], whole || ((keep >> n) & 1));
+            put_chunk<T, TL>(ty + at, y[n], whole || ((keep >> n) & 1));
         }
     }
 
@@ -320,19 +353,6 @@ private:
         for (int i = 0; i < C; ++i) {
             x[n][i] = *reinterpret_cast<const chunk16*>(bx + at_x[n] + 16 * i);
             y[n][i] = *reinterpret_cast<const chunk16*>(by + at_y[n] + 16 * i);
-        }
-    }
-    static __device__ __forceinline__ void put(L* to, const chunk16 (&v)[C], bool kept) {
-        const chunk16 zero = {0, 0, 0, 0};
-        if constexpr (C == 1) {
-            *reinterpret_cast<chunk16*>(to) = kept ? v[0] : zero;
-        } else {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = kept ? __uint_as_float(v[i / 4][i % 4]) : 0.0f;
-            const Frag<T> parts = to_frag<T>(f);
-#pragma unroll
-            for (int n = 0; n < Parts<T>::N; ++n) *reinterpret_cast<typename Mat<L>::frag*>(to + n * TL::PLANE) = parts.part[n];
         }
     }
 };
@@ -616,8 +636,8 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
             if constexpr (AXES == 0) top = __builtin_fmaf(top, a.scale_log2, -m_use);
             else if constexpr (!FOLD) top -= m_use;
             if (unset || __any(top > exponent_limit<T>())) {
-                top = half_max(top) + m_use;
-                const float mn = fmaxf(m, top), use = mn == -INFINITY ? 0.0f : mn;
+                top = half_max(top);        // a row's own need decides: its result does not depend on the rows beside it
+                const float mn = m == -INFINITY || top > exponent_limit<T>() ? fmaxf(m, top + m_use) : m, use = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m - use);
 #pragma unroll
                 for (int d = 0; d < TL::DBLOCKS; ++d)
@@ -677,6 +697,193 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, h);
         if constexpr (TWO_TERMS) store_owned<float, TL::DBLOCKS>(a.out_f32 + at * a.D, o, inv, a.D, h);
         if (TRAIN && h == 0) a.lse[stat] = l == 0.0f ? INFINITY : lse;
+    }
+}
+
+// LDS of fwd_few_kernel before its bias columns: the waves' value tiles, later their sums
+template <typename T, int DP>
+__host__ __device__ constexpr size_t few_bytes(int rows) {
+    const size_t tiles = 4 * sizeof(typename Parts<T>::Lds) * Tile<T, DP, 32>::ELEMS, sums = sizeof(float) * 4 * (2 * 32 + (size_t)rows * DP);
+    return tiles > sums ? tiles : sums;
+}
+
+// Few queries without a gradient (at most 32 rows with those of the heads that share keys: single tokens).  The rows fill one wave, and in
+// fwd_kernel the other three would only fetch for it.  Here every wave holds the same rows and takes every fourth tile of 32 keys by itself:
+// keys go from memory straight into the A operand, values through a wave's own piece of LDS (for the transposing read), no barrier until
+// the waves' sums are joined.  Bound by reading keys and values: 16 single tokens of 8 heads of 64 over 0 .. 16384 keys of 2 shared heads
+// (67 MB, bf16) 21.3 us with the join, 3.1 TB/s (fwd_kernel: 24.9); two tiles in flight instead of one: 22.1, 1024 workgroups instead of 512: 23.5.
+template <typename T, int DP, int AXES>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void fwd_few_kernel(Args a) {
+    using TL = Tile<T, DP, 32>;
+    using L = typename TL::Lds;
+    constexpr int WAVES = 4, THREADS = 64 * WAVES, ENTRY = (int)sizeof(float), N = 32 * TL::CHUNKS / 64, C = TL::E * sizeof(T) / 16;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int groups = a.H / a.pack;
+    const int split = blockIdx.x % a.splits, id = blockIdx.x / a.splits;       // pieces of a sample share nothing: spread over the XCDs
+    const int hh = id % groups, b = id / groups, kvh = hh * a.pack / (a.H / a.Hk);
+    const int rows = a.pack * a.Lq, row = lane & 31;
+    const bool exists = row < rows;
+    const int sub = exists ? row / a.Lq : 0, qi = exists ? row - sub * a.Lq : 0, head = hh * a.pack + sub;
+    L* vt = reinterpret_cast<L*>(smem) + wave * TL::ELEMS;
+    float* lut = reinterpret_cast<float*>(smem + few_bytes<T, DP>(rows));
+
+    const int len = kept_length(a, b), n_tiles = (len + 31) / 32;
+    const int t0 = split * a.tiles_per_split, t1 = min(n_tiles, t0 + a.tiles_per_split);
+    const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + kvh * a.ks.h;
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
+
+    Frag<T> qf[TL::KSTEPS];
+    load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + qi * a.qs.l + head * a.qs.h, exists, a.D, h);
+    int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
+    const int* kpos = nullptr;
+    if constexpr (AXES > 0) {
+        fill_lut<AXES, THREADS>(a.rb, lut, hh * a.pack, a.pack, a.H);
+        __syncthreads();
+        kpos = a.rb.kpos + b * a.rb.kpos_bs;
+#pragma unroll
+        for (int x = 0; x < AXES; ++x) {
+            const int centre = (int)lds_address(lut + (sub * AXES + x) * (2 * a.rb.limit + 1) + a.rb.limit);
+            qa[x] = centre + scale_pos<-ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)qi * AXES + x]);
+            lo[x] = centre - ENTRY * a.rb.limit;
+            hi[x] = centre + ENTRY * a.rb.limit;
+        }
+    }
+    const LaneMap<TL, T> map(lane);
+
+    // on its way from memory: the lane's row of keys (of the last key where there is none: masked below), its chunks of values
+    struct InFlight {
+        chunk16 k[TL::KSTEPS][C], v[N][C];
+        StreamPos<AXES, 1, ENTRY> pos;
+    };
+    auto load = [&](InFlight& in, int t) {
+        const T* k = kp + (int64_t)min(t * 32 + row, len - 1) * a.ks.l;
+#pragma unroll
+        for (int s = 0; s < TL::KSTEPS; ++s) {
+            const int c = (2 * s + h) * TL::E;
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                in.k[s][i] = chunk16{0, 0, 0, 0};
+                if (c < a.D) in.k[s][i] = reinterpret_cast<const chunk16*>(k + c)[i];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int f = lane + 64 * n, c = f % TL::CHUNKS * TL::E;
+            const T* v = vp + (int64_t)min(t * 32 + f / TL::CHUNKS, len - 1) * a.vs.l + c;
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                in.v[n][i] = chunk16{0, 0, 0, 0};
+                if (c < a.D) in.v[n][i] = reinterpret_cast<const chunk16*>(v)[i];
+            }
+        }
+        if constexpr (AXES > 0) in.pos.load(kpos, t * 32, len);
+    };
+
+    acc16 o[TL::DBLOCKS];
+#pragma unroll
+    for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = acc16{0};
+    float m = -INFINITY, m_use = 0.0f, l = 0.0f;
+    InFlight in;
+    if (t0 + wave < t1) load(in, t0 + wave);
+    for (int t = t0 + wave; t < t1; t += WAVES) {
+        const unsigned bits = (unsigned)kept_bits(mask, t * 32, len, 32);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int f = lane + 64 * n;
+            put_chunk<T, TL>(vt + TL::chunk_at(f / TL::CHUNKS, f % TL::CHUNKS), in.v[n], (bits >> (f / TL::CHUNKS)) & 1);
+        }
+        acc16 s = acc16{0};
+#pragma unroll
+        for (int ks = 0; ks < TL::KSTEPS; ++ks) s = mma<T>(chunk_frag<T>(in.k[ks]), qf[ks], s);
+        const StreamPos<AXES, 1, ENTRY> pos = in.pos;
+        if (t + WAVES < t1) load(in, t + WAVES);
+        if constexpr (AXES > 0) {
+            int off[AXES][16];
+#pragma unroll
+            for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[0][x], qa[x], off[x]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_fmaf(s[i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
+                if constexpr (AXES > 1) s[i] += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= a.scale_log2;
+        }
+        if (bits != 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = kept_row(bits, i) ? s[i] : -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+        if (__any(m == -INFINITY || top - m_use > exponent_limit<T>())) {
+            top = half_max(top);
+            const float mn = m == -INFINITY || top - m_use > exponent_limit<T>() ? fmaxf(m, top) : m;
+            m_use = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+#pragma unroll
+            for (int d = 0; d < TL::DBLOCKS; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+            l *= alpha;
+            m = mn;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+            l += s[i];
+        }
+        wave_order();       // the values are there for the other lanes
+#pragma unroll
+        for (int ps = 0; ps < TL::PSTEPS; ++ps) {
+            const Frag<T> p = pack_step<T>(s, ps);
+#pragma unroll
+            for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = mma<T>(map.read_col(vt, ps, d), p, o[d]);
+        }
+        wave_order();       // before the next tile's values take their place
+    }
+    l = half_sum(l);
+    __syncthreads();
+    // join the waves: [wave][rows][m, l], [wave][rows][DP]
+    float* stat = reinterpret_cast<float*>(smem);
+    float* sum = stat + WAVES * 2 * 32;
+    if (exists) {
+        if (h == 0) {
+            stat[(wave * 32 + row) * 2] = m;
+            stat[(wave * 32 + row) * 2 + 1] = l;
+        }
+        store_owned<float, TL::DBLOCKS>(sum + (wave * rows + row) * DP, o, 1.0f, a.D, h);
+    }
+    __syncthreads();
+    const int64_t per = (int64_t)a.B * a.Lq * a.H;
+    for (int f = tid; f < rows * (DP / 4); f += THREADS) {
+        const int r = f / (DP / 4), c = f % (DP / 4) * 4;
+        if (c >= a.D) continue;
+        float M = -INFINITY, total = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) M = fmaxf(M, stat[(w * 32 + r) * 2]);
+        const float use = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float g = __builtin_amdgcn_exp2f(stat[(w * 32 + r) * 2] - use);
+            total = __builtin_fmaf(g, stat[(w * 32 + r) * 2 + 1], total);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(g, sum[(w * rows + r) * DP + c + i], acc[i]);
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= inv;
+        const int rs = r / a.Lq, ri = r - rs * a.Lq, rh = hh * a.pack + rs;
+        const int64_t at = ((int64_t)b * a.Lq + ri) * a.H + rh;
+        if (a.splits > 1) {
+            store_f32<float, 4>(a.part_o + (split * per + at) * a.D + c, acc);
+            if (c == 0) a.part_lse[split * per + ((int64_t)b * a.H + rh) * a.Lq + ri] = total == 0.0f ? -INFINITY : use + __builtin_amdgcn_logf(total);
+        } else {
+            store_f32<T, 4>(static_cast<T*>(a.out) + at * a.D + c, acc);
+        }
     }
 }
 
@@ -1149,8 +1356,15 @@ int run_fwd_mode(const Args& a, hipStream_t s) {
 }
 
 template <typename T, int DP, int AXES>
+int run_fwd_few(const Args& a, hipStream_t s) {
+    static unsigned long long done = 0;
+    const size_t lds = few_bytes<T, DP>(a.pack * a.Lq) + lut_bytes(a, AXES, a.pack);
+    return start(fwd_few_kernel<T, DP, AXES>, "camli_cross_attention_fwd", done, dim3(a.H / a.pack * a.B * a.splits), 256, lds, a, s);
+}
+
+template <typename T, int DP, int AXES>
 int run_fwd(const Args& a, hipStream_t s) {
-    const int rc = a.lse ? run_fwd_mode<T, DP, AXES, true>(a, s) : run_fwd_mode<T, DP, AXES, false>(a, s);
+    const int rc = a.few ? run_fwd_few<T, DP, AXES>(a, s) : a.lse ? run_fwd_mode<T, DP, AXES, true>(a, s) : run_fwd_mode<T, DP, AXES, false>(a, s);
     if (rc != CAMLI_OK || a.splits == 1) return rc;
     int lanes = 2;
     while (lanes * 4 < a.D) lanes *= 2;

@@ -22,15 +22,16 @@ void split_stream(Args& a, int64_t base, int n_tiles, int tile, int want, int le
     a.splits = n_tiles ? (n_tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
 }
 
-void plan_fwd(Args& a, int type, int axes) {
+void plan_fwd(Args& a, int type, int axes, bool training) {
     const int group = a.H / a.Hk;
     // the query heads of a kv head share a workgroup where all their rows fit into one and their bias columns into LDS: keys and
     // values are then read once, not once per head
     a.pack = group > 1 && (int64_t)a.Lq * group <= 128 && xattn::lut_bytes(a, axes, group) <= 16384 ? group : 1;
     a.row_tiles = camli_divup(a.pack * a.Lq, 128);
-    // one wave of rows: the pieces are short, bound by latency, and cost little to join
-    const int least = (a.pack * (int64_t)a.Lq <= 32 ? 128 : 256) / (type == CAMLI_F32 ? 2 : 1), tile = tile_rows(a, type);
-    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile), tile, 1024, least);
+    a.few = !training && (int64_t)a.pack * a.Lq <= 32;
+    const int tile = a.few ? 32 : tile_rows(a, type);
+    // few rows: a piece is shared by four waves; 512 workgroups fill the chip and leave half the parts to join (token cases above the kernel)
+    split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile), tile, a.few ? 512 : 1024, a.few ? 512 : type == CAMLI_F32 ? 128 : 256);
 }
 
 int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.buckets > 64 ? 2 : 4; }
@@ -146,17 +147,17 @@ BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base
 
 }  // namespace
 
-extern "C" int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention* d) {
+extern "C" int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention* d, int training) {
     Args a;
     if (!make_args(a, d, "camli_cross_attention_fwd_workspace_bytes")) return CAMLI_EINVAL;
-    plan_fwd(a, d->type, d->bias_axes);
+    plan_fwd(a, d->type, d->bias_axes, training != 0);
     return fwd_workspace(a, nullptr);
 }
 
 extern "C" int camli_cross_attention_fwd(const camli_attention* d, void* out, float* out_f32, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
     Args a;
     if (!make_args(a, d, "camli_cross_attention_fwd")) return CAMLI_EINVAL;
-    plan_fwd(a, d->type, d->bias_axes);
+    plan_fwd(a, d->type, d->bias_axes, lse != nullptr);
     const int64_t need = fwd_workspace(a, static_cast<char*>(workspace));
     const bool two = lse && d->type != CAMLI_F32;
     if (!out || (((uintptr_t)out | (uintptr_t)out_f32) & 15) || (two && !out_f32) || (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))) {

@@ -784,7 +784,7 @@ typedef struct camli_attention {
     int64_t q_pos_batch_stride, k_pos_batch_stride;
     int bias_axes, bias_buckets, bias_two_sided, bias_max_distance;
 } camli_attention;
-int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention *desc);
+int64_t camli_cross_attention_fwd_workspace_bytes(const camli_attention *desc, int training);     /* training: a call with lse */
 int camli_cross_attention_fwd(const camli_attention *desc, void *out, float *out_f32, float *lse, void *workspace,
                               int64_t workspace_bytes, void *stream);
 int64_t camli_cross_attention_bwd_workspace_bytes(const camli_attention *desc, int table_gradient);

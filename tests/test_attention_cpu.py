@@ -110,20 +110,20 @@ def test_c_entries_refuse_and_report():
     assert lib.camli_rel_bias_fwd(1, 1, 0, 1, 0, 1, 1, 1, 3, 3, 1, 300, 1, 128, 0, null) == -22
     assert lib.camli_rel_bias_bwd(1, 1, 0, 1, 0, 1, 1, 0, 1, 1, 3, 3, 1, 32, 1, 128, 0, null) == -22
     d = _lib.AttentionDesc()
-    assert lib.camli_cross_attention_fwd_workspace_bytes(null) == -22
+    assert lib.camli_cross_attention_fwd_workspace_bytes(null, 0) == -22
     assert lib.camli_cross_attention_fwd(ctypes.byref(d), 16, null, null, null, 0, null) == -22
     for name, value in (('type', 0), ('B', 1), ('H', 2), ('Hk', 1), ('Lq', 3), ('Lk', 4), ('D', 32), ('scale', 0.2)):
         setattr(d, name, value)
     d.q, d.k, d.v = 4096, 8192, 12288
     for s in (d.q_stride, d.k_stride, d.v_stride):
         s[0], s[1], s[2] = 0, 64, 32
-    assert lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d)) >= 0
+    assert lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d), 0) >= 0
     assert lib.camli_cross_attention_bwd_workspace_bytes(ctypes.byref(d), 0) > 0
     for name, bad in (('D', 36), ('D', 0), ('H', 3), ('Lk', 0), ('B', 0), ('type', 3), ('scale', 0.0), ('scale', 1e-16), ('k', 8200), ('bias_axes', 1), ('Lq', 2 ** 31 - 1)):
         keep = getattr(d, name)
         d.Hk = 2 if name == 'H' else 1
         setattr(d, name, bad)
-        assert lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d)) == -22, name
+        assert lib.camli_cross_attention_fwd_workspace_bytes(ctypes.byref(d), 0) == -22, name
         assert lib.camli_cross_attention_bwd(ctypes.byref(d), 16, 16, 16, 16, 16, 16, null, 16, 1 << 30, null) == -22, name
         setattr(d, name, keep)
     for row in (-64, 2 ** 23, 66):

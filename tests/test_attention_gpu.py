@@ -121,6 +121,72 @@ def test_attention_masked_places_may_hold_anything(dtype, poison):
     assert not clean['dk'][hidden.expand_as(c['k']).cuda()].any() and not clean['dv'][hidden.expand_as(c['v']).cuda()].any()
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('dim', [8, 32, 40, 64, 96, 128])
+@pytest.mark.parametrize('lq,lk,h,hk', [(1, 1, 1, 1), (1, 31, 4, 1), (1, 700, 8, 2), (5, 129, 6, 2), (32, 40, 2, 2), (8, 1100, 4, 1)])
+def test_attention_few_queries(dtype, dim, lq, lk, h, hk):
+    """without a gradient: at most 32 rows to a kv head, every wave on its own keys"""
+    _check(_case(2, lq, lk, h, hk, dim, dtype, seed=24), grad=False)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('axes,bidirectional,buckets,max_distance', [(1, True, 32, 64), (2, False, 64, 100), (2, True, 64, 1023)])
+def test_attention_few_queries_bias_lengths_masks(dtype, axes, bidirectional, buckets, max_distance):
+    c = _case(5, 3, 1700, 4, 2, 64, dtype, axes=axes, buckets=buckets, max_distance=max_distance, lengths=[1700, 0, 1, 33, 901], masked=0.3,
+              batched_pos=True, seed=25)
+    c['mask'][3] = False        # a sample that keeps nothing, and one with its first tiles masked
+    c['mask'][4, :500] = False
+    c['keep'] = c['mask'] & (torch.arange(1700) < c['kvl'][:, None])
+    got = _check(c, bidirectional=bidirectional, grad=False)
+    assert not got['out'][1].any() and not got['out'][3].any()
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+def test_attention_few_queries_masked_places_and_rising_scores(dtype):
+    """poison in masked places; keys that grow along the row move the softmax reference tile after tile"""
+    c = _case(2, 2, 900, 4, 1, 40, dtype, lengths=[900, 610], masked=0.2, seed=26)
+    c['k'] = (c['k'].float() * torch.linspace(0, 12, 900)[:, None, None]).to(dtype)
+    want = _check(c, grad=False)['out']
+    hidden = ~c['keep'][:, :, None, None].expand_as(c['k'])
+    for poison in (float('nan'), float('inf'), torch.finfo(dtype).min):
+        p = dict(c, k=torch.where(hidden, torch.full_like(c['k'], poison), c['k']), v=torch.where(hidden, torch.full_like(c['v'], poison), c['v']))
+        assert torch.equal(_run(p, grad=False)['out'], want)
+    p = dict(c, q=c['q'].clone())
+    p['q'][1, 0, 2] = float('nan')      # one head's query: its row alone
+    out = _run(p, grad=False)['out']
+    assert out[1, 0, 2].isnan().all()
+    out[1, 0, 2] = want[1, 0, 2]
+    assert torch.equal(out, want)
+
+
+def test_attention_few_queries_in_a_graph_and_past_32_bits():
+    from camliflow_amd import csrc
+    c = _case(3, 1, 2500, 8, 2, 64, torch.bfloat16, axes=1, lengths=[2500, 7, 0], seed=27)
+    cuda = {n: _cuda(c[n]) for n in ('q', 'k', 'v', 'table', 'kvl', 'qp', 'kp')}
+
+    def run():
+        with torch.no_grad():
+            return csrc.cross_attention(cuda['q'], cuda['k'], cuda['v'], kv_lengths=cuda['kvl'], bias_table=cuda['table'], q_pos=cuda['qp'], k_pos=cuda['kp'])
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for step in range(3):
+        cuda['q'].add_(0.25)
+        cuda['kvl'].copy_(torch.tensor([2500 - 600 * step, 7 + step, 900 * step], dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, run())
+    pitch = 2 ** 30 + 2 ** 20
+    store = torch.empty(2 * pitch + 90 * 64, dtype=torch.bfloat16, device='cuda')
+    k = torch.as_strided(store, (3, 90, 1, 32), (pitch, 64, 64, 1))
+    v = torch.as_strided(store, (3, 90, 1, 32), (pitch, 64, 64, 1), 32)
+    k.normal_()
+    v.normal_()
+    q = torch.randn(3, 1, 4, 32, device='cuda').bfloat16()
+    assert torch.equal(csrc.cross_attention(q, k, v), csrc.cross_attention(q, k.contiguous(), v.contiguous()))
+
+
 @pytest.mark.parametrize('scale', [1e-15, 1e-4, 3.0])
 def test_attention_scales(scale):
     _check(_case(1, 20, 90, 2, 2, 32, torch.float32, axes=1, seed=16), scale=scale)

@@ -18,6 +18,9 @@
 //           reverse of the order in which stats read them, so that what stats read last is still in the last-level cache.
 //   sums    (backward) per channel sum dz and sum dz xhat of a chunk;  finish: joins the chunks per channel and group;
 //   dx      as apply; one extra workgroup adds dw / dbeta over the samples.
+//
+// Bound by memory.  Measured at 16 x 64 x 272 x 480 bf16, SiLU (267 MB; a large copy: 5.1 TB/s, a sum that only reads: 4.0): stats 58 us,
+// apply 106 (5.0 TB/s), sums 132 (4.0), finish 5, dx 174 (4.6); at 8 x 128 x 68 x 120 fp32 (36 MB): 10.5, 17, 14.5, 4.6 and 18 us.
 #include "typed.h"
 
 namespace {

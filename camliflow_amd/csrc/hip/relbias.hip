@@ -4,6 +4,8 @@
 // Backward: bound by reading the incoming gradient once.  dtable[a, n, h] adds up to millions of elements into each of a few dozen
 // places; every thread owns a column of an LDS histogram (address = bucket * 256 + thread: no bank conflict, no second writer), so
 // the order of every sum is fixed by the sizes alone and plain reads and writes do.  Columns are added in a fixed order at the end, workgroups in 64 bits.
+// Measured at 4 heads x 2048 x 8160, two axes of 32 buckets, bf16 (134 MB): forward 30 us (4.5 TB/s), gradient 73 us (two dependent LDS
+// read-add-writes an element) and 4 us for the join; 4 x 501 x 1237, one axis, fp32: 10, 12 and 4 us.
 #include "relbias.h"
 
 #include <math.h>

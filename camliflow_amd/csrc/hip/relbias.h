@@ -72,30 +72,40 @@ __device__ __forceinline__ int med3(int x, int lo, int hi) {
 template <int SCALE>
 __device__ __forceinline__ int scale_pos(int pos) { return min(max(pos, -(1 << 26)), 1 << 26) * SCALE; }
 
-// Two additions to a thread's own histogram column, per axis, at byte offsets.  Plain reads and writes, because nobody else touches the
-// column: an LDS float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a dependent
-// read-add-write).  The two cells of an axis may be the same one.  What stands between fetch and add covers the read's way.
-template <int AXES>
-struct HistPair {
-    float x0[AXES], x1[AXES];
+// orders a wave's LDS accesses (they execute in order; this keeps the compiler from moving them)
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
-    __device__ __forceinline__ void fetch(const char* column, const unsigned (&at0)[AXES], const unsigned (&at1)[AXES]) {
+// Two additions to a thread's own histogram column, at byte offsets.  Plain reads and writes, because nobody else touches the column: an LDS
+// float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a dependent read-add-write).  The two
+// cells may be the same one.
+__device__ __forceinline__ void hist_add2(char* cells, unsigned at0, float v0, unsigned at1, float v1) {
+    float x0 = *reinterpret_cast<float*>(cells + at0), x1 = *reinterpret_cast<float*>(cells + at1);
+    x0 += v0;
+    x1 = (at0 == at1 ? x0 : x1) + v1;
+    *reinterpret_cast<float*>(cells + at0) = x0;
+    *reinterpret_cast<float*>(cells + at1) = x1;
+}
+// ... and for every axis, whose cells never coincide: all reads on their way before the first addition
+template <int AXES>
+__device__ __forceinline__ void hist_add2(char* column, const unsigned (&at0)[AXES], float v0, const unsigned (&at1)[AXES], float v1) {
+    float x0[AXES], x1[AXES];
 #pragma unroll
-        for (int a = 0; a < AXES; ++a) {
-            x0[a] = *reinterpret_cast<const float*>(column + at0[a]);
-            x1[a] = *reinterpret_cast<const float*>(column + at1[a]);
-        }
+    for (int a = 0; a < AXES; ++a) {
+        x0[a] = *reinterpret_cast<float*>(column + at0[a]);
+        x1[a] = *reinterpret_cast<float*>(column + at1[a]);
     }
-    __device__ __forceinline__ void add(char* column, const unsigned (&at0)[AXES], float v0, const unsigned (&at1)[AXES], float v1) {
 #pragma unroll
-        for (int a = 0; a < AXES; ++a) {
-            x0[a] += v0;
-            x1[a] = (at0[a] == at1[a] ? x0[a] : x1[a]) + v1;
-        }
-#pragma unroll
-        for (int a = 0; a < AXES; ++a) {
-            *reinterpret_cast<float*>(column + at0[a]) = x0[a];
-            *reinterpret_cast<float*>(column + at1[a]) = x1[a];
-        }
+    for (int a = 0; a < AXES; ++a) {
+        x0[a] += v0;
+        x1[a] = (at0[a] == at1[a] ? x0[a] : x1[a]) + v1;
     }
-};
+#pragma unroll
+    for (int a = 0; a < AXES; ++a) {
+        *reinterpret_cast<float*>(column + at0[a]) = x0[a];
+        *reinterpret_cast<float*>(column + at1[a]) = x1[a];
+    }
+}

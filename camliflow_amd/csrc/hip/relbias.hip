@@ -4,7 +4,7 @@
 // Backward: bound by reading the incoming gradient once.  dtable[a, n, h] adds up to millions of elements into each of a few dozen
 // places; every thread owns a column of an LDS histogram (address = bucket * 256 + thread: no bank conflict, no second writer), so
 // the order of every sum is fixed by the sizes alone and plain reads and writes do.  Columns are added in a fixed order at the end, workgroups in 64 bits.
-// Measured at 4 heads x 2048 x 8160, two axes of 32 buckets, bf16 (134 MB): forward 30 us (4.5 TB/s), gradient 73 us (two dependent LDS
+// Measured at 4 heads x 2048 x 8160, two axes of 32 buckets, bf16 (134 MB): forward 30 us (4.5 TB/s), gradient 64 us (two dependent LDS
 // read-add-writes an element) and 4 us for the join; 4 x 501 x 1237, one axis, fp32: 10, 12 and 4 us.
 #include "relbias.h"
 
@@ -14,6 +14,8 @@ namespace {
 
 constexpr int BLOCK = 256;
 constexpr int ROWS = 32;        // rows of the bias a workgroup writes per column tile
+
+constexpr int bwd_columns(int axes) { return axes > 1 ? BLOCK / 2 : BLOCK; }        // of the gradient's histogram
 
 // dynamic LDS: float[axes][2 limit + 1].  grid (column tiles, row tiles, B * H)
 template <typename T, int VEC, int AXES>
@@ -56,21 +58,29 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_fwd_kernel(RelBias r, T* __res
     }
 }
 
-// dynamic LDS: float hist[axes * buckets][BLOCK], then unsigned short bucket[2 limit + 1] (two bytes an entry: the usual tables fit one
+// dynamic LDS: float hist[axes * buckets][columns], then unsigned short bucket[2 limit + 1] (two bytes an entry: the usual tables fit one
 // dword per bank, so lanes with different offsets do not collide).
+// One axis: a column per thread.  Two: lanes l and l + 32 of a wave share one.  They take the axes in opposite order, so at any time one of
+// them is among the rows of the first axis and the other among those of the second: half the LDS, twice the workgroups on a CU to cover
+// the way of a cell from LDS and back (4 heads x 2048 x 8160 bf16: 73 -> 64 us).
 // grid (row parts, column tiles, H): as in the forward a thread keeps its columns' positions in registers and walks over rows; the next
 // row's gradient is on its way while one is added.
 template <typename T, int VEC, int AXES>
 __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T* __restrict__ g, float* __restrict__ partial, int H, int Lq,
                                                              int Lk, int64_t rows, int cols) {
     extern __shared__ float hist[];
+    constexpr int COLS = bwd_columns(AXES);
     const int h = blockIdx.z, tid = threadIdx.x, span = 2 * r.limit + 1, nrows = AXES * r.buckets;
-    unsigned short* bucket = reinterpret_cast<unsigned short*>(hist + nrows * BLOCK);
+    const int half = AXES > 1 ? (tid >> 5) & 1 : 0;             // a thread's axis in turn x is x ^ half
+    unsigned short* bucket = reinterpret_cast<unsigned short*>(hist + nrows * COLS);
     const int* border = rel_stage_borders(r);
     for (int i = tid; i < span; i += BLOCK) bucket[i] = (unsigned short)rel_bucket(r, border, i);
-    for (int i = 0; i < nrows; ++i) hist[i * BLOCK + tid] = 0.0f;
+    for (int i = tid; i < nrows * COLS; i += BLOCK) hist[i] = 0.0f;
     __syncthreads();
-    char* column = reinterpret_cast<char*>(hist + tid);
+    unsigned column[AXES];
+#pragma unroll
+    for (int a = 0; a < AXES; ++a) column[a] = ((a ^ half) * r.buckets * COLS + (AXES > 1 ? (tid >> 6) * 32 + (tid & 31) : tid)) * (unsigned)sizeof(float);
+    char* cells = reinterpret_cast<char*>(hist);
     const int tx = tid % cols, ty = tid / cols, per = BLOCK / cols, j = (blockIdx.y * cols + tx) * VEC;
     const int64_t first = (int64_t)blockIdx.x * per + ty;
     const int step = gridDim.x * per, step_b = step / Lq, step_i = step - step_b * Lq;
@@ -81,7 +91,7 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
         float v[VEC];
         load_f32<T, VEC>(g + (((int64_t)b * H + h) * Lq + i) * Lk + j, v);
 #pragma unroll
-        for (int a = 0; a < AXES; ++a) q[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + a];
+        for (int a = 0; a < AXES; ++a) q[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + (a ^ half)];
         while (b < B) {
             float now[VEC];
             int qs[AXES];
@@ -99,30 +109,29 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
             if (b < B) {
                 load_f32<T, VEC>(g + (((int64_t)b * H + h) * Lq + i) * Lk + j, v);
 #pragma unroll
-                for (int a = 0; a < AXES; ++a) q[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + a];
+                for (int a = 0; a < AXES; ++a) q[a] = r.qpos[b * r.qpos_bs + (int64_t)i * AXES + (a ^ half)];
             }
             if (sample != of) {
                 of = sample;
 #pragma unroll
                 for (int a = 0; a < AXES; ++a)
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) kp[a][e] = centre + scale_pos<2>(r.kpos[sample * r.kpos_bs + (int64_t)(j + e) * AXES + a]);
+                    for (int e = 0; e < VEC; ++e) kp[a][e] = centre + scale_pos<2>(r.kpos[sample * r.kpos_bs + (int64_t)(j + e) * AXES + (a ^ half)]);
             }
-            unsigned n[VEC][AXES];
+            unsigned n[AXES][VEC];
 #pragma unroll
             for (int a = 0; a < AXES; ++a)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) n[e][a] = (a * r.buckets + lds_load<unsigned short>(med3(kp[a][e] - qs[a], lo, hi))) * (BLOCK * (unsigned)sizeof(float));
-            if constexpr (VEC > 1) {
+                for (int e = 0; e < VEC; ++e) n[a][e] = lds_load<unsigned short>(med3(kp[a][e] - qs[a], lo, hi)) * (COLS * (unsigned)sizeof(float)) + column[a];
 #pragma unroll
-                for (int e = 0; e < VEC; e += 2) {
-                    HistPair<AXES> cell;
-                    cell.fetch(column, n[e], n[e + 1]);
-                    cell.add(column, n[e], now[e], n[e + 1], now[e + 1]);
+            for (int a = 0; a < AXES; ++a) {
+                if constexpr (VEC > 1) {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) hist_add2(cells, n[a][e], now[e], n[a][e + 1], now[e + 1]);
+                } else {
+                    *reinterpret_cast<float*>(cells + n[a][0]) += now[0];
                 }
-            } else {
-#pragma unroll
-                for (int a = 0; a < AXES; ++a) *reinterpret_cast<float*>(column + n[0][a]) += now[0];
+                if constexpr (AXES > 1) wave_order();       // the halves change axes
             }
         }
     }
@@ -132,7 +141,7 @@ __global__ __launch_bounds__(BLOCK) void rel_bias_bwd_kernel(RelBias r, const T*
     for (int n = wave; n < nrows; n += BLOCK / 64) {
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < BLOCK / 64; ++k) s += hist[n * BLOCK + k * 64 + lane];
+        for (int k = 0; k < COLS / 64; ++k) s += hist[n * COLS + k * 64 + lane];
         s = wave_sum(s);
         if (lane == 0) partial[(h * parts + part) * nrows + n] = s;
     }
@@ -215,11 +224,15 @@ int pow2_cols(int n) {      // threads along a row: the power of two that covers
     return c;
 }
 
-// row parts per column tile: 512 workgroups (two per CU fit beside each other), but 16 row groups in each: a workgroup pays for its table
+size_t bwd_lds(int axes, int buckets, int limit) { return sizeof(float) * axes * buckets * bwd_columns(axes) + 2 * (2 * limit + 2); }
+
+// row parts per column tile: as many workgroups as fit on the chip at once (two to four a CU), but 16 row groups in each: a workgroup pays for its table
 // and for clearing and adding up its histogram
-int bwd_parts(int64_t rows, int Lk, int H, int vec) {
+int bwd_parts(int64_t rows, int Lk, int H, int vec, int axes, int buckets) {
+    const int fit = (int)((size_t)159 * 1024 / bwd_lds(axes, buckets, CAMLI_REL_MAX_LIMIT));
+    const int64_t want = 256 * (fit < 2 ? 2 : fit > 4 ? 4 : fit);
     const int cols = pow2_cols(camli_divup(Lk, vec)), per = BLOCK / cols, tiles = camli_divup(Lk, cols * vec);
-    const int64_t most = (512 + (int64_t)H * tiles - 1) / ((int64_t)H * tiles), few = ((rows + per - 1) / per + 15) / 16;
+    const int64_t most = (want + (int64_t)H * tiles - 1) / ((int64_t)H * tiles), few = ((rows + per - 1) / per + 15) / 16;
     return (int)(few < most ? few : most);
 }
 
@@ -234,14 +247,14 @@ int fwd(const RelBias& r, void* out, int B, int H, int Lq, int Lk, hipStream_t s
 template <typename T, int VEC, int AXES>
 int bwd(const RelBias& r, const void* g, void* gtable, float* ws, int B, int H, int Lq, int Lk, hipStream_t s) {
     static unsigned long long done = 0;
-    if (!camli_reserve_lds((const void*)rel_bias_bwd_kernel<T, VEC, AXES>, sizeof(float) * CAMLI_REL_MAX_ROWS * BLOCK + 2 * (2 * CAMLI_REL_MAX_LIMIT + 2), done)) {
+    if (!camli_reserve_lds((const void*)rel_bias_bwd_kernel<T, VEC, AXES>, bwd_lds(1, CAMLI_REL_MAX_ROWS, CAMLI_REL_MAX_LIMIT), done)) {
         camli_set_error("camli_rel_bias_bwd: cannot reserve LDS");
         return CAMLI_ELAUNCH;
     }
     const int64_t rows = (int64_t)B * Lq;
-    const int nrows = AXES * r.buckets, cols = pow2_cols(camli_divup(Lk, VEC)), parts = bwd_parts(rows, Lk, H, VEC);
+    const int nrows = AXES * r.buckets, cols = pow2_cols(camli_divup(Lk, VEC)), parts = bwd_parts(rows, Lk, H, VEC, AXES, r.buckets);
     const int tiles = camli_divup(Lk, cols * VEC);
-    const size_t lds = sizeof(float) * nrows * BLOCK + 2 * (2 * r.limit + 2);
+    const size_t lds = bwd_lds(AXES, r.buckets, r.limit);
     rel_bias_bwd_kernel<T, VEC, AXES><<<dim3(parts, tiles, H), BLOCK, lds, s>>>(r, static_cast<const T*>(g), ws, H, Lq, Lk, rows, cols);
     return rel_bias_join(ws, gtable, r.type, H, nrows, (int64_t)parts * tiles, "camli_rel_bias_bwd", s);
 }
@@ -299,8 +312,8 @@ extern "C" int64_t camli_rel_bias_bwd_workspace_bytes(int B, int H, int Lq, int 
     const int vec = 16 / camli_type_size(type);
     const int64_t rows = (int64_t)B * Lq;
     // whichever form the alignment allows
-    const int64_t a = (int64_t)bwd_parts(rows, Lk, H, vec) * camli_divup(Lk, pow2_cols(camli_divup(Lk, vec)) * vec);
-    const int64_t c = (int64_t)bwd_parts(rows, Lk, H, 1) * camli_divup(Lk, pow2_cols(Lk));
+    const int64_t a = (int64_t)bwd_parts(rows, Lk, H, vec, axes, buckets) * camli_divup(Lk, pow2_cols(camli_divup(Lk, vec)) * vec);
+    const int64_t c = (int64_t)bwd_parts(rows, Lk, H, 1, axes, buckets) * camli_divup(Lk, pow2_cols(Lk));
     return (int64_t)sizeof(float) * H * (a > c ? a : c) * axes * buckets;
 }
 

@@ -285,13 +285,6 @@ __device__ __forceinline__ void put_chunk(typename TL::Lds* to, const chunk16 (&
 #pragma unroll
     for (int n = 0; n < Parts<T>::N; ++n) *reinterpret_cast<typename Mat<L>::frag*>(to + n * TL::PLANE) = parts.part[n];
 }
-// orders a wave's LDS accesses (they execute in order; this keeps the compiler from moving them)
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // The streamed pair of tiles on its way from memory: registers now, LDS later.  A row at or beyond `limit`, a masked row and columns
 // from D on become zeros (a masked row may hold anything, and 0 * NaN is NaN); a whole, unmasked tile skips those tests.
 // A thread's place in a tile is a 32-bit byte offset computed once (row strides are below 2^23 elements); the tile's base is uniform.
@@ -944,7 +937,7 @@ __device__ __forceinline__ float unit_scale(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
-// WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, positions, lut, then
+// WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, lut, then
 // hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
 // HIST: with the table's gradient; its tiles lie in one buffer, so that two workgroups still share a CU beside their histograms (one waits at a
 // barrier while the other computes; fp32 with two buffers: 465 us where one takes 350).
@@ -1103,9 +1096,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float d0 = __is_same(T, _Float16) ? dp[i] * unscale : dp[i], d1 = __is_same(T, _Float16) ? dp[i + 1] * unscale : dp[i + 1];
-                    HistPair<AXES> cell;
-                    cell.fetch(column, at_hist[i], at_hist[i + 1]);
-                    cell.add(column, at_hist[i], d0, at_hist[i + 1], d1);
+                    hist_add2<AXES>(column, at_hist[i], d0, at_hist[i + 1], d1);
                 }
             }
 #pragma unroll

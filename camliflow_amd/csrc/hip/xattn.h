@@ -86,6 +86,11 @@ template <> struct Parts<float> {
     static constexpr int N = 3;
 };
 
+template <int I>
+struct Int {
+    static constexpr int value = I;
+};
+
 template <typename T>
 struct Frag {
     typename Mat<typename Parts<T>::Lds>::frag part[Parts<T>::N];
@@ -154,8 +159,8 @@ struct Tile {
 
 // rows of a streamed tile: what a thread of 256 can fetch at once in narrow heads, what two buffers leave room for in wide fp32 ones
 constexpr int tile_rows(int size, int dp) { return size == 2 || dp == 32 ? 64 : 32; }
-// dq with a histogram beside one buffer: two workgroups a CU need tiles of at most 12 KB
-constexpr int dq_tile_rows(int size, int dp, bool hist) { return !hist ? tile_rows(size, dp) : size == 2 && dp == 32 ? 64 : 32; }
+// dq with a histogram beside one buffer: small tiles leave LDS for three workgroups a CU in narrow heads (64 rows: 1089 us where 32 take 1063)
+constexpr int dq_tile_rows(int size, int dp, bool hist) { return hist ? 32 : tile_rows(size, dp); }
 
 // Where a lane reads in a tile (element offsets from the start of a 32-row block; loop-invariant).
 template <typename TL, typename T>
@@ -464,6 +469,30 @@ __device__ __forceinline__ void fill_lut(const RelBias& r, Entry8* lut, int head
     }
 }
 
+// the same for lanes FIRST .. FIRST + 7
+template <int FIRST>
+__device__ __forceinline__ void broadcast_plus8(int lanes, int own, int (&out)[8]) {
+    asm("s_nop 1\n\t"
+        "v_add_u32_dpp %0, %8, %9 row_newbcast:%10 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %1, %8, %9 row_newbcast:%11 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %2, %8, %9 row_newbcast:%12 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %3, %8, %9 row_newbcast:%13 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %4, %8, %9 row_newbcast:%14 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %5, %8, %9 row_newbcast:%15 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %6, %8, %9 row_newbcast:%16 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_u32_dpp %7, %8, %9 row_newbcast:%17 row_mask:0xf bank_mask:0xf"
+        : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3]), "=&v"(out[4]), "=&v"(out[5]), "=&v"(out[6]), "=&v"(out[7])
+        : "v"(lanes), "v"(own), "n"(FIRST + 0), "n"(FIRST + 1), "n"(FIRST + 2), "n"(FIRST + 3), "n"(FIRST + 4), "n"(FIRST + 5), "n"(FIRST + 6), "n"(FIRST + 7));
+}
+
+// bias of accumulator register i's pair: the axes' entries, added first (the order of two does not matter: every kernel gets the same bits)
+template <int AXES>
+__device__ __forceinline__ float pair_bias(const int (&off)[AXES][16], int i, const int (&lo)[AXES], const int (&hi)[AXES]) {
+    float b = lds_load<float>(med3(off[0][i], lo[0], hi[0]));
+    if constexpr (AXES > 1) b += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
+    return b;
+}
+
 // Positions of the streamed rows stay out of LDS: lane i of each 16-lane row holds the position of the row that accumulator register i
 // stands for (acc_row(i, h): the halves differ), and the subtraction reads it from there by a row broadcast.  As LDS broadcasts the
 // same reads took a quarter of the LDS time.
@@ -471,13 +500,15 @@ template <int AXES, int BLOCKS, int SCALE>
 struct StreamPos {
     int p[BLOCKS][AXES ? AXES : 1];
 
+    // SWAP: the upper half takes the axes in the opposite order
+    template <bool SWAP = false>
     __device__ __forceinline__ void load(const int* pos, int row0, int limit) {
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, half = SWAP ? lane >> 5 : 0;
 #pragma unroll
         for (int nb = 0; nb < BLOCKS; ++nb) {
             const int row = min(row0 + nb * 32 + acc_row(lane & 15, lane >> 5), limit - 1);
 #pragma unroll
-            for (int x = 0; x < AXES; ++x) p[nb][x] = scale_pos<SCALE>(pos[(int64_t)row * AXES + x]);
+            for (int x = 0; x < AXES; ++x) p[nb][x] = scale_pos<SCALE>(pos[(int64_t)row * AXES + (x ^ half)]);
         }
     }
 };
@@ -612,8 +643,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
                     for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], qa[x], off[x]);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
-                        if constexpr (AXES > 1) s[nb][i] += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
+                        s[nb][i] = __builtin_fmaf(s[nb][i], a.scale_log2, pair_bias<AXES>(off, i, lo, hi));
                     }
                 }
             }
@@ -801,8 +831,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void fwd_few_kernel(Args a)
             for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[0][x], qa[x], off[x]);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[i] = __builtin_fmaf(s[i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
-                if constexpr (AXES > 1) s[i] += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
+                s[i] = __builtin_fmaf(s[i], a.scale_log2, pair_bias<AXES>(off, i, lo, hi));
             }
         } else {
 #pragma unroll
@@ -937,20 +966,24 @@ __device__ __forceinline__ float unit_scale(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
-// WAVES: 4, or 2 where the histogram of four would not fit beside the tiles.  LDS: tiles, lut, then
-// hist[axes * buckets][64 WAVES] (a column per thread: sums in a fixed order, no bank conflicts).
-// HIST: with the table's gradient; its tiles lie in one buffer, so that two workgroups still share a CU beside their histograms (one waits at a
-// barrier while the other computes; fp32 with two buffers: 465 us where one takes 350).
-// Measured with a two-axis bias of 2 x 32 buckets, 4 heads of 32: 8 x 8160 queries x 2048 keys, bf16: 547 us, bound by LDS (two table reads
-// and two histogram read-add-writes a pair: 70 % busy; adding a block's ds while the next one is computed took 16 % of the vector
-// instructions away and no time); 2 x 2048 x 8160, fp32: 260 us.
+// HIST: with the table's gradient.  LDS: tiles (one buffer), lut after hist[axes * buckets][columns].  A thread adds to a column by plain reads and
+// writes: sums in a fixed order, no bank conflicts.  One axis: a column per thread, and 2 waves instead of 4 (WAVES) where more than 64
+// buckets would not fit.  Two axes: lanes l and l + 32 share a column; they take the axes in opposite order, so that one is among the rows of
+// the first axis while the other is among those of the second.  With that, 32-row tiles and eight registers' cells at a time three
+// workgroups share a CU in narrow 16-bit heads, one computing while another waits at a barrier or for LDS.
+// Measured with a two-axis bias of 2 x 32 buckets, 4 heads of 32: 8 x 8160 queries x 2048 keys, bf16: 495 us (a column per thread, two
+// workgroups: 547; adding a block's ds while the next one is computed took 16 % of the vector instructions away and no time), LDS and vector
+// arithmetic both at about 60 %; 2 x 2048 x 8160, fp32: 265 us (tiles in two buffers, one workgroup: 465 with fp32 products).
+constexpr int hist_columns(int axes, int waves) { return axes == 2 ? 32 * waves : 64 * waves; }
+
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
-__global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof(T) == 4 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
+__global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || sizeof(T) == 4 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
     constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
     using TL = Tile<T, DP, R>;
     using L = typename TL::Lds;
     using Entry = __type_pack_element<HIST ? 1 : 0, float, Entry8>;
-    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = (int)sizeof(Entry);
+    constexpr int THREADS = 64 * WAVES, OWN = 32 * WAVES, ENTRY = (int)sizeof(Entry), COLS = hist_columns(AXES, WAVES);
+    constexpr bool SHARED = HIST && AXES == 2;
     extern __shared__ __align__(16) char smem[];
     L* tiles = reinterpret_cast<L*>(smem);
     Entry* lut = reinterpret_cast<Entry*>(tiles + (HIST ? 2 : 4) * TL::ELEMS);
@@ -967,6 +1000,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
     const int qi = rt * OWN + wave * 32 + (lane & 31);
     const bool exists = qi < a.Lq;
     const int q0 = exists ? qi : 0;
+    const int half = SHARED ? h : 0;            // a lane's axis in turn x is x ^ half
 
     const int len = kept_length(a, b);
     const int n_tiles = (len + TL::ROWS - 1) / TL::ROWS;
@@ -1018,19 +1052,19 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
     if constexpr (AXES > 0) {
-        fill_lut<AXES, THREADS>(a.rb, lut, head, HIST ? 4 * THREADS : 1, a.H);
+        fill_lut<AXES, THREADS>(a.rb, lut, head, HIST ? 4 * COLS : 1, a.H);
         kpos = a.rb.kpos + b * a.rb.kpos_bs;
 #pragma unroll
         for (int x = 0; x < AXES; ++x) {
-            const int centre = (int)lds_address(lut + x * span + a.rb.limit);
-            qa[x] = centre + scale_pos<-ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + x]);
+            const int centre = (int)lds_address(lut + (x ^ half) * span + a.rb.limit);
+            qa[x] = centre + scale_pos<-ENTRY>(a.rb.qpos[b * a.rb.qpos_bs + (int64_t)q0 * AXES + (x ^ half)]);
             lo[x] = centre - ENTRY * a.rb.limit;
             hi[x] = centre + ENTRY * a.rb.limit;
         }
         if constexpr (HIST)
-            for (int i = 0; i < hist_rows; ++i) hist[i * THREADS + tid] = 0.0f;
+            for (int i = tid; i < hist_rows * COLS; i += THREADS) hist[i] = 0.0f;
     }
-    char* column = reinterpret_cast<char*>(hist + tid);
+    char* column = reinterpret_cast<char*>(hist + (SHARED ? wave * 32 + (lane & 31) : tid));
 
     acc16 dq[TL::DBLOCKS];
 #pragma unroll
@@ -1041,7 +1075,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
     int cur = 0;
     if (t0 < t1) {
         st.load(kp + t0 * (int64_t)TL::ROWS * a.ks.l, vp + t0 * (int64_t)TL::ROWS * a.vs.l, t0 * TL::ROWS, len, a.D, mask);
-        if constexpr (AXES > 0) pos_next.load(kpos, t0 * TL::ROWS, len);
+        if constexpr (AXES > 0) pos_next.template load<SHARED>(kpos, t0 * TL::ROWS, len);
         st.store(tiles, tiles + TL::ELEMS);
     }
     __syncthreads();
@@ -1050,54 +1084,68 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
         if constexpr (AXES > 0) pos = pos_next;
         if (t + 1 < t1) {
             st.load(kp + (t + 1) * (int64_t)TL::ROWS * a.ks.l, vp + (t + 1) * (int64_t)TL::ROWS * a.vs.l, (t + 1) * TL::ROWS, len, a.D, mask);
-            if constexpr (AXES > 0) pos_next.load(kpos, (t + 1) * TL::ROWS, len);
+            if constexpr (AXES > 0) pos_next.template load<SHARED>(kpos, (t + 1) * TL::ROWS, len);
         }
         const L *kt = HIST ? tiles : tiles + cur * 2 * TL::ELEMS, *vt = kt + TL::ELEMS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
-            const unsigned half = (unsigned)(bits >> (nb * 32));
-            if (half == 0) continue;
+            const unsigned half_bits = (unsigned)(bits >> (nb * 32));
+            if (half_bits == 0) continue;
             const L *kb = kt + nb * 32 * DP, *vb = vt + nb * 32 * DP;
             acc16 s = product<T, TL>(map, kb, qf, start_s), dp = product<T, TL>(map, vb, gf, start_d);
-            unsigned at_hist[16][AXES ? AXES : 1];
-            if constexpr (AXES > 0) {
-                int off[AXES][16];
+            if constexpr (HIST) {
+                auto octet = [&](auto which) {      // eight registers at a time: their cells' places need not all be held at once
+                    constexpr int F = decltype(which)::value;
+                    int off[AXES][8];
+                    unsigned at[8][AXES];
+#pragma unroll
+                    for (int x = 0; x < AXES; ++x) broadcast_plus8<F>(pos.p[nb][x], qa[x], off[x]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = F + k;
+                        float bias = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < AXES; ++x) {
+                            const uint2v e = lds_load<uint2v>(med3(off[x][k], lo[x], hi[x]));       // an Entry8
+                            bias = x ? bias + __uint_as_float(e[0]) : __uint_as_float(e[0]);
+                            at[k][x] = e[1];
+                        }
+                        s[i] = __builtin_fmaf(s[i], a.scale_log2, bias);
+                        if constexpr (!FOLD) s[i] -= lse;
+                        s[i] = kept_row(half_bits, i) ? s[i] : -INFINITY;
+                        dp[i] = (FOLD ? dp[i] : __builtin_fmaf(dp[i], sign, -delta)) * __builtin_amdgcn_exp2f(s[i]);
+                    }
+#pragma unroll
+                    for (int x = 0; x < AXES; ++x) {
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2) {
+                            const float d0 = __is_same(T, _Float16) ? dp[F + k] * unscale : dp[F + k], d1 = __is_same(T, _Float16) ? dp[F + k + 1] * unscale : dp[F + k + 1];
+                            hist_add2(column, at[k][x], d0, at[k + 1][x], d1);
+                        }
+                        if constexpr (SHARED) wave_order();         // the halves change axes
+                    }
+                };
+                octet(Int<0>{});
+                octet(Int<8>{});
+            } else {
+                int off[AXES ? AXES : 1][16];
 #pragma unroll
                 for (int x = 0; x < AXES; ++x) broadcast_plus(pos.p[nb][x], qa[x], off[x]);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float bias[AXES];
-#pragma unroll
-                    for (int x = 0; x < AXES; ++x) {
-                        const int address = med3(off[x][i], lo[x], hi[x]);
-                        if constexpr (HIST) {
-                            const uint2v e = lds_load<uint2v>(address);     // an Entry8
-                            bias[x] = __uint_as_float(e[0]);
-                            at_hist[i][x] = e[1];
-                        } else {
-                            bias[x] = lds_load<float>(address);
-                        }
+                    if constexpr (AXES > 0) {
+                        s[i] = __builtin_fmaf(s[i], a.scale_log2, pair_bias<AXES>(off, i, lo, hi));
+                        if constexpr (!FOLD) s[i] -= lse;
+                    } else {
+                        s[i] = FOLD ? s[i] * a.scale_log2 : __builtin_fmaf(s[i], a.scale_log2, -lse);
                     }
-                    s[i] = __builtin_fmaf(s[i], a.scale_log2, bias[0]);
-                    if constexpr (AXES > 1) s[i] += bias[AXES - 1];
-                    if constexpr (!FOLD) s[i] -= lse;
                 }
-            } else {
+                if (half_bits != 0xffffffffu) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = FOLD ? s[i] * a.scale_log2 : __builtin_fmaf(s[i], a.scale_log2, -lse);
-            }
-            if (half != 0xffffffffu) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = kept_row(half, i) ? s[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] = (FOLD ? dp[i] : __builtin_fmaf(dp[i], sign, -delta)) * __builtin_amdgcn_exp2f(s[i]);
-            if constexpr (HIST) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float d0 = __is_same(T, _Float16) ? dp[i] * unscale : dp[i], d1 = __is_same(T, _Float16) ? dp[i + 1] * unscale : dp[i + 1];
-                    hist_add2<AXES>(column, at_hist[i], d0, at_hist[i + 1], d1);
+                    for (int i = 0; i < 16; ++i) s[i] = kept_row(half_bits, i) ? s[i] : -INFINITY;
                 }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] = (FOLD ? dp[i] : __builtin_fmaf(dp[i], sign, -delta)) * __builtin_amdgcn_exp2f(s[i]);
             }
 #pragma unroll
             for (int ps = 0; ps < TL::PSTEPS; ++ps) {
@@ -1123,7 +1171,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? (HIST || AXES == 2 || sizeof
         for (int n = wave; n < hist_rows; n += WAVES) {
             float v = 0.0f;
 #pragma unroll
-            for (int k = 0; k < WAVES; ++k) v += hist[n * THREADS + k * 64 + lane];
+            for (int k = 0; k < COLS / 64; ++k) v += hist[n * COLS + k * 64 + lane];
             v = wave_sum(v);
             if (lane == 0) a.part_table[((int64_t)head * a.parts + part) * hist_rows + n] = v;
         }
@@ -1259,8 +1307,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
             for (int i = 0; i < 16; ++i) {
                 float x;
                 if constexpr (AXES > 0) {
-                    x = __builtin_fmaf(s[i], a.scale_log2, lds_load<float>(med3(off[0][i], lo[0], hi[0])));
-                    if constexpr (AXES > 1) x += lds_load<float>(med3(off[AXES - 1][i], lo[AXES - 1], hi[AXES - 1]));
+                    x = __builtin_fmaf(s[i], a.scale_log2, pair_bias<AXES>(off, i, lo, hi));
                 } else {
                     x = s[i] * a.scale_log2;
                 }
@@ -1376,7 +1423,7 @@ int run_dq_mode(const Args& a, hipStream_t s) {
     constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
     static unsigned long long done = 0;
     size_t lds = tile_bytes<T, DP, R>() / (HIST ? 2 : 1) + lut_bytes(a, AXES, 1);
-    if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * 64 * WAVES;      // entries of 8 bytes
+    if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * hist_columns(AXES, WAVES);      // entries of 8 bytes
     return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
 }
 
@@ -1385,7 +1432,8 @@ int run_dq(const Args& a, int waves, hipStream_t s) {
     int rc;
     if constexpr (AXES > 0) {
         if (!a.part_table) rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
-        else rc = waves == 2 ? run_dq_mode<T, DP, AXES, 2, true>(a, s) : run_dq_mode<T, DP, AXES, 4, true>(a, s);
+        else if constexpr (AXES == 1) rc = waves == 2 ? run_dq_mode<T, DP, AXES, 2, true>(a, s) : run_dq_mode<T, DP, AXES, 4, true>(a, s);
+        else rc = run_dq_mode<T, DP, AXES, 4, true>(a, s);
     } else {
         rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
     }

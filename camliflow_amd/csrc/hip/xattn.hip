@@ -34,7 +34,7 @@ void plan_fwd(Args& a, int type, int axes, bool training) {
     split_stream(a, (int64_t)a.row_tiles * (a.H / a.pack) * a.B, camli_divup(a.Lk, tile), tile, a.few ? 512 : 1024, a.few ? 512 : type == CAMLI_F32 ? 128 : 256);
 }
 
-int dq_waves(const Args& a, int axes, bool table) { return table && axes * a.rb.buckets > 64 ? 2 : 4; }
+int dq_waves(const Args& a, int axes, bool table) { return table && axes == 1 && a.rb.buckets > 64 ? 2 : 4; }
 
 void plan_dq(Args& a, int type, int axes, bool table) {
     a.pack = 1;

@@ -966,7 +966,7 @@ __device__ __forceinline__ float unit_scale(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
-// HIST: with the table's gradient.  LDS: tiles (one buffer), lut after hist[axes * buckets][columns].  A thread adds to a column by plain reads and
+// HIST: with the table's gradient.  LDS: tiles (one buffer), lut, hist[axes * buckets][columns].  A thread adds to a column by plain reads and
 // writes: sums in a fixed order, no bank conflicts.  One axis: a column per thread, and 2 waves instead of 4 (WAVES) where more than 64
 // buckets would not fit.  Two axes: lanes l and l + 32 share a column; they take the axes in opposite order, so that one is among the rows of
 // the first axis while the other is among those of the second.  With that, 32-row tiles and eight registers' cells at a time three

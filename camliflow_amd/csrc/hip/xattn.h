@@ -42,7 +42,7 @@ struct Args {
     float *lse;                 // [B][H][Lq], log2 domain; +inf where no key is kept
     float *delta;               // [B][H][Lq]
     float *go_max;              // [B][H][Lq] fp16 only: largest |go| of a row
-    float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [split][B][H][Lq] (-inf: no key)
+    float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [2][split][B][H][Lq] (two terms, -inf: no key)
     float *part_dk, *part_dv;   // splits > 1: [split][B][Lk][Hk][D]
     float *part_table;          // [H][parts][axes * buckets]
     const int *lengths;         // [B] or null
@@ -536,9 +536,32 @@ __device__ __forceinline__ void broadcast_plus(int lanes, int own, int (&out)[16
         : "v"(lanes), "v"(own));
 }
 
+// ------------------------------------------------------------------------------------------------------------ references far from zero
+// A finite table entry may be as low as its type goes, the usual mask of a bucket, and a row that so far has only such pairs (or no others
+// at all) has its softmax reference there; products of large vectors get as far without a bias.  Next to such a number a float holds no
+// digit of an ordinary score, so beyond FAR (log2 units; up to it a reference's own rounding is below 2^-16) nothing is computed
+// relative to a reference before the reference is the tile's own, and a log-sum is two floats.
+constexpr float FAR = 256.0f;
+
+// a + b exactly, as hi + lo: lo is what the sum of a large a and a small b rounds away (0 within FAR; an infinity has none)
+__device__ __forceinline__ void two_sum(float a, float b, float& hi, float& lo) {
+    const float sum = a + b, bb = sum - a, rest = (a - (sum - bb)) + (b - bb);
+    hi = sum;
+    lo = fabsf(sum) > FAR && fabsf(sum) < INFINITY ? rest : 0.0f;
+}
+template <int N>
+__device__ __forceinline__ void move_scores(acc16 (&s)[N], float by) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] += by;
+}
+// a0 + a1 > b0 + b1, for pairs as two_sum leaves them
+__device__ __forceinline__ bool two_above(float a0, float a1, float b0, float b1) { return a0 > b0 || (a0 == b0 && a1 > b1); }
+
 // ------------------------------------------------------------------------------------------------------------ forward
 // Softmax without a running maximum: the scores come out of the matrix unit already relative to m (the accumulators start at -m /
-// scale), and m is taken from the first tile that has a kept key.  p <= 2^30 (2^14 for fp16) is as good as p <= 1 in floating point, so
+// scale; at zero while m is far), and m is taken from the first tile that has a kept key.  p <= 2^30 (2^14 for fp16) is as good as p <= 1 in floating point, so
 // m moves only when a score passes that: the exchange between the half waves and the rescaling leave the loop, but for a test.
 // TRAIN (16-bit types): out has to be known to more than its own type for the backward's D = do . o, which is subtracted from
 // dp: P enters the product as two terms of the type and out is stored before its rounding as well.  Without that the bias table's
@@ -605,10 +628,10 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
 #pragma unroll
     for (int d = 0; d < TL::DBLOCKS; ++d) o[d] = acc16{0};
     // m: the reference of the row's exponents, log2 domain (-inf: no kept key yet, use 0); start: -m / scale in every accumulator (FOLD:
-    // with a bias; without one the exponent's multiply-add subtracts m at no cost)
+    // with a bias, unless any of the wave's rows is far; without one the exponent's multiply-add subtracts m at no cost)
     float m = -INFINITY, m_use = 0.0f, l = 0.0f;
     acc16 start = splat(0.0f);
-    bool unset = true;
+    bool unset = true, far = false;
 
     Stream<T, DP, R, THREADS> st;
     StreamPos<AXES, TL::BLOCKS, ENTRY> pos, pos_next;
@@ -659,34 +682,43 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
             for (int nb = 0; nb < TL::BLOCKS; ++nb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nb][i]);
-            if constexpr (AXES == 0) top = __builtin_fmaf(top, a.scale_log2, -m_use);
-            else if constexpr (!FOLD) top -= m_use;
-            if (unset || __any(top > exponent_limit<T>())) {
-                top = half_max(top);        // a row's own need decides: its result does not depend on the rows beside it
-                const float mn = m == -INFINITY || top > exponent_limit<T>() ? fmaxf(m, top + m_use) : m, use = mn == -INFINITY ? 0.0f : mn;
+            // base: what the scores are relative to.  Without a bias they are products still; the highest is rounded as the reference is, so
+            // that it comes out as 0 next to any reference
+            float base = FOLD && !far ? m_use : 0.0f;
+            if constexpr (AXES == 0) top *= a.scale_log2;
+            if (unset || __any(top + (base - m_use) > exponent_limit<T>())) {
+                // a row's own need decides: its result does not depend on the rows beside it
+                top = half_max(top);
+                const float mn = m == -INFINITY || top + (base - m_use) > exponent_limit<T>() ? fmaxf(m, top + base) : m, use = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m - use);
 #pragma unroll
                 for (int d = 0; d < TL::DBLOCKS; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
                 l *= alpha;
-                if constexpr (FOLD) {
-                    const float back = m_use - use;
-                    start = splat(-use / a.scale_log2);
-#pragma unroll
-                    for (int nb = 0; nb < TL::BLOCKS; ++nb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[nb][i] += back;
-                }
                 m = mn;
                 m_use = use;
                 unset = __any(m == -INFINITY);
+                far = __any(fabsf(m_use) > FAR);
+                if constexpr (FOLD) {
+                    start = splat(far ? 0.0f : -use / a.scale_log2);
+                    move_scores(s, base - use);
+                }
+            } else if (FOLD && far) {
+                move_scores(s, -m_use);
+            }
+            const float mul = far ? 1.0f : a.scale_log2;
+            if (AXES == 0 && far) {
+#pragma unroll
+                for (int nb = 0; nb < TL::BLOCKS; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[nb][i] *= a.scale_log2;
             }
 #pragma unroll
             for (int nb = 0; nb < TL::BLOCKS; ++nb) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[nb][i] = __builtin_amdgcn_exp2f(FOLD ? s[nb][i] : AXES > 0 ? s[nb][i] - m_use : __builtin_fmaf(s[nb][i], a.scale_log2, -m_use));
+                    s[nb][i] = __builtin_amdgcn_exp2f(FOLD ? s[nb][i] : AXES > 0 ? s[nb][i] - m_use : __builtin_fmaf(s[nb][i], mul, -m_use));
                     l += s[nb][i];
                 }
 #pragma unroll
@@ -714,11 +746,15 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (!exists) return;
     const int64_t at = ((int64_t)b * a.Lq + qi) * a.H + head, stat = ((int64_t)b * a.H + head) * a.Lq + qi;
-    const float lse = m_use + __builtin_amdgcn_logf(l);      // log2
+    float lse, lse_lo;
+    two_sum(m_use, __builtin_amdgcn_logf(l), lse, lse_lo);      // log2
     if (a.splits > 1) {
         const int64_t per = (int64_t)a.B * a.Lq * a.H;
         store_owned<float, TL::DBLOCKS>(a.part_o + (split * per + at) * a.D, o, inv, a.D, h);
-        if (h == 0) a.part_lse[split * per + stat] = l == 0.0f ? -INFINITY : lse;
+        if (h == 0) {
+            a.part_lse[split * per + stat] = l == 0.0f ? -INFINITY : lse;
+            a.part_lse[(a.splits + split) * per + stat] = l == 0.0f ? 0.0f : lse_lo;
+        }
     } else {
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, h);
         if constexpr (TWO_TERMS) store_owned<float, TL::DBLOCKS>(a.out_f32 + at * a.D, o, inv, a.D, h);
@@ -905,7 +941,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void fwd_few_kernel(Args a)
         const int64_t at = ((int64_t)b * a.Lq + ri) * a.H + rh;
         if (a.splits > 1) {
             store_f32<float, 4>(a.part_o + (split * per + at) * a.D + c, acc);
-            if (c == 0) a.part_lse[split * per + ((int64_t)b * a.H + rh) * a.Lq + ri] = total == 0.0f ? -INFINITY : use + __builtin_amdgcn_logf(total);
+            if (c == 0) {
+                float lse, lse_lo;
+                two_sum(use, __builtin_amdgcn_logf(total), lse, lse_lo);
+                float* part = a.part_lse + split * per + ((int64_t)b * a.H + rh) * a.Lq + ri;
+                part[0] = total == 0.0f ? -INFINITY : lse;
+                part[a.splits * per] = total == 0.0f ? 0.0f : lse_lo;
+            }
         } else {
             store_f32<T, 4>(static_cast<T*>(a.out) + at * a.D + c, acc);
         }
@@ -923,21 +965,31 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
     const int head = (int)(at % a.H);
     const int64_t bq = at / a.H;
     const int64_t stat = ((bq / a.Lq) * a.H + head) * a.Lq + bq % a.Lq;
-    float top = -INFINITY;
+    const float *part = a.part_lse + stat, *part_lo = part + a.splits * rows;
+    float top = -INFINITY, use_lo = 0.0f;
     bool bad = false;
+    auto higher = [&](float v, float v_lo) {
+        if (two_above(v, v_lo, top, use_lo)) {
+            top = v;
+            use_lo = v_lo;
+        }
+    };
     for (int s = lane; s < a.splits; s += 64) {
-        const float v = a.part_lse[s * rows + stat];
-        top = fmaxf(top, v);
+        const float v = part[s * rows];
+        higher(v, part_lo[s * rows]);
         bad |= v != v;
     }
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    for (int off = 32; off >= 1; off >>= 1) {
+        const float v = __shfl_xor(top, off, 64);
+        higher(v, __shfl_xor(use_lo, off, 64));
+    }
     bad = __any(bad);
     const float use = top == -INFINITY ? 0.0f : top;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
 #pragma unroll 4
     for (int s = group; s < a.splits; s += groups) {
-        const float w = __builtin_amdgcn_exp2f(a.part_lse[s * rows + stat] - use);
+        const float w = __builtin_amdgcn_exp2f((part[s * rows] - use) + (part_lo[s * rows] - use_lo));
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (c < a.D && w != 0.0f) load_f32<float, 4>(a.part_o + (s * rows + at) * a.D + c, v);
         sum += w;
@@ -951,7 +1003,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
     }
     if (group != 0) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + __builtin_amdgcn_logf(sum);
+    if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + (use_lo + __builtin_amdgcn_logf(sum));
     if (c >= a.D) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = bad ? NAN : acc[i] * inv;

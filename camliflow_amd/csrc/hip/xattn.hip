@@ -107,7 +107,7 @@ int64_t fwd_workspace(Args& a, char* base) {
     const int64_t rows = (int64_t)a.B * a.Lq * a.H, o = align256(4 * rows * a.D * a.splits);
     a.part_o = reinterpret_cast<float*>(base);
     a.part_lse = reinterpret_cast<float*>(base + o);
-    return o + align256(4 * rows * a.splits);
+    return o + align256(8 * rows * a.splits);
 }
 
 struct BwdPlan {

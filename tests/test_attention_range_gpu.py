@@ -1,0 +1,88 @@
+"""Cross attention over the range of its types: finite table entries down to the lowest (the usual mask of a bucket), rows that keep nothing
+else, scores whose neighbours in fp32 are far apart.  Against 64-bit restatements (attnsteps.py)."""
+import math
+
+import pytest
+import torch
+
+import attnref
+import attnsteps
+from test_attention_gpu import IDS, TYPES, _case, _run
+
+pytestmark = pytest.mark.gpu
+
+# what the two outermost buckets (keys far before the query, far behind it) hold
+LEVELS = {
+    torch.float32: [(-1e9, -1e9), (-1e6, -1e9), (-1e9, -1e6), (1e6, -1e30), (-1e30, -1e9)],
+    torch.bfloat16: [(-1e9, -1e9), (-1e6, -1e9), (-1e9, -1e6), (1e6, -1e30), (-1e30, -1e9)],
+    torch.float16: [(-6e4, -6e4), (-3e4, -6e4), (-6e4, -3e4), (3e4, -6e4), (-300.0, -6e4)],
+}
+LEVEL_CASES = [pytest.param(t, n, id='%s-%d' % (i, n)) for t, i in zip(TYPES, IDS) for n in range(5)]
+BEFORE, BEHIND = 15, 31         # of 32 buckets, 64 positions
+
+
+def _level_case(dtype, levels, b=2, lq=40, lk=700, h=2, hk=1, d=32, seed=0):
+    """first 300 keys far before nearly every query, then 100 far behind, then the near ones; the last six queries are far from all keys"""
+    c = _case(b, lq, lk, h, hk, d, dtype, axes=1, seed=seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    c['table'][0, BEFORE], c['table'][0, BEHIND] = levels
+    c['kp'] = torch.randint(-40, 41, (lk, 1), generator=g, dtype=torch.int32)
+    c['kp'][:3 * lk // 7], c['kp'][3 * lk // 7:4 * lk // 7] = -2000, 2000
+    c['qp'] = torch.randint(-20, 21, (lq, 1), generator=g, dtype=torch.int32)
+    c['qp'][-6:-1], c['qp'][-1] = 900, 5000
+    return c
+
+
+def _level_reference(c, training):
+    """Levels are so far apart that only the pairs of a row's highest count, at scores that differ by what fp32 holds beside that level."""
+    idx = attnref.buckets_of(c['qp'][None], c['kp'][None], 32, True, 64)
+    level = torch.zeros(32, dtype=torch.float64)
+    level[BEFORE], level[BEHIND] = c['table'][0, BEFORE, 0].double(), c['table'][0, BEHIND, 0].double()
+    pair = level[idx[0, 0]]                                  # [Lq, Lk]
+    row = pair.amax(dim=1, keepdim=True)
+    entry = torch.where((level == 0)[:, None], c['table'][0].double(), attnsteps.NO)
+    bias = torch.where((pair == row)[..., None], entry[idx[0, 0]], torch.full((), -math.inf).double()).permute(2, 0, 1)[None]
+    p, p_rel = attnsteps.softmax(c, bias, rounded_at=row[:, 0])
+    return attnsteps.attention(c, p, p_rel, training, idx=idx, buckets=32)
+
+
+@pytest.mark.parametrize('dtype,n', LEVEL_CASES)
+@pytest.mark.parametrize('d', [32, 64, 128])
+def test_attention_low_entries_forward(dtype, n, d):
+    """whole tiles of one level before the next: the digits of later scores survive, also of rows that have nothing but a low entry"""
+    c = _level_case(dtype, LEVELS[dtype][n], d=d, seed=d)
+    for training in (False, True):
+        attnref.assert_within(_run(c, grad=training)['out'], _level_reference(c, training)['out'], 'out, training %s' % training)
+
+
+@pytest.mark.parametrize('dtype,n', LEVEL_CASES)
+def test_attention_low_entries_few_queries_and_splits(dtype, n):
+    """few queries, most of them far from everything, and long rows split over workgroups, some of which see one level only"""
+    for lq, lk, d in ((7, 2500, 64), (7, 2500, 32), (7, 900, 128)):
+        c = _level_case(dtype, LEVELS[dtype][n], b=1, lq=lq, lk=lk, h=4, hk=2, d=d, seed=lq)
+        for training in (False, True):
+            attnref.assert_within(_run(c, grad=training)['out'], _level_reference(c, training)['out'], 'out, training %s' % training)
+
+
+def _tied_case(dtype, lq, lk, seed):
+    """scores of 2^30 and beyond, exact in fp32, the highest one held by two keys of different tiles: each has half of the weight"""
+    c = _case(2, lq, lk, 2, 2, 32, dtype, seed=seed)
+    big = 2.0 ** (15 if dtype == torch.float16 else 20)
+    q, k = torch.zeros_like(c['q']), torch.zeros_like(c['k'])
+    q[..., 3] = big
+    k[..., 3] = -big / 2
+    k[:, 5, :, 3] = k[:, lk - 4, :, 3] = big
+    k[:, lk // 2, :, 3] = 0.875 * big
+    return dict(c, q=q, k=k)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('lq,lk', [(3, 600), (50, 333)])
+def test_attention_huge_tied_scores(dtype, lq, lk):
+    c = _tied_case(dtype, lq, lk, seed=40)
+    pair = c['v'][:, [5, lk - 4]].double()                                     # [B, 2, H, D]
+    want = (pair.sum(1) / 2)[:, None].expand(c['q'].shape)
+    # the weights are exact in every type; a sum of two products, a reciprocal, the result's own rounding
+    bound = 6 * attnref.U * pair.abs().sum(1)[:, None] + attnref.half_step(dtype) * want.abs() + attnref.SUBNORMAL[dtype]
+    for grad in (False, True):
+        attnref.assert_within(_run(c, grad=grad)['out'], (want, bound), 'out')

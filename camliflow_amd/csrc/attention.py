@@ -214,7 +214,7 @@ def _run_attention(q, k, v, table, kv_lengths, key_mask, q_pos, k_pos, scale, bi
     lib = _lib.load()
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     out = torch.empty((b, lq, h, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if train else None
+    lse = torch.empty((2, b, h, lq), dtype=torch.float32, device=q.device) if train else None      # two terms
     out_f32 = torch.empty(out.shape, dtype=torch.float32, device=q.device) if train and q.dtype != torch.float32 else None
     desc = _descriptor(q, k, v, kv_lengths, key_mask, table, q_pos, k_pos, scale, bidirectional, max_distance)
     n = _attention_workspace_bytes(False, train, *_sizes(q, k, table, bidirectional, max_distance))

@@ -39,9 +39,10 @@ struct Args {
     Strides qs, ks, vs;         // o, go and the gradients are dense [B][L][heads][D]
     void *out, *dq, *dk, *dv;
     float *out_f32;             // 16-bit types in training: out before its rounding
-    float *lse;                 // [B][H][Lq], log2 domain; +inf where no key is kept
+    float* lse;                 // [2][B][H][Lq], log2 domain, two terms; +inf where no key is kept
     float *delta;               // [B][H][Lq]
     float *go_max;              // [B][H][Lq] fp16 only: largest |go| of a row
+    int *far_rows;              // [B][H][row_groups]: has any of 32 queries a far lse
     float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [2][split][B][H][Lq] (two terms, -inf: no key)
     float *part_dk, *part_dv;   // splits > 1: [split][B][Lk][Hk][D]
     float *part_table;          // [H][parts][axes * buckets]
@@ -51,7 +52,7 @@ struct Args {
     int B, H, Hk, Lq, Lk, D;
     bool few;                   // fwd_few_kernel
     int pack;                   // query heads of one kv head that share a workgroup's rows (few queries), else 1
-    int row_tiles, splits, tiles_per_split, parts;
+    int row_tiles, splits, tiles_per_split, parts, row_groups;
     float scale, scale_log2;
     RelBias rb;
 };
@@ -556,8 +557,7 @@ __device__ __forceinline__ void move_scores(acc16 (&s)[N], float by) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] += by;
 }
-// a0 + a1 > b0 + b1, for pairs as two_sum leaves them
-__device__ __forceinline__ bool two_above(float a0, float a1, float b0, float b1) { return a0 > b0 || (a0 == b0 && a1 > b1); }
+__device__ __forceinline__ bool is_far(float lse) { return fabsf(lse) > FAR && lse < INFINITY; }      // +inf: a row without keys
 
 // ------------------------------------------------------------------------------------------------------------ forward
 // Softmax without a running maximum: the scores come out of the matrix unit already relative to m (the accumulators start at -m /
@@ -570,7 +570,7 @@ __device__ __forceinline__ bool two_above(float a0, float a1, float b0, float b1
 // unit; 8 x 8160 x 2048, 4 heads of 32 with a two-axis bias, bf16, training: 305 us, bound by vector arithmetic (14 instructions a pair, exp
 // of four issue slots); the other way round in fp32, 2 x 2048 x 8160: 156 us.
 // fp32 with a bias starts at zero and subtracts m at the end: at -m / scale every step of the product rounds to a few bits less (a relative
-// error of p of 1e-6), which is nothing to a 16-bit product and shows in an fp32 gradient.  The adjoints do the same with the log-sum.
+// error of p of 1e-6), which is nothing to a 16-bit product and shows in an fp32 gradient.  The adjoints do the same with the log-sum and D.
 template <typename T>
 constexpr bool fold_start() { return sizeof(T) == 2; }
 template <typename T>
@@ -758,7 +758,10 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
     } else {
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.out) + at * a.D, o, inv, a.D, h);
         if constexpr (TWO_TERMS) store_owned<float, TL::DBLOCKS>(a.out_f32 + at * a.D, o, inv, a.D, h);
-        if (TRAIN && h == 0) a.lse[stat] = l == 0.0f ? INFINITY : lse;
+        if (TRAIN && h == 0) {
+            a.lse[stat] = l == 0.0f ? INFINITY : lse;
+            a.lse[(int64_t)a.B * a.Lq * a.H + stat] = l == 0.0f ? 0.0f : lse_lo;
+        }
     }
 }
 
@@ -968,34 +971,38 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
     const float *part = a.part_lse + stat, *part_lo = part + a.splits * rows;
     float top = -INFINITY, use_lo = 0.0f;
     bool bad = false;
-    auto higher = [&](float v, float v_lo) {
-        if (two_above(v, v_lo, top, use_lo)) {
-            top = v;
-            use_lo = v_lo;
-        }
-    };
     for (int s = lane; s < a.splits; s += 64) {
         const float v = part[s * rows];
-        higher(v, part_lo[s * rows]);
+        top = fmaxf(top, v);
         bad |= v != v;
     }
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const float v = __shfl_xor(top, off, 64);
-        higher(v, __shfl_xor(use_lo, off, 64));
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const bool far = is_far(top);
+    if (far) {          // the second term of the highest, so that no weight passes 1
+        use_lo = -INFINITY;
+        for (int s = lane; s < a.splits; s += 64)
+            if (part[s * rows] == top) use_lo = fmaxf(use_lo, part_lo[s * rows]);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) use_lo = fmaxf(use_lo, __shfl_xor(use_lo, off, 64));
     }
     bad = __any(bad);
     const float use = top == -INFINITY ? 0.0f : top;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+    auto add_up = [&](auto far_rows) {
 #pragma unroll 4
-    for (int s = group; s < a.splits; s += groups) {
-        const float w = __builtin_amdgcn_exp2f((part[s * rows] - use) + (part_lo[s * rows] - use_lo));
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (c < a.D && w != 0.0f) load_f32<float, 4>(a.part_o + (s * rows + at) * a.D + c, v);
-        sum += w;
+        for (int s = group; s < a.splits; s += groups) {
+            float w = part[s * rows] - use, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (decltype(far_rows)::value) w += part_lo[s * rows] - use_lo;
+            w = __builtin_amdgcn_exp2f(w);
+            if (c < a.D && w != 0.0f) load_f32<float, 4>(a.part_o + (s * rows + at) * a.D + c, v);
+            sum += w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
-    }
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+        }
+    };
+    if (far) add_up(Int<1>{});
+    else add_up(Int<0>{});
     for (int off = 32; off >= lanes; off >>= 1) {
         sum += __shfl_xor(sum, off, 64);
 #pragma unroll
@@ -1003,7 +1010,12 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
     }
     if (group != 0) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (a.lse && c == 0) a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : use + (use_lo + __builtin_amdgcn_logf(sum));
+    if (a.lse && c == 0) {
+        float lse, lse_lo;
+        two_sum(use, use_lo + __builtin_amdgcn_logf(sum), lse, lse_lo);
+        a.lse[stat] = bad ? NAN : sum == 0.0f ? INFINITY : lse;
+        a.lse[rows + stat] = sum == 0.0f ? 0.0f : lse_lo;
+    }
     if (c >= a.D) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = bad ? NAN : acc[i] * inv;
@@ -1018,6 +1030,12 @@ __device__ __forceinline__ float unit_scale(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
+constexpr int dkdv_stats(bool far_rows) { return far_rows ? 3 : 2; }       // numbers of a streamed row beside its tiles
+
+// FAR_ROWS: scores are rounded as in the forward before both terms of lse are taken off them.  That is one or two instructions more a pair, and
+// in a branch it displaces what the narrow kernels' registers are spent on (484 -> 506 to 576 us at the size below, taken or not; in dkdv 361
+// -> 370, and 658 -> 780 for a whole step of fp32 heads of 64).  So both adjoints of far rows are a launch of their own (far_kernel): its
+// workgroups leave at once (5 us), but for those of dq with a far row and those of dkdv whose kv head has one, which compute all their rows again.
 // HIST: with the table's gradient.  LDS: tiles (one buffer), lut, hist[axes * buckets][columns].  A thread adds to a column by plain reads and
 // writes: sums in a fixed order, no bank conflicts.  One axis: a column per thread, and 2 waves instead of 4 (WAVES) where more than 64
 // buckets would not fit.  Two axes: lanes l and l + 32 share a column; they take the axes in opposite order, so that one is among the rows of
@@ -1028,8 +1046,9 @@ __device__ __forceinline__ float unit_scale(float x) {
 // arithmetic both at about 60 %; 2 x 2048 x 8160, fp32: 265 us (tiles in two buffers, one workgroup: 465 with fp32 products).
 constexpr int hist_columns(int axes, int waves) { return axes == 2 ? 32 * waves : 64 * waves; }
 
-template <typename T, int DP, int AXES, int WAVES, bool HIST>
-__global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || sizeof(T) == 4 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) {
+// blocks: of the launch's workgroups those that work on this
+template <typename T, int DP, int AXES, int WAVES, bool HIST, bool FAR_ROWS>
+__device__ __forceinline__ void dq_body(const Args& a, int block, int blocks) {
     constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
     using TL = Tile<T, DP, R>;
     using L = typename TL::Lds;
@@ -1043,7 +1062,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
     float* hist = reinterpret_cast<float*>(lut + AXES * span);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int id = unit_per_xcd(blockIdx.x, gridDim.x, a.row_tiles * a.splits);
+    int id = unit_per_xcd(block, blocks, a.row_tiles * a.splits);
     const int split = id % a.splits;
     id /= a.splits;
     const int rt = id % a.row_tiles;
@@ -1062,6 +1081,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
     const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
     const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
     const int64_t at = ((int64_t)b * a.Lq + q0) * a.H + head, stat = ((int64_t)b * a.H + head) * a.Lq + q0;
+    const float lse_lo = FAR_ROWS ? a.lse[(int64_t)a.B * a.H * a.Lq + stat] : 0.0f;
 
     Frag<T> qf[TL::KSTEPS], gf[TL::KSTEPS];
     load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + q0 * a.qs.l + head * a.qs.h, exists, a.D, h);
@@ -1082,11 +1102,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
         }
     }
     delta = half_sum(delta);
-    if (exists && split == 0 && h == 0) a.delta[stat] = delta;
+    if (!FAR_ROWS && exists && split == 0 && h == 0) a.delta[stat] = delta;
     float unscale = 1.0f;
     if constexpr (__is_same(T, _Float16)) {
         most = half_max(most);
-        if (exists && split == 0 && h == 0) a.go_max[stat] = most;
+        if (!FAR_ROWS && exists && split == 0 && h == 0) a.go_max[stat] = most;
         const float f = unit_scale(most);
         unscale = unit_scale(f);
         delta *= f;
@@ -1097,9 +1117,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
     }
     // the accumulators start at -lse / scale and -delta: the products come out as the exponent and as dp - D.  +inf (a row without keys,
     // or none at all) makes every p zero.
-    constexpr bool FOLD = fold_start<T>();
+    constexpr bool FOLD = fold_start<T>(), FOLD_S = FOLD && !FAR_ROWS;
     const float lse = exists ? a.lse[stat] : INFINITY;
-    const acc16 start_s = FOLD ? splat(-lse / a.scale_log2) : acc16{0}, start_d = FOLD ? splat(-delta) : acc16{0};
+    if constexpr (!FAR_ROWS) {
+        const bool far = __any(is_far(lse));
+        if (split == 0 && lane == 0) a.far_rows[((int64_t)b * a.H + head) * a.row_groups + rt * WAVES + wave] = far;
+    }
+    const acc16 start_s = FOLD_S ? splat(-lse / a.scale_log2) : acc16{0}, start_d = FOLD ? splat(-delta) : acc16{0};
     const LaneMap<TL, T> map(lane);
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
@@ -1163,7 +1187,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
                             at[k][x] = e[1];
                         }
                         s[i] = __builtin_fmaf(s[i], a.scale_log2, bias);
-                        if constexpr (!FOLD) s[i] -= lse;
+                        if constexpr (!FOLD_S) s[i] -= lse;
+                        if constexpr (FAR_ROWS) s[i] -= lse_lo;
                         s[i] = kept_row(half_bits, i) ? s[i] : -INFINITY;
                         dp[i] = (FOLD ? dp[i] : __builtin_fmaf(dp[i], sign, -delta)) * __builtin_amdgcn_exp2f(s[i]);
                     }
@@ -1187,10 +1212,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
                 for (int i = 0; i < 16; ++i) {
                     if constexpr (AXES > 0) {
                         s[i] = __builtin_fmaf(s[i], a.scale_log2, pair_bias<AXES>(off, i, lo, hi));
-                        if constexpr (!FOLD) s[i] -= lse;
+                        if constexpr (!FOLD_S) s[i] -= lse;
+                    } else if constexpr (FAR_ROWS) {
+                        s[i] = s[i] * a.scale_log2 - lse;
                     } else {
                         s[i] = FOLD ? s[i] * a.scale_log2 : __builtin_fmaf(s[i], a.scale_log2, -lse);
                     }
+                    if constexpr (FAR_ROWS) s[i] -= lse_lo;
                 }
                 if (half_bits != 0xffffffffu) {
 #pragma unroll
@@ -1230,21 +1258,24 @@ __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || siz
     }
 }
 
+template <typename T, int DP, int AXES, int WAVES, bool HIST>
+__global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || sizeof(T) == 4 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) { dq_body<T, DP, AXES, WAVES, HIST, false>(a, blockIdx.x, gridDim.x); }
+
 // ------------------------------------------------------------------------------------------------------------ dk, dv
 // Measured at the sizes above: bf16 390 us (vector arithmetic and LDS both at 55 %, three workgroups a CU), fp32 250 us.
-template <typename T, int DP, int AXES>
-__global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64 ? 2 : 1) void dkdv_kernel(Args a) {
+template <typename T, int DP, int AXES, bool FAR_ROWS>
+__device__ __forceinline__ void dkdv_body(const Args& a, int block, int blocks) {
     constexpr int R = tile_rows(sizeof(T), DP);
     using TL = Tile<T, DP, R>;
     using L = typename TL::Lds;
-    constexpr int THREADS = 256, ENTRY = (int)sizeof(float);
+    constexpr int THREADS = 256, ENTRY = (int)sizeof(float), STATS = dkdv_stats(FAR_ROWS);
     extern __shared__ __align__(16) char smem[];
     L* tiles = reinterpret_cast<L*>(smem);                                              // [2][Q, dO]
-    float* stats = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);                     // [2][lse, delta][ROWS]
-    float* lut = reinterpret_cast<float*>(stats + 4 * TL::ROWS);
+    float* stats = reinterpret_cast<float*>(tiles + 4 * TL::ELEMS);                     // [2][lse, delta (FAR_ROWS: and lse's second term)][ROWS]
+    float* lut = reinterpret_cast<float*>(stats + 2 * STATS * TL::ROWS);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    int id = unit_per_xcd(blockIdx.x, gridDim.x, a.row_tiles * a.splits);
+    int id = unit_per_xcd(block, blocks, a.row_tiles * a.splits);
     const int split = id % a.splits;
     id /= a.splits;
     const int rt = id % a.row_tiles;
@@ -1272,7 +1303,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
             hi[x] = centre + ENTRY * a.rb.limit;
         }
     }
-    constexpr bool HALF = __is_same(T, _Float16), FOLD = fold_start<T>();
+    constexpr bool HALF = __is_same(T, _Float16), FOLD = fold_start<T>(), FOLD_S = FOLD && !FAR_ROWS;
     constexpr float P_LOG2 = HALF ? 10.0f : 0.0f, P_UNSCALE = HALF ? 1.0f / 1024.0f : 1.0f;
     float ds_scale = 1.0f, ds_unscale = 1.0f;       // of dS beside that of P
     if constexpr (HALF) {
@@ -1307,19 +1338,20 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
         const int head = kvh * group + t / q_tiles, row0 = (t % q_tiles) * TL::ROWS;
         st.load(static_cast<const T*>(a.q) + b * a.qs.b + head * a.qs.h + row0 * a.qs.l,
                 static_cast<const T*>(a.go) + (((int64_t)b * a.Lq + row0) * a.H + head) * a.D, row0, a.Lq, a.D, nullptr);
-        if (tid < 2 * TL::ROWS) {
-            const int r = row0 + tid % TL::ROWS;
-            const float* src = tid < TL::ROWS ? a.lse : a.delta;
-            // what the accumulators start at: -lse / scale (fp32: -lse, and both are added at the end) and -delta; a row that does not exist has lse = +inf, so p = 0
-            const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : tid < TL::ROWS ? INFINITY : 0.0f;
-            snext = tid < TL::ROWS && FOLD ? (P_LOG2 - x) / a.scale_log2 : -x;
+        if (tid < STATS * TL::ROWS) {
+            const int r = row0 + tid % TL::ROWS, which = tid / TL::ROWS;
+            const float* src = which == 1 ? a.delta : a.lse + (which == 2 ? (int64_t)a.B * a.H * a.Lq : 0);
+            // what the accumulators start at: -lse / scale (fp32 and FAR_ROWS: -lse, added at the end) and -delta; a row that does not exist has
+            // lse = +inf, so p = 0
+            const float x = r < a.Lq ? src[((int64_t)b * a.H + head) * a.Lq + r] : which == 0 ? INFINITY : 0.0f;
+            snext = which == 0 && FOLD_S ? (P_LOG2 - x) / a.scale_log2 : -x;
         }
         if constexpr (AXES > 0) pos_next.load(qpos, row0, a.Lq);
     };
     auto store = [&](int buf) {
         L* n = tiles + buf * 2 * TL::ELEMS;
         st.store(n, n + TL::ELEMS);
-        if (tid < 2 * TL::ROWS) stats[buf * 2 * TL::ROWS + tid] = snext;
+        if (tid < STATS * TL::ROWS) stats[buf * STATS * TL::ROWS + tid] = snext;
     };
     int lut_head = -1;
     if (t0 < t1) {
@@ -1339,7 +1371,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
             }
         }
         const L *qt = tiles + cur * 2 * TL::ELEMS, *gt = qt + TL::ELEMS;
-        const float* start = stats + cur * 2 * TL::ROWS;
+        const float* start = stats + cur * STATS * TL::ROWS;
 #pragma unroll
         for (int nb = 0; nb < TL::BLOCKS; ++nb) {
             const L *qb = qt + nb * 32 * DP, *gb = gt + nb * 32 * DP;
@@ -1347,7 +1379,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = nb * 32 + acc_row(i, h);
-                s[i] = FOLD ? start[r] : 0.0f;
+                s[i] = FOLD_S ? start[r] : 0.0f;
                 dp[i] = FOLD ? start[TL::ROWS + r] : 0.0f;
             }
             s = product<T, TL>(map, qb, kf, s);
@@ -1363,8 +1395,9 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
                 } else {
                     x = s[i] * a.scale_log2;
                 }
+                if constexpr (!FOLD_S) x += start[nb * 32 + acc_row(i, h)];
+                if constexpr (FAR_ROWS) x += start[2 * TL::ROWS + nb * 32 + acc_row(i, h)] + P_LOG2;
                 if constexpr (!FOLD) {
-                    x += start[nb * 32 + acc_row(i, h)];
                     dp[i] = __builtin_fmaf(dp[i], sign, start[TL::ROWS + nb * 32 + acc_row(i, h)]);
                 }
                 s[i] = __builtin_amdgcn_exp2f(x);
@@ -1397,6 +1430,31 @@ __global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64
     } else {
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dk) + at * a.D, dk, a.scale * ds_unscale, a.D, h);
         store_owned<T, TL::DBLOCKS>(static_cast<T*>(a.dv) + at * a.D, dv, P_UNSCALE, a.D, h);
+    }
+}
+
+template <typename T, int DP, int AXES>
+__global__ __launch_bounds__(256, DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64 ? 2 : 1) void dkdv_kernel(Args a) { dkdv_body<T, DP, AXES, false>(a, blockIdx.x, gridDim.x); }
+
+// Both adjoints of far rows: dq's workgroups first.
+template <typename T, int DP, int AXES, int WAVES, bool HIST>
+__global__ __launch_bounds__(256, 1) void far_kernel(Args dq, Args dkdv, int dq_blocks) {
+    // every wave looks for itself
+    auto none = [](const int* rows, int n) {
+        bool any = false;
+        for (int i = threadIdx.x & 63; i < n; i += 64) any |= rows[i] != 0;
+        return !__any(any);
+    };
+    int block = blockIdx.x;
+    if (block < dq_blocks) {
+        const int id = unit_per_xcd(block, dq_blocks, dq.row_tiles * dq.splits) / dq.splits;
+        if (none(dq.far_rows + (int64_t)(id / dq.row_tiles) * dq.row_groups + id % dq.row_tiles * WAVES, WAVES)) return;
+        dq_body<T, DP, AXES, WAVES, HIST, true>(dq, block, dq_blocks);
+    } else {
+        block -= dq_blocks;
+        const int blocks = gridDim.x - dq_blocks, id = unit_per_xcd(block, blocks, dkdv.row_tiles * dkdv.splits) / dkdv.splits, n = dkdv.H / dkdv.Hk * dkdv.row_groups;
+        if (none(dkdv.far_rows + (int64_t)(id / dkdv.row_tiles) * n, n)) return;
+        dkdv_body<T, DP, AXES, true>(dkdv, block, blocks);
     }
 }
 
@@ -1435,13 +1493,13 @@ constexpr size_t tile_bytes() { return 4 * sizeof(typename Parts<T>::Lds) * Tile
 
 inline size_t lut_bytes(const Args& a, int axes, int heads) { return axes ? sizeof(float) * heads * axes * (2 * a.rb.limit + 1) : 0; }
 
-template <typename K>
-int start(K kernel, const char* what, unsigned long long& done, dim3 grid, int threads, size_t lds, const Args& a, hipStream_t s) {
+template <typename K, typename... A>
+int start(K kernel, const char* what, unsigned long long& done, dim3 grid, int threads, size_t lds, hipStream_t s, const A&... args) {
     if (lds > MAX_LDS || !camli_reserve_lds((const void*)kernel, MAX_LDS, done)) {
         camli_set_error("%s: cannot reserve %zu bytes of LDS", what, lds);
         return CAMLI_ELAUNCH;
     }
-    kernel<<<grid, threads, lds, s>>>(a);
+    kernel<<<grid, threads, lds, s>>>(args...);
     return camli_check_launch(what);
 }
 
@@ -1450,14 +1508,14 @@ int run_fwd_mode(const Args& a, hipStream_t s) {
     constexpr int R = tile_rows(sizeof(T), DP);
     static unsigned long long done = 0;
     const size_t lds = tile_bytes<T, DP, R>() + lut_bytes(a, AXES, a.pack);
-    return start(fwd_kernel<T, DP, AXES, TRAIN>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, a, s);
+    return start(fwd_kernel<T, DP, AXES, TRAIN>, "camli_cross_attention_fwd", done, dim3(a.row_tiles * (a.H / a.pack) * a.B * a.splits), 256, lds, s, a);
 }
 
 template <typename T, int DP, int AXES>
 int run_fwd_few(const Args& a, hipStream_t s) {
     static unsigned long long done = 0;
     const size_t lds = few_bytes<T, DP>(a.pack * a.Lq) + lut_bytes(a, AXES, a.pack);
-    return start(fwd_few_kernel<T, DP, AXES>, "camli_cross_attention_fwd", done, dim3(a.H / a.pack * a.B * a.splits), 256, lds, a, s);
+    return start(fwd_few_kernel<T, DP, AXES>, "camli_cross_attention_fwd", done, dim3(a.H / a.pack * a.B * a.splits), 256, lds, s, a);
 }
 
 template <typename T, int DP, int AXES>
@@ -1471,41 +1529,66 @@ int run_fwd(const Args& a, hipStream_t s) {
 }
 
 template <typename T, int DP, int AXES, int WAVES, bool HIST>
-int run_dq_mode(const Args& a, hipStream_t s) {
-    constexpr int R = dq_tile_rows(sizeof(T), DP, HIST);
-    static unsigned long long done = 0;
-    size_t lds = tile_bytes<T, DP, R>() / (HIST ? 2 : 1) + lut_bytes(a, AXES, 1);
+size_t dq_lds(const Args& a) {
+    size_t lds = tile_bytes<T, DP, dq_tile_rows(sizeof(T), DP, HIST)>() / (HIST ? 2 : 1) + lut_bytes(a, AXES, 1);
     if (HIST) lds += lut_bytes(a, AXES, 1) + sizeof(float) * AXES * a.rb.buckets * hist_columns(AXES, WAVES);      // entries of 8 bytes
-    return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, lds, a, s);
+    return lds;
+}
+template <typename T, int DP, int AXES, bool FAR_ROWS>
+size_t dkdv_lds(const Args& a) {
+    constexpr int R = tile_rows(sizeof(T), DP);
+    return tile_bytes<T, DP, R>() + sizeof(float) * 2 * dkdv_stats(FAR_ROWS) * R + lut_bytes(a, AXES, 1);
 }
 
-template <typename T, int DP, int AXES>
-int run_dq(const Args& a, int waves, hipStream_t s) {
-    int rc;
-    if constexpr (AXES > 0) {
-        if (!a.part_table) rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
-        else if constexpr (AXES == 1) rc = waves == 2 ? run_dq_mode<T, DP, AXES, 2, true>(a, s) : run_dq_mode<T, DP, AXES, 4, true>(a, s);
-        else rc = run_dq_mode<T, DP, AXES, 4, true>(a, s);
-    } else {
-        rc = run_dq_mode<T, DP, AXES, 4, false>(a, s);
-    }
-    return rc;
+template <typename T, int DP, int AXES, int WAVES, bool HIST>
+int run_dq_mode(const Args& a, hipStream_t s) {
+    static unsigned long long done = 0;
+    return start(dq_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.H * a.B * a.splits), 64 * WAVES, dq_lds<T, DP, AXES, WAVES, HIST>(a), s, a);
 }
+
+template <typename T, int DP, int AXES, int WAVES, bool HIST>
+int run_far_mode(const Args& dq, const Args& dkdv, hipStream_t s) {
+    static unsigned long long done = 0;
+    const int dq_blocks = dq.dq || HIST ? dq.row_tiles * dq.H * dq.B * dq.splits : 0, dkdv_blocks = dkdv.dk ? dkdv.row_tiles * dkdv.Hk * dkdv.B * dkdv.splits : 0;
+    const size_t lq = dq_lds<T, DP, AXES, WAVES, HIST>(dq), lk = dkdv_lds<T, DP, AXES, true>(dkdv);
+    auto launch = [&](int nq, int nk, int threads) {
+        if (nq + nk == 0) return CAMLI_OK;
+        return start(far_kernel<T, DP, AXES, WAVES, HIST>, "camli_cross_attention_bwd", done, dim3(nq + nk), threads, lq > lk ? lq : lk, s, dq, dkdv, nq);
+    };
+    if (WAVES == 4 && dq_blocks + dkdv_blocks < (1 << 24)) return launch(dq_blocks, dkdv_blocks, 256);      // 2^32 threads a launch
+    const int rc = launch(dq_blocks, 0, 64 * WAVES);
+    return rc == CAMLI_OK ? launch(0, dkdv_blocks, 256) : rc;
+}
+
+// RUN<..., WAVES, HIST> for what is wanted of the table's gradient
+#define XATTN_SELECT_DQ(RUN, TABLE, ...)                                                                              \
+    if constexpr (AXES > 0) {                                                                                         \
+        if (!TABLE) return RUN<T, DP, AXES, 4, false>(__VA_ARGS__);                                                   \
+        if constexpr (AXES == 1) return waves == 2 ? RUN<T, DP, AXES, 2, true>(__VA_ARGS__) : RUN<T, DP, AXES, 4, true>(__VA_ARGS__); \
+        else return RUN<T, DP, AXES, 4, true>(__VA_ARGS__);                                                           \
+    } else {                                                                                                          \
+        return RUN<T, DP, AXES, 4, false>(__VA_ARGS__);                                                               \
+    }
+
+template <typename T, int DP, int AXES>
+int run_dq(const Args& a, int waves, hipStream_t s) { XATTN_SELECT_DQ(run_dq_mode, a.part_table, a, s) }
+
+template <typename T, int DP, int AXES>
+int run_far(const Args& dq, const Args& dkdv, int waves, hipStream_t s) { XATTN_SELECT_DQ(run_far_mode, dq.part_table, dq, dkdv, s) }
 
 template <typename T, int DP, int AXES>
 int run_dkdv(const Args& a, hipStream_t s) {
-    constexpr int R = tile_rows(sizeof(T), DP);
     static unsigned long long done = 0;
-    const size_t lds = tile_bytes<T, DP, R>() + sizeof(float) * 4 * R + lut_bytes(a, AXES, 1);
-    return start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, lds, a, s);
+    return start(dkdv_kernel<T, DP, AXES>, "camli_cross_attention_bwd", done, dim3(a.row_tiles * a.Hk * a.B * a.splits), 256, dkdv_lds<T, DP, AXES, false>(a), s, a);
 }
 
-// the three kernels by head width (padded to 32, 64 or 128) and axes of the bias
+// the kernels by head width (padded to 32, 64 or 128) and axes of the bias
 template <typename T>
 struct Launch {
     static int fwd(const Args& a, int axes, hipStream_t s);
     static int dq(const Args& a, int axes, int waves, hipStream_t s);
     static int dkdv(const Args& a, int axes, hipStream_t s);
+    static int far(const Args& dq, const Args& dkdv, int axes, int waves, hipStream_t s);
     static int sum(const SumJobs& jobs, int n, hipStream_t s);
 };
 
@@ -1518,6 +1601,11 @@ struct Launch {
     template <> int Launch<TYPE>::fwd(const Args& a, int axes, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_fwd, a, s) }
 #define XATTN_DEFINE_DQ(TYPE) \
     template <> int Launch<TYPE>::dq(const Args& a, int axes, int waves, hipStream_t s) { using T = TYPE; XATTN_SELECT(run_dq, a, waves, s) }
+#define XATTN_DEFINE_FAR(TYPE)                                                                                     \
+    template <> int Launch<TYPE>::far(const Args& a, const Args& dkdv, int axes, int waves, hipStream_t s) {       \
+        using T = TYPE;                                                                                            \
+        XATTN_SELECT(run_far, a, dkdv, waves, s)                                                                   \
+    }
 #define XATTN_DEFINE_SUM(TYPE)                                                                                     \
     template <> int Launch<TYPE>::sum(const SumJobs& jobs, int n, hipStream_t s) {                                 \
         int64_t most = 0;                                                                                          \

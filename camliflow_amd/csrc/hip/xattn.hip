@@ -115,7 +115,7 @@ struct BwdPlan {
     int64_t bytes;
 };
 
-// workspace of the backward: delta, then the parts of dq, of the table, of dk and dv
+// workspace of the backward: delta, which rows are far, then the parts of dq, of the table, of dk and dv
 BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base) {
     BwdPlan p{a, a, 0};
     plan_dq(p.dq, d->type, d->bias_axes, table);
@@ -123,6 +123,9 @@ BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base
     const int64_t rows = (int64_t)a.B * a.H * a.Lq;
     p.dq.delta = p.dkdv.delta = reinterpret_cast<float*>(base);
     int64_t end = align256(4 * rows);
+    p.dq.row_groups = p.dkdv.row_groups = p.dq.row_tiles * dq_waves(p.dq, d->bias_axes, table);
+    p.dq.far_rows = p.dkdv.far_rows = reinterpret_cast<int*>(base + end);
+    end += align256((int64_t)4 * a.B * a.H * p.dq.row_groups);
     if (d->type == CAMLI_F16) {
         p.dq.go_max = p.dkdv.go_max = reinterpret_cast<float*>(base + end);
         end += align256(4 * rows);
@@ -201,13 +204,16 @@ extern "C" int camli_cross_attention_bwd(const camli_attention* d, const float* 
     int rc = d->type == CAMLI_F32 ? xattn::Launch<float>::dq(p.dq, axes, waves, s)
              : d->type == CAMLI_BF16 ? xattn::Launch<__bf16>::dq(p.dq, axes, waves, s) : xattn::Launch<_Float16>::dq(p.dq, axes, waves, s);
     if (rc != CAMLI_OK) return rc;
-    if (gtable) {
-        rc = rel_bias_join(p.dq.part_table, gtable, d->type, a.H, axes * d->bias_buckets, p.dq.parts, "camli_cross_attention_bwd", s);
-        if (rc != CAMLI_OK) return rc;
-    }
     if (gk) {
         rc = d->type == CAMLI_F32 ? xattn::Launch<float>::dkdv(p.dkdv, axes, s)
              : d->type == CAMLI_BF16 ? xattn::Launch<__bf16>::dkdv(p.dkdv, axes, s) : xattn::Launch<_Float16>::dkdv(p.dkdv, axes, s);
+        if (rc != CAMLI_OK) return rc;
+    }
+    rc = d->type == CAMLI_F32 ? xattn::Launch<float>::far(p.dq, p.dkdv, axes, waves, s)
+         : d->type == CAMLI_BF16 ? xattn::Launch<__bf16>::far(p.dq, p.dkdv, axes, waves, s) : xattn::Launch<_Float16>::far(p.dq, p.dkdv, axes, waves, s);
+    if (rc != CAMLI_OK) return rc;
+    if (gtable) {
+        rc = rel_bias_join(p.dq.part_table, gtable, d->type, a.H, axes * d->bias_buckets, p.dq.parts, "camli_cross_attention_bwd", s);
         if (rc != CAMLI_OK) return rc;
     }
     xattn::SumJobs jobs;

@@ -1,0 +1,6 @@
+// Cross attention, both adjoints of far rows, bf16 elements: the instantiations of xattn.h (one file each, so that they compile side by side).
+#include "xattn.h"
+
+namespace xattn {
+XATTN_DEFINE_FAR(__bf16)
+}

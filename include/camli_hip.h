@@ -765,7 +765,8 @@ int camli_rel_bias_bwd(const void *gout, const int *q_pos, int64_t q_pos_batch_s
  *   zeros and takes no part in any gradient; so does a row whose scores are all -inf, if its incoming gradient is finite.
  *   bias_axes 0: no bias; else as camli_rel_bias_fwd, table [axes,buckets,H] of `type`, H <= 65535.
  *   fp32 factors are multiplied as three bf16 parts each (exact to 2^-25): a kept infinity, or a value beyond 3.38e38, gives NaN.
- *   lse [B,H,Lq]: log2 of each row's softmax sum, +inf for rows without keys; NULL if no backward follows.
+ *   lse [2,B,H,Lq]: log2 of each row's softmax sum, +inf for rows without keys, and what a float beyond 256 rounds away of it; NULL if no
+ *   backward follows.
  *   out_f32 [B,Lq,H,D]: out before its rounding to a 16-bit type, for the backward (fwd: unused for fp32 or without lse; bwd: fp32 out itself).
  *   bwd: gq may be NULL, gk and gv both or neither, gtable [axes,buckets,H] may be NULL; everything given is fully written, no atomics
  *   whose order matters: the same bits on every run.

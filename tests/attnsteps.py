@@ -9,6 +9,7 @@ import math
 
 import torch
 
+import attnref
 from attnref import SUBNORMAL, U, half_step
 
 NO = torch.zeros((), dtype=torch.float64)
@@ -22,9 +23,10 @@ def _heads(c):
     return Q, K, V, g
 
 
-def softmax(c, bias, scale=None, rounded_at=0.0):
+def softmax(c, bias, scale=None, rounded_at=0.0, roundings=1):
     """c: q, k, v, keep; bias [B|1, H|1, Lq, Lk] in 64 bits, -inf takes a pair out -> (p, relative error of p).
-    rounded_at [Lq] or number: what the scores were added to in fp32 before they were compared (a constant of the row, left out of `bias`)."""
+    rounded_at [Lq] or number: what the scores were added to in fp32 before they were compared (a constant of the row, left out of `bias`).
+    roundings: sums in fp32 at that size, each off by half a step there: that of the axes' entries (two axes), and that with the product."""
     Q, K, _, _ = _heads(c)
     scale = c['q'].shape[-1] ** -0.5 if scale is None else scale
     s = scale * Q @ K.transpose(2, 3)
@@ -42,7 +44,7 @@ def softmax(c, bias, scale=None, rounded_at=0.0):
     lk, dim = K.shape[2], Q.shape[3]
     # a dot of dim terms, scale, log2(e), the bias; the reference, of the size of the highest score, in every step of a product that starts there
     err = torch.where(out, NO, U * ((dim + 6) * mags + 6 * bias.nan_to_num(0, 0, 0).abs() + 10 * top.nan_to_num(0, 0, 0).abs())).amax(-1, keepdim=True) + 4 * U
-    err = torch.where(swallowed, 4 * U, err + torch.expm1(step * math.log(2)) / 2)
+    err = torch.where(swallowed, 4 * U, err + torch.expm1(roundings * step * math.log(2)) / 2)
     return p, 2 * err + (lk + 16) * U + 4 * U * torch.where(out, NO, s - top).abs().clamp(max=200)
 
 
@@ -94,3 +96,13 @@ def attention(c, p, p_rel, training=True, scale=None, idx=None, buckets=0):
                 err[a, :, i] = torch.bincount(flat, weights=(ds32[:, i] + 700 * U * ds[:, i].abs()).reshape(-1), minlength=buckets)
         out['dtable'] = (val, err + h * (val.abs() + err) + sub)
     return out
+
+
+def assert_within(got, want_bound, name):
+    """attnref.assert_within; a value beyond the type's largest number has to come out as infinity"""
+    want, bound = want_bound
+    largest = torch.finfo(got.dtype).max * (1 + half_step(got.dtype))
+    over = want.abs() - bound > largest
+    assert torch.equal(got.detach().cpu().double()[over], torch.copysign(torch.full_like(want, math.inf), want)[over]), name
+    bound = torch.where(want.abs() + bound > largest, math.inf, bound)      # within the bound of the border: either
+    attnref.assert_within(torch.where(over, NO, got.detach().cpu().double().clamp(-1e300, 1e300)), (torch.where(over, NO, want), torch.where(over, NO, bound)), name)

@@ -21,15 +21,16 @@ LEVEL_CASES = [pytest.param(t, n, id='%s-%d' % (i, n)) for t, i in zip(TYPES, ID
 BEFORE, BEHIND = 15, 31         # of 32 buckets, 64 positions
 
 
-def _level_case(dtype, levels, b=2, lq=40, lk=700, h=2, hk=1, d=32, seed=0):
-    """first 300 keys far before nearly every query, then 100 far behind, then the near ones; the last six queries are far from all keys"""
-    c = _case(b, lq, lk, h, hk, d, dtype, axes=1, seed=seed)
+def _level_case(dtype, levels, b=2, lq=40, lk=700, h=2, hk=1, d=32, seed=0, axes=1):
+    """on the first axis: 300 keys far before nearly every query, then 100 far behind, then the near ones; the last six queries are far
+    from all keys"""
+    c = _case(b, lq, lk, h, hk, d, dtype, axes=axes, seed=seed)
     g = torch.Generator().manual_seed(seed + 1)
     c['table'][0, BEFORE], c['table'][0, BEHIND] = levels
-    c['kp'] = torch.randint(-40, 41, (lk, 1), generator=g, dtype=torch.int32)
-    c['kp'][:3 * lk // 7], c['kp'][3 * lk // 7:4 * lk // 7] = -2000, 2000
-    c['qp'] = torch.randint(-20, 21, (lq, 1), generator=g, dtype=torch.int32)
-    c['qp'][-6:-1], c['qp'][-1] = 900, 5000
+    c['kp'] = torch.randint(-40, 41, (lk, axes), generator=g, dtype=torch.int32)
+    c['kp'][:3 * lk // 7, 0], c['kp'][3 * lk // 7:4 * lk // 7, 0] = -2000, 2000
+    c['qp'] = torch.randint(-20, 21, (lq, axes), generator=g, dtype=torch.int32)
+    c['qp'][-6:-1, 0], c['qp'][-1, 0] = 900, 5000
     return c
 
 
@@ -41,8 +42,11 @@ def _level_reference(c, training):
     pair = level[idx[0, 0]]                                  # [Lq, Lk]
     row = pair.amax(dim=1, keepdim=True)
     entry = torch.where((level == 0)[:, None], c['table'][0].double(), attnsteps.NO)
-    bias = torch.where((pair == row)[..., None], entry[idx[0, 0]], torch.full((), -math.inf).double()).permute(2, 0, 1)[None]
-    p, p_rel = attnsteps.softmax(c, bias, rounded_at=row[:, 0])
+    bias = torch.where((pair == row)[..., None], entry[idx[0, 0]], torch.full((), -math.inf).double())
+    for a in range(1, idx.shape[0]):
+        bias = bias + c['table'][a].double()[idx[a, 0]]
+    bias = bias.permute(2, 0, 1)[None]
+    p, p_rel = attnsteps.softmax(c, bias, rounded_at=row[:, 0], roundings=idx.shape[0])
     return attnsteps.attention(c, p, p_rel, training, idx=idx, buckets=32)
 
 
@@ -52,7 +56,7 @@ def test_attention_low_entries_forward(dtype, n, d):
     """whole tiles of one level before the next: the digits of later scores survive, also of rows that have nothing but a low entry"""
     c = _level_case(dtype, LEVELS[dtype][n], d=d, seed=d)
     for training in (False, True):
-        attnref.assert_within(_run(c, grad=training)['out'], _level_reference(c, training)['out'], 'out, training %s' % training)
+        attnsteps.assert_within(_run(c, grad=training)['out'], _level_reference(c, training)['out'], 'out, training %s' % training)
 
 
 @pytest.mark.parametrize('dtype,n', LEVEL_CASES)
@@ -61,7 +65,7 @@ def test_attention_low_entries_few_queries_and_splits(dtype, n):
     for lq, lk, d in ((7, 2500, 64), (7, 2500, 32), (7, 900, 128)):
         c = _level_case(dtype, LEVELS[dtype][n], b=1, lq=lq, lk=lk, h=4, hk=2, d=d, seed=lq)
         for training in (False, True):
-            attnref.assert_within(_run(c, grad=training)['out'], _level_reference(c, training)['out'], 'out, training %s' % training)
+            attnsteps.assert_within(_run(c, grad=training)['out'], _level_reference(c, training)['out'], 'out, training %s' % training)
 
 
 def _tied_case(dtype, lq, lk, seed):
@@ -85,4 +89,39 @@ def test_attention_huge_tied_scores(dtype, lq, lk):
     # the weights are exact in every type; a sum of two products, a reciprocal, the result's own rounding
     bound = 6 * attnref.U * pair.abs().sum(1)[:, None] + attnref.half_step(dtype) * want.abs() + attnref.SUBNORMAL[dtype]
     for grad in (False, True):
-        attnref.assert_within(_run(c, grad=grad)['out'], (want, bound), 'out')
+        attnsteps.assert_within(_run(c, grad=grad)['out'], (want, bound), 'out')
+
+
+@pytest.mark.parametrize('dtype,n', LEVEL_CASES)
+@pytest.mark.parametrize('d,axes', [(32, 1), (32, 2), (64, 1), (64, 2), (128, 2)])
+def test_attention_low_entries_gradients(dtype, n, d, axes):
+    """a row that has nothing but a low entry weighs its keys by the same probabilities in both directions, and the rows beside it are right"""
+    for shape in (dict(), dict(b=1, lq=8, lk=1500, h=4, hk=2), dict(b=1, lq=900, lk=40)):       # the latter two split over keys, over queries
+        c = _level_case(dtype, LEVELS[dtype][n], d=d, axes=axes, seed=d + axes, **shape)
+        want, got = _level_reference(c, True), _run(c)
+        assert set(want) == set(got)
+        for name in want:
+            attnsteps.assert_within(got[name], want[name], name)
+
+
+def test_attention_low_entries_gradients_without_the_table():
+    """a frozen table: the same gradients of the other operands"""
+    from camliflow_amd import csrc
+    for dtype in TYPES:
+        c = _level_case(dtype, LEVELS[dtype][0], axes=2, seed=5)
+        want = _level_reference(c, True)
+        leaves = [c[n].cuda().requires_grad_(True) for n in 'qkv']
+        out = csrc.cross_attention(*leaves, bias_table=c['table'].cuda(), q_pos=c['qp'].cuda(), k_pos=c['kp'].cuda(), max_distance=64)
+        for name, grad in zip(('dq', 'dk', 'dv'), torch.autograd.grad(out, leaves, c['go'].cuda())):
+            attnsteps.assert_within(grad, want[name], name)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('lq,lk', [(3, 600), (50, 333)])
+def test_attention_huge_tied_scores_gradients(dtype, lq, lk):
+    c = _tied_case(dtype, lq, lk, seed=41)
+    p = torch.zeros(2, 2, lq, lk, dtype=torch.float64)
+    p[..., 5] = p[..., lk - 4] = 0.5
+    want, got = attnsteps.attention(c, p, torch.full((1, 1, 1, 1), 8 * attnref.U).double()), _run(c)
+    for name in want:
+        attnsteps.assert_within(got[name], want[name], name)

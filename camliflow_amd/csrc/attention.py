@@ -19,6 +19,7 @@ MAX_BIAS_ROWS = 128
 MAX_BIAS_DISTANCE = 1023
 MAX_BIAS_HEADS = 65535
 MAX_POSITION = 2 ** 26
+MAX_ENTRY = 2.0 ** 125 * math.log(2)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -82,6 +83,12 @@ def _composed_bias(table, q_pos, k_pos, bidirectional, max_distance):
                   - q_pos[..., :, None, a].clamp(-MAX_POSITION, MAX_POSITION).long())
         total = total + table[a].float()[lut[offset.clamp(-max_distance, max_distance) + max_distance]]
     return total.movedim(-1, -3)            # [(B,) H, Lq, Lk]
+
+
+def _within_range(table):
+    """Finite entries beyond +-MAX_ENTRY count as that (sums of two and their distances are finite then); the gradient is the entry's own."""
+    x = table.float()
+    return x + torch.where(torch.isfinite(x), x.clamp(-MAX_ENTRY, MAX_ENTRY) - x, torch.zeros_like(x)).detach()
 
 
 @functools.lru_cache(maxsize=1024)
@@ -301,7 +308,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
     keeps no key gives zeros and takes no part in any gradient.
 
     ``bias_table`` [axes, buckets, H] of q's type with int32 ``q_pos`` [Lq, axes] or [B, Lq, axes] and ``k_pos`` likewise adds the bias
-    that :func:`relative_position_bias` describes, without storing it.  Differentiable in q, k, v and bias_table (once); the same
+    that :func:`relative_position_bias` describes, without storing it.  Entries may be as low as the type goes, or -inf, which takes their
+    pairs out (finite ones beyond +-2.9e37 count as that).  Differentiable in q, k, v and bias_table (once); the same
     bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
     name = 'cross_attention'
     if any(t.dim() != 4 for t in (q, k, v)) or q.dtype not in TYPE_CODES or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -326,7 +334,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
         bias_table, q_pos, k_pos, _, _ = _check_bias(name, bias_table, q_pos, k_pos, bidirectional, max_distance, q.dtype, h, b, lq, lk)
     same_device(name, q, k, v, kv_lengths, key_mask, bias_table)
     if not cpp_impl:
-        bias = _composed_bias(bias_table, q_pos, k_pos, bidirectional, int(max_distance)) if bias_table is not None else None
+        bias = _composed_bias(_within_range(bias_table), q_pos, k_pos, bidirectional, int(max_distance)) if bias_table is not None else None
         return _composed_attention(q, k, v, scale, kv_lengths, key_mask, bias)
     _require_cuda(name, q)
     args = (q, k, v, bias_table, kv_lengths.contiguous() if kv_lengths is not None else None,

@@ -445,6 +445,13 @@ struct Entry8 {
     unsigned hist;
 };
 
+// An entry of the table in the log2 domain.  Finite ones stay finite: the type's lowest number is a common mask, and log2 e times it is not a
+// number, nor is the sum of two axes'.  At 2^125 such a sum and its distance from another one are.
+__device__ __forceinline__ float lut_entry(const RelBias& r, int row, int H, int head) {
+    const float x = load_param(r.table, r.type, (int64_t)row * H + head);
+    return fabsf(x) < INFINITY ? fminf(fmaxf(x * LOG2E, -0x1p125f), 0x1p125f) : x;
+}
+
 // tables of `pack` heads: lut[p][axis][2 limit + 1]
 template <int AXES, int THREADS>
 __device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0, int pack, int H) {
@@ -455,7 +462,7 @@ __device__ __forceinline__ void fill_lut(const RelBias& r, float* lut, int head0
         for (int p = 0; p < pack; ++p)
 #pragma unroll
             for (int a = 0; a < AXES; ++a)
-                lut[(p * AXES + a) * span + i] = load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + head0 + p) * LOG2E;
+                lut[(p * AXES + a) * span + i] = lut_entry(r, a * r.buckets + n, H, head0 + p);
     }
 }
 template <int AXES, int THREADS>
@@ -466,7 +473,7 @@ __device__ __forceinline__ void fill_lut(const RelBias& r, Entry8* lut, int head
         const int n = rel_bucket(r, border, i);
 #pragma unroll
         for (int a = 0; a < AXES; ++a)
-            lut[a * span + i] = {load_param(r.table, r.type, (int64_t)(a * r.buckets + n) * H + head) * LOG2E, (unsigned)((a * r.buckets + n) * row_bytes)};
+            lut[a * span + i] = {lut_entry(r, a * r.buckets + n, H, head), (unsigned)((a * r.buckets + n) * row_bytes)};
     }
 }
 

@@ -763,7 +763,7 @@ int camli_rel_bias_bwd(const void *gout, const int *q_pos, int64_t q_pos_batch_s
  *   A key is kept if its index is below kv_lengths[b] (NULL: all; clamped to 0..Lk) and key_mask[b,j] != 0 (NULL: all).  Masked keys
  *   and values may hold anything, NaN included; their gradients are zero.  A row without a kept key gives
  *   zeros and takes no part in any gradient; so does a row whose scores are all -inf, if its incoming gradient is finite.
- *   bias_axes 0: no bias; else as camli_rel_bias_fwd, table [axes,buckets,H] of `type`, H <= 65535.
+ *   bias_axes 0: no bias; else as camli_rel_bias_fwd, table [axes,buckets,H] of `type`, H <= 65535; finite entries beyond +-2.9e37 count as that.
  *   fp32 factors are multiplied as three bf16 parts each (exact to 2^-25): a kept infinity, or a value beyond 3.38e38, gives NaN.
  *   lse [2,B,H,Lq]: log2 of each row's softmax sum, +inf for rows without keys, and what a float beyond 256 rounds away of it; NULL if no
  *   backward follows.

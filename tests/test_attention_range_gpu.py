@@ -125,3 +125,39 @@ def test_attention_huge_tied_scores_gradients(dtype, lq, lk):
     want, got = attnsteps.attention(c, p, torch.full((1, 1, 1, 1), 8 * attnref.U).double()), _run(c)
     for name in want:
         attnsteps.assert_within(got[name], want[name], name)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('other', ['lowest', -1e9])
+@pytest.mark.parametrize('d,axes', [(32, 1), (64, 2)])
+def test_attention_entries_of_the_lowest_value(dtype, other, d, axes):
+    """the type's lowest number is finite: a row of nothing else weighs its keys like any other (log2 e times it is not)"""
+    low = torch.finfo(dtype).min
+    for shape in (dict(), dict(b=1, lq=8, lk=1500, h=4, hk=2)):
+        c = _level_case(dtype, (low, low if other == 'lowest' else other), d=d, axes=axes, seed=d, **shape)
+        want, got = _level_reference(c, True), _run(c)
+        for name in want:
+            attnsteps.assert_within(got[name], want[name], name)
+        attnsteps.assert_within(_run(c, grad=False)['out'], _level_reference(c, False)['out'], 'out')
+
+
+def _lowest_twice(dtype, lq, lk):
+    """the second axis adds the lowest number to every pair, the first one adds it again to some: -> (case, probabilities)"""
+    c = _level_case(dtype, (torch.finfo(dtype).min,) * 2, b=1, lq=lq, lk=lk, axes=2, seed=43)
+    c['table'][1] = torch.finfo(dtype).min
+    idx = attnref.buckets_of(c['qp'][None], c['kp'][None], 32, True, 64)[0, 0]
+    once = (idx != BEFORE) & (idx != BEHIND)
+    kept = torch.where(once.any(1, keepdim=True), once, torch.ones_like(once)).double()
+    return c, (kept / kept.sum(1, keepdim=True)).expand(1, 2, -1, -1)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('lq,lk', [(40, 300), (8, 1500)])
+def test_attention_entries_of_the_lowest_value_on_both_axes(dtype, lq, lk):
+    """their sum is no number of the type, but lower than one of them"""
+    c, p = _lowest_twice(dtype, lq, lk)
+    for training in (False, True):
+        want = attnsteps.attention(c, p, torch.full((1, 1, 1, 1), (lk + 16) * attnref.U).double(), training)
+        got = _run(c, grad=training)
+        for name in want:
+            attnsteps.assert_within(got[name], want[name], name)

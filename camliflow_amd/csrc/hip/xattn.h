@@ -16,9 +16,12 @@
 //   * the A operand of the second product is the streamed tile transposed, read with the transposing LDS load.
 // Register i of half h holds streamed row 8 (i / 4) + 4 h + i % 4 of its 32-row block.
 //
-// fp16 dS: p (dp - D) of a long row is of the size of |go| / Lk, below fp16's normal numbers for quite ordinary gradients.  go is therefore taken
-// times a power of two that brings its largest element to 1 .. 2 (a row's own in dq, where the contraction is over keys; the kv head's
-// in dkdv, where it is over queries), and P times 2^10 in dkdv; both are undone exactly when the gradients are written.
+// fp16 dS: p (dp - D) is of the size of |go| |v| / Lk, for ordinary operands below fp16's normal numbers, for large values beyond its largest.
+// |dp - D| is at most 2 |go|_1 max|v| (out is a mean of values), so dS is taken times the power of two that brings this bound to 2^14 .. 2^15: it
+// cannot overflow, and what it loses is below 2^-39 of the bound.  max|v| is over the kept keys of a kv head (a launch before the others), |go|_1 a
+// row's own in dq, where the contraction is over keys, and the largest of the kv head in dkdv, where it is over queries.  In dq go itself is
+// an operand: it is taken times a power of two that brings its largest element to 1 .. 2, and p times what is left.  P is taken times 2^10 in
+// dkdv.  All of these are undone exactly when the gradients are written.
 //
 // Two adjoint kernels recompute p instead of one that adds dq with float atomics: 14 D instead of 10 D operations per pair, but
 // every sum has a fixed order (the same bits on every run).  P and dS are rounded to the element type for the second products (their
@@ -41,7 +44,8 @@ struct Args {
     float *out_f32;             // 16-bit types in training: out before its rounding
     float* lse;                 // [2][B][H][Lq], log2 domain, two terms; +inf where no key is kept
     float *delta;               // [B][H][Lq]
-    float *go_max;              // [B][H][Lq] fp16 only: largest |go| of a row
+    float* go_l1;               // [B][H][Lq] fp16 only: sum of |go| of a row
+    float* v_max;               // [B][Hk][v_chunks] fp16 only: largest |v| of a chunk of the kept keys
     int *far_rows;              // [B][H][row_groups]: has any of 32 queries a far lse
     float *part_o, *part_lse;   // splits > 1: [split][B][Lq][H][D] normalised, [2][split][B][H][Lq] (two terms, -inf: no key)
     float *part_dk, *part_dv;   // splits > 1: [split][B][Lk][Hk][D]
@@ -52,7 +56,7 @@ struct Args {
     int B, H, Hk, Lq, Lk, D;
     bool few;                   // fwd_few_kernel
     int pack;                   // query heads of one kv head that share a workgroup's rows (few queries), else 1
-    int row_tiles, splits, tiles_per_split, parts, row_groups;
+    int row_tiles, splits, tiles_per_split, parts, row_groups, v_chunks;
     float scale, scale_log2;
     RelBias rb;
 };
@@ -1030,6 +1034,51 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a, int lanes) {
     if (a.out_f32) store_f32<float, 4>(a.out_f32 + at * a.D + c, acc);
 }
 
+// power of two that brings x to 2^14 .. 2^15 (1 for zero, infinity and NaN)
+__device__ __forceinline__ float bound_scale(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
+    return x > 0.0f && e < 128 ? __uint_as_float((unsigned)(min(127 + 14 - e, 254)) << 23) : 1.0f;
+}
+
+// largest |v| of a kv head's kept keys, for whole waves
+__device__ __forceinline__ float values_max(const Args& a, int b, int kvh) {
+    const int lane = threadIdx.x & 63;
+    float x = lane < a.v_chunks ? a.v_max[((int64_t)b * a.Hk + kvh) * a.v_chunks + lane] : 0.0f;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+    return x;
+}
+
+// v_max: a workgroup per chunk of a kv head's keys, of 128 or a 64th of them.  (3 x 1237 keys of 2 heads of 40: 4.7 us, a launch.)
+constexpr int MAX_V_CHUNKS = 64;
+inline int v_chunks(const Args& a) {
+    const int n = (a.Lk + 127) / 128;
+    return n < MAX_V_CHUNKS ? n : MAX_V_CHUNKS;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void values_max_kernel(Args a) {
+    const int chunk = blockIdx.x % a.v_chunks, unit = blockIdx.x / a.v_chunks, kvh = unit % a.Hk, b = unit / a.Hk, len = kept_length(a, b);
+    const int per = (a.Lk + a.v_chunks - 1) / a.v_chunks, row0 = chunk * per, rows = min(len - row0, per), vecs = a.D / 8;
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
+    float x = 0.0f;
+    const int step = 256 / vecs, c = (int)threadIdx.x % vecs * 8;       // threads beyond step * vecs have no part
+#pragma unroll 4
+    for (int r = (int)threadIdx.x / vecs; r < rows; r += step) {
+        float v[8];
+        load8(vp + (row0 + r) * a.vs.l + c, v);
+        const bool kept = (int)threadIdx.x < step * vecs && (mask == nullptr || mask[row0 + r] != 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x = kept ? fmaxf(x, fabsf(v[e])) : x;
+    }
+    __shared__ float most[4];
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) a.v_max[blockIdx.x] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+}
+
 // power of two that brings x to 1 .. 2 (1 for zero, infinity and NaN)
 __device__ __forceinline__ float unit_scale(float x) {
     const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
@@ -1088,13 +1137,12 @@ __device__ __forceinline__ void dq_body(const Args& a, int block, int blocks) {
     const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + kvh * a.vs.h;
     const unsigned char* mask = a.mask ? a.mask + b * a.mask_bs : nullptr;
     const int64_t at = ((int64_t)b * a.Lq + q0) * a.H + head, stat = ((int64_t)b * a.H + head) * a.Lq + q0;
-    const float lse_lo = FAR_ROWS ? a.lse[(int64_t)a.B * a.H * a.Lq + stat] : 0.0f;
 
     Frag<T> qf[TL::KSTEPS], gf[TL::KSTEPS];
     load_owned<T, DP>(qf, static_cast<const T*>(a.q) + b * a.qs.b + q0 * a.qs.l + head * a.qs.h, exists, a.D, h);
     const float sign = dp_sign<T>(lane);
     load_owned<T, DP>(gf, static_cast<const T*>(a.go) + at * a.D, exists, a.D, h, sign);
-    float delta = 0.0f, most = 0.0f;
+    float delta = 0.0f, most = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < TL::KSTEPS; ++ks) {
         const int c = (2 * ks + h) * TL::E;
@@ -1105,17 +1153,22 @@ __device__ __forceinline__ void dq_body(const Args& a, int block, int blocks) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(o[e], g[e], delta);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(g[e]));
+            for (int e = 0; e < 8; ++e) {
+                most = fmaxf(most, fabsf(g[e]));
+                l1 += fabsf(g[e]);
+            }
         }
     }
     delta = half_sum(delta);
     if (!FAR_ROWS && exists && split == 0 && h == 0) a.delta[stat] = delta;
-    float unscale = 1.0f;
+    float unscale = 1.0f, p_log2 = 0.0f;       // p is taken times 2^p_log2
     if constexpr (__is_same(T, _Float16)) {
         most = half_max(most);
-        if (!FAR_ROWS && exists && split == 0 && h == 0) a.go_max[stat] = most;
-        const float f = unit_scale(most);
-        unscale = unit_scale(f);
+        l1 = half_sum(l1);
+        if (!FAR_ROWS && exists && split == 0 && h == 0) a.go_l1[stat] = l1;
+        const float f = unit_scale(most), fp = bound_scale(2.0f * l1 * f * values_max(a, b, kvh));
+        unscale = unit_scale(f) * unit_scale(fp);
+        p_log2 = (float)(((int)__float_as_uint(fp) >> 23) - 127);
         delta *= f;
 #pragma unroll
         for (int s = 0; s < TL::KSTEPS; ++s)
@@ -1126,11 +1179,12 @@ __device__ __forceinline__ void dq_body(const Args& a, int block, int blocks) {
     // or none at all) makes every p zero.
     constexpr bool FOLD = fold_start<T>(), FOLD_S = FOLD && !FAR_ROWS;
     const float lse = exists ? a.lse[stat] : INFINITY;
+    const float lse_lo = (FAR_ROWS ? a.lse[(int64_t)a.B * a.H * a.Lq + stat] : 0.0f) - p_log2;
     if constexpr (!FAR_ROWS) {
         const bool far = __any(is_far(lse));
         if (split == 0 && lane == 0) a.far_rows[((int64_t)b * a.H + head) * a.row_groups + rt * WAVES + wave] = far;
     }
-    const acc16 start_s = FOLD_S ? splat(-lse / a.scale_log2) : acc16{0}, start_d = FOLD ? splat(-delta) : acc16{0};
+    const acc16 start_s = FOLD_S ? splat((p_log2 - lse) / a.scale_log2) : acc16{0}, start_d = FOLD ? splat(-delta) : acc16{0};
     const LaneMap<TL, T> map(lane);
     int qa[AXES ? AXES : 1], lo[AXES ? AXES : 1], hi[AXES ? AXES : 1];
     const int* kpos = nullptr;
@@ -1316,14 +1370,14 @@ __device__ __forceinline__ void dkdv_body(const Args& a, int block, int blocks) 
     if constexpr (HALF) {
         __shared__ float most[THREADS / 64];
         float x = 0.0f;
-        const float* rows = a.go_max + ((int64_t)b * a.H + kvh * group) * a.Lq;
+        const float* rows = a.go_l1 + ((int64_t)b * a.H + kvh * group) * a.Lq;
         const int64_t n = (int64_t)group * a.Lq;
         for (int64_t i = tid; i < n; i += THREADS) x = fmaxf(x, rows[i]);
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
         if (lane == 0) most[wave] = x;
         __syncthreads();
-        const float f = unit_scale(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+        const float f = bound_scale(2.0f * fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * values_max(a, b, kvh));
         ds_scale = f * P_UNSCALE;
         ds_unscale = unit_scale(f);
     }
@@ -1595,6 +1649,7 @@ struct Launch {
     static int fwd(const Args& a, int axes, hipStream_t s);
     static int dq(const Args& a, int axes, int waves, hipStream_t s);
     static int dkdv(const Args& a, int axes, hipStream_t s);
+    static int values(const Args& a, hipStream_t s);        // fp16 only
     static int far(const Args& dq, const Args& dkdv, int axes, int waves, hipStream_t s);
     static int sum(const SumJobs& jobs, int n, hipStream_t s);
 };
@@ -1612,6 +1667,11 @@ struct Launch {
     template <> int Launch<TYPE>::far(const Args& a, const Args& dkdv, int axes, int waves, hipStream_t s) {       \
         using T = TYPE;                                                                                            \
         XATTN_SELECT(run_far, a, dkdv, waves, s)                                                                   \
+    }
+#define XATTN_DEFINE_VALUES(TYPE)                                                                                  \
+    template <> int Launch<TYPE>::values(const Args& a, hipStream_t s) {                                           \
+        values_max_kernel<TYPE><<<dim3((unsigned)a.B * a.Hk * a.v_chunks), 256, 0, s>>>(a);                        \
+        return camli_check_launch("camli_cross_attention_bwd");                                                    \
     }
 #define XATTN_DEFINE_SUM(TYPE)                                                                                     \
     template <> int Launch<TYPE>::sum(const SumJobs& jobs, int n, hipStream_t s) {                                 \

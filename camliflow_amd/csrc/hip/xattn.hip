@@ -127,8 +127,11 @@ BwdPlan plan_bwd(const Args& a, const camli_attention* d, bool table, char* base
     p.dq.far_rows = p.dkdv.far_rows = reinterpret_cast<int*>(base + end);
     end += align256((int64_t)4 * a.B * a.H * p.dq.row_groups);
     if (d->type == CAMLI_F16) {
-        p.dq.go_max = p.dkdv.go_max = reinterpret_cast<float*>(base + end);
+        p.dq.go_l1 = p.dkdv.go_l1 = reinterpret_cast<float*>(base + end);
         end += align256(4 * rows);
+        p.dq.v_chunks = p.dkdv.v_chunks = xattn::v_chunks(a);
+        p.dq.v_max = p.dkdv.v_max = reinterpret_cast<float*>(base + end);
+        end += align256((int64_t)4 * a.B * a.Hk * p.dq.v_chunks);
     }
     if (p.dq.splits > 1) {
         p.dq.part_o = reinterpret_cast<float*>(base + end);
@@ -201,6 +204,10 @@ extern "C" int camli_cross_attention_bwd(const camli_attention* d, const float* 
     p.dq.dq = gq;
     p.dkdv.dk = gk;
     p.dkdv.dv = gv;
+    if (d->type == CAMLI_F16) {
+        const int rc = xattn::Launch<_Float16>::values(p.dq, s);
+        if (rc != CAMLI_OK) return rc;
+    }
     int rc = d->type == CAMLI_F32 ? xattn::Launch<float>::dq(p.dq, axes, waves, s)
              : d->type == CAMLI_BF16 ? xattn::Launch<__bf16>::dq(p.dq, axes, waves, s) : xattn::Launch<_Float16>::dq(p.dq, axes, waves, s);
     if (rc != CAMLI_OK) return rc;

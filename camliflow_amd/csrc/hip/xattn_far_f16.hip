@@ -3,4 +3,5 @@
 
 namespace xattn {
 XATTN_DEFINE_FAR(_Float16)
+XATTN_DEFINE_VALUES(_Float16)
 }

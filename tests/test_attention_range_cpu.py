@@ -5,7 +5,7 @@ import torch
 import attnref
 import attnsteps
 from camliflow_amd import csrc
-from test_attention_range_gpu import _lowest_twice
+from test_attention_range_gpu import _lowest_twice, _sized_case, _sized_reference
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
@@ -17,3 +17,39 @@ def test_composed_attention_with_entries_of_the_lowest_value_on_both_axes(dtype)
     want = attnsteps.attention({n: t.detach() if isinstance(t, torch.Tensor) else t for n, t in c.items()}, p, torch.full((1, 1, 1, 1), 70 * attnref.U).double())
     for name in want:
         attnsteps.assert_within(got[name], want[name], name)
+
+
+def _rounded_steps(c, round_ds=True, p_terms=2, keep_out=True):
+    """the adjoints of c in 64 bits but for roundings to its type: of dS without any scaling, of P to one or two terms, of out before D"""
+    dtype = c['q'].dtype
+    r = lambda t: t.to(dtype).double()          # noqa: E731
+    Q, K, V, g = attnsteps._heads(c)
+    idx, bias = None, torch.zeros(1, 1, 1, 1, dtype=torch.float64)
+    if c['table'] is not None:
+        idx = attnref.buckets_of(c['qp'][None], c['kp'][None], c['buckets'], True, c['max_distance'])
+        bias = sum(c['table'][a].double()[idx[a]] for a in range(idx.shape[0])).permute(0, 3, 1, 2)
+    p, _ = attnsteps.softmax(c, bias)
+    first = r(p)
+    o = (first if p_terms == 1 else first + r(p - first)) @ V
+    G = c['go'].double().permute(0, 2, 1, 3)
+    ds = p * (G @ V.transpose(2, 3) - (G * (o if keep_out else r(o))).sum(-1, keepdim=True))
+    dsr, scale = r(ds) if round_ds else ds, Q.shape[-1] ** -0.5
+    b, h, lq, d = Q.shape
+    out = {'dq': (scale * dsr @ K).permute(0, 2, 1, 3), 'dk': (scale * dsr.transpose(2, 3) @ Q).reshape(b, h // g, g, -1, d).sum(2).permute(0, 2, 1, 3)}
+    if idx is not None:
+        out['dtable'] = torch.stack([torch.stack([torch.bincount(idx[a].expand(b, -1, -1).reshape(-1), weights=ds[:, i].reshape(-1), minlength=c['buckets'])
+                                                  for i in range(h)], -1) for a in range(idx.shape[0])])
+    return {n: t.to(dtype) for n, t in out.items()}
+
+
+
+def test_bounds_reject_half_gradients_without_a_scale():
+    """dS rounded to fp16 as it is: subnormal for small gradients, infinite for large values; and no gradient at all"""
+    for v, go, lq, lk, d, seed in ((1.0, 2.0 ** -16, 16, 3000, 32, 1), (2e4, 1.0, 16, 16, 128, 2), (2.0 ** -12, 2.0 ** -6, 16, 2000, 32, 3)):
+        for qk, name in ((2.0 ** -5, 'dq'), (2.0 ** 5, 'dk')):
+            c = _sized_case(torch.float16, lq, lk, d, v, go, qk, seed=seed)
+            want = _sized_reference(c)
+            attnsteps.assert_within(_rounded_steps(c, round_ds=False)[name], want[name], name)
+            for bad in (_rounded_steps(c)[name], torch.zeros_like(c[name[1]])):
+                with pytest.raises(AssertionError):
+                    attnsteps.assert_within(bad, want[name], name)

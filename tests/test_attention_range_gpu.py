@@ -161,3 +161,43 @@ def test_attention_entries_of_the_lowest_value_on_both_axes(dtype, lq, lk):
         got = _run(c, grad=training)
         for name in want:
             attnsteps.assert_within(got[name], want[name], name)
+
+
+def _sized_case(dtype, lq, lk, d, v, go, qk=1.0, axes=0, h=2, hk=1, seed=0, **kw):
+    """values and incoming gradients of given sizes; q times qk and k / qk (powers of two: the same scores)"""
+    c = _case(1, lq, lk, h, hk, d, dtype, axes=axes, seed=seed, **kw)
+    return dict(c, q=c['q'] * qk, k=c['k'] / qk, v=(c['v'].float() * v).clamp(-6e4, 6e4).to(dtype), go=c['go'] * go)
+
+
+def _sized_reference(c):
+    idx, bias = None, torch.zeros(1, 1, 1, 1, dtype=torch.float64)
+    if c['table'] is not None:
+        idx = attnref.buckets_of(c['qp'][None], c['kp'][None], c['buckets'], True, c['max_distance'])
+        bias = sum(c['table'][a].double()[idx[a]] for a in range(idx.shape[0])).permute(0, 3, 1, 2)
+    return attnsteps.attention(c, *attnsteps.softmax(c, bias), idx=idx, buckets=c['buckets'])
+
+
+SIZES = [(3e4, 2.0 ** -10), (3e4, 1.0), (1e3, 1.0), (1.0, 2.0 ** -12), (1.0, 2.0 ** -16), (1e-3, 1.0), (2.0 ** -12, 2.0 ** -6), (1e-3, 256.0)]
+
+
+@pytest.mark.parametrize('v,go', SIZES)
+@pytest.mark.parametrize('qk', [2.0 ** -5, 2.0 ** 5], ids=['k', 'q'])
+@pytest.mark.parametrize('lq,lk,d,axes', [(40, 16, 128, 0), (64, 5000, 32, 1), (70, 333, 64, 2)])
+def test_attention_half_gradients_of_any_size(v, go, qk, lq, lk, d, axes):
+    """fp16 has 30 powers of two: neither large values nor long rows of small ones may take dS out of them, while dq (large keys) or dk (large
+    queries) is well inside"""
+    c = _sized_case(torch.float16, lq, lk, d, v, go, qk, axes=axes, seed=lk)
+    want, got = _sized_reference(c), _run(c)
+    for name in want:
+        attnsteps.assert_within(got[name], want[name], name)
+
+
+def test_attention_half_gradients_of_masked_large_values():
+    """what is masked does not count as large"""
+    c = _sized_case(torch.float16, 60, 900, 32, 1e-3, 2.0 ** -6, 32.0, axes=1, lengths=[700], masked=0.2, seed=3)
+    want = _run(c)
+    c['v'] = torch.where(c['keep'][:, :, None, None], c['v'], torch.full_like(c['v'], 6e4))
+    for name, t in _run(c).items():
+        assert torch.equal(t, want[name]), name
+    for name, pair in _sized_reference(c).items():
+        attnsteps.assert_within(want[name], pair, name)

@@ -5,7 +5,7 @@ import torch
 import attnref
 import attnsteps
 from camliflow_amd import csrc
-from test_attention_range_gpu import _lowest_twice, _sized_case, _sized_reference
+from test_attention_range_gpu import _common_value_case, _lowest_twice, _sized_case, _sized_reference
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
@@ -53,3 +53,14 @@ def test_bounds_reject_half_gradients_without_a_scale():
             for bad in (_rounded_steps(c)[name], torch.zeros_like(c[name[1]])):
                 with pytest.raises(AssertionError):
                     attnsteps.assert_within(bad, want[name], name)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=['bf16', 'f16'])
+def test_bounds_reject_a_table_gradient_from_a_rounded_out(dtype):
+    """D from out as it is returned, or from P of one term: what the second term and the fp32 copy of out are for"""
+    c = _common_value_case(dtype)
+    want = _sized_reference(c)
+    attnsteps.assert_within(_rounded_steps(c)['dtable'], want['dtable'], 'dtable')
+    for bad in (_rounded_steps(c, keep_out=False), _rounded_steps(c, p_terms=1)):
+        with pytest.raises(AssertionError):
+            attnsteps.assert_within(bad['dtable'], want['dtable'], 'dtable')

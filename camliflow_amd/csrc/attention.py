@@ -11,7 +11,7 @@ import math
 import torch
 
 from . import _lib
-from .norm import TYPE_CODES, address, first_order, same_device
+from .norm import TYPE_CODES, address, first_order, needs_node, same_device
 from .wrapper import _on_device, _require_cuda, _stream_ptr
 
 MAX_HEAD_DIM = 128
@@ -146,7 +146,7 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
     numbers (the running index of a sequence, pixel coordinates); beyond -2^26 .. 2^26 they count as that bound.  ``bidirectional``: half the buckets for each sign, the upper half
     for keys after the query; otherwise all buckets for keys before the query, and keys after it share bucket 0.  Of the s buckets of a
     side, e = s // 2 hold one distance each; bucket e + j begins at the first distance >= e (max_distance / e)^(j / (s - e)), and the last
-    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023; at most 65535 samples x heads, 2000000 queries, 16000000 keys.  Differentiable in the table (once);
+    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023; at most 65535 samples x heads, 2000000 queries, 16000000 keys.  Differentiable in the table (once, in reverse mode);
     the same bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
     name = 'relative_position_bias'
     table, q_pos, k_pos, batch, _ = _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, table.dtype if table is not None else None)
@@ -155,7 +155,7 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
     if not cpp_impl:
         return _composed_bias(table, q_pos, k_pos, bidirectional, int(max_distance)).to(table.dtype)
     _require_cuda(name, table)
-    run = _RelativeBias.apply if table.requires_grad and torch.is_grad_enabled() else _run_bias
+    run = _RelativeBias.apply if needs_node(table) else _run_bias
     return run(table, q_pos, k_pos, batch, bool(bidirectional), int(max_distance))
 
 
@@ -309,7 +309,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
 
     ``bias_table`` [axes, buckets, H] of q's type with int32 ``q_pos`` [Lq, axes] or [B, Lq, axes] and ``k_pos`` likewise adds the bias
     that :func:`relative_position_bias` describes, without storing it.  Entries may be as low as the type goes, or -inf, which takes their
-    pairs out (finite ones beyond +-2.9e37 count as that).  Differentiable in q, k, v and bias_table (once); the same
+    pairs out (finite ones beyond +-2.9e37 count as that).  Differentiable in q, k, v and bias_table (once, in reverse mode); the same
     bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
     name = 'cross_attention'
     if any(t.dim() != 4 for t in (q, k, v)) or q.dtype not in TYPE_CODES or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -339,6 +339,6 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
     _require_cuda(name, q)
     args = (q, k, v, bias_table, kv_lengths.contiguous() if kv_lengths is not None else None,
             key_mask.contiguous() if key_mask is not None else None, q_pos, k_pos, scale, bool(bidirectional), int(max_distance))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)):
+    if needs_node(q, k, v, bias_table):
         return _CrossAttention.apply(*args)
     return _run_attention(*args, False)[0]

@@ -7,6 +7,7 @@ the ``nn.Linear`` layers of the attention modules produce.
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -31,6 +32,17 @@ def first_order(backward):
     def wrapper(ctx, *grads):
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
     return staticmethod(wrapper)
+
+
+def needs_node(*tensors):
+    """Does a call have to go through its autograd node: a gradient is wanted, or an input carries a forward-mode tangent (which the node
+    refuses; the kernels alone would drop it)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # no level, no tangents: unpacking each tensor to find that out takes a quarter of a small call's host time
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def address(t):
@@ -165,7 +177,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
     The kernels work on channels-last memory: x may be a channels-last map, rows [B, N, C] seen as x.transpose(1, 2), or a channel slice
     of a wider one; anything else is copied to that layout first.  The result is [B, C, *spatial] on dense channels-last memory, of
     x's type.  ``weight`` and ``bias`` [C] (either may be None) are fp32 or of x's type.  Differentiable in x, weight and bias
-    (once); no float atomics, the same bits on every run.  ``cpp_impl=False``: the same formula from torch primitives, on any device."""
+    (once, in reverse mode); no float atomics, the same bits on every run.  ``cpp_impl=False``: the same formula from torch primitives, on any device."""
     name = 'group_norm_act'
     shape = x.shape
     if len(shape) < 2 or x.dtype not in TYPE_CODES:
@@ -192,6 +204,6 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if needs_node(x, weight, bias):
         return _GroupNormAct.apply(x, weight, bias, num_groups, eps, NORM_ACTS[act])
     return _run_forward(x, weight, bias, num_groups, eps, NORM_ACTS[act], False)[0]

@@ -64,3 +64,14 @@ def test_bounds_reject_a_table_gradient_from_a_rounded_out(dtype):
     for bad in (_rounded_steps(c, keep_out=False), _rounded_steps(c, p_terms=1)):
         with pytest.raises(AssertionError):
             attnsteps.assert_within(bad['dtable'], want['dtable'], 'dtable')
+
+
+def test_a_tangent_goes_through_the_autograd_node():
+    from torch.autograd import forward_ad
+    from camliflow_amd.csrc.norm import needs_node
+    x, leaf = torch.ones(3), torch.ones(3, requires_grad=True)
+    assert not needs_node(x, None) and needs_node(None, leaf)
+    with torch.no_grad():
+        assert not needs_node(leaf)
+        with forward_ad.dual_level():
+            assert not needs_node(x, leaf, None) and needs_node(None, x, forward_ad.make_dual(x, torch.ones(3)))

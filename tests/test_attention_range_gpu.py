@@ -218,3 +218,27 @@ def test_attention_table_gradient_of_a_common_value(dtype):
         want, got = _sized_reference(c), _run(c)
         for name in want:
             attnsteps.assert_within(got[name], want[name], name)
+
+
+# ------------------------------------------------------------------------------------------------ forward mode
+@pytest.mark.parametrize('which', ['q', 'v', 'table', 'bias table', 'x', 'weight', 'shift'])
+def test_forward_mode_is_refused(which):
+    """a tangent is not dropped: the kernels have no forward-mode derivative"""
+    from torch.autograd import forward_ad
+    from camliflow_amd import csrc
+    c = _case(1, 5, 9, 2, 2, 32, torch.float32, axes=1, seed=1)
+    c['x'], c['weight'], c['shift'], c['bias table'] = torch.randn(2, 8, 3, 4), torch.ones(8), torch.zeros(8), c['table']
+    t = {n: c[n].cuda() for n in ('q', 'k', 'v', 'table', 'qp', 'kp', 'x', 'weight', 'shift', 'bias table')}
+
+    def call():
+        if which in ('q', 'v', 'table'):
+            return csrc.cross_attention(t['q'], t['k'], t['v'], bias_table=t['table'], q_pos=t['qp'], k_pos=t['kp'])
+        if which == 'bias table':
+            return csrc.relative_position_bias(t['bias table'], t['qp'], t['kp'])
+        return csrc.group_norm_act(t['x'], 2, t['weight'], t['shift'], act='silu')
+    want = call()
+    with forward_ad.dual_level(), torch.no_grad():
+        assert torch.equal(call(), want)                # without a tangent nothing changes
+        t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(NotImplementedError):
+            call()

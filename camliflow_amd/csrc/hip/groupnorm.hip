@@ -432,6 +432,9 @@ int gn_chunk_px(int B, int C, int P, int type) {
     return (int)(px < P ? px : P);
 }
 
+// in 64 bits: a chunk is a 256th of the map at least, and P + that passes 2^31 from 2^31 - 2^23 positions on
+int gn_chunks(int P, int chunk_px) { return (int)(((int64_t)P + chunk_px - 1) / chunk_px); }
+
 bool gn_args_ok(int B, int C, int G, int P, int type, int wtype, int act, const char* who) {
     if (B < 1 || B > 65535 || P < 1 || C < 1 || C > MAX_C || G < 1 || C % G != 0 || type < 0 || type > 2 || wtype < 0 || wtype > 2 ||
         !(act == 0 || act == 1 || act == 2 || act == 3 || act == 6)) {
@@ -450,7 +453,7 @@ GnArgs make_args(const void* x, int64_t x_bs, int64_t x_ld, const void* weight, 
     a.x = x; a.x_bs = x_bs; a.x_ld = x_ld; a.weight = weight; a.bias = bias; a.wtype = wtype;
     a.C = C; a.G = G; a.P = P; a.act = act; a.eps = eps;
     a.chunk_px = gn_chunk_px(B, C, P, type);
-    a.chunks = camli_divup(P, a.chunk_px);
+    a.chunks = gn_chunks(P, a.chunk_px);
     // half of the 256 MB last-level cache.  At 16 x 64 x 272 x 480 bf16 (267 MB) keeping nothing of the result leaves what the first
     // reading brought for the second: 196 -> 161 us forward, 305 -> 285 us backward; a smaller map is left for its next reader.
     a.stream = (int64_t)B * P * C * camli_type_size(type) >= ((int64_t)128 << 20);
@@ -489,12 +492,12 @@ bool vector_ok(const GnArgs& a, int type, const void* p0, const void* p1) {
 
 extern "C" int64_t camli_group_norm_fwd_workspace_bytes(int B, int C, int G, int P, int type) {
     if (!gn_args_ok(B, C, G, P, type, 0, 0, "camli_group_norm_fwd_workspace_bytes")) return 0;
-    return (int64_t)sizeof(float2) * B * camli_divup(P, gn_chunk_px(B, C, P, type)) * G;
+    return (int64_t)sizeof(float2) * B * gn_chunks(P, gn_chunk_px(B, C, P, type)) * G;
 }
 
 extern "C" int64_t camli_group_norm_bwd_workspace_bytes(int B, int C, int G, int P, int type) {
     if (!gn_args_ok(B, C, G, P, type, 0, 0, "camli_group_norm_bwd_workspace_bytes")) return 0;
-    return (int64_t)sizeof(float2) * B * ((int64_t)camli_divup(P, gn_chunk_px(B, C, P, type)) * C + C + G);
+    return (int64_t)sizeof(float2) * B * ((int64_t)gn_chunks(P, gn_chunk_px(B, C, P, type)) * C + C + G);
 }
 
 extern "C" int camli_group_norm_fwd(const void* x, int64_t x_batch_stride, int64_t x_pixel_stride, const void* weight, const void* bias,

@@ -5,6 +5,7 @@ import torch
 import attnref
 import attnsteps
 from camliflow_amd import csrc
+from camliflow_amd.csrc import _lib
 from test_attention_range_gpu import _common_value_case, _lowest_twice, _sized_case, _sized_reference
 
 
@@ -75,3 +76,14 @@ def test_a_tangent_goes_through_the_autograd_node():
         assert not needs_node(leaf)
         with forward_ad.dual_level():
             assert not needs_node(x, leaf, None) and needs_node(None, x, forward_ad.make_dual(x, torch.ones(3)))
+
+
+@pytest.mark.parametrize('positions', [1, 4096, 4097, 2 ** 31 - 2 ** 23 - 1, 2 ** 31 - 2 ** 23 + 1, 2 ** 31 - 2 ** 16 - 1, 2 ** 31 - 1])
+@pytest.mark.parametrize('b,c,groups,code', [(1, 1, 1, 2), (1, 1, 1, 0), (3, 8, 2, 1), (65535, 4, 4, 0)])
+def test_group_norm_workspace_sizes(positions, b, c, groups, code):
+    """one pair of floats a chunk and group (forward), and channel (backward): from 1 to 256 chunks a sample, never a negative number"""
+    lib = _lib.load()
+    size = lib.camli_group_norm_fwd_workspace_bytes(b, c, groups, positions, code)
+    chunks, rest = divmod(size, 8 * b * groups)
+    assert rest == 0 and 1 <= chunks <= min(256, positions)
+    assert lib.camli_group_norm_bwd_workspace_bytes(b, c, groups, positions, code) == 8 * b * (chunks * c + c + groups)

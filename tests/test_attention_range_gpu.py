@@ -242,3 +242,19 @@ def test_forward_mode_is_refused(which):
         t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
         with pytest.raises(NotImplementedError):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ group norm
+def test_norm_of_nearly_two_to_the_31_positions():
+    """the largest map that is taken, forward and backward: its last positions as the first ones"""
+    from camliflow_amd import csrc
+    n = 2 ** 31 - 2 ** 16 - 1
+    x = torch.empty(1, 1, n, dtype=torch.bfloat16, device='cuda')
+    x.view(-1)[:] = 1.0
+    x.view(-1)[::2] = 3.0           # exact: mean 2 and variance 1 but for 2^-31
+    leaf = x.requires_grad_(True)
+    y = csrc.group_norm_act(leaf, 1, eps=0.0)
+    gx, = torch.autograd.grad(y, leaf, y.detach())          # of a group's own values: zero
+    for part in (slice(0, 1000), slice(n // 2, n // 2 + 1000), slice(n - 1000, n)):
+        assert torch.equal(y[0, 0, part], x.detach()[0, 0, part] - 2)
+        assert gx[0, 0, part].abs().max() <= 2.0 ** -7      # a mean and a sum of 2^31 terms in fp32, rounded to bf16 once

@@ -282,16 +282,17 @@ def _composed_attention(q, k, v, scale, kv_lengths, key_mask, bias):
         keep &= key_mask
     rows = keep[:, None, :, None]
     kh, vh = torch.where(rows, kh, torch.zeros_like(kh)), torch.where(rows, vh, torch.zeros_like(vh))
-    scores = torch.matmul(qh, kh.transpose(2, 3).contiguous()) * scale
-    if bias is not None:
-        scores = scores + bias
-    scores = torch.where(keep[:, None, None, :], scores, torch.full_like(scores, -math.inf))
-    if lk == 0:
-        return torch.zeros_like(q)
-    top = scores.amax(dim=-1, keepdim=True).detach()
-    weights = torch.exp(scores - torch.where(top == -math.inf, torch.zeros_like(top), top))
-    total = weights.sum(dim=-1, keepdim=True)
-    return torch.matmul(weights / torch.where(total == 0, torch.ones_like(total), total), vh).permute(0, 2, 1, 3).to(q.dtype)
+    with torch.autocast(q.device.type, enabled=False):      # 32 bits, like the kernels' sums: autocast would take the products in 16
+        scores = torch.matmul(qh, kh.transpose(2, 3).contiguous()) * scale
+        if bias is not None:
+            scores = scores + bias
+        scores = torch.where(keep[:, None, None, :], scores, torch.full_like(scores, -math.inf))
+        if lk == 0:
+            return torch.zeros_like(q)
+        top = scores.amax(dim=-1, keepdim=True).detach()
+        weights = torch.exp(scores - torch.where(top == -math.inf, torch.zeros_like(top), top))
+        total = weights.sum(dim=-1, keepdim=True)
+        return torch.matmul(weights / torch.where(total == 0, torch.ones_like(total), total), vh).permute(0, 2, 1, 3).to(q.dtype)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=None, kv_lengths=None, key_mask=None, bias_table=None,

@@ -67,6 +67,20 @@ def test_bounds_reject_a_table_gradient_from_a_rounded_out(dtype):
             attnsteps.assert_within(bad['dtable'], want['dtable'], 'dtable')
 
 
+def test_composed_attention_is_fp32_under_autocast():
+    """as the kernels, whose inputs decide the type; the backward's products too"""
+    g = torch.Generator().manual_seed(0)
+    leaves = [torch.randn(2, n, 2, 16, generator=g).requires_grad_(True) for n in (5, 7, 7)]
+    go = torch.randn(2, 5, 2, 16, generator=g)
+    results = []
+    for enabled in (False, True):
+        with torch.autocast('cpu', torch.bfloat16, enabled=enabled):
+            out = csrc.cross_attention(*leaves, cpp_impl=False)
+        results.append((out,) + torch.autograd.grad(out, leaves, go))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_a_tangent_goes_through_the_autograd_node():
     from torch.autograd import forward_ad
     from camliflow_amd.csrc.norm import needs_node

@@ -287,8 +287,8 @@ def _composed_attention(q, k, v, scale, kv_lengths, key_mask, bias):
         if bias is not None:
             scores = scores + bias
         scores = torch.where(keep[:, None, None, :], scores, torch.full_like(scores, -math.inf))
-        if lk == 0:
-            return torch.zeros_like(q)
+        if lk == 0:         # zeros, in the graph of q, k and v
+            return torch.matmul(scores, vh).permute(0, 2, 1, 3).to(q.dtype)
         top = scores.amax(dim=-1, keepdim=True).detach()
         weights = torch.exp(scores - torch.where(top == -math.inf, torch.zeros_like(top), top))
         total = weights.sum(dim=-1, keepdim=True)

@@ -5,6 +5,7 @@ the statistics and one for normalisation, scale, shift and activation together, 
 the ``nn.Linear`` layers of the attention modules produce.
 """
 import functools
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -151,7 +152,7 @@ class _GroupNormAct(torch.autograd.Function):
 
 def _composed(x, groups, weight, bias, eps, act):
     shape = x.shape
-    grouped = x.float().reshape(shape[0], groups, -1)
+    grouped = x.float().reshape(shape[0], groups, shape[1] // groups * math.prod(shape[2:]))
     centred = grouped - grouped.mean(dim=2, keepdim=True)
     z = (centred * torch.rsqrt((centred * centred).mean(dim=2, keepdim=True) + eps)).reshape(shape)
     per_channel = (1, -1) + (1,) * (x.dim() - 2)

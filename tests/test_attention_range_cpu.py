@@ -81,6 +81,23 @@ def test_composed_attention_is_fp32_under_autocast():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('b,lq,lk', [(0, 3, 4), (2, 0, 4), (2, 3, 0)])
+def test_composed_attention_of_nothing(b, lq, lk):
+    q, k, v = (torch.randn(b, n, 2, 32, requires_grad=True) for n in (lq, lk, lk))
+    out = csrc.cross_attention(q, k, v, cpp_impl=False)
+    assert out.shape == q.shape and not out.any()
+    for t, grad in zip((q, k, v), torch.autograd.grad(out.sum(), (q, k, v))):
+        assert grad.shape == t.shape and not grad.any()
+
+
+@pytest.mark.parametrize('shape', [(0, 8, 3, 4), (2, 8, 0, 4), (0, 8)])
+def test_composed_group_norm_of_nothing(shape):
+    x, w = torch.randn(shape, requires_grad=True), torch.ones(8, requires_grad=True)
+    y = csrc.group_norm_act(x, 2, w, None, act='silu', cpp_impl=False)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    assert y.shape == x.shape and gx.shape == x.shape and not gw.any()
+
+
 def test_a_tangent_goes_through_the_autograd_node():
     from torch.autograd import forward_ad
     from camliflow_amd.csrc.norm import needs_node

@@ -53,14 +53,15 @@ class CamLiPWC_Core(nn.Module):
                                                         conv_last=not cfgs.fuse_estimator, k=k)
 
         # fusion
+        fusion_fn = getattr(cfgs, 'fusion_fn', 'sk')        # 'attn': cross attention between pixels and points (fusion.CrossAttend)
         if cfgs.fuse_pyramid:
-            self.pyramid_clfms = _per_level(lambda c: CLFM(c, c, norm=cfgs2d.norm.feature_pyramid))
+            self.pyramid_clfms = _per_level(lambda c: CLFM(c, c, fusion_fn, norm=cfgs2d.norm.feature_pyramid))
         if cfgs.fuse_correlation:
-            self.corr_clfms = _per_level(lambda c: CLFM(corr_2d, c))
+            self.corr_clfms = _per_level(lambda c: CLFM(corr_2d, c, fusion_fn))
         if cfgs.fuse_estimator:
             dim_2d = self.branch_2d_flow_estimator.flow_feat_dim
             dim_3d = self.branch_3d_flow_estimator.flow_feat_dim
-            self.estimator_clfm = CLFM(dim_2d, dim_3d)
+            self.estimator_clfm = CLFM(dim_2d, dim_3d, fusion_fn)
             self.branch_2d_conv_last = nn.Conv2d(dim_2d, 2, kernel_size=3, stride=1, padding=1)
             self.branch_3d_conv_last = nn.Conv1d(dim_3d, 3, kernel_size=1)
 

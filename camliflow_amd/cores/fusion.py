@@ -191,6 +191,8 @@ _FUSIONS = {'add': (AddFusion, {}), 'concat': (ConcatFusion, {}), 'gated': (Gate
 
 
 class CLFM(nn.Module):
+    """``norm`` is that of the interpolation's and the merge's layers; ``fusion_fn='attn'`` has neither, and group norms of its own."""
+
     def __init__(self, in_channels_2d, in_channels_3d, fusion_fn='sk', norm=None):
         super().__init__()
         self.attends = fusion_fn == 'attn'

@@ -146,8 +146,9 @@ def relative_position_bias(table: torch.Tensor, q_pos: torch.Tensor, k_pos: torc
     numbers (the running index of a sequence, pixel coordinates); beyond -2^26 .. 2^26 they count as that bound.  ``bidirectional``: half the buckets for each sign, the upper half
     for keys after the query; otherwise all buckets for keys before the query, and keys after it share bucket 0.  Of the s buckets of a
     side, e = s // 2 hold one distance each; bucket e + j begins at the first distance >= e (max_distance / e)^(j / (s - e)), and the last
-    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023; at most 65535 samples x heads, 2000000 queries, 16000000 keys.  Differentiable in the table (once, in reverse mode);
-    the same bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
+    one holds everything from there on.  1 or 2 axes, axes * buckets <= 128, max_distance <= 1023; at most 65535 samples x heads, 2000000 queries, 16000000 keys.
+    Differentiable in the table (once, in reverse mode; a workgroup's elements are added in fp32, the workgroups' sums in 64 bits); the same
+    bits on every run.  ``cpp_impl=False``: the same from torch primitives, on any device."""
     name = 'relative_position_bias'
     table, q_pos, k_pos, batch, _ = _check_bias(name, table, q_pos, k_pos, bidirectional, max_distance, table.dtype if table is not None else None)
     if (batch or 1) * table.shape[2] > 65535 or q_pos.shape[-2] > 2000000 or k_pos.shape[-2] > 16000000:
@@ -299,8 +300,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale=Non
                     q_pos=None, k_pos=None, bidirectional=True, max_distance=128, cpp_impl=True):
     """softmax(scale q k^T + bias) v of queries q [B, Lq, H, D] over keys and values k, v [B, Lk, Hk, D] of another length -> [B, Lq, H, D].
 
-    fp32, bf16 or fp16 (one type for all; sums and softmax in fp32; fp32 factors go through the matrix unit as three bf16 parts each, exact to
-    2^-25, so an infinity or a value beyond 3.38e38 among kept fp32 operands gives NaN); D a multiple of 8 up to 128; H a multiple of Hk (query heads
+    fp32, bf16 or fp16 (one type for all; sums and softmax in fp32).  16-bit types: the probabilities are rounded to the type for the product
+    with v (where a gradient is wanted they enter as two terms of it), and they and the gradients of the scores once each for the products
+    that give the gradients of v, q and k.  fp32 factors go through the matrix unit as three bf16 parts each, exact to 2^-25, so an infinity
+    or a value beyond 3.38e38 among kept fp32 operands gives NaN.  Scores that are all as low as a finite mask entry differ by what fp32 holds
+    next to it.  D a multiple of 8 up to 128; H a multiple of Hk (query heads
     h share key / value head h // (H / Hk)).  Any strides: rows that are not adjacent or 16-byte aligned are copied first.  ``scale``:
     from 1e-15 to 1e15, default D ** -0.5.  One token (Lq = 1) and other short queries are split over the keys.
 

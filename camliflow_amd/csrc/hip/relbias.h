@@ -79,33 +79,14 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Two additions to a thread's own histogram column, at byte offsets.  Plain reads and writes, because nobody else touches the column: an LDS
-// float add serialises its lanes here (193 cycles per wave instruction and CU measured, against 12 for a dependent read-add-write).  The two
-// cells may be the same one.
+// Two additions to a column of a histogram, at byte offsets.  Plain reads and writes: an LDS float add serialises its lanes here (193 cycles per
+// wave instruction and CU measured, against 12 for a dependent read-add-write).  They may be, because no other thread writes these cells at
+// the same time.  One axis: a column is one thread's.  Two: lanes l and l + 32 of a wave share a column and are among the rows of different
+// axes at any time; wave_order() stands where they change axes.  The two cells may be the same one.
 __device__ __forceinline__ void hist_add2(char* cells, unsigned at0, float v0, unsigned at1, float v1) {
     float x0 = *reinterpret_cast<float*>(cells + at0), x1 = *reinterpret_cast<float*>(cells + at1);
     x0 += v0;
     x1 = (at0 == at1 ? x0 : x1) + v1;
     *reinterpret_cast<float*>(cells + at0) = x0;
     *reinterpret_cast<float*>(cells + at1) = x1;
-}
-// ... and for every axis, whose cells never coincide: all reads on their way before the first addition
-template <int AXES>
-__device__ __forceinline__ void hist_add2(char* column, const unsigned (&at0)[AXES], float v0, const unsigned (&at1)[AXES], float v1) {
-    float x0[AXES], x1[AXES];
-#pragma unroll
-    for (int a = 0; a < AXES; ++a) {
-        x0[a] = *reinterpret_cast<float*>(column + at0[a]);
-        x1[a] = *reinterpret_cast<float*>(column + at1[a]);
-    }
-#pragma unroll
-    for (int a = 0; a < AXES; ++a) {
-        x0[a] += v0;
-        x1[a] = (at0[a] == at1[a] ? x0[a] : x1[a]) + v1;
-    }
-#pragma unroll
-    for (int a = 0; a < AXES; ++a) {
-        *reinterpret_cast<float*>(column + at0[a]) = x0[a];
-        *reinterpret_cast<float*>(column + at1[a]) = x1[a];
-    }
 }

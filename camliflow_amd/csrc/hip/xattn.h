@@ -1,6 +1,6 @@
 // Cross attention over keys and values of another length, with an optional bucketed position bias: forward, both adjoints, gfx950.
-// The three element types instantiate these kernels in files of their own (xattn_f32.hip, xattn_bf16.hip, xattn_f16.hip); checks,
-// split rules and the C entries are in xattn.hip.
+// The instantiations are in files of their own, by kernel and element type (xattn_{fwd,dq,dkdv,far}_{f32,bf16,f16}.hip); checks, split rules
+// and the C entries are in xattn.hip.
 //
 //   s_ij = scale q_i . k_j + bias[h, i, j],   p = softmax_j over the kept keys,   o_i = sum_j p_ij v_j      (no kept key: o_i = 0)
 //   D_i = do_i . o_i,   dp_ij = do_i . v_j,   ds = p (dp - D),   dq = scale ds k,   dk = scale ds^T q,   dv = p^T do,

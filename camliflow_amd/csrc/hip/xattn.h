@@ -577,7 +577,7 @@ __device__ __forceinline__ bool is_far(float lse) { return fabsf(lse) > FAR && l
 // TRAIN (16-bit types): out has to be known to more than its own type for the backward's D = do . o, which is subtracted from
 // dp: P enters the product as two terms of the type and out is stored before its rounding as well.  Without that the bias table's
 // gradient, a sum over whole rows of ds, is off by twice its own rounding.
-// Measured: 4 x 8160 queries x 8160 keys, 2 heads of 128, bf16: 280 us = 974 TFLOP/s (a large library product: 1132), bound by the matrix
+// Measured: 4 x 8160 queries x 8160 keys, 2 heads of 128, bf16: 290 to 309 us from card to card, 880 to 940 TFLOP/s (a large library product: 1132), bound by the matrix
 // unit; 8 x 8160 x 2048, 4 heads of 32 with a two-axis bias, bf16, training: 305 us, bound by vector arithmetic (14 instructions a pair, exp
 // of four issue slots); the other way round in fp32, 2 x 2048 x 8160: 156 us.
 // fp32 with a bias starts at zero and subtracts m at the end: at -m / scale every step of the product rounds to a few bits less (a relative
@@ -1097,9 +1097,10 @@ constexpr int dkdv_stats(bool far_rows) { return far_rows ? 3 : 2; }       // nu
 // buckets would not fit.  Two axes: lanes l and l + 32 share a column; they take the axes in opposite order, so that one is among the rows of
 // the first axis while the other is among those of the second.  With that, 32-row tiles and eight registers' cells at a time three
 // workgroups share a CU in narrow 16-bit heads, one computing while another waits at a barrier or for LDS.
-// Measured with a two-axis bias of 2 x 32 buckets, 4 heads of 32: 8 x 8160 queries x 2048 keys, bf16: 495 us (a column per thread, two
-// workgroups: 547; adding a block's ds while the next one is computed took 16 % of the vector instructions away and no time), LDS and vector
-// arithmetic both at about 60 %; 2 x 2048 x 8160, fp32: 265 us (tiles in two buffers, one workgroup: 465 with fp32 products).
+// Measured with a two-axis bias of 2 x 32 buckets, 4 heads of 32: 8 x 8160 queries x 2048 keys, bf16: 480 us (a column per thread, two
+// workgroups: 547; adding a block's ds while the next one is computed took 16 % of the vector instructions away and no time).  LDS and vector
+// arithmetic are both busy 61 % of the time: waves wait for LDS reads and at barriers 45 % of their cycles, and the registers allow only three
+// a SIMD to cover that.  2 x 2048 x 8160, fp32: 265 us (tiles in two buffers, one workgroup: 465 with fp32 products).
 constexpr int hist_columns(int axes, int waves) { return axes == 2 ? 32 * waves : 64 * waves; }
 
 // blocks: of the launch's workgroups those that work on this
@@ -1323,7 +1324,8 @@ template <typename T, int DP, int AXES, int WAVES, bool HIST>
 __global__ __launch_bounds__(64 * WAVES, DP == 32 ? ((!HIST && AXES == 2) || sizeof(T) == 4 ? 2 : 3) : DP == 64 && !(HIST && sizeof(T) == 4) ? 2 : 1) void dq_kernel(Args a) { dq_body<T, DP, AXES, WAVES, HIST, false>(a, blockIdx.x, gridDim.x); }
 
 // ------------------------------------------------------------------------------------------------------------ dk, dv
-// Measured at the sizes above: bf16 390 us (vector arithmetic and LDS both at 55 %, three workgroups a CU), fp32 250 us.
+// Measured at the sizes above: bf16 360 us (LDS busy 57 % of the time, vector arithmetic 52 %; waves wait 43 % of their cycles for LDS reads and at
+// barriers, three of them on a SIMD), fp32 250 us.
 template <typename T, int DP, int AXES, bool FAR_ROWS>
 __device__ __forceinline__ void dkdv_body(const Args& a, int block, int blocks) {
     constexpr int R = tile_rows(sizeof(T), DP);

@@ -24,11 +24,15 @@ def sources():
     return sorted(os.path.join(HIP_DIR, f) for f in os.listdir(HIP_DIR) if f.endswith(".hip"))
 
 
+def headers():
+    return [os.path.join(d, f) for d in (HIP_DIR, INCLUDE_DIR) for f in os.listdir(d) if f.endswith(".h")]
+
+
 def needs_build():
     if not os.path.exists(LIB_PATH):
         return True
     t = os.path.getmtime(LIB_PATH)
-    deps = sources() + [os.path.join(HIP_DIR, f) for f in os.listdir(HIP_DIR) if f.endswith(".h")]
+    deps = sources() + headers() + [os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -43,9 +47,7 @@ def build(force=False, verbose=False):
         raise RuntimeError("hipcc not found: cannot build libcamli_hip.so")
     obj_dir = os.path.join(HERE, "build")
     os.makedirs(obj_dir, exist_ok=True)
-    headers = [os.path.join(HIP_DIR, f) for f in os.listdir(HIP_DIR) if f.endswith(".h")]
-    headers += [os.path.join(INCLUDE_DIR, f) for f in os.listdir(INCLUDE_DIR) if f.endswith(".h")]
-    newest_header = max(os.path.getmtime(h) for h in headers)
+    newest_header = max(os.path.getmtime(h) for h in headers() + [os.path.abspath(__file__)])       # this file holds the flags
     compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
 
     def compile_one(src):

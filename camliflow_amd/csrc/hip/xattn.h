@@ -698,7 +698,7 @@ __global__ __launch_bounds__(256, DP == 32 ? (AXES || sizeof(T) == 4 ? 3 : 4) : 
             float base = FOLD && !far ? m_use : 0.0f;
             if constexpr (AXES == 0) top *= a.scale_log2;
             if (unset || __any(top + (base - m_use) > exponent_limit<T>())) {
-                // a row's own need decides: its result does not depend on the rows beside it
+                // a row's own need decides where its reference goes; rows beside it (far ones) change no more than when it is subtracted
                 top = half_max(top);
                 const float mn = m == -INFINITY || top + (base - m_use) > exponent_limit<T>() ? fmaxf(m, top + base) : m, use = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m - use);
